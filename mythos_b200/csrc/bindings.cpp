@@ -885,6 +885,108 @@ void paged_attn_decode_int8(const Tensor& q, const Tensor& k_cache, const Tensor
                              (int)splits, (float)scale, status_ptr(status), cur_stream(), q.stride(0));
 }
 
+// 4-bit pages: caches [pages, kv_heads, page_size * (head_dim / 2 + head_dim / 16)] uint8.
+mb::KvInt4Cache kv4_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, int64_t kv_heads, int64_t head_dim,
+                          const char* who) {
+  chk_c(k_cache, U8, "k_cache");
+  chk_c(v_cache, U8, "v_cache");
+  chk_c(block_table, I32, "block_table");
+  TORCH_CHECK(head_dim == 64 || head_dim == 128, who, ": head_dim must be 64 or 128, got ", head_dim);
+  const int64_t token = head_dim / 2 + head_dim / 16;
+  TORCH_CHECK(k_cache.dim() == 3 && k_cache.size(1) == kv_heads && k_cache.size(2) > 0 && k_cache.size(2) % (16 * token) == 0 &&
+                  v_cache.sizes() == k_cache.sizes(),
+              who, ": caches must be [pages, ", kv_heads, ", page_size * ", token, "] with page_size a multiple of 16");
+  TORCH_CHECK(block_table.dim() == 2, who, ": block_table must be [sequences, pages]");
+  TORCH_CHECK(v_cache.device() == k_cache.device() && block_table.device() == k_cache.device(), who, ": tensors on several devices");
+  return {k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr<int>(), (int)k_cache.size(0), (int)kv_heads, (int)head_dim,
+          (int)(k_cache.size(2) / token), (int)block_table.size(0), (int)block_table.size(1)};
+}
+void kv4_tokens(const Tensor& positions, const Tensor& seq_ids, const Tensor& cache, int64_t tokens, const char* who) {
+  chk_c(positions, I32, "positions");
+  chk_c(seq_ids, I32, "seq_ids");
+  TORCH_CHECK(positions.numel() == tokens && seq_ids.numel() == tokens, who, ": one position and one sequence per token");
+  TORCH_CHECK(positions.device() == cache.device() && seq_ids.device() == cache.device(), who, ": tensors on several devices");
+}
+// Rows [tokens, heads, head_dim] with contiguous heads and a token stride.
+void kv4_rows(const Tensor& t, const Tensor& cache, const char* name, const char* who) {
+  chk(t, BF16, name);
+  TORCH_CHECK(t.dim() == 3 && t.stride(2) == 1 && (t.size(1) <= 1 || t.stride(1) == t.size(2)) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * t.size(2))),
+              who, ": ", name, " must be [tokens, heads, head_dim] with contiguous heads and a token stride of a multiple of 8");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, who, ": ", name, " must be 16-byte aligned");
+  TORCH_CHECK(t.device() == cache.device(), who, ": tensors on several devices");
+}
+
+int64_t kv4_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+
+void kv_append_int4(const Tensor& k, const Tensor& v, Tensor& k_cache, Tensor& v_cache, const Tensor& block_table,
+                    const Tensor& positions, const Tensor& seq_ids) {
+  const char* who = "kv_append_int4";
+  kv4_rows(k, k_cache, "k", who);
+  kv4_rows(v, k_cache, "v", who);
+  TORCH_CHECK(k.sizes() == v.sizes(), who, ": k and v must have the same shape");
+  const auto c = kv4_cache(k_cache, v_cache, block_table, k.size(1), k.size(2), who);
+  kv4_tokens(positions, seq_ids, k_cache, k.size(0), who);
+  c10::cuda::CUDAGuard guard(k.device());
+  mb::kv_append_int4(c, k.data_ptr(), v.data_ptr(), positions.data_ptr<int>(), seq_ids.data_ptr<int>(), (int)k.size(0), kv4_stride(k),
+                     kv4_stride(v), cur_stream());
+}
+
+void kv_read_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& positions,
+                  const Tensor& seq_ids, Tensor& k, Tensor& v) {
+  const char* who = "kv_read_int4";
+  chk_c(k, BF16, "k");
+  chk_c(v, BF16, "v");
+  kv4_rows(k, k_cache, "k", who);
+  kv4_rows(v, k_cache, "v", who);
+  TORCH_CHECK(k.sizes() == v.sizes(), who, ": k and v must have the same shape");
+  const auto c = kv4_cache(k_cache, v_cache, block_table, k.size(1), k.size(2), who);
+  kv4_tokens(positions, seq_ids, k_cache, k.size(0), who);
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  mb::kv_read_int4(c, positions.data_ptr<int>(), seq_ids.data_ptr<int>(), (int)k.size(0), k.data_ptr(), v.data_ptr(), cur_stream());
+}
+
+void paged_attn_decode_int4(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                            const Tensor& context_lens, Tensor& out, double scale, const OptTensor& status) {
+  const char* who = "paged_attn_decode_int4";
+  kv4_rows(q, k_cache, "q", who);
+  chk_c(context_lens, I32, "context_lens");
+  chk_c(out, BF16, "out");
+  kv4_rows(out, k_cache, "out", who);
+  TORCH_CHECK(k_cache.dim() == 3 && k_cache.size(1) > 0 && q.size(1) % k_cache.size(1) == 0, who, ": heads must be a multiple of kv_heads");
+  TORCH_CHECK(out.sizes() == q.sizes(), who, ": out must match q");
+  TORCH_CHECK(context_lens.numel() == q.size(0) && context_lens.device() == q.device() && block_table.size(0) >= q.size(0), who,
+              ": one context length and one table row per query token");
+  const auto c = kv4_cache(k_cache, v_cache, block_table, k_cache.size(1), q.size(2), who);
+  c10::cuda::CUDAGuard guard(q.device());
+  mb::paged_attn_decode_int4(c, q.data_ptr(), kv4_stride(q), context_lens.data_ptr<int>(), out.data_ptr(), (int)q.size(0), (int)q.size(1),
+                             (float)scale, status_ptr(status), cur_stream());
+}
+
+void paged_attn_prefill_int4(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                             const Tensor& cu_q, const Tensor& kv_lens, Tensor& out, int64_t max_q_len, int64_t max_kv_len,
+                             double scale, const OptTensor& status) {
+  const char* who = "paged_attn_prefill_int4";
+  kv4_rows(q, k_cache, "q", who);
+  kv4_rows(out, k_cache, "out", who);
+  chk_c(cu_q, I32, "cu_q");
+  chk_c(kv_lens, I32, "kv_lens");
+  TORCH_CHECK(k_cache.dim() == 3 && k_cache.size(1) > 0 && q.size(1) % k_cache.size(1) == 0, who, ": heads must be a multiple of kv_heads");
+  TORCH_CHECK(out.sizes() == q.sizes(), who, ": out must match q");
+  const auto c = kv4_cache(k_cache, v_cache, block_table, k_cache.size(1), q.size(2), who);
+  const int64_t B = kv_lens.numel();
+  TORCH_CHECK(cu_q.numel() == B + 1 && block_table.size(0) >= B, who, ": cu_q must have one entry more than kv_lens, block_table a row per sequence");
+  TORCH_CHECK(cu_q.device() == q.device() && kv_lens.device() == q.device(), who, ": tensors on several devices");
+  TORCH_CHECK(max_q_len >= 0 && max_q_len <= q.size(0) && max_kv_len >= 0 && max_kv_len <= (int64_t)c.max_pages * c.page_size, who,
+              ": max_q_len must be within q and max_kv_len within the table's pages");
+  c10::cuda::CUDAGuard guard(q.device());
+  const int64_t bytes = mb::paged_attn_prefill_int4_workspace((int)B, (int)max_q_len, (int)max_kv_len, (int)q.size(1), c.kv_heads, c.head_dim);
+  Tensor work;
+  if (bytes > 0) work = torch::empty({bytes}, q.options().dtype(U8));
+  mb::paged_attn_prefill_int4(c, q.data_ptr(), kv4_stride(q), cu_q.data_ptr<int>(), kv_lens.data_ptr<int>(), out.data_ptr(), kv4_stride(out),
+                              (int)B, (int)q.size(0), (int)max_q_len, (int)max_kv_len, (int)q.size(1), (float)scale,
+                              bytes > 0 ? work.data_ptr() : nullptr, status_ptr(status), cur_stream());
+}
+
 void peer_add_f32(const Tensor& part, const std::vector<int64_t>& ptrs) {
   chk_c(part, F32, "part");
   c10::cuda::CUDAGuard guard(part.device());
@@ -1138,6 +1240,13 @@ PYBIND11_MODULE(_C, m) {
   m.def("paged_attn_decode_int8", &paged_attn_decode_int8, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"), py::arg("context_lens"), py::arg("out"),
         py::arg("scratch"), py::arg("counters"), py::arg("splits"), py::arg("scale"), py::arg("status") = py::none());
+  m.def("kv_append_int4", &kv_append_int4);
+  m.def("kv_read_int4", &kv_read_int4);
+  m.def("paged_attn_decode_int4", &paged_attn_decode_int4, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"),
+        py::arg("context_lens"), py::arg("out"), py::arg("scale"), py::arg("status") = py::none());
+  m.def("paged_attn_prefill_int4", &paged_attn_prefill_int4, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"),
+        py::arg("cu_q"), py::arg("kv_lens"), py::arg("out"), py::arg("max_q_len"), py::arg("max_kv_len"), py::arg("scale"),
+        py::arg("status") = py::none());
   m.def("sample_tokens", &sample_tokens);
   m.def("moe_topk", &moe_topk);
   m.def("moe_dispatch", &moe_dispatch, py::arg("x"), py::arg("topk_idx"), py::arg("slot"), py::arg("send_off"),

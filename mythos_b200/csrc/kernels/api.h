@@ -374,6 +374,35 @@ void paged_attn_decode_int8(const void* q, const void* k_cache, const void* v_ca
                             float* scratch, int* counters, int batch, int heads, int kv_heads, int head_dim,
                             int page_size, int max_pages, int cache_pages, int splits, float scale, int* status,
                             cudaStream_t stream, long long q_tok_stride = 0);
+// 4-bit paged KV cache (format: kv_int4.cuh). k, v: [n_pages, kv_heads, page_size * (head_dim / 2 + head_dim / 16)] bytes,
+// addressed through block_table [n_seqs, max_pages]; head_dim 64 or 128, page_size a multiple of 16.
+struct KvInt4Cache {
+  void* k;
+  void* v;
+  const int* block_table;
+  int n_pages, kv_heads, head_dim, page_size, n_seqs, max_pages;
+};
+// Quantises the rows k, v [tokens, kv_heads, head_dim] (bf16, token strides of their own) into the places of
+// (seq_ids, positions). A token without a page (sequence or position outside the table, page id outside the cache)
+// is dropped.
+void kv_append_int4(const KvInt4Cache& c, const void* k, const void* v, const int* positions, const int* seq_ids, int tokens,
+                    long long k_stride, long long v_stride, cudaStream_t stream);
+// The rows at (seq_ids, positions) as bf16 [tokens, kv_heads, head_dim]; a token without a page reads as zeros.
+void kv_read_int4(const KvInt4Cache& c, const int* positions, const int* seq_ids, int tokens, void* k, void* v, cudaStream_t stream);
+// One query token per sequence: q [batch, heads, head_dim] with a token stride, out contiguous. A sequence of length 0
+// gets zeros; a token of the context without a page is left out and reported through the status word.
+void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* context_lens, void* out, int batch,
+                            int heads, float scale, int* status, cudaStream_t stream);
+// New tokens of several sequences packed back to back, causal over the pages (as flash_attn_paged_prefill). max_q: most new
+// tokens of a sequence, max_kv: most keys. Up to P4_FEW_COLUMNS query columns (new tokens x heads of a group) a kv head, a
+// split-context kernel reads the codes directly; above, the sequences are expanded into bf16 pages in the workspace
+// (paged_attn_prefill_int4_workspace bytes, 0: none wanted), each once for all of its queries, and the tcgen05 prompt
+// kernel runs on those.
+constexpr int P4_FEW_COLUMNS = 64;
+long long paged_attn_prefill_int4_workspace(int batch, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
+void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
+                             long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale,
+                             void* workspace, int* status, cudaStream_t stream);
 // Greedy / temperature / top-k / top-p / repetition-penalty sampling of one token per row.
 struct SamplerArgs {
   float temperature, top_p, repetition_penalty;

@@ -1,0 +1,95 @@
+// Format of the 4-bit paged KV cache, shared by the kernels that write and read it.
+//
+// A row of D values (one token, one kv head, K or V; D = 64 or 128) is cut into groups of 64. A group is
+// stored as scale = bf16((max - min) / 15), low = min (a bf16 already, so exact) and 64 codes
+// clamp(round_to_even((x - low) / scale), 0, 15); it stands for scale * code + low. The range is kept
+// asymmetric because keys carry per-channel offsets: a symmetric scale would spend codes on values that do
+// not occur. The scale is rounded to bf16 (half the bytes of fp32): codes are formed against the rounded
+// scale, so its rounding moves the grid by at most 2^-9 of a step per code and adds no error of its own.
+// 64 values per group cost 4.5 bits a value; groups of 32 would cost 5 (one ninth more bytes to read per
+// decoded token). A group with a NaN, an infinity or a range beyond fp32 has a NaN or infinite scale and
+// reads back as NaN: nothing finite is made up.
+//
+// A cache is [pages, kv_heads, page_size / 16 tiles, TILE_BYTES] bytes. A tile is 16 tokens: 16 rows of codes
+// (D / 2 bytes each), then 16 rows of (scale, low) pairs (D / 16 bytes each); contiguous, a multiple of 16
+// bytes, so one bulk copy fetches it. The order inside a tile is that of the tensor-core fragments the attention
+// kernel builds, so that a thread reads its operands with 16-byte (keys) and 8-byte (values) shared loads,
+// without bank conflicts and without ldmatrix:
+//   * eight consecutive values share a 32-bit word; value 2 i + j sits in nibble i + 4 j: word >> 4 i masked by
+//     0x000F000F is the pair (2 i, 2 i + 1) in the two halves of a register;
+//   * token n of a tile has key row (and pair row, K and V) 8 (n / 8) + 2 (n % 4) + (n / 4) % 2 and value row n:
+//     the score fragment of a thread (columns 2 t, 2 t + 1 of two 8-token products) then covers tokens t, t + 4,
+//     t + 8 and t + 12, whose value rows lie in different banks for the four t;
+//   * a key row is [t = 0..3][group][2 words]: values 64 g + 16 t + 8 h ...; the words are rotated left by three
+//     bits, which puts a nibble on the top mantissa bits of a bf16: masked by 0x00780078 and joined with 0x4180 it
+//     is the number 16 + code;
+//   * a value row is [r = 0..7][group][1 word]: values 64 g + 8 r ...; chunk r is stored at place r ^ 4 ((n / 2) % 2).
+#pragma once
+#include "common.cuh"
+
+namespace mb {
+
+template <int D>
+struct KvInt4 {
+  static constexpr int GROUPS = D / 64;
+  static constexpr int ROW = D / 2;                  // code bytes of a token
+  static constexpr int PAIR = GROUPS * 4;            // (scale, low) bytes of a token
+  static constexpr int OFF_PAIR = 16 * ROW;
+  static constexpr int TILE_BYTES = 16 * (ROW + PAIR);
+};
+
+// Row of token n (0..15) among the key rows and the pair rows of a tile.
+__device__ __forceinline__ int kv4_row(int n) { return (n & 8) + ((n & 3) << 1) + ((n >> 2) & 1); }
+// Byte offset of the word that holds values 64 g + 8 u .. (u = 0..7) inside a tile.
+template <int D>
+__device__ __forceinline__ int kv4_key_word(int n, int g, int u) {
+  return kv4_row(n) * KvInt4<D>::ROW + ((u >> 1) * KvInt4<D>::GROUPS + g) * 8 + (u & 1) * 4;
+}
+template <int D>
+__device__ __forceinline__ int kv4_value_word(int n, int g, int u) {
+  return n * KvInt4<D>::ROW + ((u ^ (((n >> 1) & 1) << 2)) * KvInt4<D>::GROUPS + g) * 4;
+}
+template <int D>
+__device__ __forceinline__ int kv4_pair(int n, int g) {
+  return KvInt4<D>::OFF_PAIR + kv4_row(n) * KvInt4<D>::PAIR + g * 4;
+}
+
+// Tile of token `pos` of a sequence (its table row in `table`) and its place in the tile, or -1 for a token
+// without a page: a position outside the table, a page id outside the cache.
+__device__ __forceinline__ int kv4_tile(const int* __restrict__ table, int pos, int max_pages, int n_pages, int page_size,
+                                        int kv_heads, int head) {
+  if (pos < 0) return -1;
+  const int lp = pos / page_size;
+  if (lp >= max_pages) return -1;
+  const int page = table[lp];
+  if (page < 0 || page >= n_pages) return -1;
+  return (page * kv_heads + head) * (page_size >> 4) + ((pos - lp * page_size) >> 4);
+}
+
+// (scale, low) of a group from its extremes; the low half of the word is the scale.
+__device__ __forceinline__ uint32_t kv4_make_pair(__nv_bfloat16 lo, __nv_bfloat16 hi, float& scale, float& low) {
+  low = __bfloat162float(lo);
+  const __nv_bfloat16 s = __float2bfloat16(__fdiv_rn(__bfloat162float(hi) - low, 15.f));
+  scale = __bfloat162float(s);
+  return (uint32_t)__bfloat16_as_ushort(s) | (uint32_t)__bfloat16_as_ushort(lo) << 16;
+}
+__device__ __forceinline__ uint32_t kv4_code(float x, float scale, float low) {
+  // true division: the nearest code, ties to even, whatever the scale (a reciprocal would move ties)
+  const int c = __float2int_rn(__fdiv_rn(x - low, scale));
+  return scale > 0.f ? (uint32_t)max(0, min(15, c)) : 0u;
+}
+// Word of eight consecutive values.
+__device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], float scale, float low) {
+  uint32_t w = 0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w |= kv4_code(x[e], scale, low) << (4 * ((e >> 1) + 4 * (e & 1)));
+  return w;
+}
+__device__ __forceinline__ uint32_t kv4_rotate(uint32_t w) { return __funnelshift_l(w, w, 3); }
+__device__ __forceinline__ uint32_t kv4_unrotate(uint32_t w) { return __funnelshift_r(w, w, 3); }
+__device__ __forceinline__ float kv4_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float kv4_low(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
+// Whether a group's scale and low are finite.
+__device__ __forceinline__ bool kv4_finite(uint32_t pair) { return (pair & 0x7F80u) != 0x7F80u && (pair & 0x7F800000u) != 0x7F800000u; }
+
+}  // namespace mb

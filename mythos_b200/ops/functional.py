@@ -701,3 +701,67 @@ def sumsq(x, out=None):
     else:
         out += x.float().pow(2).sum()
     return out
+
+
+# --------------------------------------------------------------------------------------- 4-bit paged KV cache
+# Caches are uint8 [pages, kv_heads, page_size * kv4_token_bytes(head_dim)] (``infer.kv_paged.PagedKVCache(dtype=torch.uint8)``
+# makes them), page_size a multiple of 16, head_dim 64 or 128, addressed through an int32 table [sequences, pages].
+kv4_token_bytes = ref.kv4_token_bytes
+
+
+def kv_append_int4(k, v, k_cache, v_cache, block_table, positions, seq_ids) -> None:
+    """Quantise new K / V rows (bf16 [tokens, kv_heads, head_dim], token strides free) to 4 bits and store them at
+    ``(seq_ids, positions)``: per 64 values a bf16 scale and minimum. Tokens without a page (a sequence or position
+    outside the table, a page id outside the cache) are dropped. The same place twice in one call holds parts of
+    either row."""
+    if k.is_cuda:
+        _C().kv_append_int4(k, v, k_cache, v_cache, block_table, positions, seq_ids)
+    else:
+        ref.kv_append_int4(k, v, k_cache, v_cache, block_table, positions, seq_ids)
+
+
+def kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim: int):
+    """The rows at ``(seq_ids, positions)`` of 4-bit pages as bf16 ``(k, v)`` [tokens, kv_heads, head_dim]; a token
+    without a page reads as zeros."""
+    if not k_cache.is_cuda:
+        return ref.kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim)
+    shape = (positions.numel(), k_cache.shape[1], head_dim)
+    k = torch.empty(shape, device=k_cache.device, dtype=torch.bfloat16)
+    v = torch.empty(shape, device=k_cache.device, dtype=torch.bfloat16)
+    _C().kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, k, v)
+    return k, v
+
+
+def paged_attn_decode_int4(q, k_cache, v_cache, block_table, context_lens, scale: float | None = None, out=None):
+    """Attention of one new token per sequence (q bf16 [batch, heads, head_dim], already in the pages) over 4-bit
+    pages. Row b reads ``block_table[b]``; a context length of 0 gives zeros. A token of the context without a page is
+    left out and reported (``native.check_status``)."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    if not q.is_cuda:
+        if context_lens.numel() != q.shape[0]:
+            raise ValueError("paged_attn_decode_int4: one context length per query token")
+        cu = torch.arange(q.shape[0] + 1, dtype=torch.int32)
+        o = ref.paged_attn_int4(q, k_cache, v_cache, block_table, cu, context_lens, scale)
+        return o if out is None else out.copy_(o)
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+    _C().paged_attn_decode_int4(q, k_cache, v_cache, block_table, context_lens, out, scale, native.status_word(q.device))
+    return out
+
+
+def paged_attn_prefill_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q_len: int, max_kv_len: int,
+                            scale: float | None = None, out=None):
+    """Causal attention of the new tokens of several sequences (q bf16 [tokens, heads, head_dim], sequence b = rows
+    ``cu_q[b] .. cu_q[b + 1]``, already in the pages) over 4-bit pages; ``kv_lens[b]`` counts the keys its last token
+    sees. ``max_q_len`` / ``max_kv_len``: host integers that no sequence's new tokens / keys exceed. Rows of ``out`` behind the
+    last sequence are left as they are."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    if not q.is_cuda:
+        o = ref.paged_attn_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, scale)
+        if out is None:
+            return o
+        out[: int(cu_q[-1])] = o[: int(cu_q[-1])]
+        return out
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+    _C().paged_attn_prefill_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, max_q_len, max_kv_len, scale,
+                                 native.status_word(q.device))
+    return out

@@ -192,3 +192,146 @@ def load_balance_loss(probs, experts, num_experts: int):
 
 def z_loss(logits, coef: float):
     return coef * torch.logsumexp(logits.float(), dim=-1).pow(2).mean()
+
+
+# --------------------------------------------------------------------------------------- 4-bit KV cache
+# Format (csrc/kernels/kv_int4.cuh): groups of 64 values with scale = bf16((max - min) / 15), low = min and codes
+# clamp(round((x - low) / scale), 0, 15), standing for scale * code + low; caches [pages, kv_heads, page_size / 16 tiles
+# of 16 code rows and 16 (scale, low) rows] bytes.
+KV4_TILE, KV4_GROUP = 16, 64
+
+
+def kv4_token_bytes(head_dim: int) -> int:
+    """Bytes of one token's row (one kv head, K or V) in a 4-bit page: codes and one 4-byte pair per 64 values."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"4-bit pages: head_dim must be 64 or 128, got {head_dim}")
+    return head_dim // 2 + head_dim // 16
+
+
+def kv4_check(k_cache, v_cache, block_table, kv_heads: int, head_dim: int) -> int:
+    """Checks a pair of caches and their table; returns the page size."""
+    per = kv4_token_bytes(head_dim)
+    for c in (k_cache, v_cache):
+        if c.dtype != torch.uint8 or c.dim() != 3 or not c.is_contiguous():
+            raise ValueError("4-bit caches are contiguous uint8 tensors [pages, kv_heads, page bytes]")
+    if k_cache.shape != v_cache.shape or k_cache.shape[1] != kv_heads:
+        raise ValueError("4-bit caches: k and v caches of one shape, with the kv heads of the rows")
+    if k_cache.shape[2] == 0 or k_cache.shape[2] % (per * KV4_TILE):
+        raise ValueError(f"4-bit caches: a page holds a multiple of {KV4_TILE} tokens of {per} bytes each")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise ValueError("4-bit caches: block_table is int32 [sequences, pages]")
+    return k_cache.shape[2] // per
+
+
+def kv4_quantise(x):
+    """x [..., D] (bf16) -> (codes uint8 [..., D], scale, low: bf16 [..., D / 64])."""
+    g = x.float().unflatten(-1, (-1, KV4_GROUP))
+    lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    # (a tensor divisor: torch turns a division by a scalar into a product with its reciprocal)
+    scale = ((hi - lo) / torch.full_like(lo, 15.0)).to(torch.bfloat16).float()
+    code = torch.round((g - lo) / scale).clamp(0, 15)
+    code = torch.where((scale > 0) & ~code.isnan(), code, torch.zeros_like(code))
+    return code.to(torch.uint8).flatten(-2), scale.squeeze(-1).to(torch.bfloat16), lo.squeeze(-1).to(torch.bfloat16)
+
+
+def _kv4_row(n):
+    return (n & 8) + ((n & 3) << 1) + ((n >> 2) & 1)
+
+
+def kv4_places(block_table, page_size: int, n_pages: int, positions, seq_ids):
+    """(page, tile in the page, place in the tile, has a page) of every token."""
+    pos, seq = positions.long(), seq_ids.long()
+    ok = (seq >= 0) & (seq < block_table.shape[0]) & (pos >= 0) & (pos < block_table.shape[1] * page_size)
+    pos, seq = torch.where(ok, pos, 0), torch.where(ok, seq, 0)
+    if block_table.numel() == 0:
+        return pos, pos, pos, ok & False
+    page = block_table[seq, pos // page_size].long()
+    ok = ok & (page >= 0) & (page < n_pages)
+    return torch.where(ok, page, 0), pos % page_size // KV4_TILE, pos % KV4_TILE, ok
+
+
+def _kv4_views(cache, page_size: int, D: int):
+    tiles = cache.view(cache.shape[0], cache.shape[1], page_size // KV4_TILE, -1)
+    split = KV4_TILE * D // 2
+    return tiles[..., :split].unflatten(-1, (KV4_TILE, D // 2)), tiles[..., split:].unflatten(-1, (KV4_TILE, D // 16))
+
+
+def _kv4_word_order(D: int, n, is_key: bool):
+    """Word of the row that holds values 8 w .. 8 w + 7, for every token: [tokens, D / 8]."""
+    w = torch.arange(D // 8, device=n.device)
+    g, u = w // 8, w % 8
+    if is_key:
+        return ((u // 2 * (D // 64) + g) * 2 + u % 2).expand(n.numel(), -1)
+    return (u ^ (4 * (n // 2 % 2))[:, None]) * (D // 64) + g
+
+
+def kv_append_int4(k, v, k_cache, v_cache, block_table, positions, seq_ids):
+    """Quantises k, v [tokens, kv_heads, D] into the 4-bit pages (in place); tokens without a page are dropped."""
+    T, H, D = k.shape
+    page_size = kv4_check(k_cache, v_cache, block_table, H, D)
+    if v.shape != k.shape or positions.numel() != T or seq_ids.numel() != T:
+        raise ValueError("kv_append_int4: k and v of one shape, one position and one sequence per token")
+    page, tile, n, ok = kv4_places(block_table, page_size, k_cache.shape[0], positions, seq_ids)
+    page, tile, n = page[ok], tile[ok], n[ok]
+    at = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], device=k.device)      # bit position of value e of a word
+    for x, cache, is_key in ((k, k_cache, True), (v, v_cache, False)):
+        code, scale, low = kv4_quantise(x[ok])
+        w = (code.long().unflatten(-1, (-1, 8)) << at).sum(-1)              # [tokens, H, D / 8]
+        if is_key:
+            w = (w << 3 | w >> 29) & 0xFFFFFFFF
+        order = _kv4_word_order(D, n, is_key)[:, None].expand_as(w)
+        w = torch.empty_like(w).scatter_(2, order, w)
+        w = torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32).contiguous().view(torch.uint8)
+        rows, pairs = _kv4_views(cache, page_size, D)
+        rows[page, :, tile, _kv4_row(n) if is_key else n] = w
+        pairs[page, :, tile, _kv4_row(n)] = torch.stack([scale, low], -1).flatten(2).contiguous().view(torch.uint8)
+
+
+def kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim: int, dtype=torch.bfloat16):
+    """The rows at (seq_ids, positions): k, v [tokens, kv_heads, D]; zeros for tokens without a page."""
+    D, H = head_dim, k_cache.shape[1]
+    page_size = kv4_check(k_cache, v_cache, block_table, H, D)
+    if positions.numel() != seq_ids.numel():
+        raise ValueError("kv_read_int4: one position and one sequence per token")
+    page, tile, n, ok = kv4_places(block_table, page_size, k_cache.shape[0], positions, seq_ids)
+    at = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], device=k_cache.device)
+    out = []
+    for cache, is_key in ((k_cache, True), (v_cache, False)):
+        rows, pairs = _kv4_views(cache, page_size, D)
+        if cache.shape[0] == 0:
+            out.append(torch.zeros(n.numel(), H, D, dtype=dtype, device=cache.device))
+            continue
+        w = rows[page, :, tile, _kv4_row(n) if is_key else n].contiguous().view(torch.int32).long() & 0xFFFFFFFF
+        if is_key:
+            w = (w >> 3 | w << 29) & 0xFFFFFFFF
+        w = w.gather(2, _kv4_word_order(D, n, is_key)[:, None].expand_as(w))
+        code = (w[..., None] >> at & 15).flatten(2).float().unflatten(-1, (-1, KV4_GROUP))
+        pair = pairs[page, :, tile, _kv4_row(n)].contiguous().view(torch.bfloat16).float().unflatten(-1, (-1, 2))
+        x = (code * pair[..., :1] + pair[..., 1:]).flatten(2)
+        out.append(torch.where(ok[:, None, None], x, torch.zeros_like(x)).to(dtype))
+    return out[0], out[1]
+
+
+def paged_attn_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, scale: float):
+    """Causal attention of packed new tokens q [T, heads, D] (sequence b: rows cu_q[b] .. cu_q[b + 1], the last of its
+    kv_lens[b] keys) over 4-bit pages. A sequence without keys, and a query that sees none, give zeros."""
+    T, H, D = q.shape
+    Hk = k_cache.shape[1]
+    kv4_check(k_cache, v_cache, block_table, Hk, D)
+    if Hk == 0 or H % Hk or cu_q.numel() != kv_lens.numel() + 1 or block_table.shape[0] < kv_lens.numel():
+        raise ValueError("paged_attn_int4: heads in groups of the kv heads, cu_q with one entry more than kv_lens")
+    out = torch.zeros_like(q)
+    cu, lens = cu_q.tolist(), kv_lens.tolist()
+    for b, n in enumerate(lens):
+        a, e = cu[b], cu[b + 1]
+        if e <= a or n <= 0:
+            continue
+        pos = torch.arange(n, device=q.device)
+        k, v = kv_read_int4(k_cache, v_cache, block_table, pos, torch.full_like(pos, b), D, torch.float32)
+        k, v = (x.repeat_interleave(H // Hk, 1) for x in (k, v))
+        s = torch.einsum("qhd,khd->hqk", q[a:e].float(), k) * scale
+        hidden = pos[None] > n - (e - a) + torch.arange(e - a, device=q.device)[:, None]
+        p = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+        p = torch.where(hidden.all(-1)[:, None], torch.zeros_like(p), p)
+        out[a:e] = torch.einsum("hqk,khd->qhd", p, v).to(q.dtype)
+    return out
