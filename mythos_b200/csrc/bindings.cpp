@@ -979,7 +979,7 @@ void paged_attn_prefill_int4(const Tensor& q, const Tensor& k_cache, const Tenso
   TORCH_CHECK(max_q_len >= 0 && max_q_len <= q.size(0) && max_kv_len >= 0 && max_kv_len <= (int64_t)c.max_pages * c.page_size, who,
               ": max_q_len must be within q and max_kv_len within the table's pages");
   c10::cuda::CUDAGuard guard(q.device());
-  const int64_t bytes = mb::paged_attn_prefill_int4_workspace((int)B, (int)max_q_len, (int)max_kv_len, (int)q.size(1), c.kv_heads, c.head_dim);
+  const int64_t bytes = mb::paged_attn_prefill_int4_workspace((int)B, (int)q.size(0), (int)max_q_len, (int)max_kv_len, (int)q.size(1), c.kv_heads, c.head_dim);
   Tensor work;
   if (bytes > 0) work = torch::empty({bytes}, q.options().dtype(U8));
   mb::paged_attn_prefill_int4(c, q.data_ptr(), kv4_stride(q), cu_q.data_ptr<int>(), kv_lens.data_ptr<int>(), out.data_ptr(), kv4_stride(out),

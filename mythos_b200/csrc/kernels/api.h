@@ -394,15 +394,19 @@ void kv_read_int4(const KvInt4Cache& c, const int* positions, const int* seq_ids
 void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* context_lens, void* out, int batch,
                             int heads, float scale, int* status, cudaStream_t stream);
 // New tokens of several sequences packed back to back, causal over the pages (as flash_attn_paged_prefill). max_q: most new
-// tokens of a sequence, max_kv: most keys. Up to P4_FEW_COLUMNS query columns (new tokens x heads of a group) a kv head, a
-// split-context kernel reads the codes directly; above, the sequences are expanded into bf16 pages in the workspace
-// (paged_attn_prefill_int4_workspace bytes, 0: none wanted), each once for all of its queries, and the tcgen05 prompt
-// kernel runs on those.
+// tokens of a sequence, max_kv: most keys. Up to P4_FEW_COLUMNS query columns (new tokens x heads of a group) per kv head, a
+// split-context kernel reads the codes directly; above, prompt_int4 expands the sequences into the workspace
+// (paged_attn_prefill_int4_workspace bytes, 0: none wanted), each once for all of its queries.
 constexpr int P4_FEW_COLUMNS = 64;
-long long paged_attn_prefill_int4_workspace(int batch, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
+long long paged_attn_prefill_int4_workspace(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
 void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                              long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale,
                              void* workspace, int* status, cudaStream_t stream);
+// The second of its two forms (kv_int4_prefill.cu); arguments checked by the caller.
+long long prompt_int4_workspace(int batch, int total_q, int max_kv, int heads, int kv_heads, int head_dim);
+void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
+                 long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,
+                 int* status, cudaStream_t stream);
 // Greedy / temperature / top-k / top-p / repetition-penalty sampling of one token per row.
 struct SamplerArgs {
   float temperature, top_p, repetition_penalty;

@@ -104,57 +104,6 @@ kv_read_int4_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restri
   }
 }
 
-// Whole sequences into bf16 pages of 16 tokens, tile j of sequence b at page b * per_seq + j, with the block table
-// that names them so: the operands of the prompt kernel. Its matrix product multiplies masked probabilities of zero
-// by whatever the value rows hold, so nothing that is not finite goes there: tokens of a tile behind the sequence's end
-// are zeros, and a token with a scale that is not finite gets values of zero and NaN keys instead, which reach the queries
-// that see it through their scores and no others. Page 0 is always written: the prompt kernel reads it in place of tiles
-// that it masks.
-template <int D>
-__global__ void __launch_bounds__(256)
-kv_unpack_int4_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int* __restrict__ block_table,
-                      const int* __restrict__ kv_lens, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v,
-                      int* __restrict__ out_table, int kv_heads, int page_size, int max_pages, int n_pages, int per_seq,
-                      int* status) {
-  using L = KvInt4<D>;
-  constexpr int PER_ROW = D / 8;
-  const int b = blockIdx.y, j = blockIdx.x;
-  const int len = kv_lens[b];
-  if (threadIdx.x == 0) out_table[(long long)b * per_seq + j] = b * per_seq + j;
-  if (j * 16 >= len && (j > 0 || b > 0)) return;
-  const int* table = block_table + (long long)b * max_pages;
-  const int per_tok = kv_heads * PER_ROW;
-  const long long out = ((long long)b * per_seq + j) * 16 * per_tok;
-  for (int i = threadIdx.x; i < 16 * per_tok; i += blockDim.x) {
-    const int n = i / per_tok, c = i % per_tok;
-    const int head = c / PER_ROW, g = (c % PER_ROW) >> 3, u = c & 7;
-    uint32_t kw = 0u, vw = 0u, kp = 0u, vp = 0u;
-    if (j * 16 + n < len) {
-      const int tile = kv4_tile(table, j * 16, max_pages, n_pages, page_size, kv_heads, head);
-      if (tile >= 0) {
-        const uint8_t* ks = k_cache + (long long)tile * L::TILE_BYTES;
-        const uint8_t* vs = v_cache + (long long)tile * L::TILE_BYTES;
-        kw = kv4_unrotate(*reinterpret_cast<const uint32_t*>(ks + kv4_key_word<D>(n, g, u)));
-        vw = *reinterpret_cast<const uint32_t*>(vs + kv4_value_word<D>(n, g, u));
-        kp = *reinterpret_cast<const uint32_t*>(ks + kv4_pair<D>(n, g));
-        vp = *reinterpret_cast<const uint32_t*>(vs + kv4_pair<D>(n, g));
-        bool finite = true;
-#pragma unroll
-        for (int gg = 0; gg < L::GROUPS; ++gg)
-          finite = finite && kv4_finite(*reinterpret_cast<const uint32_t*>(vs + kv4_pair<D>(n, gg)));
-        if (!finite) {
-          kp = 0x7FFF7FFFu;
-          vp = vw = 0u;
-        }
-      } else if (status) {
-        atomicCAS(status, 0, ST_BAD_ARG | (91 << 16));
-      }
-    }
-    stg8(k, (out + i) * 8, kv4_expand(kw, kp));
-    stg8(v, (out + i) * 8, kv4_expand(vw, vp));
-  }
-}
-
 // ------------------------------------------------------------------------------------------------ attention
 // One (sequence, kv head, block of COLS query columns) per cluster; the CTAs of the cluster split its tiles. A column
 // is one (query token, head of the group) pair: column c is head c % G of token c / G. Four warps per CTA; warp w
@@ -696,6 +645,7 @@ void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_str
   MB_REQUIRE(heads > 0 && heads % c.kv_heads == 0, "paged_attn_decode_int4: heads must be a multiple of kv_heads");
   MB_REQUIRE(q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0,
              "paged_attn_decode_int4: q must be 16-byte aligned with a token stride of a multiple of 8 elements");
+  MB_REQUIRE(scale > 0.f, "paged_attn_decode_int4: scale must be positive");
   if (batch == 0) return;
   P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, context_lens, nullptr,
            (__nv_bfloat16*)out, q_stride, (long long)heads * c.head_dim, heads / c.kv_heads, c.kv_heads, batch, c.page_size,
@@ -703,10 +653,12 @@ void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_str
   p4_attention(a, c.head_dim, batch, 1, stream);
 }
 
-long long paged_attn_prefill_int4_workspace(int batch, int max_q, int max_kv, int heads, int kv_heads, int head_dim) {
-  if ((long long)max_q * (heads / kv_heads) <= P4_FEW_COLUMNS) return 0;
-  const long long tiles = (long long)batch * ((max_kv + 15) / 16);
-  return tiles * (2LL * 16 * kv_heads * head_dim * 2) + (tiles * 4 + 15) / 16 * 16;
+namespace {
+bool p4_few(int max_q, int group) { return (long long)max_q * group <= P4_FEW_COLUMNS; }
+}  // namespace
+
+long long paged_attn_prefill_int4_workspace(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int head_dim) {
+  return p4_few(max_q, heads / kv_heads) ? 0 : prompt_int4_workspace(batch, total_q, max_kv, heads, kv_heads, head_dim);
 }
 
 void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
@@ -716,8 +668,9 @@ void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_st
   MB_REQUIRE(heads > 0 && heads % c.kv_heads == 0, "paged_attn_prefill_int4: heads must be a multiple of kv_heads");
   MB_REQUIRE(q_stride % 8 == 0 && o_stride % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
              "paged_attn_prefill_int4: q and out must be 16-byte aligned with token strides of multiples of 8 elements");
+  MB_REQUIRE(scale > 0.f, "paged_attn_prefill_int4: scale must be positive");
   if (batch == 0 || total_q == 0 || max_q == 0) return;
-  if (paged_attn_prefill_int4_workspace(batch, max_q, max_kv, heads, c.kv_heads, c.head_dim) == 0) {
+  if (p4_few(max_q, heads / c.kv_heads)) {
     P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, kv_lens, cu_q, (__nv_bfloat16*)out,
              q_stride, o_stride, heads / c.kv_heads, c.kv_heads, total_q, c.page_size, c.max_pages, c.n_pages, 1,
              scale * 1.4426950408889634f, status};
@@ -725,23 +678,7 @@ void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_st
     return;
   }
   MB_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "paged_attn_prefill_int4: workspace missing or not aligned");
-  const int per_seq = (max_kv + 15) / 16;
-  const long long tiles = (long long)batch * per_seq, values = tiles * 16 * c.kv_heads * c.head_dim;
-  MB_REQUIRE(batch <= 65535 && tiles < (1LL << 31), "paged_attn_prefill_int4: batch too large");
-  __nv_bfloat16* wk = (__nv_bfloat16*)workspace;
-  __nv_bfloat16* wv = wk + values;
-  int* wt = (int*)(wv + values);
-  const dim3 grid(per_seq, batch);
-  const auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, stream>>>((const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, kv_lens, wk, wv, wt, c.kv_heads,
-                                   c.page_size, c.max_pages, c.n_pages, per_seq, status);
-  };
-  if (c.head_dim == 128) go(kv_unpack_int4_kernel<128>);
-  else go(kv_unpack_int4_kernel<64>);
-  count_launch();
-  check_launch();
-  flash_attn_paged_prefill(q, q_stride, wk, wv, (int)tiles, wt, per_seq, cu_q, kv_lens, out, o_stride, batch, total_q, max_q, heads,
-                           c.kv_heads, c.head_dim, c.head_dim, AttnExtras{}, scale, status, stream);
+  prompt_int4(c, q, q_stride, cu_q, kv_lens, out, o_stride, batch, total_q, max_q, max_kv, heads, scale, workspace, status, stream);
 }
 
 }  // namespace mb

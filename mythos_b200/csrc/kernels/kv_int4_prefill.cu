@@ -1,0 +1,628 @@
+// Attention of prompts over the 4-bit paged KV cache: tcgen05 products on fp16 images of the pages.
+//
+// Two launches. kv4_expand_kernel turns every sequence's pages into 128-token tiles [batch, kv_heads, tokens, D] of
+// fp16 in a workspace, once for all the queries that read them, and the queries into fp16 rows; fa_int4_kernel is the
+// persistent two-tile flash attention kernel of attention_fwd2.cu over those images (128 x 128 score tiles, P in tensor memory).
+//
+// Why fp16 and not bf16: a value scale * code + low has up to 20 significant bits. Rounded to bf16 (half a step, 2^-9)
+// every key moves its score by 2^-9 of sum |q k|, which is several times the error of all other roundings together
+// (measured 4.5e-3 of the output in bf16 against 1.7e-3 here, of which 1.65e-3 is the output's own rounding). fp16
+// has three bits more but a range of 2^-14 .. 2^15, so exponents are factored out, all powers of two (exact):
+//   * a query row is divided by 2^eq (its largest value then lies in 2^14 .. 2^15); the thread that owns the row's softmax
+//     multiplies it back with the softmax scale;
+//   * a tile of keys (128 tokens of one head) is divided by 2^ek, which joins the same factor per step;
+//   * a tile of values is divided by 2^ev, and the probabilities of the step are multiplied by it: the running reference
+//     M is the maximum of score + ev, so that p 2^(ev - M) stays within fp16, and the row sum is taken back by 2^-ev.
+// The matrix product multiplies masked probabilities of zero by whatever the value rows hold, so nothing that is not
+// finite goes there: tokens behind a sequence's end are zeros, and a token with a scale that is not finite gets values of
+// zero and NaN keys, which reach the queries that see it through their scores, and no others.
+//
+// Rows of a query tile are (token, head) pairs of one kv head when the group divides 128 (a box of GP heads x 128 / GP tokens
+// in one TMA load), so that short prompts fill their tiles and the heads of a group read a K / V tile once; other groups run one
+// head at a time.
+#include <cuda_fp16.h>
+
+#include "api.h"
+#include "host_util.h"
+#include "kv_int4.cuh"
+#include "tc.cuh"
+
+namespace mb {
+namespace {
+
+constexpr int PF_TILE = 128;      // tokens of a K / V tile, rows of a query tile
+constexpr int PF_EXPAND = 256;    // threads of the expansion
+
+// Exponent e so that a value of magnitude m lies in 2^14 .. 2^15 after division by 2^e. Bounded so that 2^-e is a number.
+__device__ __forceinline__ int pf_exponent(float m) {
+  if (!(m > 0.f)) return 0;
+  const int e = (int)(__float_as_uint(m) >> 23) - 127 - 14;      // subnormals: -141 -> bounded
+  return max(-126, min(113, e));
+}
+__device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
+__device__ __forceinline__ uint32_t pf_half2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ uint4 pf_expand8(uint32_t w, uint32_t pair, float inv) {
+  const float s = kv4_scale(pair), low = kv4_low(pair);
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = fmaf((float)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u), s, low) * inv;
+  return make_uint4(pf_half2(f[0], f[1]), pf_half2(f[2], f[3]), pf_half2(f[4], f[5]), pf_half2(f[6], f[7]));
+}
+
+struct PfExpand {
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const int* block_table;
+  const int* kv_lens;
+  const __nv_bfloat16* q;
+  long long q_stride;
+  __half* k;            // [batch * kv_heads, tokens, D]
+  __half* v;
+  __half* qh;           // [total_q, heads, D]
+  float* q_factor;      // [total_q, heads]: 2^eq
+  int* exponents;       // [batch * kv_heads, tiles]: ek in the low, ev in the high half
+  int kv_heads, heads, page_size, max_pages, n_pages, tiles, kv_blocks, total_q;
+  int* status;
+};
+
+// Blocks [0, kv_blocks): one 128-token tile of one (sequence, kv head). The rest: query rows, one per D / 8 lanes.
+template <int D>
+__global__ void __launch_bounds__(PF_EXPAND)
+kv4_expand_kernel(const __grid_constant__ PfExpand a) {
+  using L = KvInt4<D>;
+  constexpr int WORDS = D / 8;
+  if ((int)blockIdx.x >= a.kv_blocks) {
+    const long long row = ((long long)blockIdx.x - a.kv_blocks) * (PF_EXPAND / WORDS) + threadIdx.x / WORDS;
+    const int c = threadIdx.x % WORDS;
+    const bool live = row < (long long)a.total_q * a.heads;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) unpack8(ldg8(a.q, row / a.heads * a.q_stride + row % a.heads * D + c * 8), f);
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(f[e]));
+#pragma unroll
+    for (int o = WORDS / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (!live) return;
+    const int e = pf_exponent(m);
+    const float inv = pf_pow2(-e);
+    *reinterpret_cast<uint4*>(a.qh + row * D + c * 8) =
+        make_uint4(pf_half2(f[0] * inv, f[1] * inv), pf_half2(f[2] * inv, f[3] * inv), pf_half2(f[4] * inv, f[5] * inv),
+                   pf_half2(f[6] * inv, f[7] * inv));
+    if (c == 0) a.q_factor[row] = pf_pow2(e);
+    return;
+  }
+  __shared__ uint32_t s_pair[2][PF_TILE][L::GROUPS];
+  __shared__ int s_tile[8];
+  __shared__ float s_max[2][PF_EXPAND / 32];
+  const int j = blockIdx.x % a.tiles, bh = blockIdx.x / a.tiles, b = bh / a.kv_heads, head = bh % a.kv_heads;
+  const int len = a.kv_lens[b], n0 = j * PF_TILE;
+  if (n0 >= len) return;
+  if (threadIdx.x < 8) {
+    int tile = -1;
+    if (n0 + 16 * (int)threadIdx.x < len) {
+      tile = kv4_tile(a.block_table + (long long)b * a.max_pages, n0 + 16 * threadIdx.x, a.max_pages, a.n_pages, a.page_size, a.kv_heads, head);
+      if (tile < 0 && a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (91 << 16));
+    }
+    s_tile[threadIdx.x] = tile;
+  }
+  __syncthreads();
+  // pairs of both tensors; the largest magnitude a group can stand for lies at one of its ends
+  float km = 0.f, vm = 0.f;
+  for (int i = threadIdx.x; i < PF_TILE * L::GROUPS; i += PF_EXPAND) {
+    const int n = i / L::GROUPS, g = i % L::GROUPS, tile = s_tile[n >> 4];
+    uint32_t kp = 0u, vp = 0u;
+    if (tile >= 0 && n0 + n < len) {
+      const long long at = (long long)tile * L::TILE_BYTES;
+      kp = *reinterpret_cast<const uint32_t*>(a.k_cache + at + kv4_pair<D>(n & 15, g));
+      bool finite = true;
+#pragma unroll
+      for (int gg = 0; gg < L::GROUPS; ++gg) {
+        const uint32_t p = *reinterpret_cast<const uint32_t*>(a.v_cache + at + kv4_pair<D>(n & 15, gg));
+        finite = finite && kv4_finite(p);
+        if (gg == g) vp = p;
+      }
+      if (!finite) {
+        kp = 0x7FFF7FFFu;
+        vp = 0u;
+      }
+    }
+    s_pair[0][n][g] = kp;
+    s_pair[1][n][g] = vp;
+    if (kv4_finite(kp)) km = fmaxf(km, fmaxf(fabsf(kv4_low(kp)), fabsf(fmaf(15.f, kv4_scale(kp), kv4_low(kp)))));
+    vm = fmaxf(vm, fmaxf(fabsf(kv4_low(vp)), fabsf(fmaf(15.f, kv4_scale(vp), kv4_low(vp)))));
+  }
+  km = warp_max(km);
+  vm = warp_max(vm);
+  if ((threadIdx.x & 31) == 0) {
+    s_max[0][threadIdx.x >> 5] = km;
+    s_max[1][threadIdx.x >> 5] = vm;
+  }
+  __syncthreads();
+  km = vm = 0.f;
+#pragma unroll
+  for (int w = 0; w < PF_EXPAND / 32; ++w) {
+    km = fmaxf(km, s_max[0][w]);
+    vm = fmaxf(vm, s_max[1][w]);
+  }
+  const int ek = pf_exponent(km), ev = pf_exponent(vm);
+  if (threadIdx.x == 0) a.exponents[blockIdx.x] = (ek & 0xFFFF) | ev << 16;
+  const float ik = pf_pow2(-ek), iv = pf_pow2(-ev);
+  const long long out = ((long long)bh * a.tiles + j) * PF_TILE * D;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < PF_TILE * WORDS; i += PF_EXPAND) {
+    const int n = i / WORDS, c = i % WORDS, g = c >> 3, u = c & 7, tile = s_tile[n >> 4];
+    const uint32_t kp = s_pair[0][n][g], vp = s_pair[1][n][g];
+    uint32_t kw = 0u, vw = 0u;
+    if (tile >= 0 && n0 + n < len) {
+      const long long at = (long long)tile * L::TILE_BYTES;
+      kw = kv4_unrotate(*reinterpret_cast<const uint32_t*>(a.k_cache + at + kv4_key_word<D>(n & 15, g, u)));
+      vw = *reinterpret_cast<const uint32_t*>(a.v_cache + at + kv4_value_word<D>(n & 15, g, u));
+    }
+    *reinterpret_cast<uint4*>(a.k + out + (long long)i * 8) = pf_expand8(kw, kp, ik);
+    *reinterpret_cast<uint4*>(a.v + out + (long long)i * 8) = pf_expand8(vw, vp, iv);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ attention
+constexpr int PF_THREADS = 384;   // service warps, softmax of tile 0, softmax of tile 1
+
+template <int D>
+struct PfCfg {
+  static constexpr int KS = D == 128 ? 2 : 4, VS = D == 128 ? 3 : 4;    // K and V stages
+  static constexpr int CHUNKS = D / 64;
+  static constexpr int TILE_BYTES = PF_TILE * D * 2;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = 2 * TILE_BYTES;
+  static constexpr int OFF_V = OFF_K + KS * TILE_BYTES;
+  static constexpr int OFF_BAR = OFF_V + VS * TILE_BYTES;
+  static constexpr int NUM_BARS = 4 + 2 * KS + 2 * VS + 6;
+  static constexpr int SMEM_BYTES = OFF_BAR + NUM_BARS * 8 + 16 + 1024;
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
+  static constexpr int COL_S = 0;     // S_t at t * 128 (P_t over its first 64 columns)
+  static constexpr int COL_O = 256;   // O_t at 256 + t * D
+};
+
+struct PfArgs {
+  const int* cu_q;
+  const int* kv_lens;
+  const float* q_factor;
+  const int* exponents;
+  __nv_bfloat16* out;
+  long long o_stride;
+  int batch, heads, group, pack, units, n_qb, n_items, tiles, total_q;   // pack: heads in a row block; units = heads / pack
+  float scale_log2;
+  int* status;
+};
+
+struct PfItem {
+  int b, unit, row0, q_len, q_off, kv_len, tok[2], J[2], Jmax;   // tok: first token of each tile; J: its key tiles
+  bool live[2];
+};
+// Work item w: last (heaviest under the causal mask) blocks first. False: the sequence has no such block.
+__device__ __forceinline__ bool pf_item(const PfArgs& a, int w, PfItem& it) {
+  const int bu = w % (a.units * a.batch), blk = a.n_qb - 1 - w / (a.units * a.batch);
+  it.unit = bu % a.units;
+  it.b = bu / a.units;
+  it.row0 = a.cu_q[it.b];
+  it.q_len = a.cu_q[it.b + 1] - it.row0;
+  const int per = PF_TILE / a.pack;                              // tokens of a tile
+  it.tok[0] = blk * 2 * per;
+  it.tok[1] = it.tok[0] + per;
+  if (it.tok[0] >= it.q_len) return false;
+  it.kv_len = a.kv_lens[it.b];
+  it.q_off = it.kv_len - it.q_len;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    it.live[t] = it.tok[t] < it.q_len;
+    const int hi = it.live[t] ? min(it.kv_len, it.q_off + min(it.q_len, it.tok[t] + per)) : 0;
+    it.J[t] = min(a.tiles, (max(hi, 0) + PF_TILE - 1) / PF_TILE);
+  }
+  it.Jmax = max(it.J[0], it.J[1]);
+  return true;
+}
+
+__host__ __device__ constexpr uint32_t pf_idesc(int M, int N, bool b_mn_major) {   // fp16 operands, fp32 accumulator
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+template <int D>
+__global__ void __launch_bounds__(PF_THREADS, 1)
+fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PfArgs a) {
+  using Cfg = PfCfg<D>;
+  constexpr int KS = Cfg::KS, VS = Cfg::VS, CHUNKS = Cfg::CHUNKS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* q_full = bars;                 // [2]
+  uint64_t* q_free = bars + 2;             // [2]
+  uint64_t* k_full = bars + 4;             // [KS]
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* v_full = k_empty + KS;         // [VS]
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* s_full = v_empty + VS;         // [2]
+  uint64_t* p_full = s_full + 2;           // [2]
+  uint64_t* o_full = p_full + 2;           // [2]
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(o_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  int* status = a.status;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kv_heads = a.heads / a.group;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_free[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 128);
+      mbar_init(&o_full[t], 1);
+    }
+    for (int s = 0; s < KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+    for (int s = 0; s < VS; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_ptr, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr;
+
+  if (warp == 2) {
+    // ------------------------------------------------------------------ Q loader
+    if (lane == 0) {
+      uint32_t n_q[2] = {0, 0};   // loads issued per tile (phase of q_free / q_full)
+      PfItem it;
+      bool ok = true;
+      for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
+        if (!pf_item(a, w, it)) continue;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (it.J[t] == 0 || !ok) continue;
+          if (!mbar_wait(&q_free[t], (n_q[t] & 1) ^ 1, abort_flag, status, 94)) { ok = false; break; }
+          mbar_arrive_expect_tx(&q_full[t], Cfg::TILE_BYTES);
+          for (int c = 0; c < CHUNKS; ++c)
+            tma_load_3d(smem + Cfg::OFF_Q + t * Cfg::TILE_BYTES + c * (PF_TILE * 128), &tm_q, &q_full[t], c * 64,
+                        it.unit * a.pack, it.row0 + it.tok[t]);
+          ++n_q[t];
+        }
+      }
+    }
+  } else if (warp == 0) {
+    // ------------------------------------------------------------------ K / V loader
+    if (lane == 0) {
+      uint32_t kc = 0, vc = 0;
+      PfItem it;
+      bool ok = true;
+      for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
+        if (!pf_item(a, w, it)) continue;
+        const int bh = it.b * kv_heads + it.unit * a.pack / a.group;
+        for (int j = 0; j < it.Jmax; ++j) {
+          const int ks = kc % KS, vs = vc % VS;
+          if (!mbar_wait(&k_empty[ks], ((kc / KS) & 1) ^ 1, abort_flag, status, 95)) { ok = false; break; }
+          mbar_arrive_expect_tx(&k_full[ks], Cfg::TILE_BYTES);
+          for (int c = 0; c < CHUNKS; ++c)
+            tma_load_3d(smem + Cfg::OFF_K + ks * Cfg::TILE_BYTES + c * (PF_TILE * 128), &tm_k, &k_full[ks], c * 64, j * PF_TILE, bh);
+          ++kc;
+          if (!mbar_wait(&v_empty[vs], ((vc / VS) & 1) ^ 1, abort_flag, status, 96)) { ok = false; break; }
+          mbar_arrive_expect_tx(&v_full[vs], Cfg::TILE_BYTES);
+          for (int c = 0; c < CHUNKS; ++c)
+            tma_load_3d(smem + Cfg::OFF_V + vs * Cfg::TILE_BYTES + c * (PF_TILE * 128), &tm_v, &v_full[vs], c * 64, j * PF_TILE, bh);
+          ++vc;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t IDESC_S = pf_idesc(PF_TILE, PF_TILE, false);
+      constexpr uint32_t IDESC_O = pf_idesc(PF_TILE, D, true);
+      const uint32_t q_addr = smem_u32(smem + Cfg::OFF_Q);
+      const uint32_t k_addr = smem_u32(smem + Cfg::OFF_K);
+      const uint32_t v_addr = smem_u32(smem + Cfg::OFF_V);
+      uint32_t kc = 0, vc = 0;              // K / V tiles consumed so far (ring position and phase)
+      uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
+      bool ok = true;
+      auto issue_s = [&](int t, uint32_t kpos) {
+        const uint32_t qa = q_addr + t * Cfg::TILE_BYTES;
+        const uint32_t ka = k_addr + (kpos % KS) * Cfg::TILE_BYTES;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const int c = k >> 2, kk = k & 3;
+          umma_f16(tmem_base + Cfg::COL_S + t * 128, umma_desc_sw128(qa + c * (PF_TILE * 128) + kk * 32, 0, 1024),
+                   umma_desc_sw128(ka + c * (PF_TILE * 128) + kk * 32, 0, 1024), IDESC_S, k > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[t]);
+      };
+      PfItem it;
+      for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
+        if (!pf_item(a, w, it) || it.Jmax == 0) continue;
+        // scores of step 0 for both tiles
+        if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 97)) { ok = false; break; }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (it.J[t] == 0 || !ok) continue;
+          if (!mbar_wait(&q_full[t], n_q[t] & 1, abort_flag, status, 98)) { ok = false; break; }
+          tc_fence_after();
+          issue_s(t, kc);
+          if (it.J[t] == 1) umma_commit(&q_free[t]);
+        }
+        if (!ok) break;
+        umma_commit(&k_empty[kc % KS]);   // every score product of key tile 0 has been issued
+        ++kc;
+        for (int j = 0; j < it.Jmax && ok; ++j) {
+          bool v_ready = false, k_ready = false;
+          const bool have_next = j + 1 < it.Jmax;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= it.J[t] || !ok) continue;
+            if (!mbar_wait(&p_full[t], n_p[t] & 1, abort_flag, status, 99)) { ok = false; break; }
+            ++n_p[t];
+            if (!v_ready) {
+              if (!mbar_wait(&v_full[vc % VS], (vc / VS) & 1, abort_flag, status, 100)) { ok = false; break; }
+              v_ready = true;
+            }
+            tc_fence_after();
+            const uint32_t va = v_addr + (vc % VS) * Cfg::TILE_BYTES;
+#pragma unroll
+            for (int k = 0; k < PF_TILE / 16; ++k)   // O_t += P_t(tmem) V
+              umma_f16_ts(tmem_base + Cfg::COL_O + t * D, tmem_base + Cfg::COL_S + t * 128 + k * 8,
+                          umma_desc_sw128(va + k * 2048, PF_TILE * 128, 1024), IDESC_O, (j > 0 || k > 0) ? 1u : 0u);
+            if (j == it.J[t] - 1) umma_commit(&o_full[t]);
+            if (j + 1 < it.J[t]) {
+              if (!k_ready) {
+                if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 101)) { ok = false; break; }
+                tc_fence_after();
+                k_ready = true;
+              }
+              issue_s(t, kc);               // overwrites S_t / P_t: ordered behind the PV product just issued
+              if (j + 2 == it.J[t]) umma_commit(&q_free[t]);   // that was the tile's last score product
+            }
+          }
+          if (!ok) break;
+          umma_commit(&v_empty[vc % VS]);
+          ++vc;
+          if (have_next) {
+            umma_commit(&k_empty[kc % KS]);
+            ++kc;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (it.J[t] > 0) ++n_q[t];
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ softmax + epilogue
+    const int t = (warp - 4) >> 2;           // query tile
+    const int quarter = warp & 3;            // TMEM lane quarter this warp may access
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tmem_base + Cfg::COL_S + t * 128 + lane_sel;
+    const uint32_t t_o = tmem_base + Cfg::COL_O + t * D + lane_sel;
+    uint32_t n_s = 0, n_o = 0;
+    bool ok = true;
+    PfItem it;
+    for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
+      // (selects, not indexing: the item stays in registers)
+      if (!pf_item(a, w, it) || !(t ? it.live[1] : it.live[0])) continue;
+      const int Jt = t ? it.J[1] : it.J[0];
+      const int tok = (t ? it.tok[1] : it.tok[0]) + r / a.pack, head = it.unit * a.pack + r % a.pack;
+      const int row = it.row0 + tok;
+      const bool live = tok < it.q_len && (unsigned)row < (unsigned)a.total_q;
+      const int limit = min(it.kv_len - 1, it.q_off + tok);
+      const int* ex = a.exponents + (long long)(it.b * kv_heads + it.unit * a.pack / a.group) * a.tiles;
+      const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 1.f;
+      float m_ref = 0.f, l = 0.f;
+      int e0 = 0;                             // exponent of the first tile's values: the row sum is kept in units of 2^-e0
+      int e_next = Jt > 0 ? ex[0] : 0;
+      for (int j = 0; j < Jt && ok; ++j) {
+        const int ek = (short)e_next, e = e_next >> 16;
+        if (j + 1 < Jt) e_next = ex[j + 1];
+        if (j == 0) e0 = e;
+        // (never zero: a masked score of minus infinity has to stay one)
+        const float sc = fmaxf(row_f * pf_pow2(ek), 1e-37f), ev = (float)e;
+        ok = mbar_wait(&s_full[t], n_s & 1, abort_flag, status, 102);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++n_s;
+        tc_fence_after();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, sr[c]);
+        tmem_ld_wait();
+        float* s = reinterpret_cast<float*>(&sr[0][0]);
+        const int kv0 = j * PF_TILE;
+        if (kv0 + PF_TILE - 1 > limit) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (kv0 + i > limit) s[i] = -INFINITY;
+        }
+        float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < 124; i += 8) {
+          mx4[0] = fmax3(mx4[0], s[i], s[i + 1]);
+          mx4[1] = fmax3(mx4[1], s[i + 2], s[i + 3]);
+          mx4[2] = fmax3(mx4[2], s[i + 4], s[i + 5]);
+          mx4[3] = fmax3(mx4[3], s[i + 6], s[i + 7]);
+        }
+        mx4[0] = fmax3(mx4[0], s[124], s[125]);
+        mx4[1] = fmax3(mx4[1], s[126], s[127]);
+        const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sc, ev);
+        float alpha = 1.f;
+        bool need = false;
+        if (j == 0) {
+          m_ref = (m_new == -INFINITY) ? 0.f : m_new;
+        } else if (m_new - m_ref > 6.f) {     // lazy: p up to 2^6 until the reference moves
+          need = true;
+          alpha = fast_exp2(m_ref - m_new);
+          m_ref = m_new;
+        }
+        // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):
+        // O_t is quiescent until this warpgroup arrives on p_full, so a rescale can happen right here.
+        if (j > 0 && __any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t orr[32];
+            tmem_ld32(t_o + c * 32, orr);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * alpha);
+            tmem_st32(t_o + c * 32, orr);
+          }
+        }
+        const float shift = ev - m_ref;
+        const uint64_t sc2 = f32x2(sc, sc), nm2 = f32x2(shift, shift);
+        uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
+        uint32_t* pk = &sr[0][0];         // packed in place: pair i lands in word i / 2, behind the read position
+#pragma unroll
+        for (int i = 0; i < 128; i += 2) {
+          float e0f, e1f;
+          f32x2_unpack(fma_f32x2(f32x2(s[i], s[i + 1]), sc2, nm2), e0f, e1f);
+          const float p0 = fast_exp2(e0f), p1 = fast_exp2(e1f);
+          rs2[(i >> 1) & 3] = add_f32x2(rs2[(i >> 1) & 3], f32x2(p0, p1));
+          pk[i >> 1] = pf_half2(p0, p1);
+        }
+        float rs[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
+        l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(e0 - e);
+        tmem_st32(t_s, sr[0]);            // P_t: fp16 pairs over the first 64 columns of S_t
+        tmem_st32(t_s + 32, sr[1]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      if (Jt > 0) {
+        ok = mbar_wait(&o_full[t], n_o & 1, abort_flag, status, 103);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++n_o;
+        tc_fence_after();
+      }
+      // p 2^ev and the values' 2^-ev cancel in O; l is in units of 2^-e0
+      const float inv_l = l == 0.f ? 0.f : 1.f / l, unit = pf_pow2(e0);
+      __nv_bfloat16* orow = a.out + (long long)row * a.o_stride + (long long)head * D;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t orr[32];                 // (without a key: whatever the columns hold, not used)
+        tmem_ld32(t_o + c * 32, orr);
+        tmem_ld_wait();
+        if (live) {
+          uint4* p4 = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              v[k] = l == 0.f ? 0u
+                              : pack_bf16x2(__uint_as_float(orr[8 * i + 2 * k]) * inv_l * unit, __uint_as_float(orr[8 * i + 2 * k + 1]) * inv_l * unit);
+            p4[i] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+      // The TMEM loads above have completed (tmem_ld_wait); the next item's first PV product waits for
+      // this warpgroup's next arrives on p_full, so O_t is not overwritten before it was read.
+      tc_fence_before();
+    }
+  }
+
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 10000000LL) {}
+    __syncthreads();
+  }
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
+}
+
+int pf_tiles(int max_kv) { return (max_kv + PF_TILE - 1) / PF_TILE; }
+long long pf_align(long long n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+long long prompt_int4_workspace(int batch, int total_q, int max_kv, int heads, int kv_heads, int head_dim) {
+  const long long tiles = (long long)batch * kv_heads * pf_tiles(max_kv);
+  return 2 * tiles * PF_TILE * head_dim * 2 + pf_align((long long)total_q * heads * head_dim * 2) +
+         pf_align((long long)total_q * heads * 4) + pf_align(tiles * 4);
+}
+
+void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
+                 long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,
+                 int* status, cudaStream_t stream) {
+  const int D = c.head_dim, G = heads / c.kv_heads, tiles = pf_tiles(max_kv);
+  const int pack = 128 % G == 0 ? G : 1;
+  const long long all = (long long)batch * c.kv_heads * tiles;
+  uint8_t* p = (uint8_t*)workspace;
+  PfExpand x{(const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, kv_lens, (const __nv_bfloat16*)q, q_stride};
+  x.k = (__half*)p;
+  x.v = x.k + all * PF_TILE * D;
+  p += 2 * all * PF_TILE * D * 2;
+  x.qh = (__half*)p;
+  p += pf_align((long long)total_q * heads * D * 2);
+  x.q_factor = (float*)p;
+  p += pf_align((long long)total_q * heads * 4);
+  x.exponents = (int*)p;
+  x.kv_heads = c.kv_heads;
+  x.heads = heads;
+  x.page_size = c.page_size;
+  x.max_pages = c.max_pages;
+  x.n_pages = c.n_pages;
+  x.tiles = tiles;
+  x.total_q = total_q;
+  x.status = status;
+  const int rows_per = PF_EXPAND / (D / 8);
+  const long long q_blocks = ((long long)total_q * heads + rows_per - 1) / rows_per;
+  MB_REQUIRE(all + q_blocks < (1LL << 31) && all < (1LL << 31), "paged_attn_prefill_int4: batch too large");
+  x.kv_blocks = (int)all;
+  if (D == 128) kv4_expand_kernel<128><<<(unsigned)(all + q_blocks), PF_EXPAND, 0, stream>>>(x);
+  else kv4_expand_kernel<64><<<(unsigned)(all + q_blocks), PF_EXPAND, 0, stream>>>(x);
+  count_launch();
+  check_launch();
+
+  // (copies only: TMA moves fp16 as it moves bf16)
+  uint64_t qd[3] = {(uint64_t)D, (uint64_t)heads, (uint64_t)total_q}, qs[2] = {(uint64_t)D * 2, (uint64_t)heads * D * 2};
+  uint32_t qb[3] = {64, (uint32_t)pack, (uint32_t)(PF_TILE / pack)};
+  uint64_t kd[3] = {(uint64_t)D, (uint64_t)tiles * PF_TILE, (uint64_t)batch * c.kv_heads};
+  uint64_t ks[2] = {(uint64_t)D * 2, (uint64_t)tiles * PF_TILE * D * 2};
+  uint32_t kb[3] = {64, PF_TILE, 1};
+  const CUtensorMap tq = make_tensor_map(x.qh, TmaDType::BF16, 3, qd, qs, qb, true);
+  const CUtensorMap tk = make_tensor_map(x.k, TmaDType::BF16, 3, kd, ks, kb, true);
+  const CUtensorMap tv = make_tensor_map(x.v, TmaDType::BF16, 3, kd, ks, kb, true);
+  PfArgs a{cu_q, kv_lens, x.q_factor, x.exponents, (__nv_bfloat16*)out, o_stride};
+  a.batch = batch;
+  a.heads = heads;
+  a.group = G;
+  a.pack = pack;
+  a.units = heads / pack;
+  a.n_qb = (int)(((long long)max_q * pack + 2 * PF_TILE - 1) / (2 * PF_TILE));
+  MB_REQUIRE((long long)a.n_qb * a.units * batch < (1LL << 31), "paged_attn_prefill_int4: batch too large");
+  a.n_items = a.n_qb * a.units * batch;
+  a.tiles = tiles;
+  a.total_q = total_q;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.status = status;
+  const int grid = a.n_items < sm_count() ? a.n_items : sm_count();
+  const auto go = [&](auto kern, int smem) {
+    MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kern<<<grid, PF_THREADS, smem, stream>>>(tq, tk, tv, a);
+  };
+  if (D == 128) go(fa_int4_kernel<128>, PfCfg<128>::SMEM_BYTES);
+  else go(fa_int4_kernel<64>, PfCfg<64>::SMEM_BYTES);
+  count_launch();
+  check_launch();
+}
+
+}  // namespace mb
