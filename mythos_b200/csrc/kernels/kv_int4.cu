@@ -4,6 +4,10 @@
 //   kv_read_int4              tokens of the cache -> bf16 rows
 //   paged_attn_decode_int4    one query token per sequence
 //   paged_attn_prefill_int4   several new query tokens per sequence, causal, over everything in the pages
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
 #include "api.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -105,47 +109,56 @@ kv_read_int4_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restri
 }
 
 // ------------------------------------------------------------------------------------------------ attention
-// One (sequence, kv head, block of COLS query columns) per cluster; the CTAs of the cluster split its tiles. A column
+// One (sequence, kv head, block of COLS query columns) per cluster; the CTAs of the cluster split its tokens. A column
 // is one (query token, head of the group) pair: column c is head c % G of token c / G. Four warps per CTA; warp w
-// takes every fourth tile of its CTA's range through a ring of its own, filled with one bulk copy per tile
-// for K and one for V.
+// takes every fourth chunk (32 tokens, two tiles) of its CTA's range through a ring of its own, filled with one bulk copy per
+// tile for K and one for V.
 //
-// Scores: q . k = sum over groups of scale (q_g . c_g) + low sum(q_g). The matrix product runs on 16 + code, exact in
-// bf16, one AND-OR per pair of values; the offset leaves with (low - 16 scale) sum(q_g) in fp32. Values:
-// o = sum_t (p_t scale_t) (c_t - 8) + sum_t p_t (low_t + 8 scale_t): the codes are centred here, because this sum runs
-// over the whole context and the tensor cores truncate what they add; the second sum is a scalar per column and group.
-// p_t scale_t is rounded to bf16 (half a step, 2^-9 of each term; the rounding errors of the terms are independent),
-// everything else is fp32. mma.sync rather than tcgen05: at 8 columns the tile would be 128 rows for 8 useful ones,
-// and the codes would have to be expanded through shared memory.
+// What bounds it is the integer pipe (half rate) that takes the codes apart, so operands are formed by one AND each:
+// the low eleven bits of an fp16 are linear in its value (subnormals and the first normal binade share one step,
+// 2^-24), so a nibble anywhere in them is its code times a power of two. Keys: bits 3-6 (code 2^-21) and 7-10 (code 2^-17)
+// of a rotated word, then the word rotated by eight; queries of the second kind are multiplied by 2^-4. Values: bits 0-3
+// (2^-24) and 4-7 (2^-20) of two tokens' halves side by side; they are different output values, scaled at the end.
+//
+// Scores: q . k = sum over groups of scale (q_g . c_g) + low sum(q_g), the product exact in fp16 (a query column is divided
+// by a power of two first, so that its bf16 values fit). Values: o = sum_t (p_t scale_t) (c_t - 8) + sum_t p_t (low_t + 8
+// scale_t): the codes are centred (one packed subtraction on the idle FMA pipe), because this sum runs over the whole
+// context and the tensor cores truncate what they add; the second sum is a scalar per column and group in fp32.
+// p_t scale_t is rounded to fp16 (2^-12 of each term); the running reference M is the maximum of the scores plus the
+// exponent of the chunk's values, so it fits whatever the values' size. Everything else is fp32. mma.sync rather than tcgen05:
+// with 8 columns a 128-row tile would be filled to a sixteenth, and the codes would have to go through shared memory
+// once more.
 //
 // The CTAs of a cluster merge their partial softmax states through distributed shared memory: no scratch, no
 // counters, one result for the same inputs, and calls on several streams share nothing.
 constexpr int P4_WARPS = 4;
 constexpr int P4_THREADS = 32 * P4_WARPS;
+constexpr int P4_CHUNK = 32;      // tokens
 
 template <int D, int COLS>
 struct P4Cfg {
   using L = KvInt4<D>;
-  static constexpr int STAGES = D == 128 ? 6 : 8;
-  static constexpr int STAGE = 2 * L::TILE_BYTES;             // K tile, V tile
+  static constexpr int STAGES = 3;
+  static constexpr int HALF = 2 * L::TILE_BYTES;              // K (or V) of a chunk
+  static constexpr int STAGE = 2 * HALF;
   static constexpr int WARP_BYTES = STAGES * STAGE;
   static constexpr int OFF_BAR = P4_WARPS * WARP_BYTES;
-  static constexpr int OFF_ML = OFF_BAR + P4_WARPS * STAGES * 8 + 16;              // m, l: [warps][COLS] each
+  static constexpr int OFF_ML = OFF_BAR + P4_WARPS * STAGES * 8 + 16;               // m, l: [warps][COLS] each
   static constexpr int OFF_Z = OFF_ML + 2 * P4_WARPS * COLS * 4;                    // [warps][COLS][groups]
-  static constexpr int OFF_CTA = OFF_Z + P4_WARPS * COLS * L::GROUPS * 4;           // m, l of the CTA, weight, 1 / l
+  static constexpr int OFF_CTA = OFF_Z + P4_WARPS * COLS * L::GROUPS * 4;           // m, l of the CTA
   static constexpr int BYTES = OFF_CTA + 2 * COLS * 4 + 128;
   static_assert(COLS * D * 4 <= WARP_BYTES, "a warp's output state is staged in its own (drained) ring");
 };
 
 __device__ __forceinline__ void p4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                "{%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void p4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+__device__ __forceinline__ void p4_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ uint32_t p4_rank() {
   uint32_t r;
@@ -165,17 +178,15 @@ __device__ __forceinline__ float p4_ld_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-// The pair of values 2 i, 2 i + 1 of a rotated key word as the bf16 numbers 16 + code.
-template <int I>
-__device__ __forceinline__ uint32_t p4_key_pair(uint32_t w) {
-  const uint32_t s = I == 0 ? w : (I == 3 ? __funnelshift_r(w, w, 12) : w >> (4 * I));
-  return (s & 0x00780078u) | 0x41804180u;
+__device__ __forceinline__ uint32_t p4_half2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-// Nibble i of both halves as the bf16 numbers code - 8: 128 + code by bit pattern, minus 136 (exact).
-template <int I>
-__device__ __forceinline__ uint32_t p4_value_pair(uint32_t w) {
-  const uint32_t x = ((w >> (4 * I)) & 0x000F000Fu) | 0x43004300u;
-  const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
+__device__ __forceinline__ float p4_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// x - c on both halves (c: 8 steps of the subnormal range, so the difference is exact).
+__device__ __forceinline__ uint32_t p4_centre(uint32_t x, uint32_t c) {
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
@@ -193,8 +204,190 @@ struct P4Args {
   int* status;
 };
 
+// A warp's running state: accumulators (units of 2^-24 / 2^-20), offset sums, reference and row sum.
 template <int D, int COLS>
-__global__ void __launch_bounds__(P4_THREADS)
+struct P4State {
+  static constexpr int NB = COLS / 8, GR = KvInt4<D>::GROUPS;
+  uint32_t qa[NB][GR][8];
+  float qsum[NB][GR], factor[NB];
+  int limit[NB];
+  float o[NB][GR][4][4];
+  float z[NB][GR], m[NB], l[NB];
+};
+
+// One chunk: tile u (0, 1) at `at` + u * TILE_BYTES for K, HALF behind for V; tok0: its first token plus this thread's t.
+// MASK: some token is not seen by some column (visible: those seen by any), or not held at all.
+template <int D, int COLS, bool MASK>
+__device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at, int tok0, int lane, int visible, uint32_t absent) {
+  using L = KvInt4<D>;
+  using C = P4Cfg<D, COLS>;
+  constexpr int GR = L::GROUPS, NB = COLS / 8;
+  const int r = lane >> 2, t = lane & 3;
+  // ---- scores of tokens tok0 + 16 u + 4 (2 j + e): the matrix product's columns 2 t + e, rows r and r + 8
+  float sc[2][2][GR][4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t kw[GR][2];
+      const uint8_t* kp = at + u * L::TILE_BYTES + (8 * j + r) * L::ROW + t * (8 * GR);
+      if constexpr (GR == 2) {
+        const uint4 x = *reinterpret_cast<const uint4*>(kp);
+        kw[0][0] = x.x; kw[0][1] = x.y; kw[1][0] = x.z; kw[1][1] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(kp);
+        kw[0][0] = x.x; kw[0][1] = x.y;
+      }
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        float (&c)[4] = sc[u][j][g];
+        c[0] = c[1] = c[2] = c[3] = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w = kw[g][h], w8 = __funnelshift_r(w, w, 8);
+          const uint32_t (&q0)[8] = s.qa[0][g];
+          const uint32_t (&q1)[8] = s.qa[NB - 1][g];
+          p4_mma(c, q0[4 * h], NB > 1 ? q1[4 * h] : 0u, q0[4 * h + 1], NB > 1 ? q1[4 * h + 1] : 0u, w & 0x00780078u, w & 0x07800780u);
+          p4_mma(c, q0[4 * h + 2], NB > 1 ? q1[4 * h + 2] : 0u, q0[4 * h + 3], NB > 1 ? q1[4 * h + 3] : 0u, w8 & 0x00780078u, w8 & 0x07800780u);
+        }
+      }
+    }
+  // ---- exponent of the chunk's values: one group of one token per thread and tile
+  uint32_t mag = 0u;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if (GR == 1 && u == 1) break;                 // 16 groups a tile: the warp's halves take the two tiles
+    const int tile = GR == 2 ? u : lane >> 4, row = GR == 2 ? lane >> 1 : lane & 15, g = GR == 2 ? lane & 1 : 0;
+    const uint32_t p = *reinterpret_cast<const uint32_t*>(at + C::HALF + tile * L::TILE_BYTES + L::OFF_PAIR + row * L::PAIR + 4 * g);
+    const float sv = kv4_scale(p), a = fmaxf(8.f * sv, fabsf(fmaf(8.f, sv, kv4_low(p))));
+    bool use = kv4_finite(p);
+    if (MASK) {                                   // a place behind the context may hold anything
+      const int n = (row & 8) + ((row >> 1) & 3) + ((row & 1) << 2);       // token at this pair row
+      use = use && tok0 - t + 16 * tile + n < visible && !(absent >> tile & 1u);
+    }
+    if (use) mag = max(mag, __float_as_uint(a));
+  }
+  mag = __reduce_max_sync(0xffffffffu, mag);
+  // p is kept up to 2^9 (and 2^6 more until the reference moves) times the largest value's inverse: p times a scale,
+  // an eighth of it at most, then stays below 2^14, and is exact to 2^-12 over 24 octaves below. Bounded so that p, its sum
+  // and its product with any value stay within fp32.
+  const float ev = (float)(max(-80, min(112, (int)(mag >> 23) - 127)) - 9);
+  // ---- online softmax per column; the reference moves only when it grew by more than 2^6
+  uint32_t pb[2][NB][GR][2];
+  float x[2][NB][2][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t kq[2][GR];
+        const uint8_t* kp = at + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + 2 * t) * L::PAIR;
+        if constexpr (GR == 2) {
+          const uint4 y = *reinterpret_cast<const uint4*>(kp);
+          kq[0][0] = y.x; kq[0][1] = y.y; kq[1][0] = y.z; kq[1][1] = y.w;
+        } else {
+          const uint2 y = *reinterpret_cast<const uint2*>(kp);
+          kq[0][0] = y.x; kq[1][0] = y.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = 0.f;
+#pragma unroll
+          for (int g = 0; g < GR; ++g)
+            v = fmaf(kv4_scale(kq[e][g]), sc[u][j][g][2 * nb + e], fmaf(kv4_low(kq[e][g]), s.qsum[nb][g], v));
+          v *= s.factor[nb];
+          if (MASK && (tok0 + 16 * u + 4 * (2 * j + e) >= s.limit[nb] || (absent >> u & 1u))) v = -INFINITY;
+          x[u][nb][j][e] = v;
+        }
+        mx = fmax3(mx, x[u][nb][j][0], x[u][nb][j][1]);
+      }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) + ev;
+    const bool need = mx > s.m[nb] + 6.f || (s.m[nb] == -INFINITY && mx > -INFINITY);
+    if (__any_sync(0xffffffffu, need)) {
+      const float alpha = need ? fast_exp2(s.m[nb] - mx) : 1.f;
+      if (need) s.m[nb] = mx;
+      s.l[nb] *= alpha;
+      const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        s.z[nb][g] *= alpha;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          s.o[nb][g][q][0] *= a0; s.o[nb][g][q][1] *= a1; s.o[nb][g][q][2] *= a0; s.o[nb][g][q][3] *= a1;
+        }
+      }
+    }
+    const float m = MASK && s.m[nb] == -INFINITY ? 0.f : s.m[nb];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t vq[2][GR];
+        const uint8_t* vp = at + C::HALF + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + 2 * t) * L::PAIR;
+        if constexpr (GR == 2) {
+          const uint4 y = *reinterpret_cast<const uint4*>(vp);
+          vq[0][0] = y.x; vq[0][1] = y.y; vq[1][0] = y.z; vq[1][1] = y.w;
+        } else {
+          const uint2 y = *reinterpret_cast<const uint2*>(vp);
+          vq[0][0] = y.x; vq[1][0] = y.y;
+        }
+        const float p0 = fast_exp2(x[u][nb][j][0] - m), p1 = fast_exp2(x[u][nb][j][1] - m);
+        s.l[nb] += p0 + p1;
+        // a token the column does not see may hold anything, behind the sequence's end too: it is left out, not
+        // multiplied by zero
+        const bool s0 = !MASK || x[u][nb][j][0] != -INFINITY, s1 = !MASK || x[u][nb][j][1] != -INFINITY;
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          const float w0 = kv4_scale(vq[0][g]), w1 = kv4_scale(vq[1][g]);
+          const float b0 = fmaf(8.f, w0, kv4_low(vq[0][g])), b1 = fmaf(8.f, w1, kv4_low(vq[1][g]));
+          if (MASK) s.z[nb][g] += (s0 ? p0 * b0 : 0.f) + (s1 ? p1 * b1 : 0.f);
+          else s.z[nb][g] = fmaf(p0, b0, fmaf(p1, b1, s.z[nb][g]));
+          pb[u][nb][g][j] = p4_half2(s0 ? p0 * w0 : 0.f, s1 ? p1 * w1 : 0.f);
+        }
+      }
+  }
+  // ---- values: the A operand holds values x tokens, B the probabilities
+  const int chunk = r ^ ((t >> 1) << 2);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t vw[2][2][GR];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint8_t* vp = at + C::HALF + u * L::TILE_BYTES + (t + 4 * (2 * j + e)) * L::ROW + chunk * (4 * GR);
+        if constexpr (GR == 2) {
+          const uint2 w = *reinterpret_cast<const uint2*>(vp);
+          vw[j][e][0] = w.x; vw[j][e][1] = w.y;
+        } else {
+          vw[j][e][0] = *reinterpret_cast<const uint32_t*>(vp);
+        }
+      }
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      // halves of the two tokens' words side by side: lo holds values 0, 2, 4, 6 and hi values 1, 3, 5, 7 of both
+      uint32_t lo0 = __byte_perm(vw[0][0][g], vw[0][1][g], 0x5410), hi0 = __byte_perm(vw[0][0][g], vw[0][1][g], 0x7632);
+      uint32_t lo1 = __byte_perm(vw[1][0][g], vw[1][1][g], 0x5410), hi1 = __byte_perm(vw[1][0][g], vw[1][1][g], 0x7632);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i == 2) {
+          lo0 >>= 8; hi0 >>= 8; lo1 >>= 8; hi1 >>= 8;
+        }
+        const uint32_t mask = (i & 1) ? 0x00F000F0u : 0x000F000Fu, eight = (i & 1) ? 0x00800080u : 0x00080008u;
+        const uint32_t a0 = p4_centre(lo0 & mask, eight), a1 = p4_centre(hi0 & mask, eight), a2 = p4_centre(lo1 & mask, eight),
+                       a3 = p4_centre(hi1 & mask, eight);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) p4_mma(s.o[nb][g][i], a0, a1, a2, a3, pb[u][nb][g][0], pb[u][nb][g][1]);
+      }
+    }
+  }
+}
+
+template <int D, int COLS>
+__global__ void __launch_bounds__(P4_THREADS, COLS == 8 ? 4 : 2)
 paged_attn_int4_kernel(const __grid_constant__ P4Args a) {
   using L = KvInt4<D>;
   using C = P4Cfg<D, COLS>;
@@ -221,258 +414,161 @@ paged_attn_int4_kernel(const __grid_constant__ P4Args a) {
   }
   __syncthreads();
 
-  // tiles of this CTA: what the last query of the block sees, cut into equal ranges
-  const int last_q = (col0 + n_cols - 1) / a.G;
-  const int visible = min(kv_len, kv_len - q_len + last_q + 1);
-  const int n_tiles = (max(0, visible) + 15) >> 4;
-  const int per = (n_tiles + a.splits - 1) / a.splits;
-  const int tile0 = split * per, tile1 = min(n_tiles, tile0 + per);
-  const int my_tiles = (tile1 - tile0 - warp + P4_WARPS - 1) / P4_WARPS;      // tile0 + warp, + 4, ... (<= 0: none)
+  // chunks of this CTA: what the last query of the block sees, cut into equal ranges
+  const int first_q = col0 / a.G, last_q = (col0 + n_cols - 1) / a.G;
+  const int visible = max(0, min(kv_len, kv_len - q_len + last_q + 1));       // to some column
+  const int common = min(kv_len, kv_len - q_len + first_q + 1);               // to every column
+  const int n_chunks = (visible + P4_CHUNK - 1) / P4_CHUNK;
+  const int per = (n_chunks + a.splits - 1) / a.splits;
+  const int chunk0 = split * per + warp, chunk_end = min(n_chunks, split * per + per);
+  const int mine = (chunk_end - chunk0 + P4_WARPS - 1) / P4_WARPS;            // chunk0, + 4, ... (<= 0: none)
   const int* table = a.block_table + (long long)b * a.max_pages;
 
-  // lane l holds the tile index of the warp's tile 32 n + l for the block n being issued, and of the next block
+  // lane l holds tile l % 2 of the warp's chunk 16 n + l / 2 for the block n being issued, and of the next block:
+  // its index, -1 without a page, -2 behind the visible tokens
   auto locate = [&](int i) {
-    return i < my_tiles ? kv4_tile(table, (tile0 + warp + P4_WARPS * i) * 16, a.max_pages, a.n_pages, a.page_size, a.kv_heads, hkv) : -1;
+    const int token = (chunk0 + P4_WARPS * i) * P4_CHUNK + (lane & 1) * 16;
+    return i < mine && token < visible ? kv4_tile(table, token, a.max_pages, a.n_pages, a.page_size, a.kv_heads, hkv) : -2;
   };
-  int ids = locate(lane), ids_next = locate(32 + lane);
-  uint32_t present = 0u;                          // bit s: stage s holds a tile
-  auto issue = [&](int i) {                       // all lanes; lane 0 starts the copies of the warp's tile i
-    if (i > 0 && (i & 31) == 0) {
+  int ids = locate(lane >> 1), ids_next = locate(16 + (lane >> 1));
+  uint32_t absent = 0u;                           // bits 2 s, 2 s + 1: tiles of stage s that were not loaded
+  auto issue = [&](int i, int st) {               // all lanes; lane 0 starts the copies of the warp's chunk i
+    if (i > 0 && (i & 15) == 0) {
       ids = ids_next;
-      ids_next = locate(i + 32 + lane);
+      ids_next = locate(i + 16 + (lane >> 1));
     }
-    const int id = __shfl_sync(0xffffffffu, ids, i & 31), st = i % C::STAGES;
-    if (id >= 0) {
-      present |= 1u << st;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&full[st], C::STAGE);
-        p4_bulk_load(ring + st * C::STAGE, a.k_cache + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[st]);
-        p4_bulk_load(ring + st * C::STAGE + L::TILE_BYTES, a.v_cache + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[st]);
-      }
-    } else {                                      // a token of the context without a page: reported, left out
-      present &= ~(1u << st);
-      if (lane == 0) {
-        if (a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (92 << 16));
-        mbar_arrive(&full[st]);
+    const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + 1);
+    absent = (absent & ~(3u << (2 * st))) | ((id0 < 0 ? 1u : 0u) | (id1 < 0 ? 2u : 0u)) << (2 * st);
+    if (lane == 0) {
+      const uint32_t dst = smem_u32(ring) + st * C::STAGE;
+      const uint32_t bytes = ((id0 >= 0 ? 2 : 0) + (id1 >= 0 ? 2 : 0)) * L::TILE_BYTES;
+      if (bytes) mbar_arrive_expect_tx(&full[st], bytes);
+      else mbar_arrive(&full[st]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int id = u ? id1 : id0;
+        if (id >= 0) {
+          p4_bulk_load(dst + u * L::TILE_BYTES, a.k_cache + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[st]);
+          p4_bulk_load(dst + C::HALF + u * L::TILE_BYTES, a.v_cache + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[st]);
+        } else if (id == -1 && a.status) {        // a token of the context without a page: reported, left out
+          atomicCAS(a.status, 0, ST_BAD_ARG | (92 << 16));
+        }
       }
     }
   };
-  for (int i = 0; i < C::STAGES - 1 && i < my_tiles; ++i) issue(i);
+#pragma unroll
+  for (int i = 0; i < C::STAGES - 1; ++i)
+    if (i < mine) issue(i, i);
 
-  // Queries: the A operand, columns r and r + 8; k-step j of group g holds values 64 g + 16 t + 4 j .. + 3.
-  uint32_t qa[NB][GR][8];
-  float qsum[NB][GR];
-  int limit[NB];                                  // tokens the column sees
+  // Queries: the A operand, columns r and r + 8; word h of group g holds values 64 g + 16 t + 8 h ..
+  P4State<D, COLS> s;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int col = col0 + nb * 8 + r;
     const int qi = col / a.G, g_head = col % a.G;
     const bool live = nb * 8 + r < n_cols && (unsigned)(row0 + qi) < (unsigned)a.total_q;
-    limit[nb] = live ? min(kv_len, kv_len - q_len + qi + 1) : 0;
+    s.limit[nb] = live ? min(kv_len, kv_len - q_len + qi + 1) : 0;
     const __nv_bfloat16* qp = a.q + (long long)(row0 + qi) * a.q_stride + (long long)(hkv * a.G + g_head) * D + 16 * t;
+    uint32_t raw[GR][8];
+    float big = 0.f;
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (live) v = *reinterpret_cast<const uint4*>(qp + 64 * g + 8 * h);
+        raw[g][4 * h] = v.x; raw[g][4 * h + 1] = v.y; raw[g][4 * h + 2] = v.z; raw[g][4 * h + 3] = v.w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)               // (both halves of a word)
+          big = fmax3(big, fabsf(kv4_scale(raw[g][4 * h + e])), fabsf(kv4_low(raw[g][4 * h + e])));
+      }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // the column's largest value in 2^14 .. 2^15
+    const int eq = big > 0.f ? max(-100, min(113, (int)(__float_as_uint(big) >> 23) - 127 - 14)) : 0;
+    const float down = p4_pow2(-eq), down4 = p4_pow2(-eq - 4);
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
       float sum = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (live) x = *reinterpret_cast<const uint4*>(qp + 64 * g + 8 * h);
-        qa[nb][g][4 * h] = x.x; qa[nb][g][4 * h + 1] = x.y; qa[nb][g][4 * h + 2] = x.z; qa[nb][g][4 * h + 3] = x.w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += kv4_scale(qa[nb][g][4 * h + e]) + kv4_low(qa[nb][g][4 * h + e]);   // both halves
+      for (int e = 0; e < 8; ++e) {
+        const float q0 = kv4_scale(raw[g][e]), q1 = kv4_low(raw[g][e]), f = (e & 1) ? down4 : down;
+        s.qa[nb][g][e] = p4_half2(q0 * f, q1 * f);
+        sum += q0 * down + q1 * down;
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      qsum[nb][g] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      s.qsum[nb][g] = sum * 0x1p-21f;             // the products are in units of 2^-21
     }
-  }
-  float o[NB][GR][4][4];
-  float z[NB][GR], m_ref[NB], l_run[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    m_ref[nb] = -INFINITY;
-    l_run[nb] = 0.f;
+    s.factor[nb] = a.scale_log2 * 0x1p21f * p4_pow2(eq);
+    s.m[nb] = -INFINITY;
+    s.l[nb] = 0.f;
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
-      z[nb][g] = 0.f;
+      s.z[nb][g] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[nb][g][i][0] = o[nb][g][i][1] = o[nb][g][i][2] = o[nb][g][i][3] = 0.f;
+      for (int i = 0; i < 4; ++i) s.o[nb][g][i][0] = s.o[nb][g][i][1] = s.o[nb][g][i][2] = s.o[nb][g][i][3] = 0.f;
     }
   }
 
   bool ok = true;
-  int done = 0;
-  for (int i = 0; i < my_tiles; ++i) {
+  int st = 0, st_issue = C::STAGES - 1;
+  uint32_t parity = 0u;
+  int i = 0;
+  for (; i < mine; ++i) {
     // the stage read in the step before is free now: every value read from it has gone through a product
-    if (i + C::STAGES - 1 < my_tiles) issue(i + C::STAGES - 1);
-    const int st = i % C::STAGES;
-    ok = mbar_wait(&full[st], (i / C::STAGES) & 1, abort_flag, a.status, 93);
+    if (i + C::STAGES - 1 < mine) {
+      issue(i + C::STAGES - 1, st_issue);
+      st_issue = st_issue == C::STAGES - 1 ? 0 : st_issue + 1;
+    }
+    ok = mbar_wait(&full[st], parity, abort_flag, a.status, 93);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
-    done = i + 1;
-    if (!(present >> st & 1u)) continue;
-    const uint8_t* kt = ring + st * C::STAGE;
-    const uint8_t* vt = kt + L::TILE_BYTES;
-
-    // ---- scores of tokens t + 4 (2 j + e): sc[j][g][2 nb' + e] over the matrix product's rows r and r + 8
-    float sc[2][GR][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t kw[GR][2];
-      const uint8_t* kp = kt + (8 * j + r) * L::ROW + t * (8 * GR);
-      if constexpr (GR == 2) {
-        const uint4 x = *reinterpret_cast<const uint4*>(kp);
-        kw[0][0] = x.x; kw[0][1] = x.y; kw[1][0] = x.z; kw[1][1] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(kp);
-        kw[0][0] = x.x; kw[0][1] = x.y;
-      }
-#pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        sc[j][g][0] = sc[j][g][1] = sc[j][g][2] = sc[j][g][3] = 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w = kw[g][h];
-          const uint32_t p0 = p4_key_pair<0>(w), p1 = p4_key_pair<1>(w), p2 = p4_key_pair<2>(w), p3 = p4_key_pair<3>(w);
-          p4_mma(sc[j][g], qa[0][g][4 * h], NB > 1 ? qa[NB - 1][g][4 * h] : 0u, qa[0][g][4 * h + 1], NB > 1 ? qa[NB - 1][g][4 * h + 1] : 0u, p0, p1);
-          p4_mma(sc[j][g], qa[0][g][4 * h + 2], NB > 1 ? qa[NB - 1][g][4 * h + 2] : 0u, qa[0][g][4 * h + 3], NB > 1 ? qa[NB - 1][g][4 * h + 3] : 0u, p2, p3);
-        }
-      }
-    }
-    // ---- scales and lows of this thread's four tokens
-    const int tok0 = (tile0 + warp + P4_WARPS * i) * 16 + t;
-    float ks[2][2][GR], kl[2][2][GR], vs[2][2][GR], vl[2][2][GR];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t kq[2][GR], vq[2][GR];
-      const uint8_t* kp = kt + L::OFF_PAIR + (8 * j + 2 * t) * L::PAIR;
-      const uint8_t* vp = vt + L::OFF_PAIR + (8 * j + 2 * t) * L::PAIR;
-      if constexpr (GR == 2) {
-        const uint4 x = *reinterpret_cast<const uint4*>(kp), y = *reinterpret_cast<const uint4*>(vp);
-        kq[0][0] = x.x; kq[0][1] = x.y; kq[1][0] = x.z; kq[1][1] = x.w;
-        vq[0][0] = y.x; vq[0][1] = y.y; vq[1][0] = y.z; vq[1][1] = y.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(kp), y = *reinterpret_cast<const uint2*>(vp);
-        kq[0][0] = x.x; kq[1][0] = x.y;
-        vq[0][0] = y.x; vq[1][0] = y.y;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          ks[j][e][g] = kv4_scale(kq[e][g]);
-          kl[j][e][g] = fmaf(-16.f, ks[j][e][g], kv4_low(kq[e][g]));
-          vs[j][e][g] = kv4_scale(vq[e][g]);
-          vl[j][e][g] = fmaf(8.f, vs[j][e][g], kv4_low(vq[e][g]));
-        }
-    }
-    // ---- online softmax per column; the reference maximum moves only when it grew by more than 2^8
-    uint32_t pb[NB][GR][2];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float x[2][2], mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = 0.f;
-#pragma unroll
-          for (int g = 0; g < GR; ++g) v += fmaf(ks[j][e][g], sc[j][g][2 * nb + e], kl[j][e][g] * qsum[nb][g]);
-          x[j][e] = tok0 + 4 * (2 * j + e) < limit[nb] ? v * a.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, x[j][e]);
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const bool need = mx > m_ref[nb] + 8.f || (m_ref[nb] == -INFINITY && mx > -INFINITY);
-      if (__any_sync(0xffffffffu, need)) {
-        const float alpha = need ? fast_exp2(m_ref[nb] - mx) : 1.f;
-        if (need) m_ref[nb] = mx;
-        l_run[nb] *= alpha;
-        const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
-#pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          z[nb][g] *= alpha;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            o[nb][g][q][0] *= a0; o[nb][g][q][1] *= a1; o[nb][g][q][2] *= a0; o[nb][g][q][3] *= a1;
-          }
-        }
-      }
-      const float m_use = m_ref[nb] == -INFINITY ? 0.f : m_ref[nb];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float p0 = fast_exp2(x[j][0] - m_use), p1 = fast_exp2(x[j][1] - m_use);
-        l_run[nb] += p0 + p1;
-        // a token the column does not see may hold anything, behind the sequence's end too: it is left out, not
-        // multiplied by zero
-        const bool s0 = tok0 + 8 * j < limit[nb], s1 = tok0 + 8 * j + 4 < limit[nb];
-#pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          z[nb][g] += (s0 ? p0 * vl[j][0][g] : 0.f) + (s1 ? p1 * vl[j][1][g] : 0.f);
-          pb[nb][g][j] = pack_bf16x2(s0 ? p0 * vs[j][0][g] : 0.f, s1 ? p1 * vs[j][1][g] : 0.f);
-        }
-      }
-    }
-    // ---- values: the A operand holds values x tokens, B the probabilities
-    uint32_t vw[2][2][GR];
-    const int chunk = r ^ ((t >> 1) << 2);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint8_t* vp = vt + (t + 4 * (2 * j + e)) * L::ROW + chunk * (4 * GR);
-        if constexpr (GR == 2) {
-          const uint2 w = *reinterpret_cast<const uint2*>(vp);
-          vw[j][e][0] = w.x; vw[j][e][1] = w.y;
-        } else {
-          vw[j][e][0] = *reinterpret_cast<const uint32_t*>(vp);
-        }
-      }
-#pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      // halves of the two tokens' words side by side: lo holds values 0, 2, 4, 6 and hi values 1, 3, 5, 7 of both
-      const uint32_t lo0 = __byte_perm(vw[0][0][g], vw[0][1][g], 0x5410), hi0 = __byte_perm(vw[0][0][g], vw[0][1][g], 0x7632);
-      const uint32_t lo1 = __byte_perm(vw[1][0][g], vw[1][1][g], 0x5410), hi1 = __byte_perm(vw[1][0][g], vw[1][1][g], 0x7632);
-#define P4_PV(I)                                                                                              \
-  do {                                                                                                        \
-    const uint32_t a0 = p4_value_pair<I>(lo0), a1 = p4_value_pair<I>(hi0), a2 = p4_value_pair<I>(lo1),        \
-                   a3 = p4_value_pair<I>(hi1);                                                                \
-    _Pragma("unroll") for (int nb = 0; nb < NB; ++nb) p4_mma(o[nb][g][I], a0, a1, a2, a3, pb[nb][g][0], pb[nb][g][1]); \
-  } while (0)
-      P4_PV(0);
-      P4_PV(1);
-      P4_PV(2);
-      P4_PV(3);
-#undef P4_PV
-    }
+    const int tok = (chunk0 + P4_WARPS * i) * P4_CHUNK;
+    const uint32_t gone = absent >> (2 * st) & 3u;
+    const uint8_t* at = ring + st * C::STAGE;
+    if (gone == 0u && tok + P4_CHUNK <= common) p4_chunk<D, COLS, false>(s, at, tok + t, lane, visible, 0u);
+    else p4_chunk<D, COLS, true>(s, at, tok + t, lane, visible, gone);
     __syncwarp();
+    if (++st == C::STAGES) {
+      st = 0;
+      parity ^= 1u;
+    }
   }
   if (!ok)                                        // copies in flight land before the ring's memory goes away
-    for (int i = done; i < my_tiles && i < done + C::STAGES; ++i) mbar_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
+    for (int k = 0; k < C::STAGES && i < mine; ++k, ++i) {
+      mbar_drain(&full[st], parity);
+      if (++st == C::STAGES) {
+        st = 0;
+        parity ^= 1u;
+      }
+    }
 
   // ---- the warp's state: row c of w_acc is column c, values in order
   float* w_acc = reinterpret_cast<float*>(ring);
   __syncwarp();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    float l = l_run[nb];
+    float l = s.l[nb];
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (t == 0) {
-      s_m[warp * COLS + nb * 8 + r] = ok ? m_ref[nb] : -INFINITY;
+      s_m[warp * COLS + nb * 8 + r] = ok ? s.m[nb] : -INFINITY;
       s_l[warp * COLS + nb * 8 + r] = ok ? l : 0.f;
     }
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
-      float zz = z[nb][g];
+      float zz = s.z[nb][g];
       zz += __shfl_xor_sync(0xffffffffu, zz, 1);
       zz += __shfl_xor_sync(0xffffffffu, zz, 2);
       if (t == 0) s_z[(warp * COLS + nb * 8 + r) * GR + g] = zz;
-      // thread (r, t): columns 2 t and 2 t + 1, values 64 g + 8 r + (0 .. 7)
+      // thread (r, t): columns 2 t and 2 t + 1, values 64 g + 8 r + (0 .. 7), out of their units
+      float (&o)[4][4] = s.o[nb][g];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float* dst = w_acc + (nb * 8 + 2 * t + c) * D + 64 * g + 8 * r;
-        *reinterpret_cast<float4*>(dst) = make_float4(o[nb][g][0][c], o[nb][g][0][2 + c], o[nb][g][1][c], o[nb][g][1][2 + c]);
-        *reinterpret_cast<float4*>(dst + 4) = make_float4(o[nb][g][2][c], o[nb][g][2][2 + c], o[nb][g][3][c], o[nb][g][3][2 + c]);
+        *reinterpret_cast<float4*>(dst) = make_float4(o[0][c] * 0x1p24f, o[0][2 + c] * 0x1p24f, o[1][c] * 0x1p20f, o[1][2 + c] * 0x1p20f);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(o[2][c] * 0x1p24f, o[2][2 + c] * 0x1p24f, o[3][c] * 0x1p20f, o[3][2 + c] * 0x1p20f);
       }
     }
   }
@@ -556,11 +652,11 @@ void p4_launch(P4Args& a, int batch, int max_q, cudaStream_t stream) {
   p4_configure(paged_attn_int4_kernel<D, COLS>, P4Cfg<D, COLS>::BYTES, seen);
   const long long blocks = ((long long)max_q * a.G + COLS - 1) / COLS;
   MB_REQUIRE(blocks * a.kv_heads <= 65535, "paged attention over 4-bit pages: too many query columns for one launch");
-  // Enough CTAs for two to four per SM, each with two tiles or more per warp if the table were full.
+  // As many CTAs as fit the GPU at once, four per SM, with a chunk or more per warp if the table were full.
   const long long pairs = (long long)batch * a.kv_heads * blocks;
-  const long long tiles = (long long)a.max_pages * (a.page_size >> 4);
-  int splits = 1;
-  while (splits < 16 && pairs * splits < 2LL * sm_count() && tiles > 8LL * splits) splits *= 2;
+  const long long chunks = ((long long)a.max_pages * a.page_size + P4_CHUNK - 1) / P4_CHUNK;
+  const long long fit = 4LL * sm_count() / pairs, use = (chunks + P4_WARPS - 1) / P4_WARPS;
+  const int splits = (int)std::max(1LL, std::min({16LL, fit, use}));
   a.splits = splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(batch, (unsigned)(blocks * a.kv_heads), splits);

@@ -21,8 +21,7 @@
 //     the score fragment of a thread (columns 2 t, 2 t + 1 of two 8-token products) then covers tokens t, t + 4,
 //     t + 8 and t + 12, whose value rows lie in different banks for the four t;
 //   * a key row is [t = 0..3][group][2 words]: values 64 g + 16 t + 8 h ...; the words are rotated left by three
-//     bits, which puts a nibble on the top mantissa bits of a bf16: masked by 0x00780078 and joined with 0x4180 it
-//     is the number 16 + code;
+//     bits, so that two nibbles of a half lie within the top bits of a 16-bit float's mantissa;
 //   * a value row is [r = 0..7][group][1 word]: values 64 g + 8 r ...; chunk r is stored at place r ^ 4 ((n / 2) % 2).
 #pragma once
 #include "common.cuh"
