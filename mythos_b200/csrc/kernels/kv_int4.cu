@@ -184,12 +184,6 @@ __device__ __forceinline__ uint32_t p4_half2(float lo, float hi) {
   return r;
 }
 __device__ __forceinline__ float p4_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// x - c on both halves (c: 8 steps of the subnormal range, so the difference is exact).
-__device__ __forceinline__ uint32_t p4_centre(uint32_t x, uint32_t c) {
-  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&c));
-  return *reinterpret_cast<const uint32_t*>(&y);
-}
-
 struct P4Args {
   const __nv_bfloat16* q;
   const uint8_t* k_cache;
@@ -204,18 +198,24 @@ struct P4Args {
   int* status;
 };
 
-// A warp's running state: accumulators (units of 2^-24 / 2^-20), offset sums, reference and row sum.
+// A warp's running state. Thread (r, t) of the warp holds columns 2 t and 2 t + 1 of every block of eight.
 template <int D, int COLS>
 struct P4State {
   static constexpr int NB = COLS / 8, GR = KvInt4<D>::GROUPS;
-  uint32_t qa[NB][GR][8];
-  float qsum[NB][GR], factor[NB];
-  int limit[NB];
-  float o[NB][GR][4][4];
-  float z[NB][GR], m[NB], l[NB];
+  uint32_t qb[NB][GR][8];                 // B operand: column r
+  float qsum[NB][GR][2], factor[NB][2];   // of columns 2 t, 2 t + 1, as everything below
+  int limit[NB][2];
+  float o[NB][GR][4][4];                  // units of 2^-24 (even i) and 2^-20
+  float z[NB][GR][2], m[NB][2], l[NB][2];
 };
 
-// One chunk: tile u (0, 1) at `at` + u * TILE_BYTES for K, HALF behind for V; tok0: its first token plus this thread's t.
+__device__ __forceinline__ uint32_t p4_transpose(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// One chunk: tile u (0, 1) at `at` + u * TILE_BYTES for K, HALF behind for V; tok0: its first token.
 // MASK: some token is not seen by some column (visible: those seen by any), or not held at all.
 template <int D, int COLS, bool MASK>
 __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at, int tok0, int lane, int visible, uint32_t absent) {
@@ -223,133 +223,175 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
   using C = P4Cfg<D, COLS>;
   constexpr int GR = L::GROUPS, NB = COLS / 8;
   const int r = lane >> 2, t = lane & 3;
-  // ---- scores of tokens tok0 + 16 u + 4 (2 j + e): the matrix product's columns 2 t + e, rows r and r + 8
-  float sc[2][2][GR][4];
+  // ---- scores: rows of the product are key rows 8 j + r of a tile, columns 2 t + c
+  float sc[2][NB][GR][4];                         // [tile][block][group][2 j + c]
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t kw[2][GR][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint8_t* kp = at + u * L::TILE_BYTES + (8 * j + r) * L::ROW + t * (8 * GR);
+      if constexpr (GR == 2) {
+        const uint4 x = *reinterpret_cast<const uint4*>(kp);
+        kw[j][0][0] = x.x; kw[j][0][1] = x.y; kw[j][1][0] = x.z; kw[j][1][1] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(kp);
+        kw[j][0][0] = x.x; kw[j][0][1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w0 = kw[0][g][h], w1 = kw[1][g][h], v0 = __funnelshift_r(w0, w0, 8), v1 = __funnelshift_r(w1, w1, 8);
+        const uint32_t a0 = w0 & 0x00780078u, a1 = w1 & 0x00780078u, a2 = w0 & 0x07800780u, a3 = w1 & 0x07800780u;
+        const uint32_t b0 = v0 & 0x00780078u, b1 = v1 & 0x00780078u, b2 = v0 & 0x07800780u, b3 = v1 & 0x07800780u;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float (&c)[4] = sc[u][nb][g];
+          if (h == 0) c[0] = c[1] = c[2] = c[3] = 0.f;
+          p4_mma(c, a0, a1, a2, a3, s.qb[nb][g][4 * h], s.qb[nb][g][4 * h + 1]);
+          p4_mma(c, b0, b1, b2, b3, s.qb[nb][g][4 * h + 2], s.qb[nb][g][4 * h + 3]);
+        }
+      }
+  }
+  // ---- exponent of the chunk's values: one group of one token per thread and tile
+  float mag = 0.f;
+#pragma unroll
+  for (int u = 0; u < GR; ++u) {                  // (one group a token: the warp's halves take the two tiles)
+    const int tile = GR == 2 ? u : lane >> 4, row = GR == 2 ? lane >> 1 : lane & 15, g = GR == 2 ? lane & 1 : 0;
+    const uint32_t p = *reinterpret_cast<const uint32_t*>(at + C::HALF + tile * L::TILE_BYTES + L::OFF_PAIR + row * L::PAIR + 4 * g);
+    const float top = fmaf(15.f, kv4_scale(p), kv4_low(p));
+    bool use = true;                              // (what every column sees may be infinite: the result is no number then)
+    if (MASK) {                                   // a place behind the context may hold anything
+      const int n = (row & 8) + ((row >> 1) & 3) + ((row & 1) << 2);       // token at this pair row
+      use = kv4_finite(p) && tok0 + 16 * tile + n < visible && !(absent >> tile & 1u);
+    }
+    mag = fmax3(mag, use ? fabsf(top) : 0.f, use ? fabsf(kv4_low(p)) : 0.f);
+  }
+  // p is kept up to 2^8 (and 2^6 more until the reference moves) times the inverse of the largest magnitude, which is at
+  // least 7 scales: p times a scale then stays below 2^13, and is exact to 2^-12 over 24 octaves below. Bounded so that p, its
+  // sum and its product with any value stay within fp32.
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(mag));
+  const float ev = fminf(fmaxf(__uint_as_float(0x4B000000u | (bits >> 23)) - (8388608.f + 127.f), -80.f), 112.f) - 8.f;
+  // ---- online softmax: scores relative to the reference; it moves only when one of them passes it by 2^6
+  float x[2][NB][2][2];                           // [tile][block][j][c]
+  float top = -INFINITY;
+  const int tok_r = tok0 + ((r >> 1) & 3) + ((r & 1) << 2);                // token of key row r of the first tile; row r + 8: 8 on
+  float mm[NB][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) mm[nb][c] = s.m[nb][c] == -INFINITY ? 0.f : s.m[nb][c];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      uint32_t kw[GR][2];
-      const uint8_t* kp = at + u * L::TILE_BYTES + (8 * j + r) * L::ROW + t * (8 * GR);
+      uint32_t kq[GR];
+      const uint8_t* kp = at + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + r) * L::PAIR;
       if constexpr (GR == 2) {
-        const uint4 x = *reinterpret_cast<const uint4*>(kp);
-        kw[0][0] = x.x; kw[0][1] = x.y; kw[1][0] = x.z; kw[1][1] = x.w;
+        const uint2 y = *reinterpret_cast<const uint2*>(kp);
+        kq[0] = y.x; kq[1] = y.y;
       } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(kp);
-        kw[0][0] = x.x; kw[0][1] = x.y;
+        kq[0] = *reinterpret_cast<const uint32_t*>(kp);
       }
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        float (&c)[4] = sc[u][j][g];
-        c[0] = c[1] = c[2] = c[3] = 0.f;
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w = kw[g][h], w8 = __funnelshift_r(w, w, 8);
-          const uint32_t (&q0)[8] = s.qa[0][g];
-          const uint32_t (&q1)[8] = s.qa[NB - 1][g];
-          p4_mma(c, q0[4 * h], NB > 1 ? q1[4 * h] : 0u, q0[4 * h + 1], NB > 1 ? q1[4 * h + 1] : 0u, w & 0x00780078u, w & 0x07800780u);
-          p4_mma(c, q0[4 * h + 2], NB > 1 ? q1[4 * h + 2] : 0u, q0[4 * h + 3], NB > 1 ? q1[4 * h + 3] : 0u, w8 & 0x00780078u, w8 & 0x07800780u);
+        for (int c = 0; c < 2; ++c) {
+          float v = kv4_low(kq[0]) * s.qsum[nb][0][c];
+          if constexpr (GR == 2) v = fmaf(kv4_low(kq[1]), s.qsum[nb][1][c], v);
+#pragma unroll
+          for (int g = 0; g < GR; ++g) v = fmaf(kv4_scale(kq[g]), sc[u][nb][g][2 * j + c], v);
+          v = fmaf(v, s.factor[nb][c], -mm[nb][c]);
+          if (MASK && (tok_r + 16 * u + 8 * j >= s.limit[nb][c] || (absent >> u & 1u))) v = -INFINITY;
+          x[u][nb][j][c] = v;
         }
-      }
     }
-  // ---- exponent of the chunk's values: one group of one token per thread and tile
-  uint32_t mag = 0u;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    if (GR == 1 && u == 1) break;                 // 16 groups a tile: the warp's halves take the two tiles
-    const int tile = GR == 2 ? u : lane >> 4, row = GR == 2 ? lane >> 1 : lane & 15, g = GR == 2 ? lane & 1 : 0;
-    const uint32_t p = *reinterpret_cast<const uint32_t*>(at + C::HALF + tile * L::TILE_BYTES + L::OFF_PAIR + row * L::PAIR + 4 * g);
-    const float sv = kv4_scale(p), a = fmaxf(8.f * sv, fabsf(fmaf(8.f, sv, kv4_low(p))));
-    bool use = kv4_finite(p);
-    if (MASK) {                                   // a place behind the context may hold anything
-      const int n = (row & 8) + ((row >> 1) & 3) + ((row & 1) << 2);       // token at this pair row
-      use = use && tok0 - t + 16 * tile + n < visible && !(absent >> tile & 1u);
-    }
-    if (use) mag = max(mag, __float_as_uint(a));
-  }
-  mag = __reduce_max_sync(0xffffffffu, mag);
-  // p is kept up to 2^9 (and 2^6 more until the reference moves) times the largest value's inverse: p times a scale,
-  // an eighth of it at most, then stays below 2^14, and is exact to 2^-12 over 24 octaves below. Bounded so that p, its sum
-  // and its product with any value stay within fp32.
-  const float ev = (float)(max(-80, min(112, (int)(mag >> 23) - 127)) - 9);
-  // ---- online softmax per column; the reference moves only when it grew by more than 2^6
-  uint32_t pb[2][NB][GR][2];
-  float x[2][NB][2][2];
+  bool first = false;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) first = first || s.m[nb][c] == -INFINITY;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t kq[2][GR];
-        const uint8_t* kp = at + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + 2 * t) * L::PAIR;
-        if constexpr (GR == 2) {
-          const uint4 y = *reinterpret_cast<const uint4*>(kp);
-          kq[0][0] = y.x; kq[0][1] = y.y; kq[1][0] = y.z; kq[1][1] = y.w;
-        } else {
-          const uint2 y = *reinterpret_cast<const uint2*>(kp);
-          kq[0][0] = y.x; kq[1][0] = y.y;
-        }
+      for (int j = 0; j < 2; ++j) top = fmax3(top, x[u][nb][j][0], x[u][nb][j][1]);
+  }
+  if (__any_sync(0xffffffffu, first || top + ev > 6.f)) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = 0.f;
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int g = 0; g < GR; ++g)
-            v = fmaf(kv4_scale(kq[e][g]), sc[u][j][g][2 * nb + e], fmaf(kv4_low(kq[e][g]), s.qsum[nb][g], v));
-          v *= s.factor[nb];
-          if (MASK && (tok0 + 16 * u + 4 * (2 * j + e) >= s.limit[nb] || (absent >> u & 1u))) v = -INFINITY;
-          x[u][nb][j][e] = v;
+      for (int c = 0; c < 2; ++c) {
+        float mx = fmaxf(fmax3(x[0][nb][0][c], x[0][nb][1][c], x[1][nb][0][c]), x[1][nb][1][c]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        mx += ev;                                 // relative to the reference used so far
+        if (s.m[nb][c] == -INFINITY ? mx > -INFINITY : mx > 0.f) {
+          const float alpha = s.m[nb][c] == -INFINITY ? 0.f : fast_exp2(-mx);
+          s.m[nb][c] = mm[nb][c] + mx;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) x[u][nb][j][c] -= mx;
+          s.l[nb][c] *= alpha;
+#pragma unroll
+          for (int g = 0; g < GR; ++g) {
+            s.z[nb][g][c] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s.o[nb][g][i][c] *= alpha;
+              s.o[nb][g][i][2 + c] *= alpha;
+            }
+          }
         }
-        mx = fmax3(mx, x[u][nb][j][0], x[u][nb][j][1]);
       }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) + ev;
-    const bool need = mx > s.m[nb] + 6.f || (s.m[nb] == -INFINITY && mx > -INFINITY);
-    if (__any_sync(0xffffffffu, need)) {
-      const float alpha = need ? fast_exp2(s.m[nb] - mx) : 1.f;
-      if (need) s.m[nb] = mx;
-      s.l[nb] *= alpha;
-      const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
+  }
+  // ---- weights p scale as the B operand (k = tokens, n = columns): transposed in blocks of eight by eight. Odd key rows
+  // are the tokens that enter with the complement of their codes.
+  uint32_t pb[2][NB][GR][2];
+  const uint32_t flip = (uint32_t)(r & 1) << 31;
+  const float whole = (r & 1) ? -15.f : 0.f;      // low + 15 scale, the scale's sign already turned
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t vq[GR];
+      const uint8_t* vp = at + C::HALF + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + r) * L::PAIR;
+      if constexpr (GR == 2) {
+        const uint2 y = *reinterpret_cast<const uint2*>(vp);
+        vq[0] = y.x; vq[1] = y.y;
+      } else {
+        vq[0] = *reinterpret_cast<const uint32_t*>(vp);
+      }
+      float w[GR], b[GR];
 #pragma unroll
       for (int g = 0; g < GR; ++g) {
-        s.z[nb][g] *= alpha;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          s.o[nb][g][q][0] *= a0; s.o[nb][g][q][1] *= a1; s.o[nb][g][q][2] *= a0; s.o[nb][g][q][3] *= a1;
-        }
+        w[g] = __uint_as_float(vq[g] << 16 ^ flip);
+        b[g] = fmaf(whole, w[g], kv4_low(vq[g]));
       }
-    }
-    const float m = MASK && s.m[nb] == -INFINITY ? 0.f : s.m[nb];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t vq[2][GR];
-        const uint8_t* vp = at + C::HALF + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + 2 * t) * L::PAIR;
-        if constexpr (GR == 2) {
-          const uint4 y = *reinterpret_cast<const uint4*>(vp);
-          vq[0][0] = y.x; vq[0][1] = y.y; vq[1][0] = y.z; vq[1][1] = y.w;
-        } else {
-          const uint2 y = *reinterpret_cast<const uint2*>(vp);
-          vq[0][0] = y.x; vq[1][0] = y.y;
-        }
-        const float p0 = fast_exp2(x[u][nb][j][0] - m), p1 = fast_exp2(x[u][nb][j][1] - m);
-        s.l[nb] += p0 + p1;
+      for (int nb = 0; nb < NB; ++nb) {
+        const float p0 = fast_exp2(x[u][nb][j][0]), p1 = fast_exp2(x[u][nb][j][1]);
+        s.l[nb][0] += p0;
+        s.l[nb][1] += p1;
         // a token the column does not see may hold anything, behind the sequence's end too: it is left out, not
         // multiplied by zero
         const bool s0 = !MASK || x[u][nb][j][0] != -INFINITY, s1 = !MASK || x[u][nb][j][1] != -INFINITY;
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
-          const float w0 = kv4_scale(vq[0][g]), w1 = kv4_scale(vq[1][g]);
-          const float b0 = fmaf(8.f, w0, kv4_low(vq[0][g])), b1 = fmaf(8.f, w1, kv4_low(vq[1][g]));
-          if (MASK) s.z[nb][g] += (s0 ? p0 * b0 : 0.f) + (s1 ? p1 * b1 : 0.f);
-          else s.z[nb][g] = fmaf(p0, b0, fmaf(p1, b1, s.z[nb][g]));
-          pb[u][nb][g][j] = p4_half2(s0 ? p0 * w0 : 0.f, s1 ? p1 * w1 : 0.f);
+          if (MASK) {
+            s.z[nb][g][0] += s0 ? p0 * b[g] : 0.f;
+            s.z[nb][g][1] += s1 ? p1 * b[g] : 0.f;
+          } else {
+            s.z[nb][g][0] = fmaf(p0, b[g], s.z[nb][g][0]);
+            s.z[nb][g][1] = fmaf(p1, b[g], s.z[nb][g][1]);
+          }
+          pb[u][nb][g][j] = p4_transpose(p4_half2(s0 ? p0 * w[g] : 0.f, s1 ? p1 * w[g] : 0.f));
         }
       }
-  }
-  // ---- values: the A operand holds values x tokens, B the probabilities
+    }
+  // ---- values: the A operand holds values x tokens (t, t + 4, t + 8, t + 12: those of key rows 2 t, 2 t + 1 and 8 on)
   const int chunk = r ^ ((t >> 1) << 2);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -376,9 +418,9 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
         if (i == 2) {
           lo0 >>= 8; hi0 >>= 8; lo1 >>= 8; hi1 >>= 8;
         }
-        const uint32_t mask = (i & 1) ? 0x00F000F0u : 0x000F000Fu, eight = (i & 1) ? 0x00800080u : 0x00080008u;
-        const uint32_t a0 = p4_centre(lo0 & mask, eight), a1 = p4_centre(hi0 & mask, eight), a2 = p4_centre(lo1 & mask, eight),
-                       a3 = p4_centre(hi1 & mask, eight);
+        const uint32_t mask = (i & 1) ? 0x00F000F0u : 0x000F000Fu;
+        const uint32_t a0 = (lo0 ^ 0xFFFF0000u) & mask, a1 = (hi0 ^ 0xFFFF0000u) & mask, a2 = (lo1 ^ 0xFFFF0000u) & mask,
+                       a3 = (hi1 ^ 0xFFFF0000u) & mask;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) p4_mma(s.o[nb][g][i], a0, a1, a2, a3, pb[u][nb][g][0], pb[u][nb][g][1]);
       }
@@ -432,42 +474,38 @@ paged_attn_int4_kernel(const __grid_constant__ P4Args a) {
   };
   int ids = locate(lane >> 1), ids_next = locate(16 + (lane >> 1));
   uint32_t absent = 0u;                           // bits 2 s, 2 s + 1: tiles of stage s that were not loaded
-  auto issue = [&](int i, int st) {               // all lanes; lane 0 starts the copies of the warp's chunk i
+  // lanes 0 .. 3 start one copy each: tile l % 2, K (l < 2) or V
+  const uint8_t* base = (lane & 2) ? a.v_cache : a.k_cache;
+  const uint32_t dst0 = smem_u32(ring) + ((lane & 2) ? C::HALF : 0) + (lane & 1) * L::TILE_BYTES;
+  auto issue = [&](int i, int st) {               // all lanes: the warp's chunk i into stage st
     if (i > 0 && (i & 15) == 0) {
       ids = ids_next;
       ids_next = locate(i + 16 + (lane >> 1));
     }
-    const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + 1);
-    absent = (absent & ~(3u << (2 * st))) | ((id0 < 0 ? 1u : 0u) | (id1 < 0 ? 2u : 0u)) << (2 * st);
+    const int id = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + (lane & 1));
+    const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 3u;
+    absent = (absent & ~(3u << (2 * st))) | gone << (2 * st);
     if (lane == 0) {
-      const uint32_t dst = smem_u32(ring) + st * C::STAGE;
-      const uint32_t bytes = ((id0 >= 0 ? 2 : 0) + (id1 >= 0 ? 2 : 0)) * L::TILE_BYTES;
-      if (bytes) mbar_arrive_expect_tx(&full[st], bytes);
-      else mbar_arrive(&full[st]);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int id = u ? id1 : id0;
-        if (id >= 0) {
-          p4_bulk_load(dst + u * L::TILE_BYTES, a.k_cache + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[st]);
-          p4_bulk_load(dst + C::HALF + u * L::TILE_BYTES, a.v_cache + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[st]);
-        } else if (id == -1 && a.status) {        // a token of the context without a page: reported, left out
-          atomicCAS(a.status, 0, ST_BAD_ARG | (92 << 16));
-        }
-      }
+      if (gone == 3u) mbar_arrive(&full[st]);
+      else mbar_arrive_expect_tx(&full[st], gone ? C::STAGE / 2 : C::STAGE);
+    }
+    if (lane < 4) {
+      if (id >= 0) p4_bulk_load(dst0 + st * C::STAGE, base + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[st]);
+      else if (id == -1 && a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (92 << 16));   // a token of the context without a page
     }
   };
 #pragma unroll
   for (int i = 0; i < C::STAGES - 1; ++i)
     if (i < mine) issue(i, i);
 
-  // Queries: the A operand, columns r and r + 8; word h of group g holds values 64 g + 16 t + 8 h ..
+  // Queries: the B operand, column r of every block; word h of group g holds values 64 g + 16 t + 8 h ..
   P4State<D, COLS> s;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int col = col0 + nb * 8 + r;
     const int qi = col / a.G, g_head = col % a.G;
     const bool live = nb * 8 + r < n_cols && (unsigned)(row0 + qi) < (unsigned)a.total_q;
-    s.limit[nb] = live ? min(kv_len, kv_len - q_len + qi + 1) : 0;
+    const int limit = live ? min(kv_len, kv_len - q_len + qi + 1) : 0;
     const __nv_bfloat16* qp = a.q + (long long)(row0 + qi) * a.q_stride + (long long)(hkv * a.G + g_head) * D + 16 * t;
     uint32_t raw[GR][8];
     float big = 0.f;
@@ -486,29 +524,38 @@ paged_attn_int4_kernel(const __grid_constant__ P4Args a) {
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
     // the column's largest value in 2^14 .. 2^15
     const int eq = big > 0.f ? max(-100, min(113, (int)(__float_as_uint(big) >> 23) - 127 - 14)) : 0;
-    const float down = p4_pow2(-eq), down4 = p4_pow2(-eq - 4);
+    const float down = p4_pow2(-eq), down4 = p4_pow2(-eq - 4), factor = a.scale_log2 * 0x1p21f * p4_pow2(eq);
+    float qsum[GR];
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float q0 = kv4_scale(raw[g][e]), q1 = kv4_low(raw[g][e]), f = (e & 1) ? down4 : down;
-        s.qa[nb][g][e] = p4_half2(q0 * f, q1 * f);
+        s.qb[nb][g][e] = p4_half2(q0 * f, q1 * f);
         sum += q0 * down + q1 * down;
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      s.qsum[nb][g] = sum * 0x1p-21f;             // the products are in units of 2^-21
+      qsum[g] = sum * 0x1p-21f;                   // the products are in units of 2^-21
     }
-    s.factor[nb] = a.scale_log2 * 0x1p21f * p4_pow2(eq);
-    s.m[nb] = -INFINITY;
-    s.l[nb] = 0.f;
 #pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      s.z[nb][g] = 0.f;
+    for (int c = 0; c < 2; ++c) {                 // what concerns columns 2 t + c sits in the threads of r = 2 t + c
+      const int from = 8 * t + 4 * c;
+      s.limit[nb][c] = __shfl_sync(0xffffffffu, limit, from);
+      s.factor[nb][c] = __shfl_sync(0xffffffffu, factor, from);
+      s.m[nb][c] = -INFINITY;
+      s.l[nb][c] = 0.f;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        s.qsum[nb][g][c] = __shfl_sync(0xffffffffu, qsum[g], from);
+        s.z[nb][g][c] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s.o[nb][g][i][0] = s.o[nb][g][i][1] = s.o[nb][g][i][2] = s.o[nb][g][i][3] = 0.f;
-    }
   }
 
   bool ok = true;
@@ -521,14 +568,16 @@ paged_attn_int4_kernel(const __grid_constant__ P4Args a) {
       issue(i + C::STAGES - 1, st_issue);
       st_issue = st_issue == C::STAGES - 1 ? 0 : st_issue + 1;
     }
-    ok = mbar_wait(&full[st], parity, abort_flag, a.status, 93);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) break;
+    if (!__all_sync(0xffffffffu, mbar_try_wait(&full[st], parity))) {
+      ok = mbar_wait(&full[st], parity, abort_flag, a.status, 93);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+    }
     const int tok = (chunk0 + P4_WARPS * i) * P4_CHUNK;
     const uint32_t gone = absent >> (2 * st) & 3u;
     const uint8_t* at = ring + st * C::STAGE;
-    if (gone == 0u && tok + P4_CHUNK <= common) p4_chunk<D, COLS, false>(s, at, tok + t, lane, visible, 0u);
-    else p4_chunk<D, COLS, true>(s, at, tok + t, lane, visible, gone);
+    if (gone == 0u && tok + P4_CHUNK <= common) p4_chunk<D, COLS, false>(s, at, tok, lane, visible, 0u);
+    else p4_chunk<D, COLS, true>(s, at, tok, lane, visible, gone);
     __syncwarp();
     if (++st == C::STAGES) {
       st = 0;
@@ -548,30 +597,30 @@ paged_attn_int4_kernel(const __grid_constant__ P4Args a) {
   float* w_acc = reinterpret_cast<float*>(ring);
   __syncwarp();
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    float l = s.l[nb];
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (t == 0) {
-      s_m[warp * COLS + nb * 8 + r] = ok ? s.m[nb] : -INFINITY;
-      s_l[warp * COLS + nb * 8 + r] = ok ? l : 0.f;
-    }
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      float zz = s.z[nb][g];
-      zz += __shfl_xor_sync(0xffffffffu, zz, 1);
-      zz += __shfl_xor_sync(0xffffffffu, zz, 2);
-      if (t == 0) s_z[(warp * COLS + nb * 8 + r) * GR + g] = zz;
-      // thread (r, t): columns 2 t and 2 t + 1, values 64 g + 8 r + (0 .. 7), out of their units
-      float (&o)[4][4] = s.o[nb][g];
+    for (int c = 0; c < 2; ++c) {
+      const int col = nb * 8 + 2 * t + c;
+      float l = s.l[nb][c];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float* dst = w_acc + (nb * 8 + 2 * t + c) * D + 64 * g + 8 * r;
+      for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      if (r == 0) {
+        s_m[warp * COLS + col] = ok ? s.m[nb][c] : -INFINITY;
+        s_l[warp * COLS + col] = ok ? l : 0.f;
+      }
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        float z = s.z[nb][g][c];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+        if (r == 0) s_z[(warp * COLS + col) * GR + g] = z;
+        // values 64 g + 8 r + (0 .. 7), out of their units
+        float (&o)[4][4] = s.o[nb][g];
+        float* dst = w_acc + col * D + 64 * g + 8 * r;
         *reinterpret_cast<float4*>(dst) = make_float4(o[0][c] * 0x1p24f, o[0][2 + c] * 0x1p24f, o[1][c] * 0x1p20f, o[1][2 + c] * 0x1p20f);
         *reinterpret_cast<float4*>(dst + 4) = make_float4(o[2][c] * 0x1p24f, o[2][2 + c] * 0x1p24f, o[3][c] * 0x1p20f, o[3][2 + c] * 0x1p20f);
       }
     }
-  }
   __syncthreads();
 
   // ---- the CTA's state, in the first warp's ring: every element is read and written by one thread
