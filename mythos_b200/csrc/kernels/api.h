@@ -392,17 +392,24 @@ void kv_read_int4(const KvInt4Cache& c, const int* positions, const int* seq_ids
 // One query token per sequence: q [batch, heads, head_dim] with a token stride, out contiguous. A sequence of length 0
 // gets zeros; a token of the context without a page is left out and reported through the status word.
 void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* context_lens, void* out, int batch,
-                            int heads, float scale, int* status, cudaStream_t stream);
+                            int heads, float scale, void* workspace, int* status, cudaStream_t stream);
 // New tokens of several sequences packed back to back, causal over the pages (as flash_attn_paged_prefill). max_q: most new
 // tokens of a sequence, max_kv: most keys. Up to P4_FEW_COLUMNS query columns (new tokens x heads of a group) per kv head, a
-// split-context kernel reads the codes directly; above, prompt_int4 expands the sequences into the workspace
-// (paged_attn_prefill_int4_workspace bytes, 0: none wanted), each once for all of its queries.
+// split-context kernel reads the codes directly; above, prompt_int4 expands the sequences into the workspace, each once
+// for all of its queries.
 constexpr int P4_FEW_COLUMNS = 64;
-long long paged_attn_prefill_int4_workspace(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
+// Bytes of the workspace of both attention calls (decode: total_q = batch, max_q = 1); 16-byte aligned, free again when the call's
+// kernels have run.
+long long paged_attn_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads);
 void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                              long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale,
                              void* workspace, int* status, cudaStream_t stream);
-// The second of its two forms (kv_int4_prefill.cu); arguments checked by the caller.
+// Their two forms, arguments checked by the caller: kv_int4_decode.cu (cu_q null: one query token per sequence) and
+// kv_int4_prefill.cu.
+long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads);
+void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
+                    long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,
+                    cudaStream_t stream);
 long long prompt_int4_workspace(int batch, int total_q, int max_kv, int heads, int kv_heads, int head_dim);
 void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                  long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,

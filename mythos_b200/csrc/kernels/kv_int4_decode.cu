@@ -1,0 +1,1040 @@
+// Attention over the 4-bit paged KV cache for one or a few query tokens per sequence (format: kv_int4.cuh).
+//
+// Queries of one (sequence, kv head) are columns: column c is head c % G of token c / G. A warp takes chunks of 32 tokens
+// (two tiles) for a block of COLS columns through a ring of its own, filled with one bulk copy per tile for K and one for V.
+//
+// What bounds it is the integer pipe (half rate) that takes the codes apart, so operands are formed by one AND each:
+// the low eleven bits of an fp16 are linear in its value (subnormals and the first normal binade share one step,
+// 2^-24), so a nibble anywhere in them is its code times a power of two. Keys: bits 3-6 (code 2^-21) and 7-10 (code 2^-17)
+// of a rotated word, then the word rotated by eight; queries of the second kind are multiplied by 2^-4. Values: bits 0-3
+// (2^-24) and 4-7 (2^-20) of two tokens' halves side by side; they are different output values, scaled at the end.
+//
+// Scores: q . k = sum over groups of scale (q_g . c_g) + low sum(q_g), the product exact in fp16 (a query column is
+// divided by a power of two first, so that its bf16 values fit). Values: o = sum_t (p_t scale_t) c_t + sum_t p_t low_t, the
+// second sum a scalar per column and group in fp32. The tensor cores truncate what they add, and the codes are all
+// positive: over a long context that would drift. So every second token (the upper halves of the operand) enters as
+// -(p scale) (15 - c) + p (low + 15 scale): complementing costs one NOT per word, and the running sum stays near zero.
+// p_t scale_t is rounded to fp16 (2^-12 of each term); the running reference M is the maximum of the scores plus the
+// exponent of the chunk's values, so it fits whatever the values' size. Everything else is fp32. mma.sync rather than tcgen05:
+// with 8 columns a 128-row tile would be filled to a sixteenth, and the codes would have to go through shared memory
+// once more.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "api.h"
+#include "common.cuh"
+#include "host_util.h"
+#include "kv_int4.cuh"
+#include "tc.cuh"
+
+namespace mb {
+namespace {
+
+constexpr int P4_WARPS = 4;
+constexpr int P4_THREADS = 32 * P4_WARPS;
+constexpr int P4_CHUNK = 32;      // tokens
+
+template <int D, int COLS>
+struct P4Cfg {
+  using L = KvInt4<D>;
+  // One chunk ahead: sixteen warps keep 74 KB (D = 128) in flight per SM, about twice what its share of the memory rate
+  // times the latency asks for.
+  static constexpr int STAGES = 2;
+  static constexpr int HALF = 2 * L::TILE_BYTES;              // K (or V) of a chunk
+  static constexpr int STAGE = 2 * HALF;
+  static constexpr int WARP_BYTES = STAGES * STAGE;
+  static constexpr int PART = COLS * D * 4;                   // a part's sums, [COLS][D]
+  static_assert(PART <= WARP_BYTES, "a warp's last part is staged in its own (drained) ring");
+};
+
+__device__ __forceinline__ void p4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void p4_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t p4_half2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float p4_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ uint32_t p4_transpose(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Quotient by a number the host knows: n * mul / 2^shift with mul = ceil(2^shift / d), shift = 31 + ceil(log2 d); exact for
+// 0 <= n < 2^31.
+struct P4Div {
+  uint32_t mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)((unsigned long long)(unsigned)n * mul >> shift); }
+};
+P4Div p4_div(int d) {
+  int s = 0;
+  while ((1LL << s) < d) ++s;
+  return {(uint32_t)(((1ULL << (31 + s)) + (unsigned)d - 1) / (unsigned)d), 31 + s};
+}
+
+struct P4Args {
+  const __nv_bfloat16* q;
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const int* block_table;
+  const int* kv_lens;
+  const int* cu_q;          // first query row of every sequence, or null: one query token per sequence
+  __nv_bfloat16* out;
+  long long q_stride, o_stride;
+  int batch, G, kv_heads, total_q, page_size, max_pages, n_pages;
+  P4Div by_group, by_heads, by_page;
+  float scale_log2;
+  int* status;
+  // Tile of a token, -1 without a page.
+  __device__ __forceinline__ int tile(int b, int token, int head) const {
+    const int lp = by_page(token);
+    if (lp >= max_pages) return -1;
+    const int page = block_table[(long long)b * max_pages + lp];
+    if ((unsigned)page >= (unsigned)n_pages) return -1;
+    return (page * kv_heads + head) * (page_size >> 4) + ((token - lp * page_size) >> 4);
+  }
+};
+
+// A unit: one (sequence, kv head, block of columns).
+struct P4Unit {
+  int b, hkv, col0, n_cols, row0, q_len, kv_len;
+  __device__ __forceinline__ P4Unit(const P4Args& a, int cols, int b_, int y) : b(b_) {
+    const int block = a.by_heads(y);
+    hkv = y - block * a.kv_heads;
+    col0 = block * cols;
+    row0 = a.cu_q ? a.cu_q[b] : b;
+    q_len = a.cu_q ? a.cu_q[b + 1] - row0 : 1;
+    kv_len = a.kv_lens[b];
+    n_cols = min(cols, q_len * a.G - col0);
+  }
+  // Where the value d of column c goes, or null: a row that the output does not have.
+  __device__ __forceinline__ __nv_bfloat16* out(const P4Args& a, int D, int c, int d) const {
+    const int col = col0 + c, qi = a.by_group(col), row = row0 + qi;
+    if (c >= n_cols || (unsigned)row >= (unsigned)a.total_q) return nullptr;
+    return a.out + row * a.o_stride + (hkv * a.G + col - qi * a.G) * D + d;
+  }
+};
+
+// A warp's running state. Thread (r, t) of the warp holds columns 2 t and 2 t + 1 of every block of eight.
+template <int D, int COLS>
+struct P4State {
+  static constexpr int NB = COLS / 8, GR = KvInt4<D>::GROUPS;
+  uint32_t qb[NB][GR][8];                 // B operand: column r
+  float qsum[NB][GR][2], factor[NB][2];   // of columns 2 t, 2 t + 1, as everything below
+  int limit[NB][2];
+  float o[NB][GR][4][4];                  // units of 2^-24 (even i) and 2^-20
+  float z[NB][GR][2], m[NB][2], l[NB][2];
+};
+
+// One chunk: tile u (0, 1) at `at` + u * TILE_BYTES for K, HALF behind for V; tok0: its first token.
+// MASK: some token is not seen by some column (visible: those seen by any), or not held at all.
+template <int D, int COLS, bool MASK>
+__device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at, int tok0, int lane, int visible, uint32_t absent) {
+  using L = KvInt4<D>;
+  using C = P4Cfg<D, COLS>;
+  constexpr int GR = L::GROUPS, NB = COLS / 8;
+  const int r = lane >> 2, t = lane & 3;
+  // ---- scores: rows of the product are key rows 8 j + r of a tile, columns 2 t + c
+  float sc[2][NB][GR][4];                         // [tile][block][group][2 j + c]
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t kw[2][GR][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint8_t* kp = at + u * L::TILE_BYTES + (8 * j + r) * L::ROW + t * (8 * GR);
+      if constexpr (GR == 2) {
+        const uint4 x = *reinterpret_cast<const uint4*>(kp);
+        kw[j][0][0] = x.x; kw[j][0][1] = x.y; kw[j][1][0] = x.z; kw[j][1][1] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(kp);
+        kw[j][0][0] = x.x; kw[j][0][1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w0 = kw[0][g][h], w1 = kw[1][g][h], v0 = __funnelshift_r(w0, w0, 8), v1 = __funnelshift_r(w1, w1, 8);
+        const uint32_t a0 = w0 & 0x00780078u, a1 = w1 & 0x00780078u, a2 = w0 & 0x07800780u, a3 = w1 & 0x07800780u;
+        const uint32_t b0 = v0 & 0x00780078u, b1 = v1 & 0x00780078u, b2 = v0 & 0x07800780u, b3 = v1 & 0x07800780u;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float (&c)[4] = sc[u][nb][g];
+          if (h == 0) c[0] = c[1] = c[2] = c[3] = 0.f;
+          p4_mma(c, a0, a1, a2, a3, s.qb[nb][g][4 * h], s.qb[nb][g][4 * h + 1]);
+          p4_mma(c, b0, b1, b2, b3, s.qb[nb][g][4 * h + 2], s.qb[nb][g][4 * h + 3]);
+        }
+      }
+  }
+  // ---- exponent of the chunk's values: one group of one token per thread and tile
+  float mag = 0.f;
+#pragma unroll
+  for (int u = 0; u < GR; ++u) {                  // (one group a token: the warp's halves take the two tiles)
+    const int tile = GR == 2 ? u : lane >> 4, row = GR == 2 ? lane >> 1 : lane & 15, g = GR == 2 ? lane & 1 : 0;
+    const uint32_t p = *reinterpret_cast<const uint32_t*>(at + C::HALF + tile * L::TILE_BYTES + L::OFF_PAIR + row * L::PAIR + 4 * g);
+    const float top = fmaf(15.f, kv4_scale(p), kv4_low(p));
+    bool use = true;                              // (what every column sees may be infinite: the result is no number then)
+    if (MASK) {                                   // a place behind the context may hold anything
+      const int n = (row & 8) + ((row >> 1) & 3) + ((row & 1) << 2);       // token at this pair row
+      use = kv4_finite(p) && tok0 + 16 * tile + n < visible && !(absent >> tile & 1u);
+    }
+    mag = fmax3(mag, use ? fabsf(top) : 0.f, use ? fabsf(kv4_low(p)) : 0.f);
+  }
+  // p is kept up to 2^8 (and 2^6 more until the reference moves) times the inverse of the largest magnitude, which is at
+  // least 7 scales: p times a scale then stays below 2^13, and is exact to 2^-12 over 24 octaves below. Bounded so that p, its
+  // sum and its product with any value stay within fp32.
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(mag));
+  const float ev = fminf(fmaxf(__uint_as_float(0x4B000000u | (bits >> 23)) - (8388608.f + 127.f), -80.f), 112.f) - 8.f;
+  // ---- online softmax: scores relative to the reference; it moves only when one of them passes it by 2^6
+  float x[2][NB][2][2];                           // [tile][block][j][c]
+  float top = -INFINITY;
+  const int tok_r = tok0 + ((r >> 1) & 3) + ((r & 1) << 2);                // token of key row r of the first tile; row r + 8: 8 on
+  float mm[NB][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) mm[nb][c] = s.m[nb][c] == -INFINITY ? 0.f : s.m[nb][c];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t kq[GR];
+      const uint8_t* kp = at + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + r) * L::PAIR;
+      if constexpr (GR == 2) {
+        const uint2 y = *reinterpret_cast<const uint2*>(kp);
+        kq[0] = y.x; kq[1] = y.y;
+      } else {
+        kq[0] = *reinterpret_cast<const uint32_t*>(kp);
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float v = kv4_low(kq[0]) * s.qsum[nb][0][c];
+          if constexpr (GR == 2) v = fmaf(kv4_low(kq[1]), s.qsum[nb][1][c], v);
+#pragma unroll
+          for (int g = 0; g < GR; ++g) v = fmaf(kv4_scale(kq[g]), sc[u][nb][g][2 * j + c], v);
+          v = fmaf(v, s.factor[nb][c], -mm[nb][c]);
+          if (MASK && (tok_r + 16 * u + 8 * j >= s.limit[nb][c] || (absent >> u & 1u))) v = -INFINITY;
+          x[u][nb][j][c] = v;
+        }
+    }
+  bool first = false;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) first = first || s.m[nb][c] == -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) top = fmax3(top, x[u][nb][j][0], x[u][nb][j][1]);
+  }
+  if (__any_sync(0xffffffffu, first || top + ev > 6.f)) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float mx = fmaxf(fmax3(x[0][nb][0][c], x[0][nb][1][c], x[1][nb][0][c]), x[1][nb][1][c]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        mx += ev;                                 // relative to the reference used so far
+        if (s.m[nb][c] == -INFINITY ? mx > -INFINITY : mx > 0.f) {
+          const float alpha = s.m[nb][c] == -INFINITY ? 0.f : fast_exp2(-mx);
+          s.m[nb][c] = mm[nb][c] + mx;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) x[u][nb][j][c] -= mx;
+          s.l[nb][c] *= alpha;
+#pragma unroll
+          for (int g = 0; g < GR; ++g) {
+            s.z[nb][g][c] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s.o[nb][g][i][c] *= alpha;
+              s.o[nb][g][i][2 + c] *= alpha;
+            }
+          }
+        }
+      }
+  }
+  // ---- weights p scale as the B operand (k = tokens, n = columns): transposed in blocks of eight by eight. Odd key rows
+  // are the tokens that enter with the complement of their codes.
+  uint32_t pb[2][NB][GR][2];
+  const uint32_t flip = (uint32_t)(r & 1) << 31;
+  const float whole = (r & 1) ? -15.f : 0.f;      // low + 15 scale, the scale's sign already turned
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t vq[GR];
+      const uint8_t* vp = at + C::HALF + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + r) * L::PAIR;
+      if constexpr (GR == 2) {
+        const uint2 y = *reinterpret_cast<const uint2*>(vp);
+        vq[0] = y.x; vq[1] = y.y;
+      } else {
+        vq[0] = *reinterpret_cast<const uint32_t*>(vp);
+      }
+      float w[GR], b[GR];
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        w[g] = __uint_as_float(vq[g] << 16 ^ flip);
+        b[g] = fmaf(whole, w[g], kv4_low(vq[g]));
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float p0 = fast_exp2(x[u][nb][j][0]), p1 = fast_exp2(x[u][nb][j][1]);
+        s.l[nb][0] += p0;
+        s.l[nb][1] += p1;
+        // a token the column does not see may hold anything, behind the sequence's end too: it is left out, not
+        // multiplied by zero
+        const bool s0 = !MASK || x[u][nb][j][0] != -INFINITY, s1 = !MASK || x[u][nb][j][1] != -INFINITY;
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          if (MASK) {
+            s.z[nb][g][0] += s0 ? p0 * b[g] : 0.f;
+            s.z[nb][g][1] += s1 ? p1 * b[g] : 0.f;
+          } else {
+            s.z[nb][g][0] = fmaf(p0, b[g], s.z[nb][g][0]);
+            s.z[nb][g][1] = fmaf(p1, b[g], s.z[nb][g][1]);
+          }
+          pb[u][nb][g][j] = p4_transpose(p4_half2(s0 ? p0 * w[g] : 0.f, s1 ? p1 * w[g] : 0.f));
+        }
+      }
+    }
+  // ---- values: the A operand holds values x tokens (t, t + 4, t + 8, t + 12: those of key rows 2 t, 2 t + 1 and 8 on)
+  const int chunk = r ^ ((t >> 1) << 2);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t vw[2][2][GR];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint8_t* vp = at + C::HALF + u * L::TILE_BYTES + (t + 4 * (2 * j + e)) * L::ROW + chunk * (4 * GR);
+        if constexpr (GR == 2) {
+          const uint2 w = *reinterpret_cast<const uint2*>(vp);
+          vw[j][e][0] = w.x; vw[j][e][1] = w.y;
+        } else {
+          vw[j][e][0] = *reinterpret_cast<const uint32_t*>(vp);
+        }
+      }
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      // halves of the two tokens' words side by side: lo holds values 0, 2, 4, 6 and hi values 1, 3, 5, 7 of both; the
+      // second token's codes enter as 15 - code
+      const uint32_t n0 = ~vw[0][1][g], n1 = ~vw[1][1][g];
+      uint32_t lo0 = __byte_perm(vw[0][0][g], n0, 0x5410), hi0 = __byte_perm(vw[0][0][g], n0, 0x7632);
+      uint32_t lo1 = __byte_perm(vw[1][0][g], n1, 0x5410), hi1 = __byte_perm(vw[1][0][g], n1, 0x7632);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i == 2) {
+          lo0 >>= 8; hi0 >>= 8; lo1 >>= 8; hi1 >>= 8;
+        }
+        const uint32_t mask = (i & 1) ? 0x00F000F0u : 0x000F000Fu;
+        const uint32_t a0 = lo0 & mask, a1 = hi0 & mask, a2 = lo1 & mask, a3 = hi1 & mask;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) p4_mma(s.o[nb][g][i], a0, a1, a2, a3, pb[u][nb][g][0], pb[u][nb][g][1]);
+      }
+    }
+  }
+}
+
+// Queries of a unit into the state. The B operand: column r of every block; word h of group g holds values 64 g + 16 t + 8 h ..
+template <int D, int COLS>
+__device__ __forceinline__ void p4_queries(P4State<D, COLS>& s, const P4Args& a, const P4Unit& u, int lane) {
+  constexpr int GR = KvInt4<D>::GROUPS, NB = COLS / 8;
+  const int r = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int col = u.col0 + nb * 8 + r, qi = a.by_group(col);
+    const bool live = nb * 8 + r < u.n_cols && (unsigned)(u.row0 + qi) < (unsigned)a.total_q;
+    const int limit = live ? min(u.kv_len, u.kv_len - u.q_len + qi + 1) : 0;
+    const __nv_bfloat16* qp = a.q + (u.row0 + qi) * a.q_stride + (u.hkv * a.G + col - qi * a.G) * D + 16 * t;
+    uint32_t raw[GR][8];
+    __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (live) v = *reinterpret_cast<const uint4*>(qp + 64 * g + 8 * h);
+        raw[g][4 * h] = v.x; raw[g][4 * h + 1] = v.y; raw[g][4 * h + 2] = v.z; raw[g][4 * h + 3] = v.w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&raw[g][4 * h + e])));
+      }
+    top = __hmax2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __hmax2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float big = fmaxf(__low2float(top), __high2float(top));
+    // the column's largest value in 2^14 .. 2^15
+    const int eq = big > 0.f ? max(-100, min(113, (int)(__float_as_uint(big) >> 23) - 127 - 14)) : 0;
+    const float down = p4_pow2(-eq), down4 = p4_pow2(-eq - 4);
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = (e & 1) ? down4 : down;
+        s.qb[nb][g][e] = p4_half2(kv4_scale(raw[g][e]) * f, kv4_low(raw[g][e]) * f);     // (both halves of a word)
+      }
+      // sum(q_g) in the scores' units of 2^-21: the product with a key whose codes are all one
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) p4_mma(c, 0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u, s.qb[nb][g][e], s.qb[nb][g][e + 1]);
+      s.qsum[nb][g][0] = c[0];
+      s.qsum[nb][g][1] = c[1];
+      s.z[nb][g][0] = s.z[nb][g][1] = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s.o[nb][g][q][0] = s.o[nb][g][q][1] = s.o[nb][g][q][2] = s.o[nb][g][q][3] = 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {                 // what concerns columns 2 t + c sits in the threads of r = 2 t + c
+      const int from = 8 * t + 4 * c;
+      s.limit[nb][c] = __shfl_sync(0xffffffffu, limit, from);
+      s.factor[nb][c] = a.scale_log2 * 0x1p21f * p4_pow2(__shfl_sync(0xffffffffu, eq, from));
+      s.m[nb][c] = -INFINITY;
+      s.l[nb][c] = 0.f;
+    }
+  }
+}
+
+// The state's sums, complete over the warp: into `out` (whole) or as a part to w_acc [COLS][D] with references and row sums
+// in ml [2][COLS]. Thread (r, t) has columns 2 t and 2 t + 1 of every block, values 64 g + 8 r + (0 .. 7).
+template <int D, int COLS>
+__device__ __forceinline__ void p4_result(const P4State<D, COLS>& s, const P4Args& a, const P4Unit& u, bool whole, float* w_acc, float* ml,
+                                          int lane) {
+  constexpr int GR = KvInt4<D>::GROUPS, NB = COLS / 8;
+  const int r = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int cc = nb * 8 + 2 * t + c;
+      float l = s.l[nb][c];
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;      // nothing visible: zeros
+      if (!whole && r == 0) {
+        ml[cc] = s.m[nb][c];
+        ml[COLS + cc] = l;
+      }
+      __nv_bfloat16* dst = whole ? u.out(a, D, cc, 8 * r) : nullptr;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        float z = s.z[nb][g][c];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+        float v[8];                               // out of their units, with the offset sum
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float unit = (q & 1) ? 0x1p20f : 0x1p24f;
+          v[2 * q] = fmaf(s.o[nb][g][q][c], unit, z) * inv;
+          v[2 * q + 1] = fmaf(s.o[nb][g][q][2 + c], unit, z) * inv;
+        }
+        if (!whole) {
+          float* p = w_acc + cc * D + 64 * g + 8 * r;
+          *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else if (dst) {
+          *reinterpret_cast<uint4*>(dst + 64 * g) =
+              make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        }
+      }
+    }
+}
+
+// A warp's chunks 0 .. mine - 1 through its ring. locate(i) gives the tile of the lane's half (lane & 1) of chunk i: -1 without
+// a page (reported, left out), -2 behind the keys.
+template <int D, int COLS>
+struct P4Feed {
+  using L = KvInt4<D>;
+  using C = P4Cfg<D, COLS>;
+  const P4Args& a;
+  uint8_t* ring;
+  uint64_t* full;
+  int lane, mine;
+  int ids = -2, ids_next = -2;    // lane l: tile l % 2 of chunk 16 n + l / 2 for the block n being issued, and of the next one
+  uint32_t absent = 0u, parity = 0u;   // bits 2 s, 2 s + 1: tiles of stage s that were not loaded
+  int st = 0;                     // stage of the next chunk to use
+  template <class F>
+  __device__ __forceinline__ void issue(int i, int stage, const F& locate) {
+    if ((i & 15) == 0) ids = i == 0 ? locate(lane >> 1) : ids_next;
+    if ((i & 15) == 4 && i + 12 < mine) ids_next = locate(i + 12 + (lane >> 1));
+    const int id = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + (lane & 1));
+    const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 3u;
+    absent = (absent & ~(3u << (2 * stage))) | gone << (2 * stage);
+    if (lane == 0) {
+      if (gone == 3u) mbar_arrive(&full[stage]);
+      else mbar_arrive_expect_tx(&full[stage], gone ? C::STAGE / 2 : C::STAGE);
+    }
+    if (lane < 4) {               // one copy each: tile lane % 2, K (lane < 2) or V
+      if (id >= 0)
+        p4_bulk_load(smem_u32(ring) + stage * C::STAGE + ((lane & 2) ? C::HALF : 0) + (lane & 1) * L::TILE_BYTES,
+                     ((lane & 2) ? a.v_cache : a.k_cache) + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[stage]);
+      else if (id == -1 && a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (92 << 16));
+    }
+  }
+  // Waits for chunk i, with the next one under way. False: the wait ran out.
+  template <class F>
+  __device__ __forceinline__ bool wait(int i, volatile int* abort_flag, const F& locate) {
+    // the stage read in the step before is free now: every value read from it has gone through a product
+    if (i + 1 < mine) issue(i + 1, st ^ 1, locate);
+    if (__all_sync(0xffffffffu, mbar_try_wait(&full[st], parity))) return true;
+    const bool ok = mbar_wait(&full[st], parity, abort_flag, a.status, 93);
+    return __all_sync(0xffffffffu, ok);
+  }
+  __device__ __forceinline__ const uint8_t* at() const { return ring + st * C::STAGE; }
+  __device__ __forceinline__ uint32_t gone() const { return absent >> (2 * st) & 3u; }
+  __device__ __forceinline__ void next() {
+    __syncwarp();
+    parity ^= (uint32_t)st;
+    st ^= 1;
+  }
+  // After a wait that ran out at chunk i: copies in flight land before the ring's memory goes away.
+  __device__ __forceinline__ void drain(int i) {
+    for (int k = 0; k < C::STAGES && i + k < mine; ++k) {
+      mbar_drain(&full[st], parity);
+      parity ^= (uint32_t)st;
+      st ^= 1;
+    }
+  }
+};
+static_assert(P4Cfg<128, 8>::STAGES == 2, "P4Feed alternates between two stages");
+
+template <int D, int COLS>
+__device__ __forceinline__ void p4_step(P4State<D, COLS>& s, const P4Feed<D, COLS>& feed, const P4Unit& u, const P4Args& a, int chunk) {
+  const int tok = chunk * P4_CHUNK, to_some = min(u.kv_len, u.kv_len - u.q_len + a.by_group(u.col0 + u.n_cols - 1) + 1),
+            to_all = min(u.kv_len, u.kv_len - u.q_len + a.by_group(u.col0) + 1);
+  const uint32_t gone = feed.gone();
+  if (gone == 0u && tok + P4_CHUNK <= to_all) p4_chunk<D, COLS, false>(s, feed.at(), tok, feed.lane, to_some, 0u);
+  else p4_chunk<D, COLS, true>(s, feed.at(), tok, feed.lane, to_some, gone);
+}
+
+// Joins the parts of a unit that shared memory holds (bits of `parts`), column c, values d .. d + 3: sums, and the column's
+// reference and row sum.
+template <int D, int COLS, class At>
+__device__ __forceinline__ float4 p4_join(uint32_t parts, const float* ml, const At& at, int c, int d, float& M, float& l) {
+  M = -INFINITY;
+  for (uint32_t w = parts; w; w &= w - 1) M = fmaxf(M, ml[(__ffs(w) - 1) * 2 * COLS + c]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f;
+  for (uint32_t w = parts; w; w &= w - 1) {
+    const int k = __ffs(w) - 1;
+    const float lk = ml[(2 * k + 1) * COLS + c];
+    if (lk == 0.f) continue;                      // nothing seen (a NaN is not nothing)
+    const float e = fast_exp2(ml[2 * k * COLS + c] - M);
+    const float4 v = *reinterpret_cast<const float4*>(at(k) + c * D + d);
+    l = fmaf(e, lk, l);
+    acc.x = fmaf(e, v.x, acc.x);
+    acc.y = fmaf(e, v.y, acc.y);
+    acc.z = fmaf(e, v.z, acc.z);
+    acc.w = fmaf(e, v.w, acc.w);
+  }
+  return acc;
+}
+__device__ __forceinline__ void p4_store(__nv_bfloat16* dst, const float4& v, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (dst) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
+}
+
+// ------------------------------------------------------------------------------------------------ few units
+// One unit per cluster, whose CTAs split its chunks and join their sums through distributed shared memory: one launch, which
+// counts where the whole call takes a few microseconds.
+__device__ __forceinline__ uint32_t p4_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void p4_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t p4_mapa(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float p4_ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 p4_ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int D, int COLS>
+struct P4SmemCluster {
+  using C = P4Cfg<D, COLS>;
+  static constexpr int OFF_CTA = P4_WARPS * C::WARP_BYTES;                  // the CTA's sums
+  static constexpr int OFF_ML = OFF_CTA + C::PART;                          // [warps][m, l][COLS]
+  static constexpr int OFF_CML = OFF_ML + P4_WARPS * 2 * COLS * 4;          // of the CTA: [m, l][COLS]
+  static constexpr int OFF_BAR = OFF_CML + 2 * COLS * 4;
+  static constexpr int OFF_FLAG = OFF_BAR + P4_WARPS * C::STAGES * 8;
+  static constexpr int BYTES = OFF_FLAG + 16;
+};
+
+template <int D, int COLS>
+__global__ void __launch_bounds__(P4_THREADS, COLS == 8 ? 3 : 2)
+paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
+  using C = P4Cfg<D, COLS>;
+  using S = P4SmemCluster<D, COLS>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, splits = gridDim.z;
+  const P4Unit u(a, COLS, blockIdx.x, blockIdx.y);
+  if (u.n_cols <= 0) return;                      // the same for every CTA of the cluster
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * C::STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::OFF_FLAG);
+  float* s_ml = reinterpret_cast<float*>(smem + S::OFF_ML);
+  float* s_cml = reinterpret_cast<float*>(smem + S::OFF_CML);
+  float* s_cta = reinterpret_cast<float*>(smem + S::OFF_CTA);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) {
+    for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int n = (max(u.kv_len, 0) + P4_CHUNK - 1) / P4_CHUNK, per = (n + splits - 1) / splits;
+  const int chunk0 = blockIdx.z * per + warp, end = min(n, (int)blockIdx.z * per + per);
+  const int mine = max(0, (end - chunk0 + P4_WARPS - 1) / P4_WARPS);        // chunk0, + 4, ...
+  const auto locate = [&](int i) {
+    const int token = (chunk0 + P4_WARPS * i) * P4_CHUNK + (lane & 1) * 16;
+    return i < mine && token < u.kv_len ? a.tile(u.b, token, u.hkv) : -2;
+  };
+  P4Feed<D, COLS> feed{a, smem + warp * C::WARP_BYTES, full, lane, mine};
+  if (mine > 0) feed.issue(0, 0, locate);
+  P4State<D, COLS> s;
+  p4_queries(s, a, u, lane);
+  bool ok = true;
+  for (int i = 0; i < mine; ++i) {
+    ok = feed.wait(i, abort_flag, locate);
+    if (!ok) {
+      feed.drain(i);
+      break;
+    }
+    p4_step(s, feed, u, a, chunk0 + P4_WARPS * i);
+    feed.next();
+  }
+  p4_result(s, a, u, false, reinterpret_cast<float*>(feed.ring), s_ml + warp * 2 * COLS, lane);
+  __syncwarp();
+  if (!ok) s_ml[warp * 2 * COLS + COLS + lane % COLS] = 0.f;                // counts as nothing seen
+  __syncthreads();
+  for (int i = threadIdx.x; i < COLS * D / 4; i += P4_THREADS) {
+    const int c = 4 * i / D, d = 4 * i % D;
+    float M, l;
+    const float4 v = p4_join<D, COLS>((1u << P4_WARPS) - 1u, s_ml, [&](int k) { return reinterpret_cast<const float*>(smem + k * C::WARP_BYTES); }, c, d, M, l);
+    *reinterpret_cast<float4*>(s_cta + 4 * i) = v;
+    if (d == 0) {
+      s_cml[c] = M;
+      s_cml[COLS + c] = l;
+    }
+  }
+  p4_cluster_sync();
+  // every CTA writes a share of the block's outputs, four values a thread
+  const int share = (COLS * D / 4 + splits - 1) / splits, rank = p4_rank();
+  for (int i = rank * share + threadIdx.x; i < min(COLS * D / 4, (rank + 1) * share); i += P4_THREADS) {
+    const int c = 4 * i / D, d = 4 * i % D;
+    if (c >= u.n_cols) break;
+    const uint32_t m_at = smem_u32(s_cml + c), l_at = smem_u32(s_cml + COLS + c), v_at = smem_u32(s_cta + 4 * i);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f, M = -INFINITY;
+#pragma unroll 4
+    for (int p = 0; p < splits; ++p) {
+      const float m = p4_ld_cluster(p4_mapa(m_at, p)), lp = p4_ld_cluster(p4_mapa(l_at, p));
+      const float4 v = p4_ld_cluster4(p4_mapa(v_at, p));
+      if (lp == 0.f) continue;
+      const float Mn = fmaxf(M, m), e0 = M == -INFINITY ? 0.f : fast_exp2(M - Mn), e1 = fast_exp2(m - Mn);
+      acc.x = fmaf(e1, v.x, acc.x * e0);
+      acc.y = fmaf(e1, v.y, acc.y * e0);
+      acc.z = fmaf(e1, v.z, acc.z * e0);
+      acc.w = fmaf(e1, v.w, acc.w * e0);
+      l = fmaf(e1, lp, l * e0);
+      M = Mn;
+    }
+    p4_store(u.out(a, D, c, d), acc, l);
+  }
+  p4_cluster_sync();                              // nobody leaves while a peer still reads its shared memory
+}
+
+// ------------------------------------------------------------------------------------------------ many units
+// A unit has n = ceil(keys / 32) chunks. All chunks of all units stand in one line, units of a sequence side by side, and every
+// warp takes an equal stretch of it, so that ragged batches and any number of units load the GPU evenly (with equal splits
+// of each unit, 148 SMs x 16 warps were filled to three quarters: 8 x 32768 tokens and 5 kv heads took 73 us, 60 this way). A
+// warp that meets a whole unit writes its outputs; parts of units go to shared memory and are joined by the CTA, and what
+// crosses a CTA's border goes to a scratch buffer of the call (two slots a CTA) and is joined by p4_merge_kernel.
+struct P4Line {
+  int batch, G, kv_heads, cols;
+  const int* kv_lens;
+  const int* cu_q;
+  __device__ __forceinline__ int chunks(int b) const { return (max(kv_lens[b], 0) + P4_CHUNK - 1) / P4_CHUNK; }
+  __device__ __forceinline__ int units(int b) const {
+    return kv_heads * (cu_q ? (max(cu_q[b + 1] - cu_q[b], 0) * G + cols - 1) / cols : (G + cols - 1) / cols);
+  }
+  __device__ __forceinline__ int size(int b) const { return b < batch ? chunks(b) * units(b) : 0; }
+};
+// Equal stretches: the first `rem` of them one chunk longer.
+struct P4Share {
+  int per, rem;
+  __device__ __forceinline__ P4Share(int total, int workers) : per(total / workers), rem(total - total / workers * workers) {}
+  __device__ __forceinline__ int start(int worker) const { return worker * per + min(worker, rem); }
+  __device__ __forceinline__ int worker(int place) const {       // whose stretch holds it
+    const int longer = rem * (per + 1);
+    return place < longer ? place / (per + 1) : rem + (place - longer) / max(per, 1);
+  }
+};
+// What a warp knows of the line: the size of sequence `lane` (of the first 32) and the sum of those up to it.
+struct P4Scan {
+  int size, sum, total;
+  __device__ __forceinline__ P4Scan(const P4Line& line, int lane) {
+    size = line.size(lane);
+    sum = size;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    total = __shfl_sync(0xffffffffu, sum, 31);
+    for (int b0 = 32; b0 < line.batch; b0 += 32) total += __reduce_add_sync(0xffffffffu, (unsigned)line.size(b0 + lane));
+  }
+  // The sequence that holds a place below the total, and where it begins.
+  __device__ __forceinline__ int find(const P4Line& line, int place, int lane, int& begin) const {
+    int base = 0, n = size, up = sum;
+    for (int b0 = 0;; b0 += 32) {
+      const unsigned past = __ballot_sync(0xffffffffu, base + up > place);
+      if (past || b0 + 32 >= line.batch) {
+        const int l = past ? __ffs(past) - 1 : 31;
+        begin = base + __shfl_sync(0xffffffffu, up - n, l);
+        return b0 + l;
+      }
+      base += __shfl_sync(0xffffffffu, up, 31);
+      n = line.size(b0 + 32 + lane);
+      up = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += v;
+      }
+    }
+  }
+  // Where sequence b begins.
+  __device__ __forceinline__ int begin(const P4Line& line, int b, int lane) const {
+    if (b < 32) return __shfl_sync(0xffffffffu, sum - size, b);
+    int s = __shfl_sync(0xffffffffu, sum, 31);
+    for (int b0 = 32; b0 < b; b0 += 32) s += __reduce_add_sync(0xffffffffu, (unsigned)(b0 + lane < b ? line.size(b0 + lane) : 0));
+    return s;
+  }
+};
+
+template <int D, int COLS>
+struct P4SmemLine {
+  using C = P4Cfg<D, COLS>;
+  static constexpr int OFF_HEAD = P4_WARPS * C::WARP_BYTES;                 // head parts; tail parts lie in the drained rings
+  static constexpr int OFF_ML = OFF_HEAD + P4_WARPS * C::PART;              // [warps][head, tail][m, l][COLS]
+  static constexpr int OFF_UNIT = OFF_ML + P4_WARPS * 4 * COLS * 4;         // [warps][head, tail] int4: sequence, unit, begins, ends
+  static constexpr int OFF_LEAD = OFF_UNIT + P4_WARPS * 2 * 16;             // int2: sequence and unit of the CTA's first chunk
+  static constexpr int OFF_BAR = OFF_LEAD + 16;
+  static constexpr int OFF_FLAG = OFF_BAR + P4_WARPS * C::STAGES * 8;
+  static constexpr int BYTES = OFF_FLAG + 16;
+};
+
+template <int D, int COLS>
+__global__ void __launch_bounds__(P4_THREADS, COLS == 8 ? 4 : 2)
+paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict__ scratch) {
+  using C = P4Cfg<D, COLS>;
+  using S = P4SmemLine<D, COLS>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * C::STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::OFF_FLAG);
+  float* s_ml = reinterpret_cast<float*>(smem + S::OFF_ML);
+  int4* s_unit = reinterpret_cast<int4*>(smem + S::OFF_UNIT);
+  int2* s_lead = reinterpret_cast<int2*>(smem + S::OFF_LEAD);
+  // the merge may start as soon as there is room; it waits for this grid's end before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) {
+    for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+  }
+  if (lane < 2) s_unit[warp * 2 + lane] = make_int4(-1, 0, 0, 0);
+  __syncthreads();
+
+  const P4Line line{a.batch, a.G, a.kv_heads, COLS, a.kv_lens, a.cu_q};
+  const P4Scan scan(line, lane);
+  const P4Share share(scan.total, gridDim.x * P4_WARPS);
+  const int worker = blockIdx.x * P4_WARPS + warp;
+  const int f0 = share.start(worker), mine = share.start(worker + 1) - f0;
+  int begin = 0, b = 0, n = 1, left_units = 0, y = 0, chunk = 0;
+  if (mine > 0) {
+    b = scan.find(line, f0, lane, begin);
+    n = line.chunks(b);
+    y = (f0 - begin) / n;
+    chunk = f0 - begin - y * n;
+    left_units = line.units(b) - y;
+    if (warp == 0 && lane == 0) *s_lead = make_int2(b, y);       // (where the first warp has nothing, no warp has)
+  }
+  // Every lane walks the line from where it was.
+  int lb = b, ln = n, lbegin = begin, lsize = mine > 0 ? line.size(b) : 0;
+  const auto locate = [&](int i) {
+    if (i >= mine) return -2;
+    const int f = f0 + i;
+    while (f >= lbegin + lsize) {
+      lbegin += lsize;
+      lsize = line.size(++lb);
+      ln = line.chunks(lb);
+    }
+    const int at = f - lbegin, ly = at / ln, token = (at - ly * ln) * P4_CHUNK + (lane & 1) * 16;
+    return token < a.kv_lens[lb] ? a.tile(lb, token, ly - a.by_heads(ly) * a.kv_heads) : -2;
+  };
+  P4Feed<D, COLS> feed{a, smem + warp * C::WARP_BYTES, full, lane, mine};
+  if (mine > 0) feed.issue(0, 0, locate);
+  P4State<D, COLS> s;
+  bool ok = true;
+  int i = 0;
+  while (i < mine) {
+    // ---- one unit, or the part of it in this warp's stretch
+    const P4Unit u(a, COLS, b, y);
+    const bool begins = chunk == 0;
+    p4_queries(s, a, u, lane);
+    for (const int end = i + min(n - chunk, mine - i); i < end; ++i, ++chunk) {
+      ok = feed.wait(i, abort_flag, locate);
+      if (!ok) break;
+      p4_step(s, feed, u, a, chunk);
+      feed.next();
+    }
+    if (!ok) {
+      feed.drain(i);
+      break;
+    }
+    const bool ends = chunk == n;
+    const int slot = ends ? 0 : 1;                // (a part that does not end its unit is the warp's last)
+    p4_result(s, a, u, begins && ends, reinterpret_cast<float*>(slot ? feed.ring : smem + S::OFF_HEAD + warp * C::PART),
+              s_ml + (warp * 2 + slot) * 2 * COLS, lane);
+    if (!(begins && ends) && lane == 0) s_unit[warp * 2 + slot] = make_int4(b, y, begins ? 1 : 0, ends ? 1 : 0);
+    if (ends) {
+      chunk = 0;
+      ++y;
+      if (--left_units == 0 && i < mine) {
+        do {
+          ++b;
+          n = line.chunks(b);
+          left_units = line.units(b);
+        } while (n == 0 || left_units == 0);      // (the line has mine chunks: some later sequence holds the next)
+        y = 0;
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---- parts of one unit follow each other in the order (warp, head / tail): joined by the CTA
+  const auto at = [&](int k) {
+    return reinterpret_cast<const float*>((k & 1) ? smem + (k >> 1) * C::WARP_BYTES : smem + S::OFF_HEAD + (k >> 1) * C::PART);
+  };
+  for (int p = 0; p < 2 * P4_WARPS;) {
+    const int4 g = s_unit[p];
+    if (g.x < 0) {
+      ++p;
+      continue;
+    }
+    uint32_t parts = 1u << p;
+    int e = p + 1, last_end = g.w;
+    for (; e < 2 * P4_WARPS; ++e) {
+      const int4 v = s_unit[e];
+      if (v.x < 0) continue;
+      if (v.x != g.x || v.y != g.y) break;
+      parts |= 1u << e;
+      last_end = v.w;
+    }
+    p = e;
+    const bool whole = g.z && last_end;
+    const P4Unit u(a, COLS, g.x, g.y);
+    // the unit that holds the CTA's first chunk goes to the first slot
+    float* dst = scratch + (blockIdx.x * 2 + (s_lead->x == g.x && s_lead->y == g.y ? 0 : 1)) * COLS * (D + 2);
+    for (int k = threadIdx.x; k < u.n_cols * D / 4; k += P4_THREADS) {
+      const int c = 4 * k / D, d = 4 * k % D;
+      float M, l;
+      const float4 v = p4_join<D, COLS>(parts, s_ml, at, c, d, M, l);
+      if (whole) {
+        p4_store(u.out(a, D, c, d), v, l);
+      } else {
+        *reinterpret_cast<float4*>(dst + 4 * k) = v;
+        if (d == 0) {
+          dst[COLS * D + c] = M;
+          dst[COLS * D + COLS + c] = l;
+        }
+      }
+    }
+  }
+}
+
+// One CTA per unit and 32 of its values: joins the parts of a unit that lies in several CTAs' stretches; zeros for a sequence
+// without keys. First the weights of all parts (one thread per part and column), then the sums with every load in flight.
+constexpr int P4_MERGE = 64;      // parts whose weights are held at a time
+template <int D, int COLS>
+__global__ void __launch_bounds__(COLS * 8)
+p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scratch, int ctas) {
+  constexpr int PART = COLS * (D + 2);
+  __shared__ float s_w[P4_MERGE][COLS], s_lw[P4_MERGE][COLS], s_m[COLS];
+  __shared__ int s_at[P4_MERGE];
+  const int b = blockIdx.x, y = blockIdx.y, lane = threadIdx.x & 31;
+  const P4Line line{a.batch, a.G, a.kv_heads, COLS, a.kv_lens, a.cu_q};
+  const P4Scan scan(line, lane);
+  const P4Share share(scan.total, ctas * P4_WARPS);
+  const int u0 = scan.begin(line, b, lane) + y * line.chunks(b), n = line.chunks(b);
+  const bool here = y < line.units(b);
+  int c0 = 0, c1 = -1;
+  if (n > 0 && here) {
+    c0 = share.worker(u0) / P4_WARPS;
+    c1 = share.worker(u0 + n - 1) / P4_WARPS;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");             // every CTA, so that this grid ends behind the one before
+  if (!here || (n > 0 && c0 == c1)) return;       // no such unit, or written by that CTA
+  const P4Unit u(a, COLS, b, y);
+  const int c = threadIdx.x >> 3, d = blockIdx.z * 32 + (threadIdx.x & 7) * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f, M = -INFINITY;
+  for (int k0 = c0; k0 <= c1; k0 += P4_MERGE) {   // (a unit of more than 64 CTAs: joined in turns)
+    const int parts = min(P4_MERGE, c1 - k0 + 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i < parts * COLS; i += COLS * 8) {
+      const int p = i / COLS, cc = i % COLS, k = k0 + p;
+      // the first CTA has the unit in its first slot only where the unit holds the first chunk of its stretch; with fewer
+      // chunks than warps a CTA in between may have an empty stretch
+      const int first = share.start(k * P4_WARPS);
+      const bool empty = first == share.start((k + 1) * P4_WARPS);
+      const int at = (2 * k + (u0 > first ? 1 : 0)) * PART;
+      if (cc == 0) s_at[p] = empty ? -1 : at;
+      s_w[p][cc] = empty ? -INFINITY : scratch[at + COLS * D + cc];
+      s_lw[p][cc] = empty ? 0.f : scratch[at + COLS * D + COLS + cc];
+    }
+    __syncthreads();
+    if (threadIdx.x < COLS) {
+      float m = -INFINITY;
+      for (int p = 0; p < parts; ++p)
+        if (s_lw[p][threadIdx.x] != 0.f) m = fmaxf(m, s_w[p][threadIdx.x]);    // nothing seen is left out, a NaN is not
+      s_m[threadIdx.x] = m;
+    }
+    __syncthreads();
+    if (c < u.n_cols) {
+      const float Mn = fmaxf(M, s_m[c]), e = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
+      acc.x *= e; acc.y *= e; acc.z *= e; acc.w *= e; l *= e;
+      M = Mn;
+#pragma unroll 8
+      for (int p = 0; p < parts; ++p) {
+        const float lw = s_lw[p][c];
+        const float4 v = lw != 0.f ? *reinterpret_cast<const float4*>(scratch + s_at[p] + c * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float w = lw != 0.f ? fast_exp2(s_w[p][c] - M) : 0.f;
+        l = fmaf(w, lw, l);
+        acc.x = fmaf(w, v.x, acc.x);
+        acc.y = fmaf(w, v.y, acc.y);
+        acc.z = fmaf(w, v.z, acc.z);
+        acc.w = fmaf(w, v.w, acc.w);
+      }
+    }
+  }
+  p4_store(u.out(a, D, c, d), acc, l);
+}
+
+// A kernel's limits, raised once per device.
+template <typename K>
+void p4_configure(K kern, int smem, bool cluster, unsigned long long& seen) {
+  int dev = 0;
+  MB_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64 && (seen >> dev & 1ull)) return;
+  MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (cluster) MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (dev < 64) seen |= 1ull << dev;
+}
+
+// How a call runs, by its sizes (the table's width stands for the contexts, which only the device knows).
+struct P4Plan {
+  int cols, ctas, splits;         // splits > 0: clusters; else stretches of the line over that many CTAs
+  long long blocks, units, chunks;
+};
+P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, long long max_tokens) {
+  P4Plan p;
+  p.cols = (long long)max_q * G > 8 ? 16 : 8;
+  p.blocks = ((long long)max_q * G + p.cols - 1) / p.cols;
+  p.units = (long long)batch * kv_heads * p.blocks;
+  p.chunks = std::max(1LL, (max_tokens + P4_CHUNK - 1) / P4_CHUNK);
+  const long long resident = (p.cols == 8 ? 4LL : 2LL) * sm_count();
+  p.ctas = (int)std::max(1LL, std::min(resident, (p.units * p.chunks + P4_WARPS - 1) / P4_WARPS));
+  // A cluster per unit while sixteen CTAs a unit fit beside each other and no warp gets more than eight chunks.
+  const long long want = std::min(16LL, (p.chunks + P4_WARPS - 1) / P4_WARPS);
+  p.splits = p.units * want <= resident && p.chunks <= 8 * P4_WARPS * want ? (int)want : 0;
+  return p;
+}
+
+template <int D, int COLS>
+void p4_launch(P4Args& a, const P4Plan& plan, float* scratch, cudaStream_t stream) {
+  MB_REQUIRE(plan.blocks * a.kv_heads <= 65535, "paged attention over 4-bit pages: too many query columns for one launch");
+  MB_REQUIRE(plan.units * plan.chunks < (1LL << 31), "paged attention over 4-bit pages: too many chunks for one launch");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (plan.splits > 0) {
+    static unsigned long long seen = 0;
+    p4_configure(paged_attn_int4_cluster_kernel<D, COLS>, P4SmemCluster<D, COLS>::BYTES, true, seen);
+    cfg.gridDim = dim3(a.batch, (unsigned)(plan.blocks * a.kv_heads), plan.splits);
+    cfg.blockDim = dim3(P4_THREADS);
+    cfg.dynamicSmemBytes = P4SmemCluster<D, COLS>::BYTES;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = plan.splits;
+    MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_attn_int4_cluster_kernel<D, COLS>, a));
+    count_launch();
+    return;
+  }
+  static unsigned long long seen = 0;
+  p4_configure(paged_attn_int4_line_kernel<D, COLS>, P4SmemLine<D, COLS>::BYTES, false, seen);
+  paged_attn_int4_line_kernel<D, COLS><<<plan.ctas, P4_THREADS, P4SmemLine<D, COLS>::BYTES, stream>>>(a, scratch);
+  count_launch();
+  check_launch();
+  cfg.gridDim = dim3(a.batch, (unsigned)(plan.blocks * a.kv_heads), D / 32);
+  cfg.blockDim = dim3(COLS * 8);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, p4_merge_kernel<D, COLS>, a, (const float*)scratch, plan.ctas));
+  count_launch();
+}
+
+}  // namespace
+
+long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads) {
+  const P4Plan p = p4_plan(batch, max_q, heads / c.kv_heads, c.kv_heads, (long long)c.max_pages * c.page_size);
+  return p.splits > 0 ? 0 : 2LL * p.ctas * p.cols * (c.head_dim + 2) * 4;
+}
+
+void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
+                    long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,
+                    cudaStream_t stream) {
+  const int G = heads / c.kv_heads;
+  const P4Plan plan = p4_plan(batch, max_q, G, c.kv_heads, (long long)c.max_pages * c.page_size);
+  P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, kv_lens, cu_q, (__nv_bfloat16*)out,
+           q_stride, o_stride, batch, G, c.kv_heads, total_q, c.page_size, c.max_pages, c.n_pages,
+           p4_div(G), p4_div(c.kv_heads), p4_div(c.page_size), scale * 1.4426950408889634f, status};
+  float* scratch = (float*)workspace;
+  if (c.head_dim == 128) {
+    if (plan.cols == 16) p4_launch<128, 16>(a, plan, scratch, stream);
+    else p4_launch<128, 8>(a, plan, scratch, stream);
+  } else {
+    if (plan.cols == 16) p4_launch<64, 16>(a, plan, scratch, stream);
+    else p4_launch<64, 8>(a, plan, scratch, stream);
+  }
+}
+
+}  // namespace mb
