@@ -49,10 +49,17 @@ struct P4Cfg {
 };
 
 __device__ __forceinline__ void p4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                "{%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same into a fresh accumulator.
+__device__ __forceinline__ void p4_mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void p4_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -109,6 +116,7 @@ struct P4Args {
 // A unit: one (sequence, kv head, block of columns).
 struct P4Unit {
   int b, hkv, col0, n_cols, row0, q_len, kv_len;
+  int to_some, to_all;      // tokens that some column sees, and that all see
   __device__ __forceinline__ P4Unit(const P4Args& a, int cols, int b_, int y) : b(b_) {
     const int block = a.by_heads(y);
     hkv = y - block * a.kv_heads;
@@ -117,6 +125,8 @@ struct P4Unit {
     q_len = a.cu_q ? a.cu_q[b + 1] - row0 : 1;
     kv_len = a.kv_lens[b];
     n_cols = min(cols, q_len * a.G - col0);
+    to_some = min(kv_len, kv_len - q_len + a.by_group(col0 + max(n_cols, 1) - 1) + 1);
+    to_all = min(kv_len, kv_len - q_len + a.by_group(col0) + 1);
   }
   // Where the value d of column c goes, or null: a row that the output does not have.
   __device__ __forceinline__ __nv_bfloat16* out(const P4Args& a, int D, int c, int d) const {
@@ -171,8 +181,8 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           float (&c)[4] = sc[u][nb][g];
-          if (h == 0) c[0] = c[1] = c[2] = c[3] = 0.f;
-          p4_mma(c, a0, a1, a2, a3, s.qb[nb][g][4 * h], s.qb[nb][g][4 * h + 1]);
+          if (h == 0) p4_mma0(c, a0, a1, a2, a3, s.qb[nb][g][0], s.qb[nb][g][1]);
+          else p4_mma(c, a0, a1, a2, a3, s.qb[nb][g][4], s.qb[nb][g][5]);
           p4_mma(c, b0, b1, b2, b3, s.qb[nb][g][4 * h + 2], s.qb[nb][g][4 * h + 3]);
         }
       }
@@ -272,8 +282,7 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
   // ---- weights p scale as the B operand (k = tokens, n = columns): transposed in blocks of eight by eight. Odd key rows
   // are the tokens that enter with the complement of their codes.
   uint32_t pb[2][NB][GR][2];
-  const uint32_t flip = (uint32_t)(r & 1) << 31;
-  const float whole = (r & 1) ? -15.f : 0.f;      // low + 15 scale, the scale's sign already turned
+  const float sign = (r & 1) ? -1.f : 1.f, whole = (r & 1) ? 15.f : 0.f;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -289,8 +298,8 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
       float w[GR], b[GR];
 #pragma unroll
       for (int g = 0; g < GR; ++g) {
-        w[g] = __uint_as_float(vq[g] << 16 ^ flip);
-        b[g] = fmaf(whole, w[g], kv4_low(vq[g]));
+        w[g] = kv4_scale(vq[g]) * sign;
+        b[g] = fmaf(whole, kv4_scale(vq[g]), kv4_low(vq[g]));
       }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -511,13 +520,30 @@ struct P4Feed {
 };
 static_assert(P4Cfg<128, 8>::STAGES == 2, "P4Feed alternates between two stages");
 
-template <int D, int COLS>
-__device__ __forceinline__ void p4_step(P4State<D, COLS>& s, const P4Feed<D, COLS>& feed, const P4Unit& u, const P4Args& a, int chunk) {
-  const int tok = chunk * P4_CHUNK, to_some = min(u.kv_len, u.kv_len - u.q_len + a.by_group(u.col0 + u.n_cols - 1) + 1),
-            to_all = min(u.kv_len, u.kv_len - u.q_len + a.by_group(u.col0) + 1);
-  const uint32_t gone = feed.gone();
-  if (gone == 0u && tok + P4_CHUNK <= to_all) p4_chunk<D, COLS, false>(s, feed.at(), tok, feed.lane, to_some, 0u);
-  else p4_chunk<D, COLS, true>(s, feed.at(), tok, feed.lane, to_some, gone);
+// Chunks i .. end - 1 of the warp, which are the unit's chunks chunk, chunk + step, ...; false: a wait ran out. Those that every
+// column sees whole come first and have a loop of their own: with both forms in one loop the accumulators were copied
+// between them.
+template <int D, int COLS, class F>
+__device__ __forceinline__ bool p4_run(P4State<D, COLS>& s, P4Feed<D, COLS>& feed, const P4Unit& u, int& i, int end, int chunk, int step,
+                                       volatile int* abort_flag, const F& locate) {
+  bool waited = false;
+  for (; i < end && (chunk + 1) * P4_CHUNK <= u.to_all; ++i, chunk += step) {
+    if (!feed.wait(i, abort_flag, locate)) return false;
+    if (feed.gone() != 0u) {
+      waited = true;
+      break;
+    }
+    p4_chunk<D, COLS, false>(s, feed.at(), chunk * P4_CHUNK, feed.lane, u.to_some, 0u);
+    feed.next();
+  }
+#pragma unroll 1
+  for (; i < end; ++i, chunk += step) {
+    if (!waited && !feed.wait(i, abort_flag, locate)) return false;
+    waited = false;
+    p4_chunk<D, COLS, true>(s, feed.at(), chunk * P4_CHUNK, feed.lane, u.to_some, feed.gone());
+    feed.next();
+  }
+  return true;
 }
 
 // Joins the parts of a unit that shared memory holds (bits of `parts`), column c, values d .. d + 3: sums, and the column's
@@ -616,25 +642,18 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   if (mine > 0) feed.issue(0, 0, locate);
   P4State<D, COLS> s;
   p4_queries(s, a, u, lane);
-  bool ok = true;
-  for (int i = 0; i < mine; ++i) {
-    ok = feed.wait(i, abort_flag, locate);
-    if (!ok) {
-      feed.drain(i);
-      break;
-    }
-    p4_step(s, feed, u, a, chunk0 + P4_WARPS * i);
-    feed.next();
-  }
+  int i = 0;
+  const bool ok = p4_run(s, feed, u, i, mine, chunk0, P4_WARPS, abort_flag, locate);
+  if (!ok) feed.drain(i);
   p4_result(s, a, u, false, reinterpret_cast<float*>(feed.ring), s_ml + warp * 2 * COLS, lane);
   __syncwarp();
   if (!ok) s_ml[warp * 2 * COLS + COLS + lane % COLS] = 0.f;                // counts as nothing seen
   __syncthreads();
-  for (int i = threadIdx.x; i < COLS * D / 4; i += P4_THREADS) {
-    const int c = 4 * i / D, d = 4 * i % D;
+  for (int k = threadIdx.x; k < COLS * D / 4; k += P4_THREADS) {
+    const int c = 4 * k / D, d = 4 * k % D;
     float M, l;
-    const float4 v = p4_join<D, COLS>((1u << P4_WARPS) - 1u, s_ml, [&](int k) { return reinterpret_cast<const float*>(smem + k * C::WARP_BYTES); }, c, d, M, l);
-    *reinterpret_cast<float4*>(s_cta + 4 * i) = v;
+    const float4 v = p4_join<D, COLS>((1u << P4_WARPS) - 1u, s_ml, [&](int w) { return reinterpret_cast<const float*>(smem + w * C::WARP_BYTES); }, c, d, M, l);
+    *reinterpret_cast<float4*>(s_cta + 4 * k) = v;
     if (d == 0) {
       s_cml[c] = M;
       s_cml[COLS + c] = l;
@@ -643,10 +662,10 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   p4_cluster_sync();
   // every CTA writes a share of the block's outputs, four values a thread
   const int share = (COLS * D / 4 + splits - 1) / splits, rank = p4_rank();
-  for (int i = rank * share + threadIdx.x; i < min(COLS * D / 4, (rank + 1) * share); i += P4_THREADS) {
-    const int c = 4 * i / D, d = 4 * i % D;
+  for (int k = rank * share + threadIdx.x; k < min(COLS * D / 4, (rank + 1) * share); k += P4_THREADS) {
+    const int c = 4 * k / D, d = 4 * k % D;
     if (c >= u.n_cols) break;
-    const uint32_t m_at = smem_u32(s_cml + c), l_at = smem_u32(s_cml + COLS + c), v_at = smem_u32(s_cta + 4 * i);
+    const uint32_t m_at = smem_u32(s_cml + c), l_at = smem_u32(s_cml + COLS + c), v_at = smem_u32(s_cta + 4 * k);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f, M = -INFINITY;
 #pragma unroll 4
@@ -800,23 +819,18 @@ paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict_
   P4Feed<D, COLS> feed{a, smem + warp * C::WARP_BYTES, full, lane, mine};
   if (mine > 0) feed.issue(0, 0, locate);
   P4State<D, COLS> s;
-  bool ok = true;
   int i = 0;
   while (i < mine) {
     // ---- one unit, or the part of it in this warp's stretch
     const P4Unit u(a, COLS, b, y);
     const bool begins = chunk == 0;
     p4_queries(s, a, u, lane);
-    for (const int end = i + min(n - chunk, mine - i); i < end; ++i, ++chunk) {
-      ok = feed.wait(i, abort_flag, locate);
-      if (!ok) break;
-      p4_step(s, feed, u, a, chunk);
-      feed.next();
-    }
-    if (!ok) {
+    const int part = min(n - chunk, mine - i);
+    if (!p4_run(s, feed, u, i, i + part, chunk, 1, abort_flag, locate)) {
       feed.drain(i);
       break;
     }
+    chunk += part;
     const bool ends = chunk == n;
     const int slot = ends ? 0 : 1;                // (a part that does not end its unit is the warp's last)
     p4_result(s, a, u, begins && ends, reinterpret_cast<float*>(slot ? feed.ring : smem + S::OFF_HEAD + warp * C::PART),
