@@ -14,94 +14,124 @@ namespace mb {
 namespace {
 
 // ------------------------------------------------------------------------------------------------ write
-// Eight lanes share a group of 64 values, one 16-byte load each; extremes travel as bf16 pairs (min and max
-// that keep a NaN), codes leave as one word per lane. Moves 2 + 0.5625 bytes per value.
+// Four lanes share a group of 64 values, sixteen each; extremes travel as bf16 pairs (min and max that keep a NaN), codes
+// leave as two words per lane. Moves 2 + 0.5625 bytes per value.
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
 kv_append_int4_kernel(const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, uint8_t* __restrict__ k_cache,
-                      uint8_t* __restrict__ v_cache, const int* __restrict__ block_table, const int* __restrict__ positions,
-                      const int* __restrict__ seq_ids, long long units, int kv_heads, int page_size, int max_pages, int n_seqs,
-                      int n_pages, long long k_stride, long long v_stride) {
+                      uint8_t* __restrict__ v_cache, const Kv4Pages pages, const int* __restrict__ positions,
+                      const int* __restrict__ seq_ids, int units, Kv4Div by_token, long long k_stride, long long v_stride) {
   using L = KvInt4<D>;
-  constexpr int PER_ROW = D / 8;
-  const int per_tok = kv_heads * PER_ROW;
-  const long long step = (long long)gridDim.x * blockDim.x;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < units; i += step) {
-    const unsigned mask = 0xFFu << (threadIdx.x & 24);           // units is a multiple of 8: a group is here as a whole
-    const int t = (int)(i / per_tok), c = (int)(i % per_tok);
-    const int head = c / PER_ROW, g = (c % PER_ROW) >> 3, u = c & 7;
-    const bf16x8 kx = ldg8(k, t * k_stride + (long long)c * 8), vx = ldg8(v, t * v_stride + (long long)c * 8);
-    __nv_bfloat162 lo[2], hi[2];
+  constexpr int PER_ROW = D / 16, GR = L::GROUPS;
+  // units is a multiple of the lanes of a row: groups and rows are here as a whole
+  const unsigned mask = 0xFu << (threadIdx.x & 28), row_mask = ((1u << PER_ROW) - 1u) << (threadIdx.x & (32 - PER_ROW));
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= units) return;
+  const int t = by_token(i), c = i - t * pages.kv_heads * PER_ROW;
+  const int head = c / PER_ROW, g = (c % PER_ROW) >> 2, u = c & 3;
+  const int seq = seq_ids[t], pos = positions[t];
+  bf16x8 x[2][2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const bf16x8& x = s ? vx : kx;
-      lo[s] = __hmin2_nan(__hmin2_nan(x.v[0], x.v[1]), __hmin2_nan(x.v[2], x.v[3]));
-      hi[s] = __hmax2_nan(__hmax2_nan(x.v[0], x.v[1]), __hmax2_nan(x.v[2], x.v[3]));
+  for (int h = 0; h < 2; ++h) {
+    x[0][h] = ldg8(k, t * k_stride + c * 16 + 8 * h);
+    x[1][h] = ldg8(v, t * v_stride + c * 16 + 8 * h);
+  }
+  const int tile = pages.tile(seq, pos, head);
+  const int n = pos & 15;                                        // (page sizes are multiples of 16)
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        lo[s] = __hmin2_nan(lo[s], __shfl_xor_sync(mask, lo[s], o));
-        hi[s] = __hmax2_nan(hi[s], __shfl_xor_sync(mask, hi[s], o));
-      }
+  for (int s = 0; s < 2; ++s) {
+    __nv_bfloat162 lo = x[s][0].v[0], hi = lo;
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+      lo = __hmin2_nan(lo, x[s][e >> 2].v[e & 3]);
+      hi = __hmax2_nan(hi, x[s][e >> 2].v[e & 3]);
     }
-    const int seq = seq_ids[t], pos = positions[t];
-    const int tile = seq >= 0 && seq < n_seqs
-        ? kv4_tile(block_table + (long long)seq * max_pages, pos, max_pages, n_pages, page_size, kv_heads, head) : -1;
+#pragma unroll
+    for (int o = 2; o > 0; o >>= 1) {
+      lo = __hmin2_nan(lo, __shfl_xor_sync(mask, lo, o));
+      hi = __hmax2_nan(hi, __shfl_xor_sync(mask, hi, o));
+    }
     if (tile < 0) continue;
-    const int n = (pos % page_size) & 15;
+    float scale, low;
+    const uint32_t pair = kv4_make_pair(__hmin_nan(lo.x, lo.y), __hmax_nan(hi.x, hi.y), scale, low);
+    const float inv = __frcp_rn(scale);
+    uint32_t w[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      float f[8], scale, low;
-      unpack8(s ? vx : kx, f);
-      const uint32_t pair = kv4_make_pair(__hmin_nan(lo[s].x, lo[s].y), __hmax_nan(hi[s].x, hi[s].y), scale, low);
-      const uint32_t w = kv4_word(f, scale, low);
-      uint8_t* dst = (s ? v_cache : k_cache) + (long long)tile * L::TILE_BYTES;
-      if (s == 0) *reinterpret_cast<uint32_t*>(dst + kv4_key_word<D>(n, g, u)) = kv4_rotate(w);
-      else *reinterpret_cast<uint32_t*>(dst + kv4_value_word<D>(n, g, u)) = w;
-      if (u == 0) *reinterpret_cast<uint32_t*>(dst + kv4_pair<D>(n, g)) = pair;
+    for (int h = 0; h < 2; ++h) w[h] = kv4_word(x[s][h], scale, low, inv);
+    uint8_t* dst = (s ? v_cache : k_cache) + (long long)tile * L::TILE_BYTES;
+    if (s == 0) {
+      *reinterpret_cast<uint2*>(dst + kv4_key_word<D>(n, g, 2 * u)) = make_uint2(kv4_rotate(w[0]), kv4_rotate(w[1]));
+    } else if (GR == 1) {
+      *reinterpret_cast<uint2*>(dst + kv4_value_word<D>(n, g, 2 * u)) = make_uint2(w[0], w[1]);
+    } else {
+      // the two groups' words of a place lie side by side: this lane stores those of place 2 u + g
+      const uint32_t other = __shfl_xor_sync(row_mask, g ? w[0] : w[1], 4);
+      *reinterpret_cast<uint2*>(dst + kv4_value_word<D>(n, 0, 2 * u + g)) = g ? make_uint2(other, w[1]) : make_uint2(w[0], other);
     }
+    if (u == 0) *reinterpret_cast<uint32_t*>(dst + kv4_pair<D>(n, g)) = pair;
   }
 }
 
 // ------------------------------------------------------------------------------------------------ read
-// Eight values of a row: scale * code + low, rounded once (the product of a bf16 and a 4-bit integer is exact
-// in fp32).
+// Eight values of a row. 0x4300 | code is the bf16 number 128 + code; taking 128 off is exact, and the fused bf16
+// multiply-add rounds scale * code + low once.
 __device__ __forceinline__ bf16x8 kv4_expand(uint32_t w, uint32_t pair) {
-  const float s = kv4_scale(pair), low = kv4_low(pair);
-  float f[8];
+  const __nv_bfloat16 s = __ushort_as_bfloat16((unsigned short)pair), low = __ushort_as_bfloat16((unsigned short)(pair >> 16));
+  const __nv_bfloat162 s2(s, s), low2(low, low), k128(__ushort_as_bfloat16(0x4300), __ushort_as_bfloat16(0x4300));
+  bf16x8 y;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = fmaf((float)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u), s, low);
-  return pack8(f);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = (w >> (4 * i) & 0x000F000Fu) | 0x43004300u;
+    y.v[i] = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), k128), s2, low2);
+  }
+  return y;
 }
 
-// Tokens named by (sequence, position): the counterpart of the append. One word per thread and tensor.
-template <int D>
+// Tokens named by (sequence, position): the counterpart of the append. One word per thread, tensor and step, so that a warp's
+// stores are 512 bytes side by side (two words per thread left half-written 32-byte sectors between its stores: 174 us
+// instead of 62 for 8 ragged sequences of up to 8192 tokens); four steps at once (50 us), because a word is behind three
+// loads that wait for one another (position, page, code). Calls that one step per thread spreads over the GPU at once take one
+// (1000 tokens of 5 heads: 2.8 us against 3.5).
+constexpr int KV4_READ = 4;
+template <int D, int STEPS>
 __global__ void __launch_bounds__(256)
-kv_read_int4_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int* __restrict__ block_table,
+kv_read_int4_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const Kv4Pages pages,
                     const int* __restrict__ positions, const int* __restrict__ seq_ids, __nv_bfloat16* __restrict__ k,
-                    __nv_bfloat16* __restrict__ v, long long units, int kv_heads, int page_size, int max_pages, int n_seqs,
-                    int n_pages) {
+                    __nv_bfloat16* __restrict__ v, int units, Kv4Div by_token) {
   using L = KvInt4<D>;
   constexpr int PER_ROW = D / 8;
-  const int per_tok = kv_heads * PER_ROW;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < units; i += (long long)gridDim.x * blockDim.x) {
-    const int t = (int)(i / per_tok), c = (int)(i % per_tok);
-    const int head = c / PER_ROW, g = (c % PER_ROW) >> 3, u = c & 7;
-    const int seq = seq_ids[t], pos = positions[t];
-    const int tile = seq >= 0 && seq < n_seqs
-        ? kv4_tile(block_table + (long long)seq * max_pages, pos, max_pages, n_pages, page_size, kv_heads, head) : -1;
-    uint32_t kw = 0u, vw = 0u, kp = 0u, vp = 0u;                 // a token without a page reads as zeros
-    if (tile >= 0) {
-      const int n = (pos % page_size) & 15;
-      const uint8_t* ks = k_cache + (long long)tile * L::TILE_BYTES;
-      const uint8_t* vs = v_cache + (long long)tile * L::TILE_BYTES;
-      kw = kv4_unrotate(*reinterpret_cast<const uint32_t*>(ks + kv4_key_word<D>(n, g, u)));
-      vw = *reinterpret_cast<const uint32_t*>(vs + kv4_value_word<D>(n, g, u));
-      kp = *reinterpret_cast<const uint32_t*>(ks + kv4_pair<D>(n, g));
-      vp = *reinterpret_cast<const uint32_t*>(vs + kv4_pair<D>(n, g));
+  const int first = blockIdx.x * (256 * STEPS) + threadIdx.x;
+  uint32_t kw[STEPS], vw[STEPS], kp[STEPS], vp[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int i = first + 256 * s;
+    kw[s] = vw[s] = kp[s] = vp[s] = 0u;                          // a token without a page reads as zeros
+    if (i < units) {
+      const int t = by_token(i), c = i - t * pages.kv_heads * PER_ROW;
+      const int head = c / PER_ROW, g = (c % PER_ROW) >> 3, u = c & 7;
+      const int pos = positions[t], tile = pages.tile(seq_ids[t], pos, head), n = pos & 15;
+      if (tile >= 0) {
+        const uint8_t* ks = k_cache + (long long)tile * L::TILE_BYTES;
+        const uint8_t* vs = v_cache + (long long)tile * L::TILE_BYTES;
+        kw[s] = *reinterpret_cast<const uint32_t*>(ks + kv4_key_word<D>(n, g, u));
+        vw[s] = *reinterpret_cast<const uint32_t*>(vs + kv4_value_word<D>(n, g, u));
+        kp[s] = *reinterpret_cast<const uint32_t*>(ks + kv4_pair<D>(n, g));
+        vp[s] = *reinterpret_cast<const uint32_t*>(vs + kv4_pair<D>(n, g));
+      }
     }
-    stg8(k, i * 8, kv4_expand(kw, kp));
-    stg8(v, i * 8, kv4_expand(vw, vp));
   }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int i = first + 256 * s;
+    if (i < units) {
+      stg8(k, i * 8LL, kv4_expand(kv4_unrotate(kw[s]), kp[s]));
+      stg8(v, i * 8LL, kv4_expand(vw[s], vp[s]));
+    }
+  }
+}
+
+Kv4Pages kv4_pages(const KvInt4Cache& c) {
+  return {c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)};
 }
 
 void kv4_check(const KvInt4Cache& c, const char* who) {
@@ -113,9 +143,11 @@ void kv4_check(const KvInt4Cache& c, const char* who) {
              std::string(who) + ": caches must be 16-byte aligned");
 }
 
-int kv4_grid(long long units, int per_sm) {
-  const long long g = (units + 255) / 256, cap = (long long)sm_count() * per_sm;
-  return (int)(g < cap ? g : cap);
+// Threads of an append or a read, one per `values` of each tensor.
+int kv4_units(const KvInt4Cache& c, int tokens, int values, const char* who) {
+  const long long n = (long long)tokens * c.kv_heads * (c.head_dim / values);
+  MB_REQUIRE(n < (1LL << 31) - 256 * KV4_READ, std::string(who) + ": too many tokens in one call");
+  return (int)n;
 }
 
 }  // namespace
@@ -126,11 +158,10 @@ void kv_append_int4(const KvInt4Cache& c, const void* k, const void* v, const in
   MB_REQUIRE(k_stride % 8 == 0 && v_stride % 8 == 0, "kv_append_int4: token strides must be multiples of 8 elements");
   MB_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0, "kv_append_int4: k and v must be 16-byte aligned");
   if (tokens == 0) return;
-  const long long units = (long long)tokens * c.kv_heads * (c.head_dim / 8);
+  const int units = kv4_units(c, tokens, 16, "kv_append_int4"), per_token = c.kv_heads * (c.head_dim / 16);
   const auto go = [&](auto kern) {
-    kern<<<kv4_grid(units, 16), 256, 0, stream>>>((const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (uint8_t*)c.k, (uint8_t*)c.v,
-                                                  c.block_table, positions, seq_ids, units, c.kv_heads, c.page_size, c.max_pages,
-                                                  c.n_seqs, c.n_pages, k_stride, v_stride);
+    kern<<<(units + 255) / 256, 256, 0, stream>>>((const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (uint8_t*)c.k, (uint8_t*)c.v,
+                                                  kv4_pages(c), positions, seq_ids, units, kv4_div(per_token), k_stride, v_stride);
   };
   if (c.head_dim == 128) go(kv_append_int4_kernel<128>);
   else go(kv_append_int4_kernel<64>);
@@ -142,14 +173,20 @@ void kv_read_int4(const KvInt4Cache& c, const int* positions, const int* seq_ids
   kv4_check(c, "kv_read_int4");
   MB_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0, "kv_read_int4: k and v must be 16-byte aligned");
   if (tokens == 0) return;
-  const long long units = (long long)tokens * c.kv_heads * (c.head_dim / 8);
+  const int units = kv4_units(c, tokens, 8, "kv_read_int4"), per_token = c.kv_heads * (c.head_dim / 8);
+  const bool small = units <= 8 * 256 * sm_count();
+  const int per = 256 * (small ? 1 : KV4_READ);
   const auto go = [&](auto kern) {
-    kern<<<kv4_grid(units, 16), 256, 0, stream>>>((const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, positions, seq_ids,
-                                                  (__nv_bfloat16*)k, (__nv_bfloat16*)v, units, c.kv_heads, c.page_size,
-                                                  c.max_pages, c.n_seqs, c.n_pages);
+    kern<<<(units + per - 1) / per, 256, 0, stream>>>((const uint8_t*)c.k, (const uint8_t*)c.v, kv4_pages(c), positions, seq_ids,
+                                                      (__nv_bfloat16*)k, (__nv_bfloat16*)v, units, kv4_div(per_token));
   };
-  if (c.head_dim == 128) go(kv_read_int4_kernel<128>);
-  else go(kv_read_int4_kernel<64>);
+  if (c.head_dim == 128) {
+    if (small) go(kv_read_int4_kernel<128, 1>);
+    else go(kv_read_int4_kernel<128, KV4_READ>);
+  } else {
+    if (small) go(kv_read_int4_kernel<64, 1>);
+    else go(kv_read_int4_kernel<64, KV4_READ>);
+  }
   count_launch();
   check_launch();
 }

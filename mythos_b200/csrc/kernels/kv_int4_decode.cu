@@ -77,40 +77,19 @@ __device__ __forceinline__ uint32_t p4_transpose(uint32_t x) {
   return y;
 }
 
-// Quotient by a number the host knows: n * mul / 2^shift with mul = ceil(2^shift / d), shift = 31 + ceil(log2 d); exact for
-// 0 <= n < 2^31.
-struct P4Div {
-  uint32_t mul;
-  int shift;
-  __device__ __forceinline__ int operator()(int n) const { return (int)((unsigned long long)(unsigned)n * mul >> shift); }
-};
-P4Div p4_div(int d) {
-  int s = 0;
-  while ((1LL << s) < d) ++s;
-  return {(uint32_t)(((1ULL << (31 + s)) + (unsigned)d - 1) / (unsigned)d), 31 + s};
-}
-
 struct P4Args {
   const __nv_bfloat16* q;
   const uint8_t* k_cache;
   const uint8_t* v_cache;
-  const int* block_table;
+  Kv4Pages pages;
   const int* kv_lens;
   const int* cu_q;          // first query row of every sequence, or null: one query token per sequence
   __nv_bfloat16* out;
   long long q_stride, o_stride;
-  int batch, G, kv_heads, total_q, page_size, max_pages, n_pages;
-  P4Div by_group, by_heads, by_page;
+  int batch, G, kv_heads, total_q;
+  Kv4Div by_group, by_heads;
   float scale_log2;
   int* status;
-  // Tile of a token, -1 without a page.
-  __device__ __forceinline__ int tile(int b, int token, int head) const {
-    const int lp = by_page(token);
-    if (lp >= max_pages) return -1;
-    const int page = block_table[(long long)b * max_pages + lp];
-    if ((unsigned)page >= (unsigned)n_pages) return -1;
-    return (page * kv_heads + head) * (page_size >> 4) + ((token - lp * page_size) >> 4);
-  }
 };
 
 // A unit: one (sequence, kv head, block of columns).
@@ -636,7 +615,7 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   const int mine = max(0, (end - chunk0 + P4_WARPS - 1) / P4_WARPS);        // chunk0, + 4, ...
   const auto locate = [&](int i) {
     const int token = (chunk0 + P4_WARPS * i) * P4_CHUNK + (lane & 1) * 16;
-    return i < mine && token < u.kv_len ? a.tile(u.b, token, u.hkv) : -2;
+    return i < mine && token < u.kv_len ? a.pages.tile(u.b, token, u.hkv) : -2;
   };
   P4Feed<D, COLS> feed{a, smem + warp * C::WARP_BYTES, full, lane, mine};
   if (mine > 0) feed.issue(0, 0, locate);
@@ -814,7 +793,7 @@ paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict_
       ln = line.chunks(lb);
     }
     const int at = f - lbegin, ly = at / ln, token = (at - ly * ln) * P4_CHUNK + (lane & 1) * 16;
-    return token < a.kv_lens[lb] ? a.tile(lb, token, ly - a.by_heads(ly) * a.kv_heads) : -2;
+    return token < a.kv_lens[lb] ? a.pages.tile(lb, token, ly - a.by_heads(ly) * a.kv_heads) : -2;
   };
   P4Feed<D, COLS> feed{a, smem + warp * C::WARP_BYTES, full, lane, mine};
   if (mine > 0) feed.issue(0, 0, locate);
@@ -1038,9 +1017,10 @@ void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, con
                     cudaStream_t stream) {
   const int G = heads / c.kv_heads;
   const P4Plan plan = p4_plan(batch, max_q, G, c.kv_heads, (long long)c.max_pages * c.page_size);
-  P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, kv_lens, cu_q, (__nv_bfloat16*)out,
-           q_stride, o_stride, batch, G, c.kv_heads, total_q, c.page_size, c.max_pages, c.n_pages,
-           p4_div(G), p4_div(c.kv_heads), p4_div(c.page_size), scale * 1.4426950408889634f, status};
+  P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v,
+           {c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)}, kv_lens, cu_q,
+           (__nv_bfloat16*)out, q_stride, o_stride, batch, G, c.kv_heads, total_q, kv4_div(G), kv4_div(c.kv_heads),
+           scale * 1.4426950408889634f, status};
   float* scratch = (float*)workspace;
   if (c.head_dim == 128) {
     if (plan.cols == 16) p4_launch<128, 16>(a, plan, scratch, stream);

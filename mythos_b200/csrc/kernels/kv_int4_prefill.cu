@@ -45,18 +45,23 @@ __device__ __forceinline__ uint32_t pf_half2(float a, float b) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
+// Eight values times inv (a power of two) as fp16. 0x4300 | code is the bf16 number 128 + code; the 128 scale leaves with the low
+// (both exact to 2^-17 of a step, far below fp16's rounding).
 __device__ __forceinline__ uint4 pf_expand8(uint32_t w, uint32_t pair, float inv) {
-  const float s = kv4_scale(pair), low = kv4_low(pair);
-  float f[8];
+  const float s = kv4_scale(pair) * inv, low = fmaf(-128.f, s, kv4_low(pair) * inv);
+  uint32_t y[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = fmaf((float)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u), s, low) * inv;
-  return make_uint4(pf_half2(f[0], f[1]), pf_half2(f[2], f[3]), pf_half2(f[4], f[5]), pf_half2(f[6], f[7]));
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = (w >> (4 * i) & 0x000F000Fu) | 0x43004300u;
+    y[i] = pf_half2(fmaf(kv4_scale(x), s, low), fmaf(kv4_low(x), s, low));           // (both halves of a word)
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
 struct PfExpand {
   const uint8_t* k_cache;
   const uint8_t* v_cache;
-  const int* block_table;
+  Kv4Pages pages;
   const int* kv_lens;
   const __nv_bfloat16* q;
   long long q_stride;
@@ -65,7 +70,7 @@ struct PfExpand {
   __half* qh;           // [total_q, heads, D]
   float* q_factor;      // [total_q, heads]: 2^eq
   int* exponents;       // [batch * kv_heads, tiles]: ek in the low, ev in the high half
-  int kv_heads, heads, page_size, max_pages, n_pages, tiles, kv_blocks, total_q;
+  int kv_heads, heads, tiles, kv_blocks, total_q;
   int* status;
 };
 
@@ -104,7 +109,7 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
   if (threadIdx.x < 8) {
     int tile = -1;
     if (n0 + 16 * (int)threadIdx.x < len) {
-      tile = kv4_tile(a.block_table + (long long)b * a.max_pages, n0 + 16 * threadIdx.x, a.max_pages, a.n_pages, a.page_size, a.kv_heads, head);
+      tile = a.pages.tile(b, n0 + 16 * threadIdx.x, head);
       if (tile < 0 && a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (91 << 16));
     }
     s_tile[threadIdx.x] = tile;
@@ -566,7 +571,9 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   const int pack = 128 % G == 0 ? G : 1;
   const long long all = (long long)batch * c.kv_heads * tiles;
   uint8_t* p = (uint8_t*)workspace;
-  PfExpand x{(const uint8_t*)c.k, (const uint8_t*)c.v, c.block_table, kv_lens, (const __nv_bfloat16*)q, q_stride};
+  PfExpand x{(const uint8_t*)c.k, (const uint8_t*)c.v,
+             {c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)}, kv_lens,
+             (const __nv_bfloat16*)q, q_stride};
   x.k = (__half*)p;
   x.v = x.k + all * PF_TILE * D;
   p += 2 * all * PF_TILE * D * 2;
@@ -577,9 +584,6 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.exponents = (int*)p;
   x.kv_heads = c.kv_heads;
   x.heads = heads;
-  x.page_size = c.page_size;
-  x.max_pages = c.max_pages;
-  x.n_pages = c.n_pages;
   x.tiles = tiles;
   x.total_q = total_q;
   x.status = status;
