@@ -931,25 +931,26 @@ void kv_append_int4(const Tensor& k, const Tensor& v, Tensor& k_cache, Tensor& v
                      kv4_stride(v), cur_stream());
 }
 
-void kv_read_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& positions,
-                  const Tensor& seq_ids, Tensor& k, Tensor& v) {
+std::tuple<Tensor, Tensor> kv_read_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& positions,
+                                        const Tensor& seq_ids, int64_t head_dim) {
   const char* who = "kv_read_int4";
-  chk_c(k, BF16, "k");
-  chk_c(v, BF16, "v");
-  kv4_rows(k, k_cache, "k", who);
-  kv4_rows(v, k_cache, "v", who);
-  TORCH_CHECK(k.sizes() == v.sizes(), who, ": k and v must have the same shape");
-  const auto c = kv4_cache(k_cache, v_cache, block_table, k.size(1), k.size(2), who);
-  kv4_tokens(positions, seq_ids, k_cache, k.size(0), who);
+  TORCH_CHECK(k_cache.dim() == 3, who, ": caches must be [pages, kv_heads, page bytes]");
+  const int64_t T = positions.numel(), Hkv = k_cache.size(1);
+  const auto c = kv4_cache(k_cache, v_cache, block_table, Hkv, head_dim, who);
+  kv4_tokens(positions, seq_ids, k_cache, T, who);
   c10::cuda::CUDAGuard guard(k_cache.device());
-  mb::kv_read_int4(c, positions.data_ptr<int>(), seq_ids.data_ptr<int>(), (int)k.size(0), k.data_ptr(), v.data_ptr(), cur_stream());
+  const auto opt = k_cache.options().dtype(BF16);
+  Tensor k = torch::empty({T, Hkv, head_dim}, opt), v = torch::empty({T, Hkv, head_dim}, opt);
+  mb::kv_read_int4(c, positions.data_ptr<int>(), seq_ids.data_ptr<int>(), (int)T, k.data_ptr(), v.data_ptr(), cur_stream());
+  return {k, v};
 }
 
-void paged_attn_decode_int4(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
-                            const Tensor& context_lens, Tensor& out, double scale, const OptTensor& status) {
+Tensor paged_attn_decode_int4(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                              const Tensor& context_lens, const OptTensor& out_, double scale, const OptTensor& status) {
   const char* who = "paged_attn_decode_int4";
   kv4_rows(q, k_cache, "q", who);
   chk_c(context_lens, I32, "context_lens");
+  Tensor out = out_.has_value() ? *out_ : torch::empty(q.sizes(), q.options());
   chk_c(out, BF16, "out");
   kv4_rows(out, k_cache, "out", who);
   TORCH_CHECK(k_cache.dim() == 3 && k_cache.size(1) > 0 && q.size(1) % k_cache.size(1) == 0, who, ": heads must be a multiple of kv_heads");
@@ -959,16 +960,19 @@ void paged_attn_decode_int4(const Tensor& q, const Tensor& k_cache, const Tensor
   const auto c = kv4_cache(k_cache, v_cache, block_table, k_cache.size(1), q.size(2), who);
   c10::cuda::CUDAGuard guard(q.device());
   const int64_t bytes = mb::paged_attn_int4_workspace(c, (int)q.size(0), (int)q.size(0), 1, c.max_pages * c.page_size, (int)q.size(1));
-  Tensor work = torch::empty({bytes}, q.options().dtype(U8));
+  Tensor work;
+  if (bytes > 0) work = torch::empty({bytes}, q.options().dtype(U8));
   mb::paged_attn_decode_int4(c, q.data_ptr(), kv4_stride(q), context_lens.data_ptr<int>(), out.data_ptr(), (int)q.size(0), (int)q.size(1),
-                             (float)scale, work.data_ptr(), status_ptr(status), cur_stream());
+                             (float)scale, bytes > 0 ? work.data_ptr() : nullptr, status_ptr(status), cur_stream());
+  return out;
 }
 
-void paged_attn_prefill_int4(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
-                             const Tensor& cu_q, const Tensor& kv_lens, Tensor& out, int64_t max_q_len, int64_t max_kv_len,
-                             double scale, const OptTensor& status) {
+Tensor paged_attn_prefill_int4(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                               const Tensor& cu_q, const Tensor& kv_lens, const OptTensor& out_, int64_t max_q_len,
+                               int64_t max_kv_len, double scale, const OptTensor& status) {
   const char* who = "paged_attn_prefill_int4";
   kv4_rows(q, k_cache, "q", who);
+  Tensor out = out_.has_value() ? *out_ : torch::empty(q.sizes(), q.options());
   kv4_rows(out, k_cache, "out", who);
   chk_c(cu_q, I32, "cu_q");
   chk_c(kv_lens, I32, "kv_lens");
@@ -982,10 +986,12 @@ void paged_attn_prefill_int4(const Tensor& q, const Tensor& k_cache, const Tenso
               ": max_q_len must be within q and max_kv_len within the table's pages");
   c10::cuda::CUDAGuard guard(q.device());
   const int64_t bytes = mb::paged_attn_int4_workspace(c, (int)B, (int)q.size(0), (int)max_q_len, (int)max_kv_len, (int)q.size(1));
-  Tensor work = torch::empty({bytes}, q.options().dtype(U8));
+  Tensor work;
+  if (bytes > 0) work = torch::empty({bytes}, q.options().dtype(U8));
   mb::paged_attn_prefill_int4(c, q.data_ptr(), kv4_stride(q), cu_q.data_ptr<int>(), kv_lens.data_ptr<int>(), out.data_ptr(), kv4_stride(out),
-                              (int)B, (int)q.size(0), (int)max_q_len, (int)max_kv_len, (int)q.size(1), (float)scale, work.data_ptr(),
-                              status_ptr(status), cur_stream());
+                              (int)B, (int)q.size(0), (int)max_q_len, (int)max_kv_len, (int)q.size(1), (float)scale,
+                              bytes > 0 ? work.data_ptr() : nullptr, status_ptr(status), cur_stream());
+  return out;
 }
 
 void peer_add_f32(const Tensor& part, const std::vector<int64_t>& ptrs) {

@@ -725,11 +725,7 @@ def kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim: in
     without a page reads as zeros."""
     if not k_cache.is_cuda:
         return ref.kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim)
-    shape = (positions.numel(), k_cache.shape[1], head_dim)
-    k = torch.empty(shape, device=k_cache.device, dtype=torch.bfloat16)
-    v = torch.empty(shape, device=k_cache.device, dtype=torch.bfloat16)
-    _C().kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, k, v)
-    return k, v
+    return _C().kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim)
 
 
 def paged_attn_decode_int4(q, k_cache, v_cache, block_table, context_lens, scale: float | None = None, out=None):
@@ -743,9 +739,7 @@ def paged_attn_decode_int4(q, k_cache, v_cache, block_table, context_lens, scale
         cu = torch.arange(q.shape[0] + 1, dtype=torch.int32)
         o = ref.paged_attn_int4(q, k_cache, v_cache, block_table, cu, context_lens, scale)
         return o if out is None else out.copy_(o)
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
-    _C().paged_attn_decode_int4(q, k_cache, v_cache, block_table, context_lens, out, scale, native.status_word(q.device))
-    return out
+    return _C().paged_attn_decode_int4(q, k_cache, v_cache, block_table, context_lens, out, scale, native.status_word(q.device))
 
 
 def paged_attn_prefill_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q_len: int, max_kv_len: int,
@@ -761,7 +755,5 @@ def paged_attn_prefill_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, max
             return o
         out[: int(cu_q[-1])] = o[: int(cu_q[-1])]
         return out
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
-    _C().paged_attn_prefill_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, max_q_len, max_kv_len, scale,
-                                 native.status_word(q.device))
-    return out
+    return _C().paged_attn_prefill_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, max_q_len, max_kv_len, scale,
+                                        native.status_word(q.device))

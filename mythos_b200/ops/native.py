@@ -37,7 +37,7 @@ def available() -> bool:
 
 def require():
     """Return the extension module or raise with the import error and the build command."""
-    ext = _load()
+    ext = _ext if _ext is not None else _load()
     if ext is None:
         raise RuntimeError(
             "mythos_b200 native kernels are not built or failed to import "
@@ -72,10 +72,14 @@ def launch_count() -> int:
 
 
 _status: dict = {}
+_status_of: dict = {}
 
 
 def status_word(device) -> torch.Tensor:
     """Per-device int32 word that kernels with bounded waits write a non-zero code into."""
+    t = _status_of.get(device)          # (a torch.device with an index, seen before)
+    if t is not None:
+        return t
     dev = torch.device(device)
     key = (dev.type, dev.index if dev.index is not None else torch.cuda.current_device())
     t = _status.get(key)
@@ -85,6 +89,8 @@ def status_word(device) -> torch.Tensor:
         ext = _load()
         if dev.type == "cuda" and ext is not None and hasattr(ext, "comm_set_abort_word"):
             ext.comm_set_abort_word(t)    # collective kernels stop writing once a bounded wait has expired
+    if isinstance(device, torch.device) and device.index is not None:
+        _status_of[device] = t
     return t
 
 
