@@ -691,6 +691,37 @@ void tp_sum_residual_rmsnorm(OptTensor acc, const std::vector<int64_t>& staging_
                               (int)rows, (int)dim, (float)eps, epoch_dev.data_ptr<int>(), arrive.data_ptr<int>(),
                               limit_cycles, status_ptr(status), cur_stream());
 }
+// 4-bit pages: caches [pages, kv_heads, page_size * (head_dim / 2 + head_dim / 16)] uint8.
+mb::KvInt4Cache kv4_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, int64_t kv_heads, int64_t head_dim,
+                          const char* who) {
+  chk_c(k_cache, U8, "k_cache");
+  chk_c(v_cache, U8, "v_cache");
+  chk_c(block_table, I32, "block_table");
+  TORCH_CHECK(head_dim == 64 || head_dim == 128, who, ": head_dim must be 64 or 128, got ", head_dim);
+  const int64_t token = head_dim / 2 + head_dim / 16;
+  TORCH_CHECK(k_cache.dim() == 3 && k_cache.size(1) == kv_heads && k_cache.size(2) > 0 && k_cache.size(2) % (16 * token) == 0 &&
+                  v_cache.sizes() == k_cache.sizes(),
+              who, ": caches must be [pages, ", kv_heads, ", page_size * ", token, "] with page_size a multiple of 16");
+  TORCH_CHECK(block_table.dim() == 2, who, ": block_table must be [sequences, pages]");
+  TORCH_CHECK(v_cache.device() == k_cache.device() && block_table.device() == k_cache.device(), who, ": tensors on several devices");
+  return {k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr<int>(), (int)k_cache.size(0), (int)kv_heads, (int)head_dim,
+          (int)(k_cache.size(2) / token), (int)block_table.size(0), (int)block_table.size(1)};
+}
+void kv4_tokens(const Tensor& positions, const Tensor& seq_ids, const Tensor& cache, int64_t tokens, const char* who) {
+  chk_c(positions, I32, "positions");
+  chk_c(seq_ids, I32, "seq_ids");
+  TORCH_CHECK(positions.numel() == tokens && seq_ids.numel() == tokens, who, ": one position and one sequence per token");
+  TORCH_CHECK(positions.device() == cache.device() && seq_ids.device() == cache.device(), who, ": tensors on several devices");
+}
+// Rows [tokens, heads, head_dim] with contiguous heads and a token stride.
+void kv4_rows(const Tensor& t, const Tensor& cache, const char* name, const char* who) {
+  chk(t, BF16, name);
+  TORCH_CHECK(t.dim() == 3 && t.stride(2) == 1 && (t.size(1) <= 1 || t.stride(1) == t.size(2)) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * t.size(2))),
+              who, ": ", name, " must be [tokens, heads, head_dim] with contiguous heads and a token stride of a multiple of 8");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, who, ": ", name, " must be 16-byte aligned");
+  TORCH_CHECK(t.device() == cache.device(), who, ": tensors on several devices");
+}
+
 void qkv_rope_append(Tensor& acc, const Tensor& pos, const Tensor& seq_ids, const Tensor& block_table, Tensor& q_out,
                      Tensor& k_cache, Tensor& v_cache, double theta, OptTensor k_scale, OptTensor v_scale) {
   chk_c(acc, F32, "acc");
@@ -698,6 +729,17 @@ void qkv_rope_append(Tensor& acc, const Tensor& pos, const Tensor& seq_ids, cons
   chk_c(seq_ids, I32, "seq_ids");
   chk_c(block_table, I32, "block_table");
   chk_c(q_out, BF16, "q_out");
+  if (k_cache.scalar_type() == U8) {   // 4-bit pages
+    const int64_t T4 = q_out.size(0), H4 = q_out.size(1), D4 = q_out.size(2), Hkv4 = k_cache.size(1);
+    TORCH_CHECK(!k_scale.has_value() && !v_scale.has_value(), "qkv_rope_append: 4-bit pages hold their scales");
+    TORCH_CHECK(acc.numel() == T4 * (H4 + 2 * Hkv4) * D4, "qkv_rope_append: accumulator shape mismatch");
+    const auto c = kv4_cache(k_cache, v_cache, block_table, Hkv4, D4, "qkv_rope_append");
+    kv4_tokens(pos, seq_ids, k_cache, T4, "qkv_rope_append");
+    c10::cuda::CUDAGuard guard4(acc.device());
+    mb::qkv_rope_append_int4(acc.data_ptr<float>(), pos.data_ptr<int>(), seq_ids.data_ptr<int>(), q_out.data_ptr(), c, (int)T4, (int)H4,
+                             (float)theta, cur_stream());
+    return;
+  }
   const bool int8 = k_scale.has_value();
   TORCH_CHECK(int8 == v_scale.has_value(), "qkv_rope_append: give both scale tensors or neither");
   chk_c(k_cache, int8 ? torch::kInt8 : BF16, "k_cache");
@@ -883,37 +925,6 @@ void paged_attn_decode_int8(const Tensor& q, const Tensor& k_cache, const Tensor
                              out.data_ptr(), scratch.data_ptr<float>(), counters.data_ptr<int>(), (int)B, (int)H,
                              (int)Hkv, (int)D, (int)k_cache.size(1), (int)block_table.size(1), (int)k_cache.size(0),
                              (int)splits, (float)scale, status_ptr(status), cur_stream(), q.stride(0));
-}
-
-// 4-bit pages: caches [pages, kv_heads, page_size * (head_dim / 2 + head_dim / 16)] uint8.
-mb::KvInt4Cache kv4_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, int64_t kv_heads, int64_t head_dim,
-                          const char* who) {
-  chk_c(k_cache, U8, "k_cache");
-  chk_c(v_cache, U8, "v_cache");
-  chk_c(block_table, I32, "block_table");
-  TORCH_CHECK(head_dim == 64 || head_dim == 128, who, ": head_dim must be 64 or 128, got ", head_dim);
-  const int64_t token = head_dim / 2 + head_dim / 16;
-  TORCH_CHECK(k_cache.dim() == 3 && k_cache.size(1) == kv_heads && k_cache.size(2) > 0 && k_cache.size(2) % (16 * token) == 0 &&
-                  v_cache.sizes() == k_cache.sizes(),
-              who, ": caches must be [pages, ", kv_heads, ", page_size * ", token, "] with page_size a multiple of 16");
-  TORCH_CHECK(block_table.dim() == 2, who, ": block_table must be [sequences, pages]");
-  TORCH_CHECK(v_cache.device() == k_cache.device() && block_table.device() == k_cache.device(), who, ": tensors on several devices");
-  return {k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr<int>(), (int)k_cache.size(0), (int)kv_heads, (int)head_dim,
-          (int)(k_cache.size(2) / token), (int)block_table.size(0), (int)block_table.size(1)};
-}
-void kv4_tokens(const Tensor& positions, const Tensor& seq_ids, const Tensor& cache, int64_t tokens, const char* who) {
-  chk_c(positions, I32, "positions");
-  chk_c(seq_ids, I32, "seq_ids");
-  TORCH_CHECK(positions.numel() == tokens && seq_ids.numel() == tokens, who, ": one position and one sequence per token");
-  TORCH_CHECK(positions.device() == cache.device() && seq_ids.device() == cache.device(), who, ": tensors on several devices");
-}
-// Rows [tokens, heads, head_dim] with contiguous heads and a token stride.
-void kv4_rows(const Tensor& t, const Tensor& cache, const char* name, const char* who) {
-  chk(t, BF16, name);
-  TORCH_CHECK(t.dim() == 3 && t.stride(2) == 1 && (t.size(1) <= 1 || t.stride(1) == t.size(2)) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * t.size(2))),
-              who, ": ", name, " must be [tokens, heads, head_dim] with contiguous heads and a token stride of a multiple of 8");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, who, ": ", name, " must be 16-byte aligned");
-  TORCH_CHECK(t.device() == cache.device(), who, ": tensors on several devices");
 }
 
 int64_t kv4_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }

@@ -389,6 +389,9 @@ void kv_append_int4(const KvInt4Cache& c, const void* k, const void* v, const in
                     long long k_stride, long long v_stride, cudaStream_t stream);
 // The rows at (seq_ids, positions) as bf16 [tokens, kv_heads, head_dim]; a token without a page reads as zeros.
 void kv_read_int4(const KvInt4Cache& c, const int* positions, const int* seq_ids, int tokens, void* k, void* v, cudaStream_t stream);
+// The fused QKV epilogue (qkv_rope_append) with 4-bit pages.
+void qkv_rope_append_int4(float* acc, const int* pos, const int* seq_ids, void* q_out, const KvInt4Cache& c, int tokens, int heads,
+                          float theta, cudaStream_t stream);
 // One query token per sequence: q [batch, heads, head_dim] with a token stride, out contiguous. A sequence of length 0
 // gets zeros; a token of the context without a page is left out and reported through the status word.
 void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* context_lens, void* out, int batch,

@@ -20,6 +20,7 @@
 #include "api.h"
 #include "common.cuh"
 #include "host_util.h"
+#include "kv_int4.cuh"
 
 namespace mb {
 namespace {
@@ -225,13 +226,33 @@ tp_sum_residual_rmsnorm_kernel(float* __restrict__ acc, PeerPtrs staging, PeerPt
 // With k_cache8 / v_cache8 set the pages are int8: the head_dim / 16 threads of a head slot (adjacent
 // lanes, aligned in the warp) find max|x| with shuffles and store 8 + 8 bytes each plus one fp32
 // scale = max|x| / 127 per (token, kv head). Every lane of a warp reaches the shuffles: lanes past
-// the end of the work carry zeros and store nothing.
+// the end of the work carry zeros and store nothing. INT4: the pages (k_cache4 / v_cache4) are 4-bit (kv_int4.cuh): the
+// lanes of a head slot hold 8 + 8 values of two groups of 64 (head_dim 128) or of one (64).
+__device__ __forceinline__ void store_int4(uint8_t* tile, int n, bool is_k, int head_dim, int g, const bf16x8 (&x)[2],
+                                           const __nv_bfloat162 (&lo)[2], const __nv_bfloat162 (&hi)[2]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float scale, low;
+    const uint32_t pair = kv4_make_pair(__hmin_nan(lo[s].x, lo[s].y), __hmax_nan(hi[s].x, hi[s].y), scale, low);
+    const uint32_t w = kv4_word(x[s], scale, low, __frcp_rn(scale));
+    if (head_dim == 128) {
+      *reinterpret_cast<uint32_t*>(tile + (is_k ? kv4_key_word<128>(n, s, g) : kv4_value_word<128>(n, s, g))) = is_k ? kv4_rotate(w) : w;
+      if (g == 0) *reinterpret_cast<uint32_t*>(tile + kv4_pair<128>(n, s)) = pair;
+    } else {
+      *reinterpret_cast<uint32_t*>(tile + (is_k ? kv4_key_word<64>(n, 0, 4 * s + g) : kv4_value_word<64>(n, 0, 4 * s + g))) = is_k ? kv4_rotate(w) : w;
+      if (g == 0 && s == 0) *reinterpret_cast<uint32_t*>(tile + kv4_pair<64>(n, 0)) = pair;
+    }
+  }
+}
+
+template <bool INT4>
 __global__ void qkv_rope_append_kernel(float* __restrict__ acc, const int* __restrict__ pos,
                                        const int* __restrict__ seq_ids, const int* __restrict__ block_table,
                                        __nv_bfloat16* __restrict__ q_out, __nv_bfloat16* __restrict__ k_cache,
                                        __nv_bfloat16* __restrict__ v_cache, signed char* __restrict__ k_cache8,
                                        signed char* __restrict__ v_cache8, float* __restrict__ k_scale,
-                                       float* __restrict__ v_scale, int tokens, int heads, int kv_heads,
+                                       float* __restrict__ v_scale, uint8_t* __restrict__ k_cache4,
+                                       uint8_t* __restrict__ v_cache4, const Kv4Pages pages4, int tokens, int heads, int kv_heads,
                                        int head_dim, int page_size, int max_pages, float log2_theta) {
   const int half = head_dim >> 1, groups = half >> 3, slots = heads + 2 * kv_heads;
   const long long raw_gid = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -281,6 +302,27 @@ __global__ void qkv_rope_append_kernel(float* __restrict__ acc, const int* __res
     }
     for (int o = groups >> 1; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   }
+  bf16x8 x4[2];
+  __nv_bfloat162 lo4[2], hi4[2];
+  if constexpr (INT4) {
+    x4[0] = pack8(a);
+    x4[1] = pack8(b);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      lo4[s] = __hmin2_nan(__hmin2_nan(x4[s].v[0], x4[s].v[1]), __hmin2_nan(x4[s].v[2], x4[s].v[3]));
+      hi4[s] = __hmax2_nan(__hmax2_nan(x4[s].v[0], x4[s].v[1]), __hmax2_nan(x4[s].v[2], x4[s].v[3]));
+    }
+    if (head_dim == 64) {      // both halves belong to one group
+      lo4[0] = lo4[1] = __hmin2_nan(lo4[0], lo4[1]);
+      hi4[0] = hi4[1] = __hmax2_nan(hi4[0], hi4[1]);
+    }
+    for (int o = groups >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        lo4[s] = __hmin2_nan(lo4[s], __shfl_xor_sync(0xffffffffu, lo4[s], o));
+        hi4[s] = __hmax2_nan(hi4[s], __shfl_xor_sync(0xffffffffu, hi4[s], o));
+      }
+  }
   if (!valid) return;
   if (hs < heads) {
     __nv_bfloat16* dst = q_out + ((long long)t * heads + hs) * head_dim;
@@ -289,10 +331,16 @@ __global__ void qkv_rope_append_kernel(float* __restrict__ acc, const int* __res
     return;
   }
   const int seq = seq_ids[t];
-  const int page = block_table[(long long)seq * max_pages + p / page_size];
-  if (page < 0) return;
   const bool is_k = hs < heads + kv_heads;
   const int kvh = is_k ? hs - heads : hs - heads - kv_heads;
+  if constexpr (INT4) {
+    const int tile = pages4.tile(seq, p, kvh);
+    if (tile >= 0)
+      store_int4((is_k ? k_cache4 : v_cache4) + (long long)tile * (16 * (head_dim / 2 + head_dim / 16)), p & 15, is_k, head_dim, g, x4, lo4, hi4);
+    return;
+  }
+  const int page = block_table[(long long)seq * max_pages + p / page_size];
+  if (page < 0) return;
   const long long row = ((long long)page * page_size + p % page_size) * kv_heads + kvh;
   if (k_cache8 != nullptr) {
     const float inv = amax > 0.f ? 127.f / amax : 0.f;
@@ -387,11 +435,25 @@ void qkv_rope_append(float* acc, const int* pos, const int* seq_ids, const int* 
              "qkv_rope_append: int8 pages need head_dim / 16 lanes per head to be a power of two up to 16");
   if (tokens == 0) return;
   const long long work = (long long)tokens * (heads + 2 * kv_heads) * (head_dim / 16);
-  qkv_rope_append_kernel<<<(unsigned)ceil_div(work, 128), 128, 0, stream>>>(
+  qkv_rope_append_kernel<false><<<(unsigned)ceil_div(work, 128), 128, 0, stream>>>(
       acc, pos, seq_ids, block_table, (__nv_bfloat16*)q_out, int8 ? nullptr : (__nv_bfloat16*)k_cache,
       int8 ? nullptr : (__nv_bfloat16*)v_cache, int8 ? (signed char*)k_cache : nullptr,
-      int8 ? (signed char*)v_cache : nullptr, k_scale, v_scale, tokens, heads, kv_heads, head_dim, page_size, max_pages,
+      int8 ? (signed char*)v_cache : nullptr, k_scale, v_scale, nullptr, nullptr, Kv4Pages{}, tokens, heads, kv_heads, head_dim, page_size, max_pages,
       theta > 0.f ? log2f(theta) : 0.f);
+  count_launch();
+  check_launch();
+}
+
+void qkv_rope_append_int4(float* acc, const int* pos, const int* seq_ids, void* q_out, const KvInt4Cache& c, int tokens, int heads,
+                          float theta, cudaStream_t stream) {
+  MB_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "qkv_rope_append: 4-bit pages need a head_dim of 64 or 128");
+  MB_REQUIRE(c.page_size > 0 && c.page_size % 16 == 0, "qkv_rope_append: 4-bit pages hold a multiple of 16 tokens");
+  if (tokens == 0) return;
+  const long long work = (long long)tokens * (heads + 2 * c.kv_heads) * (c.head_dim / 16);
+  qkv_rope_append_kernel<true><<<(unsigned)ceil_div(work, 128), 128, 0, stream>>>(
+      acc, pos, seq_ids, c.block_table, (__nv_bfloat16*)q_out, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, (uint8_t*)c.k,
+      (uint8_t*)c.v, Kv4Pages{c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)}, tokens,
+      heads, c.kv_heads, c.head_dim, c.page_size, c.max_pages, theta > 0.f ? log2f(theta) : 0.f);
   count_launch();
   check_launch();
 }

@@ -177,6 +177,9 @@ def _embed_block(cfg: TransformerConfig) -> int:
     return cfg.oil_block_size if cfg.hidden_size % cfg.oil_block_size == 0 else 64
 
 
+KV_DTYPES = {"bf16": torch.bfloat16, "int8": torch.int8, "int4": torch.uint8}
+
+
 class _Layer:
     __slots__ = ("attn_norm", "ffn_norm", "qkv", "o", "up", "down")
 
@@ -188,11 +191,14 @@ class InferenceEngine:
     def __init__(self, cfg: TransformerConfig, device="cuda", max_batch: int = 64, max_seq_len: int | None = None,
                  page_size: int = 16, tp: TPContext | None = None, kv_pages: int | None = None,
                  kv_dtype: str = "bf16"):
-        """``kv_dtype``: "bf16", or "int8" for pages of int8 rows with one scale per (token, kv head)
+        """``kv_dtype``: "bf16", "int8" for pages of int8 rows with one scale per (token, kv head)
         (half the KV bytes per decode step; the reference's block-quantised cache mode,
-        src/kv_cache.cpp:13-42, 78-137)."""
-        if kv_dtype not in ("bf16", "int8"):
-            raise ValueError(f"kv_dtype must be 'bf16' or 'int8', got {kv_dtype!r}")
+        src/kv_cache.cpp:13-42, 78-137), or "int4" for pages of 4-bit codes with a scale and a minimum per 64
+        values (9/32 of the bytes; head widths 64 and 128)."""
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype must be one of {sorted(KV_DTYPES)}, got {kv_dtype!r}")
+        if kv_dtype == "int4" and (cfg.head_dim not in (64, 128) or page_size % 16):
+            raise ValueError("4-bit pages need a head width of 64 or 128 and pages of a multiple of 16 tokens")
         self.cfg, self.device, self.tp = cfg, torch.device(device), tp
         self.max_batch = max_batch
         self.max_seq_len = max_seq_len or cfg.max_seq_len
@@ -215,7 +221,7 @@ class InferenceEngine:
         pages_per_seq = (self.max_seq_len + page_size - 1) // page_size
         self.cache = PagedKVCache(cfg.num_layers, self.hkv_local, cfg.head_dim, kv_pages or max_batch * pages_per_seq,
                                   page_size, max_batch, pages_per_seq, self.device,
-                                  dtype=torch.int8 if kv_dtype == "int8" else torch.bfloat16)
+                                  dtype=KV_DTYPES[kv_dtype])
         self.layers: list[_Layer] = []
         self.embed = None        # bf16 [V, d], or a QuantLinear when the table is stored in an OIL format
         self.final_norm = None
@@ -472,6 +478,9 @@ class InferenceEngine:
                 C.qkv_rope_append(acc, pos, seq_ids, table, q, self.cache.k[li], self.cache.v[li], cfg.rope_theta, ks, vs)
                 C.paged_attn_decode_int8(q, self.cache.k[li], self.cache.v[li], ks, vs, table, ctx_lens, o,
                                          self._scratch, self._counters, self._splits, scale, st)
+            elif self.cache.int4:
+                C.qkv_rope_append(acc, pos, seq_ids, table, q, self.cache.k[li], self.cache.v[li], cfg.rope_theta)
+                C.paged_attn_decode_int4(q, self.cache.k[li], self.cache.v[li], table, ctx_lens, o, scale, st)
             else:
                 C.qkv_rope_append(acc, pos, seq_ids, table, q, self.cache.k[li], self.cache.v[li], cfg.rope_theta)
                 C.paged_attn_decode(q, self.cache.k[li], self.cache.v[li], table, ctx_lens, o, self._scratch,
@@ -516,14 +525,12 @@ class InferenceEngine:
             if self.cache.int8:
                 C.kv_append_int8(k, v, self.cache.k[li], self.cache.v[li], self.cache.k_scale[li],
                                  self.cache.v_scale[li], table, pos, seq_ids)
+            elif self.cache.int4:
+                C.kv_append_int4(k, v, self.cache.k[li], self.cache.v[li], table, pos, seq_ids)
             else:
                 C.kv_append(k, v, self.cache.k[li], self.cache.v[li], table, pos, seq_ids)
             if paged is not None:
-                cu_q, kv_lens, rows, max_q = paged[:4]
-                o = torch.empty(T, H, D, device=self.device, dtype=torch.bfloat16)
-                C.flash_attn_paged_prefill(q, self.cache.k[li], self.cache.v[li], rows, cu_q, kv_lens, o, max_q, scale,
-                                           native.status_word(self.device))
-                o = o.view(T, H * D)
+                o = self._paged_attention(li, q, paged, scale).view(T, H * D)
             elif prefill_shape is not None:
                 B, S = prefill_shape
                 o = torch.empty(B, S, H, D, device=self.device, dtype=torch.bfloat16)
@@ -539,6 +546,9 @@ class InferenceEngine:
                     C.paged_attn_decode_int8(q, self.cache.k[li], self.cache.v[li], self.cache.k_scale[li],
                                              self.cache.v_scale[li], table, ctx_lens, o, self._scratch,
                                              self._counters, self._splits, scale, native.status_word(self.device))
+                elif self.cache.int4:
+                    C.paged_attn_decode_int4(q, self.cache.k[li], self.cache.v[li], table, ctx_lens, o, scale,
+                                             native.status_word(self.device))
                 else:
                     C.paged_attn_decode(q, self.cache.k[li], self.cache.v[li], table, ctx_lens, o,
                                         self._scratch, self._counters, self._splits, scale,
@@ -567,6 +577,18 @@ class InferenceEngine:
         return (cfg.hidden_size >= 256 and cfg.hidden_size % 64 == 0
                 and all(m.K % 64 == 0 for L in self.layers for m in (L.qkv, L.up)))
 
+    def _paged_attention(self, li, q, paged, scale):
+        """Attention of packed new tokens over the pages of layer ``li`` (which hold them already)."""
+        C = native.require()
+        cu_q, kv_lens, rows, max_q = paged[:4]
+        o = torch.empty(q.shape, device=self.device, dtype=torch.bfloat16)
+        k, v, st = self.cache.k[li], self.cache.v[li], native.status_word(self.device)
+        if self.cache.int4:
+            C.paged_attn_prefill_int4(q, k, v, rows, cu_q, kv_lens, o, max_q, paged[6], scale, st)
+        else:
+            C.flash_attn_paged_prefill(q, k, v, rows, cu_q, kv_lens, o, max_q, scale, st)
+        return o
+
     def _attention_prefill(self, li, qkv, pos, seq_ids, prefill_shape, paged):
         """RoPE, K/V append and prefill attention for all tokens over this rank's heads -> [T, H_local * D]."""
         cfg, C = self.cfg, native.require()
@@ -582,14 +604,12 @@ class InferenceEngine:
         if self.cache.int8:
             C.kv_append_int8(k, v, self.cache.k[li], self.cache.v[li], self.cache.k_scale[li], self.cache.v_scale[li],
                              table, pos, seq_ids)
+        elif self.cache.int4:
+            C.kv_append_int4(k, v, self.cache.k[li], self.cache.v[li], table, pos, seq_ids)
         else:
             C.kv_append(k, v, self.cache.k[li], self.cache.v[li], table, pos, seq_ids)
         if paged is not None:
-            cu_q, kv_lens, rows, max_q = paged[:4]
-            o = torch.empty(T, H, D, device=self.device, dtype=torch.bfloat16)
-            C.flash_attn_paged_prefill(q, self.cache.k[li], self.cache.v[li], rows, cu_q, kv_lens, o, max_q, scale,
-                                       native.status_word(self.device))
-            return o.view(T, H * D)
+            return self._paged_attention(li, q, paged, scale).view(T, H * D)
         B, S = prefill_shape
         o = torch.empty(B, S, H, D, device=self.device, dtype=torch.bfloat16)
         lse = torch.empty(B, H, S, device=self.device, dtype=torch.float32)
@@ -668,7 +688,7 @@ class InferenceEngine:
 
     # ------------------------------------------------------------------ paged / chunked prefill
     def _paged_prefill_ok(self) -> bool:
-        return not self.cache.int8 and self.cfg.head_dim in (64, 128) and self.cache.page_size == 16
+        return self.cache.int4 or (not self.cache.int8 and self.cfg.head_dim in (64, 128) and self.cache.page_size == 16)
 
     @torch.no_grad()
     def _prefill_paged(self, seqs, token_lists, bases):

@@ -4,7 +4,7 @@ reference counts (shared prefix pages), optional host offload of cold pages.
 Covers the reference's ``KVCache`` (contiguous, src/kv_cache.cpp:44-238), ``PagedAttention`` block
 pool (src/inference_opt.cpp:14-57), ``PagedKVCache1T`` (hierarchical table + LRU offload to disk,
 src/kv_cache.cpp:244-642) and ``PrefixCache`` (src/inference_opt.cpp:460-520) with one design: a
-flat page pool per layer on the GPU (``[pages, page_size, kv_heads, head_dim]`` bf16), an int32
+flat page pool per layer on the GPU (``[pages, page_size, kv_heads, head_dim]`` bf16; int8 and 4-bit pages), an int32
 block table ``[max_seqs, max_pages_per_seq]`` that the attention kernels index directly, and an
 offload tier in pinned host memory (the disk files of the reference are replaced by host RAM;
 ``save_pages`` / ``load_pages`` still give a file tier when asked for).
@@ -15,6 +15,8 @@ import hashlib
 from collections import OrderedDict
 
 import torch
+
+from ..ops.reference import KV4_TILE, kv4_token_bytes
 
 
 class PageAllocator:
@@ -76,7 +78,9 @@ class PagedKVCache:
     def __init__(self, num_layers: int, kv_heads: int, head_dim: int, num_pages: int, page_size: int = 16,
                  max_seqs: int = 64, max_pages_per_seq: int = 256, device="cuda", dtype=torch.bfloat16,
                  layer_shapes=None, states: RecurrentStatePool | None = None):
-        """``layer_shapes``: per attention layer ``(kv_heads, key width, value width)`` where the layers
+        """``dtype``: bfloat16, float32, int8 (rows with one scale per token and kv head) or uint8 (4-bit pages
+        ``[pages, kv_heads, page_size * kv4_token_bytes(head_dim)]``, ``ops.functional.kv_append_int4``);
+        ``layer_shapes``: per attention layer ``(kv_heads, key width, value width)`` where the layers
         differ or the two widths do; ``states``: the recurrent layers' per-sequence state, which follows
         the sequence slots (a prefix is then never shared: its pages alone do not determine the rest)."""
         self.num_layers, self.kv_heads, self.head_dim = num_layers, kv_heads, head_dim
@@ -84,10 +88,18 @@ class PagedKVCache:
         self.device = torch.device(device)
         self.states = states
         shapes = layer_shapes if layer_shapes is not None else [(kv_heads, head_dim, head_dim)] * num_layers
-        if len(shapes) != num_layers or (layer_shapes is not None and dtype == torch.int8):
-            raise ValueError("layer_shapes: one entry per layer, not with int8 pages")
-        self.k = [torch.zeros((num_pages, page_size, g, dk), device=self.device, dtype=dtype) for g, dk, _ in shapes]
-        self.v = [torch.zeros((num_pages, page_size, g, dv), device=self.device, dtype=dtype) for g, _, dv in shapes]
+        if len(shapes) != num_layers or (layer_shapes is not None and dtype in (torch.int8, torch.uint8)):
+            raise ValueError("layer_shapes: one entry per layer, not with int8 or 4-bit pages")
+        self.int4 = dtype == torch.uint8
+        if self.int4:
+            if page_size % KV4_TILE:
+                raise ValueError(f"4-bit pages hold a multiple of {KV4_TILE} tokens, got {page_size}")
+            record = (num_pages, kv_heads, page_size * kv4_token_bytes(head_dim))
+            self.k = [torch.zeros(record, device=self.device, dtype=dtype) for _ in range(num_layers)]
+            self.v = [torch.zeros(record, device=self.device, dtype=dtype) for _ in range(num_layers)]
+        else:
+            self.k = [torch.zeros((num_pages, page_size, g, dk), device=self.device, dtype=dtype) for g, dk, _ in shapes]
+            self.v = [torch.zeros((num_pages, page_size, g, dv), device=self.device, dtype=dtype) for g, _, dv in shapes]
         # int8 pages carry one fp32 scale (max|x| / 127) per (token, kv head); the append kernel
         # writes them and the decode kernel folds them into the score and the probability
         self.int8 = dtype == torch.int8

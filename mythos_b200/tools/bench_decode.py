@@ -34,7 +34,7 @@ def main(argv=None) -> int:
     ap.add_argument("--layers", type=int, default=0, help="use only this many layers (0 = all)")
     ap.add_argument("--vocab", type=int, default=0, help="override the vocabulary size (0 = preset)")
     ap.add_argument("--repeat", type=int, default=3)
-    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "int8"], help="KV page storage")
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "int8", "int4"], help="KV page storage")
     ap.add_argument("--no-graph", action="store_true", help="launch decode steps one by one (for launch lists)")
     a = ap.parse_args(argv)
     world = int(os.environ.get("WORLD_SIZE", "1"))

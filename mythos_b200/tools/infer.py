@@ -31,8 +31,9 @@ def build_parser():
     ap.add_argument("--batch-size", type=int, default=1)
     ap.add_argument("--output", "-o", default=None)
     ap.add_argument("--gpu", "--device", dest="device", default="auto")
-    ap.add_argument("--precision", default="auto", choices=["auto", "fp32", "fp16", "bf16", "int8"],
-                    help="int8: int8 KV pages on the GPU engine, int8 activations on the CPU path; the other "
+    ap.add_argument("--precision", default="auto", choices=["auto", "fp32", "fp16", "bf16", "int8", "int4"],
+                    help="int8: int8 KV pages on the GPU engine, int8 activations on the CPU path; int4: 4-bit KV pages on the "
+                         "GPU engine (the CPU path keeps no cache and refuses it); the other "
                          "values keep the engine's bf16 compute (GPU) / fp32 reference ops (CPU). Layer-list models: fp32 runs "
                          "everything in 32-bit floats, other values bf16")
     ap.add_argument("--verbose", action="store_true")
@@ -54,10 +55,10 @@ def generate_text(model, tokenizer, prompt: str, max_tokens: int, sampler, devic
         S = len(ids)
         if isinstance(model.cfg, TransformerConfig):
             kw = {"max_seq_len": min(model.cfg.max_seq_len, S + max_tokens) + 16,
-                  "kv_dtype": "int8" if precision == "int8" else "bf16"}
+                  "kv_dtype": precision if precision in ("int8", "int4") else "bf16"}
         else:
-            if precision == "int8":
-                raise ValueError("int8 pages are not available for layer-list models")
+            if precision in ("int8", "int4"):
+                raise ValueError(f"{precision} pages are not available for layer-list models")
             kw = {"max_seq_len": min(model.cfg.max_seq_len, S + max_tokens + 16),
                   "dtype": "float32" if precision == "fp32" else "bfloat16"}
         eng = InferenceEngine.from_model(model, device=device, max_batch=1, **kw)
@@ -67,6 +68,8 @@ def generate_text(model, tokenizer, prompt: str, max_tokens: int, sampler, devic
         new = res.tokens[0]
         stats = {"tokens_per_s": res.stats.tokens_per_s, "ttft_s": res.stats.ttft_s}
     else:
+        if precision == "int4":
+            raise ValueError("4-bit KV pages need the GPU engine")
         seq = torch.tensor([ids], dtype=torch.int32)
         new = []
         ttft = None

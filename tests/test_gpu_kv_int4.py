@@ -253,3 +253,96 @@ def test_refusals_on_the_gpu():
             pytest.fail(f"call {i} was not refused")
     empty = F.paged_attn_decode_int4(q[:0], kc, vc, table, ctx[:0])
     assert empty.shape == (0, 4, 128)
+
+
+# ------------------------------------------------------------------------------------------------ together, in the engine
+@pytest.mark.parametrize("D", [128, 64])
+def test_fused_epilogue_writes_what_rope_and_append_write(D):
+    C = native.require()
+    torch.manual_seed(D)
+    H, Hk, page, T = 4, 2, 32, 5
+    kc, vc, table = make_cache([40] * T, Hk, D, page, "cuda")
+    kr, vr = kc.clone(), vc.clone()
+    acc = torch.randn(T, (H + 2 * Hk) * D, device="cuda") * 2
+    qkv = acc.to(torch.bfloat16)
+    pos = torch.tensor([5, 17, 0, 33, 2], device="cuda", dtype=torch.int32)
+    sid = torch.arange(T, device="cuda", dtype=torch.int32)
+    sid[4] = T + 3                                  # outside the table: dropped
+    q = torch.empty(T, H, D, device="cuda", dtype=torch.bfloat16)
+    C.qkv_rope_append(acc, pos, sid, table, q, kc, vc, 10000.0)
+    qk = qkv[:, : (H + Hk) * D].clone().unflatten(-1, (H + Hk, D))
+    C.rope(qk, pos, 10000.0, False)
+    F.kv_append_int4(qk[:, H:].contiguous(), qkv[:, (H + Hk) * D:].unflatten(-1, (Hk, D)), kr, vr, table, pos, sid)
+    assert torch.equal(vc, vr) and float(acc.abs().max()) == 0.0
+    # the two rotations round differently in places: a key may be a bf16 step off, its code then one step of the grid
+    got, want = (F.kv_read_int4(c, vc, table, pos, sid, D)[0].float() for c in (kc, kr))
+    step = (want.unflatten(-1, (-1, 64)).amax(-1) - want.unflatten(-1, (-1, 64)).amin(-1)) / 15
+    assert ((got - want).abs().unflatten(-1, (-1, 64)) <= 1.1 * step[..., None] + 2 * HALF * want.abs().amax()).all()
+    assert float((q.float() - qk[:, :H].float()).abs().max()) <= 2 * HALF * float(qk.float().abs().max())
+
+
+def _engine(kv_dtype, D=128, **kw):
+    from mythos_b200.infer.engine import InferenceEngine
+    from mythos_b200.models import TransformerConfig
+
+    cfg = TransformerConfig(vocab_size=512, hidden_size=256, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=D,
+                            ffn_hidden_size=512, max_seq_len=512, oil_block_size=256, codebook_group=2)
+    return InferenceEngine.random(cfg, seed=7, device="cuda", max_batch=8, max_seq_len=512, kv_dtype=kv_dtype, **kw)
+
+
+def _off(a, b):
+    return float((a.float() - b.float()).norm() / b.float().norm())
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_engine_over_4_bit_pages(D):
+    """Prompts, portions, prefix hits, decoding, offload: logits of the 4-bit engine against the bf16 engine's and against
+    each other. A 4-bit value is a step / sqrt(12) off, a tenth of its spread: logits stay within a quarter; two ways to the
+    same pages differ by bf16 roundings that move a few codes by a step: half of that."""
+    g = torch.Generator().manual_seed(1)
+    head = torch.randint(0, 512, (150,), generator=g).tolist()
+    a, b = head + [5, 6, 7], head + [9, 10, 11, 12, 13]
+    wide, eng = _engine("bf16", D), _engine("int4", D)
+    assert eng.cache.int4 and eng.cache.size_bytes() * 32 == wide.cache.size_bytes() * 9
+    ref_logits = wide.start_sequence(b, reuse_prefix=False)[1]
+    sa, la = eng.start_sequence(a)
+    sb, lb = eng.start_sequence(b)                       # over the shared pages of the first prompt
+    assert eng.last_prefix_hit == 144
+    sc, lc = eng.start_sequence(b, reuse_prefix=False)
+    assert _off(lb, ref_logits) < 0.25 and _off(lc, ref_logits) < 0.25 and _off(lb, lc) < 0.25
+    seq = eng.cache.new_sequence()                       # the same prompt in portions through step()
+    for lo in range(0, len(b), 61):
+        ls = eng.step([seq], [b[lo:lo + 61]])
+    assert _off(ls, lb) < 0.125
+    tokens = [int(lb.float().argmax())] * 4
+    out = eng.decode([sa, sb, sc, seq], tokens)
+    assert _off(out[1], out[3]) < 0.125 and out.isfinite().all()
+    eng.fused_decode = False                             # one more token through the separate kernels and through step()
+    handle = eng.cache.offload_sequence(sb)
+    sb = eng.cache.restore_sequence(handle)
+    eng.cache.sync_tables()
+    one = eng.decode([sb], [3])
+    many = eng.step([seq], [[3]])
+    assert _off(one, many) < 0.125
+    for s in (sa, sb, sc, seq):
+        eng.release(s)
+    assert eng.cache.alloc.used == 0
+    native.check_status("cuda")
+
+
+def test_engine_generates_over_4_bit_pages():
+    from mythos_b200.infer.serving import ContinuousBatcher
+
+    eng = _engine("int4")
+    g = torch.Generator().manual_seed(3)
+    prompts = torch.randint(0, 512, (2, 128), generator=g, dtype=torch.int32)
+    eager = eng.generate(prompts, max_new_tokens=12, use_graph=False).tokens
+    assert eng.generate(prompts, max_new_tokens=12, use_graph=True).tokens == eager
+    ragged = [prompts[0].tolist(), prompts[1, :77].tolist(), [4]]
+    res = eng.generate(ragged, max_new_tokens=5)
+    assert [len(t) for t in res.tokens] == [5, 5, 5]
+    batcher = ContinuousBatcher(eng, chunk_tokens=40)
+    reqs = [batcher.submit(p, max_new_tokens=6) for p in ragged]
+    batcher.run_until_idle()
+    assert all(len(r.output) == 6 for r in reqs) and eng.cache.alloc.used == 0
+    native.check_status("cuda")

@@ -127,3 +127,46 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_paged_cache_of_4_bit_pages():
+    from mythos_b200.infer.kv_paged import PagedKVCache
+
+    c = PagedKVCache(2, 3, 128, num_pages=8, page_size=32, max_seqs=2, max_pages_per_seq=4, device="cpu", dtype=torch.uint8)
+    wide = PagedKVCache(2, 3, 128, num_pages=8, page_size=32, max_seqs=2, max_pages_per_seq=4, device="cpu")
+    assert c.int4 and not wide.int4 and c.size_bytes() * 32 == wide.size_bytes() * 9
+    s = c.new_sequence()
+    c.reserve(s, 40)
+    c.sync_tables()
+    k, v = random_rows(40, 3, 128, 0, "cpu")
+    pos, sid = token_lists([0], [40], "cpu")
+    for li in range(2):
+        F.kv_append_int4(k, v, c.k[li], c.v[li], c.block_table, pos, sid)
+    c.advance(s, 40)
+    want = F.kv_read_int4(c.k[1], c.v[1], c.block_table, pos, sid, 128)
+    other = c.new_sequence()
+    c.reserve(other, 20)                          # so that the pages move
+    s = c.restore_sequence(c.offload_sequence(s))
+    c.sync_tables()
+    got = F.kv_read_int4(c.k[1], c.v[1], c.block_table, pos, torch.full_like(sid, s), 128)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 1, 128, 4, page_size=24, device="cpu", dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 1, 96, 4, device="cpu", dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 1, 64, 4, device="cpu", dtype=torch.uint8, layer_shapes=[(1, 64, 64)])
+
+
+def test_engine_refuses_what_4_bit_pages_cannot_hold():
+    from mythos_b200.infer.engine import InferenceEngine
+    from mythos_b200.models import TransformerConfig
+
+    cfg = TransformerConfig(vocab_size=64, hidden_size=96, num_layers=1, num_heads=1, head_dim=96, ffn_hidden_size=64, max_seq_len=64)
+    with pytest.raises(ValueError):
+        InferenceEngine(cfg, device="cpu", kv_dtype="int4")
+    cfg.head_dim = 64
+    with pytest.raises(ValueError):
+        InferenceEngine(cfg, device="cpu", kv_dtype="int4", page_size=8)
+    with pytest.raises(ValueError):
+        InferenceEngine(cfg, device="cpu", kv_dtype="fp4")
