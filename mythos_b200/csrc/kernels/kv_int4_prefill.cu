@@ -184,7 +184,7 @@ struct PfCfg {
   static constexpr int OFF_K = 2 * TILE_BYTES;
   static constexpr int OFF_V = OFF_K + KS * TILE_BYTES;
   static constexpr int OFF_BAR = OFF_V + VS * TILE_BYTES;
-  static constexpr int NUM_BARS = 4 + 2 * KS + 2 * VS + 6;
+  static constexpr int NUM_BARS = 4 + 2 * KS + 2 * VS + 8;
   static constexpr int SMEM_BYTES = OFF_BAR + NUM_BARS * 8 + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
   static constexpr int COL_S = 0;     // S_t at t * 128 (P_t over its first 64 columns)
@@ -250,8 +250,8 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   uint64_t* v_full = k_empty + KS;         // [VS]
   uint64_t* v_empty = v_full + VS;
   uint64_t* s_full = v_empty + VS;         // [2]
-  uint64_t* p_full = s_full + 2;           // [2]
-  uint64_t* o_full = p_full + 2;           // [2]
+  uint64_t* p_full = s_full + 2;           // [2 tiles][2 halves of the keys]
+  uint64_t* o_full = p_full + 4;           // [2]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   int* status = a.status;
@@ -263,7 +263,8 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       mbar_init(&q_full[t], 1);
       mbar_init(&q_free[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 128);
+      mbar_init(&p_full[2 * t], 128);
+      mbar_init(&p_full[2 * t + 1], 128);
       mbar_init(&o_full[t], 1);
     }
     for (int s = 0; s < KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
@@ -371,8 +372,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (j >= it.J[t] || !ok) continue;
-            if (!mbar_wait(&p_full[t], n_p[t] & 1, abort_flag, status, 99)) { ok = false; break; }
-            ++n_p[t];
+            if (!mbar_wait(&p_full[2 * t], n_p[t] & 1, abort_flag, status, 99)) { ok = false; break; }
             if (!v_ready) {
               if (!mbar_wait(&v_full[vc % VS], (vc / VS) & 1, abort_flag, status, 100)) { ok = false; break; }
               v_ready = true;
@@ -380,9 +380,16 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             tc_fence_after();
             const uint32_t va = v_addr + (vc % VS) * Cfg::TILE_BYTES;
 #pragma unroll
-            for (int k = 0; k < PF_TILE / 16; ++k)   // O_t += P_t(tmem) V
+            for (int k = 0; k < PF_TILE / 16; ++k) {   // O_t += P_t(tmem) V, the second half while its exponentials run
+              if (k == PF_TILE / 32) {
+                if (!mbar_wait(&p_full[2 * t + 1], n_p[t] & 1, abort_flag, status, 104)) { ok = false; break; }
+                tc_fence_after();
+              }
               umma_f16_ts(tmem_base + Cfg::COL_O + t * D, tmem_base + Cfg::COL_S + t * 128 + k * 8,
                           umma_desc_sw128(va + k * 2048, PF_TILE * 128, 1024), IDESC_O, (j > 0 || k > 0) ? 1u : 0u);
+            }
+            if (!ok) break;
+            ++n_p[t];
             if (j == it.J[t] - 1) umma_commit(&o_full[t]);
             if (j + 1 < it.J[t]) {
               if (!k_ready) {
@@ -491,22 +498,24 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
         uint32_t* pk = &sr[0][0];         // packed in place: pair i lands in word i / 2, behind the read position
 #pragma unroll
-        for (int i = 0; i < 128; i += 2) {
-          float e0f, e1f;
-          f32x2_unpack(fma_f32x2(f32x2(s[i], s[i + 1]), sc2, nm2), e0f, e1f);
-          const float p0 = fast_exp2(e0f), p1 = fast_exp2(e1f);
-          rs2[(i >> 1) & 3] = add_f32x2(rs2[(i >> 1) & 3], f32x2(p0, p1));
-          pk[i >> 1] = pf_half2(p0, p1);
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int i = 64 * h; i < 64 * h + 64; i += 2) {
+            float e0f, e1f;
+            f32x2_unpack(fma_f32x2(f32x2(s[i], s[i + 1]), sc2, nm2), e0f, e1f);
+            const float p0 = fast_exp2(e0f), p1 = fast_exp2(e1f);
+            rs2[(i >> 1) & 3] = add_f32x2(rs2[(i >> 1) & 3], f32x2(p0, p1));
+            pk[i >> 1] = pf_half2(p0, p1);
+          }
+          tmem_st32(t_s + 32 * h, sr[h]);   // P_t: fp16 pairs over the first 64 columns of S_t
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&p_full[2 * t + h]);
         }
         float rs[8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
         l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(e0 - e);
-        tmem_st32(t_s, sr[0]);            // P_t: fp16 pairs over the first 64 columns of S_t
-        tmem_st32(t_s + 32, sr[1]);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
       if (Jt > 0) {
