@@ -413,7 +413,7 @@ long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, i
 void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                     long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,
                     cudaStream_t stream);
-long long prompt_int4_workspace(int batch, int total_q, int max_kv, int heads, int kv_heads, int head_dim);
+long long prompt_int4_workspace(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
 void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                  long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,
                  int* status, cudaStream_t stream);

@@ -202,7 +202,7 @@ bool p4_few(int max_q, int group) { return (long long)max_q * group <= P4_FEW_CO
 long long paged_attn_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads) {
   if (batch == 0 || max_q == 0 || c.kv_heads <= 0) return 0;
   const int G = heads / c.kv_heads;
-  if (!p4_few(max_q, G)) return prompt_int4_workspace(batch, total_q, max_kv, heads, c.kv_heads, c.head_dim);
+  if (!p4_few(max_q, G)) return prompt_int4_workspace(batch, total_q, max_q, max_kv, heads, c.kv_heads, c.head_dim);
   return few_query_int4_workspace(c, batch, max_q, heads);
 }
 

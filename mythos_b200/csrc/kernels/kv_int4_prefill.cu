@@ -1,6 +1,6 @@
 // Attention of prompts over the 4-bit paged KV cache: tcgen05 products on fp16 images of the pages.
 //
-// Two launches. kv4_expand_kernel turns every sequence's pages into 128-token tiles [batch, kv_heads, tokens, D] of
+// kv4_expand_kernel turns every sequence's pages into 128-token tiles [batch, kv_heads, tokens, D] of
 // fp16 in a workspace, once for all the queries that read them, and the queries into fp16 rows; fa_int4_kernel is the
 // persistent two-tile flash attention kernel of attention_fwd2.cu over those images (128 x 128 score tiles, P in tensor memory).
 //
@@ -17,10 +17,16 @@
 // finite goes there: tokens behind a sequence's end are zeros, and a token with a scale that is not finite gets values of
 // zero and NaN keys, which reach the queries that see it through their scores, and no others.
 //
+// The work is a line of (item, key tile) steps, an item being 256 query rows of one kv head, cut into equal stretches, one per
+// CTA: with whole items per CTA the 256 items of 2048 new tokens left every fourth SM idle for half of the time. What a border
+// cuts is written as an unnormalised part and joined by a third kernel.
+//
 // Rows of a query tile are (token, head) pairs of one kv head when the group divides 128 (a box of GP heads x 128 / GP tokens
 // in one TMA load), so that short prompts fill their tiles and the heads of a group read a K / V tile once; other groups run one
 // head at a time.
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "api.h"
 #include "host_util.h"
@@ -58,6 +64,52 @@ __device__ __forceinline__ uint4 pf_expand8(uint32_t w, uint32_t pair, float inv
   return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
+// ------------------------------------------------------------------------------------------------ the line of steps
+// A pair is (sequence, block of 256 query rows); its items, one per unit (`pack` heads of a kv head), stand side by side, each
+// with as many steps as its last row sees key tiles (at least one, so that rows that see nothing get their zeros).
+struct PfLine {
+  const int* cu_q;
+  const int* kv_lens;
+  int batch, pack, units, n_qb, tiles;
+};
+struct PfItem {
+  int b, row0, q_len, q_off, kv_len, tok[2], J[2], steps;   // tok: first token of each tile; J: its key tiles
+  bool live[2];
+  __device__ __forceinline__ PfItem(const PfLine& a, int pair) {
+    b = pair / a.n_qb;
+    const int blk = pair - b * a.n_qb, per = PF_TILE / a.pack;     // tokens of a tile
+    row0 = a.cu_q[b];
+    q_len = a.cu_q[b + 1] - row0;
+    kv_len = a.kv_lens[b];
+    q_off = kv_len - q_len;
+    steps = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      tok[t] = (2 * blk + t) * per;
+      live[t] = tok[t] < q_len;
+      const int hi = live[t] ? min(kv_len, q_off + min(q_len, tok[t] + per)) : 0;
+      J[t] = min(a.tiles, (max(hi, 0) + PF_TILE - 1) / PF_TILE);
+      if (live[t]) steps = max(steps, max(1, J[t]));
+    }
+  }
+};
+// Written by the expansion, read by the attention and the merge: [0] steps of a stretch, [1] how many stretches have one more,
+// [2] stretches; then where every pair begins (pairs + 1), then (pair, unit, step, steps) of every stretch's start.
+struct PfPlan {
+  int* p;
+  int pairs;
+  __device__ __forceinline__ int per() const { return p[0]; }
+  __device__ __forceinline__ int rem() const { return p[1]; }
+  __device__ __forceinline__ int count() const { return p[2]; }
+  __device__ __forceinline__ int* begin() const { return p + 3; }
+  __device__ __forceinline__ int* start(int c) const { return p + 4 + pairs + 4 * c; }
+};
+__device__ __forceinline__ int pf_start(int per, int rem, int c) { return c * per + min(c, rem); }
+__device__ __forceinline__ int pf_owner(int per, int rem, int place) {       // whose stretch holds it
+  const int longer = rem * (per + 1);
+  return place < longer ? place / (per + 1) : rem + (place - longer) / max(per, 1);
+}
+
 struct PfExpand {
   const uint8_t* k_cache;
   const uint8_t* v_cache;
@@ -70,16 +122,92 @@ struct PfExpand {
   __half* qh;           // [total_q, heads, D]
   float* q_factor;      // [total_q, heads]: 2^eq
   int* exponents;       // [batch * kv_heads, tiles]: ek in the low, ev in the high half
-  int kv_heads, heads, tiles, kv_blocks, total_q;
+  int kv_heads, heads, tiles, kv_blocks, q_blocks, total_q;
+  PfLine line;
+  PfPlan plan;
+  int ctas;
+  bool whole;           // a whole item per stretch
   int* status;
 };
 
-// Blocks [0, kv_blocks): one 128-token tile of one (sequence, kv head). The rest: query rows, one per D / 8 lanes.
+constexpr int PF_MIN_STEPS = 4;   // of a stretch: a step is about 2 us, setting up and writing a part a few
+// Where there are no more items than CTAs and none has more steps than this, every CTA takes a whole one, and there is no merge:
+// 6 ragged prompts of up to 700 tokens take 21 us so and 26 with equal stretches.
+constexpr int PF_WHOLE_STEPS = 12;
+
+// One block: the plan. Every thread takes a run of pairs.
+__device__ void pf_make_plan(const PfExpand& a) {
+  __shared__ int s_sum[PF_EXPAND / 32], s_total;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (a.plan.pairs + PF_EXPAND - 1) / PF_EXPAND, p0 = min(a.plan.pairs, (int)threadIdx.x * each), p1 = min(a.plan.pairs, p0 + each);
+  int sum = 0;
+  for (int p = p0; p < p1; ++p) sum += PfItem(a.line, p).steps * a.line.units;
+  int up = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += v;
+  }
+  if (lane == 31) s_sum[warp] = up;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int t = 0;
+    for (int w = 0; w < PF_EXPAND / 32; ++w) {
+      const int v = s_sum[w];
+      s_sum[w] = t;
+      t += v;
+    }
+    s_total = t;
+  }
+  __syncthreads();
+  const int total = s_total;
+  if (a.whole) {                                  // one item per stretch; items without steps in between are none
+    for (int p = p0; p < p1; ++p) {
+      const int steps = PfItem(a.line, p).steps;
+      for (int u = 0; u < a.line.units; ++u) {
+        int* s = a.plan.start(p * a.line.units + u);
+        s[0] = p;
+        s[1] = u;
+        s[2] = 0;
+        s[3] = steps;
+      }
+    }
+    if (threadIdx.x == 0) a.plan.p[2] = a.plan.pairs * a.line.units;
+    return;
+  }
+  const int count = max(1, min(a.ctas, total / PF_MIN_STEPS)), per = total / count, rem = total - per * count;
+  int place = s_sum[warp] + up - sum;
+  for (int p = p0; p < p1; ++p) {
+    const int steps = PfItem(a.line, p).steps, end = place + steps * a.line.units;
+    a.plan.begin()[p] = place;
+    for (int c = place > 0 ? pf_owner(per, rem, place - 1) + 1 : 0; c < count && pf_start(per, rem, c) < end; ++c) {
+      const int at = pf_start(per, rem, c) - place;
+      int* s = a.plan.start(c);
+      s[0] = p;
+      s[1] = at / steps;
+      s[2] = at - at / steps * steps;
+      s[3] = per + (c < rem ? 1 : 0);
+    }
+    place = end;
+  }
+  if (threadIdx.x == 0) {
+    a.plan.p[0] = per;
+    a.plan.p[1] = rem;
+    a.plan.p[2] = total > 0 ? count : 0;
+    a.plan.begin()[a.plan.pairs] = total;
+  }
+}
+
+// Blocks [0, kv_blocks): one 128-token tile of one (sequence, kv head). Then query rows, one per D / 8 lanes; then the plan.
 template <int D>
 __global__ void __launch_bounds__(PF_EXPAND)
 kv4_expand_kernel(const __grid_constant__ PfExpand a) {
   using L = KvInt4<D>;
   constexpr int WORDS = D / 8;
+  if ((int)blockIdx.x == a.kv_blocks + a.q_blocks) {
+    pf_make_plan(a);
+    return;
+  }
   if ((int)blockIdx.x >= a.kv_blocks) {
     const long long row = ((long long)blockIdx.x - a.kv_blocks) * (PF_EXPAND / WORDS) + threadIdx.x / WORDS;
     const int c = threadIdx.x % WORDS;
@@ -192,43 +320,59 @@ struct PfCfg {
 };
 
 struct PfArgs {
-  const int* cu_q;
-  const int* kv_lens;
+  PfLine line;
+  PfPlan plan;
   const float* q_factor;
   const int* exponents;
   __nv_bfloat16* out;
+  float* parts;         // [stretches][2 slots][2 tiles]: see pf_part_floats
   long long o_stride;
-  int batch, heads, group, pack, units, n_qb, n_items, tiles, total_q;   // pack: heads in a row block; units = heads / pack
+  int heads, group, total_q;
   float scale_log2;
   int* status;
 };
+// A part of a query tile: sums [D / 4][128 rows][4], reference, row sum and its exponent per row.
+template <int D>
+__host__ __device__ constexpr int pf_part_floats() { return PF_TILE * (D + 4); }
 
-struct PfItem {
-  int b, unit, row0, q_len, q_off, kv_len, tok[2], J[2], Jmax;   // tok: first token of each tile; J: its key tiles
-  bool live[2];
-};
-// Work item w: last (heaviest under the causal mask) blocks first. False: the sequence has no such block.
-__device__ __forceinline__ bool pf_item(const PfArgs& a, int w, PfItem& it) {
-  const int bu = w % (a.units * a.batch), blk = a.n_qb - 1 - w / (a.units * a.batch);
-  it.unit = bu % a.units;
-  it.b = bu / a.units;
-  it.row0 = a.cu_q[it.b];
-  it.q_len = a.cu_q[it.b + 1] - it.row0;
-  const int per = PF_TILE / a.pack;                              // tokens of a tile
-  it.tok[0] = blk * 2 * per;
-  it.tok[1] = it.tok[0] + per;
-  if (it.tok[0] >= it.q_len) return false;
-  it.kv_len = a.kv_lens[it.b];
-  it.q_off = it.kv_len - it.q_len;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    it.live[t] = it.tok[t] < it.q_len;
-    const int hi = it.live[t] ? min(it.kv_len, it.q_off + min(it.q_len, it.tok[t] + per)) : 0;
-    it.J[t] = min(a.tiles, (max(hi, 0) + PF_TILE - 1) / PF_TILE);
+// The parts of a CTA's stretch, in order: the steps j0 .. j1 of an item.
+struct PfCursor {
+  int pair, unit, step, left, slot = -1;
+  int j0, j1;           // of the part
+  int of_pair, of_unit;
+  __device__ __forceinline__ explicit PfCursor(const PfArgs& a) {
+    const int c = blockIdx.x;
+    left = 0;
+    pair = unit = step = 0;
+    if (c < a.plan.count()) {
+      const int* s = a.plan.start(c);
+      left = s[3];
+      pair = s[0];
+      unit = s[1];
+      step = s[2];
+    }
   }
-  it.Jmax = max(it.J[0], it.J[1]);
-  return true;
-}
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  // The item of the next part, and past it.
+  __device__ __forceinline__ PfItem next(const PfArgs& a) {
+    PfItem it(a.line, pair);
+    while (it.steps == 0) it = PfItem(a.line, ++pair);     // (a later pair holds the steps that are left)
+    slot = slot < 0 ? 0 : 1;
+    of_pair = pair;
+    of_unit = unit;
+    j0 = step;
+    j1 = min(it.steps, step + left);
+    left -= j1 - j0;
+    step = 0;
+    if (j1 == it.steps) {
+      if (++unit == a.line.units) {
+        unit = 0;
+        ++pair;
+      }
+    }
+    return it;
+  }
+};
 
 __host__ __device__ constexpr uint32_t pf_idesc(int M, int N, bool b_mn_major) {   // fp16 operands, fp32 accumulator
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
@@ -257,6 +401,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   int* status = a.status;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kv_heads = a.heads / a.group;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge waits for this grid's end before it reads
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -288,18 +433,17 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // ------------------------------------------------------------------ Q loader
     if (lane == 0) {
       uint32_t n_q[2] = {0, 0};   // loads issued per tile (phase of q_free / q_full)
-      PfItem it;
       bool ok = true;
-      for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
-        if (!pf_item(a, w, it)) continue;
+      for (PfCursor c(a); c.more() && ok;) {
+        const PfItem it = c.next(a);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (it.J[t] == 0 || !ok) continue;
+          if (min(c.j1, it.J[t]) <= c.j0 || !ok) continue;
           if (!mbar_wait(&q_free[t], (n_q[t] & 1) ^ 1, abort_flag, status, 94)) { ok = false; break; }
           mbar_arrive_expect_tx(&q_full[t], Cfg::TILE_BYTES);
-          for (int c = 0; c < CHUNKS; ++c)
-            tma_load_3d(smem + Cfg::OFF_Q + t * Cfg::TILE_BYTES + c * (PF_TILE * 128), &tm_q, &q_full[t], c * 64,
-                        it.unit * a.pack, it.row0 + it.tok[t]);
+          for (int k = 0; k < CHUNKS; ++k)
+            tma_load_3d(smem + Cfg::OFF_Q + t * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_q, &q_full[t], k * 64,
+                        c.of_unit * a.line.pack, it.row0 + it.tok[t]);
           ++n_q[t];
         }
       }
@@ -308,22 +452,21 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // ------------------------------------------------------------------ K / V loader
     if (lane == 0) {
       uint32_t kc = 0, vc = 0;
-      PfItem it;
       bool ok = true;
-      for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
-        if (!pf_item(a, w, it)) continue;
-        const int bh = it.b * kv_heads + it.unit * a.pack / a.group;
-        for (int j = 0; j < it.Jmax; ++j) {
+      for (PfCursor c(a); c.more() && ok;) {
+        const PfItem it = c.next(a);
+        const int bh = it.b * kv_heads + c.of_unit * a.line.pack / a.group, end = min(c.j1, max(it.J[0], it.J[1]));
+        for (int j = c.j0; j < end; ++j) {
           const int ks = kc % KS, vs = vc % VS;
           if (!mbar_wait(&k_empty[ks], ((kc / KS) & 1) ^ 1, abort_flag, status, 95)) { ok = false; break; }
           mbar_arrive_expect_tx(&k_full[ks], Cfg::TILE_BYTES);
-          for (int c = 0; c < CHUNKS; ++c)
-            tma_load_3d(smem + Cfg::OFF_K + ks * Cfg::TILE_BYTES + c * (PF_TILE * 128), &tm_k, &k_full[ks], c * 64, j * PF_TILE, bh);
+          for (int k = 0; k < CHUNKS; ++k)
+            tma_load_3d(smem + Cfg::OFF_K + ks * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_k, &k_full[ks], k * 64, j * PF_TILE, bh);
           ++kc;
           if (!mbar_wait(&v_empty[vs], ((vc / VS) & 1) ^ 1, abort_flag, status, 96)) { ok = false; break; }
           mbar_arrive_expect_tx(&v_full[vs], Cfg::TILE_BYTES);
-          for (int c = 0; c < CHUNKS; ++c)
-            tma_load_3d(smem + Cfg::OFF_V + vs * Cfg::TILE_BYTES + c * (PF_TILE * 128), &tm_v, &v_full[vs], c * 64, j * PF_TILE, bh);
+          for (int k = 0; k < CHUNKS; ++k)
+            tma_load_3d(smem + Cfg::OFF_V + vs * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_v, &v_full[vs], k * 64, j * PF_TILE, bh);
           ++vc;
         }
       }
@@ -350,28 +493,33 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         }
         umma_commit(&s_full[t]);
       };
-      PfItem it;
-      for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
-        if (!pf_item(a, w, it) || it.Jmax == 0) continue;
-        // scores of step 0 for both tiles
+      for (PfCursor c(a); c.more() && ok;) {
+        const PfItem it = c.next(a);
+        const int j0 = c.j0;
+        int end[2];                         // steps of each tile in this part: j0 .. end - 1
+#pragma unroll
+        for (int t = 0; t < 2; ++t) end[t] = min(c.j1, it.J[t]);
+        const int last = max(end[0], end[1]);
+        if (last <= j0) continue;
+        // scores of the first step for both tiles
         if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 97)) { ok = false; break; }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (it.J[t] == 0 || !ok) continue;
+          if (end[t] <= j0 || !ok) continue;
           if (!mbar_wait(&q_full[t], n_q[t] & 1, abort_flag, status, 98)) { ok = false; break; }
           tc_fence_after();
           issue_s(t, kc);
-          if (it.J[t] == 1) umma_commit(&q_free[t]);
+          if (end[t] == j0 + 1) umma_commit(&q_free[t]);
         }
         if (!ok) break;
-        umma_commit(&k_empty[kc % KS]);   // every score product of key tile 0 has been issued
+        umma_commit(&k_empty[kc % KS]);   // every score product of the first key tile has been issued
         ++kc;
-        for (int j = 0; j < it.Jmax && ok; ++j) {
+        for (int j = j0; j < last && ok; ++j) {
           bool v_ready = false, k_ready = false;
-          const bool have_next = j + 1 < it.Jmax;
+          const bool have_next = j + 1 < last;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (j >= it.J[t] || !ok) continue;
+            if (j >= end[t] || !ok) continue;
             if (!mbar_wait(&p_full[2 * t], n_p[t] & 1, abort_flag, status, 99)) { ok = false; break; }
             if (!v_ready) {
               if (!mbar_wait(&v_full[vc % VS], (vc / VS) & 1, abort_flag, status, 100)) { ok = false; break; }
@@ -386,19 +534,19 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 tc_fence_after();
               }
               umma_f16_ts(tmem_base + Cfg::COL_O + t * D, tmem_base + Cfg::COL_S + t * 128 + k * 8,
-                          umma_desc_sw128(va + k * 2048, PF_TILE * 128, 1024), IDESC_O, (j > 0 || k > 0) ? 1u : 0u);
+                          umma_desc_sw128(va + k * 2048, PF_TILE * 128, 1024), IDESC_O, (j > j0 || k > 0) ? 1u : 0u);
             }
             if (!ok) break;
             ++n_p[t];
-            if (j == it.J[t] - 1) umma_commit(&o_full[t]);
-            if (j + 1 < it.J[t]) {
+            if (j == end[t] - 1) umma_commit(&o_full[t]);
+            if (j + 1 < end[t]) {
               if (!k_ready) {
                 if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 101)) { ok = false; break; }
                 tc_fence_after();
                 k_ready = true;
               }
               issue_s(t, kc);               // overwrites S_t / P_t: ordered behind the PV product just issued
-              if (j + 2 == it.J[t]) umma_commit(&q_free[t]);   // that was the tile's last score product
+              if (j + 2 == end[t]) umma_commit(&q_free[t]);   // that was the tile's last score product
             }
           }
           if (!ok) break;
@@ -411,7 +559,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (it.J[t] > 0) ++n_q[t];
+          if (end[t] > j0) ++n_q[t];
       }
     }
   } else if (warp >= 4) {
@@ -424,24 +572,25 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t t_o = tmem_base + Cfg::COL_O + t * D + lane_sel;
     uint32_t n_s = 0, n_o = 0;
     bool ok = true;
-    PfItem it;
-    for (int w = blockIdx.x; w < a.n_items && ok; w += gridDim.x) {
+    for (PfCursor c(a); c.more() && ok;) {
+      const PfItem it = c.next(a);
       // (selects, not indexing: the item stays in registers)
-      if (!pf_item(a, w, it) || !(t ? it.live[1] : it.live[0])) continue;
-      const int Jt = t ? it.J[1] : it.J[0];
-      const int tok = (t ? it.tok[1] : it.tok[0]) + r / a.pack, head = it.unit * a.pack + r % a.pack;
+      const int Jt = t ? it.J[1] : it.J[0], j0 = c.j0, end = min(c.j1, Jt);
+      const bool whole = j0 == 0 && end == Jt && (t ? it.live[1] : it.live[0]);     // the tile's outputs are complete here
+      if (end <= j0 && !whole) continue;
+      const int tok = (t ? it.tok[1] : it.tok[0]) + r / a.line.pack, head = c.of_unit * a.line.pack + r % a.line.pack;
       const int row = it.row0 + tok;
       const bool live = tok < it.q_len && (unsigned)row < (unsigned)a.total_q;
       const int limit = min(it.kv_len - 1, it.q_off + tok);
-      const int* ex = a.exponents + (long long)(it.b * kv_heads + it.unit * a.pack / a.group) * a.tiles;
+      const int* ex = a.exponents + (long long)(it.b * kv_heads + c.of_unit * a.line.pack / a.group) * a.line.tiles;
       const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 1.f;
       float m_ref = 0.f, l = 0.f;
-      int e0 = 0;                             // exponent of the first tile's values: the row sum is kept in units of 2^-e0
-      int e_next = Jt > 0 ? ex[0] : 0;
-      for (int j = 0; j < Jt && ok; ++j) {
+      int e0 = 0;                             // exponent of the part's first values: the row sum is kept in units of 2^-e0
+      int e_next = end > j0 ? ex[j0] : 0;
+      for (int j = j0; j < end && ok; ++j) {
         const int ek = (short)e_next, e = e_next >> 16;
-        if (j + 1 < Jt) e_next = ex[j + 1];
-        if (j == 0) e0 = e;
+        if (j + 1 < end) e_next = ex[j + 1];
+        if (j == j0) e0 = e;
         // (never zero: a masked score of minus infinity has to stay one)
         const float sc = fmaxf(row_f * pf_pow2(ek), 1e-37f), ev = (float)e;
         ok = mbar_wait(&s_full[t], n_s & 1, abort_flag, status, 102);
@@ -473,7 +622,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sc, ev);
         float alpha = 1.f;
         bool need = false;
-        if (j == 0) {
+        if (j == j0) {
           m_ref = (m_new == -INFINITY) ? 0.f : m_new;
         } else if (m_new - m_ref > 6.f) {     // lazy: p up to 2^6 until the reference moves
           need = true;
@@ -482,7 +631,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         }
         // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):
         // O_t is quiescent until this warpgroup arrives on p_full, so a rescale can happen right here.
-        if (j > 0 && __any_sync(0xffffffffu, need)) {
+        if (j > j0 && __any_sync(0xffffffffu, need)) {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t orr[32];
@@ -518,7 +667,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(e0 - e);
       }
       if (!ok) break;
-      if (Jt > 0) {
+      if (end > j0) {
         ok = mbar_wait(&o_full[t], n_o & 1, abort_flag, status, 103);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -528,25 +677,36 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       // p 2^ev and the values' 2^-ev cancel in O; l is in units of 2^-e0
       const float inv_l = l == 0.f ? 0.f : 1.f / l, unit = pf_pow2(e0);
       __nv_bfloat16* orow = a.out + (long long)row * a.o_stride + (long long)head * D;
+      float* part = a.parts + (long long)((blockIdx.x * 2 + c.slot) * 2 + t) * pf_part_floats<D>();
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int k = 0; k < D / 32; ++k) {
         uint32_t orr[32];                 // (without a key: whatever the columns hold, not used)
-        tmem_ld32(t_o + c * 32, orr);
+        tmem_ld32(t_o + k * 32, orr);
         tmem_ld_wait();
-        if (live) {
-          uint4* p4 = reinterpret_cast<uint4*>(orow + c * 32);
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(part + ((k * 8 + i) * PF_TILE + r) * 4) =
+                make_uint4(orr[4 * i], orr[4 * i + 1], orr[4 * i + 2], orr[4 * i + 3]);
+        } else if (live) {
+          uint4* p4 = reinterpret_cast<uint4*>(orow + k * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              v[k] = l == 0.f ? 0u
-                              : pack_bf16x2(__uint_as_float(orr[8 * i + 2 * k]) * inv_l * unit, __uint_as_float(orr[8 * i + 2 * k + 1]) * inv_l * unit);
+            for (int q = 0; q < 4; ++q)
+              v[q] = l == 0.f ? 0u
+                              : pack_bf16x2(__uint_as_float(orr[8 * i + 2 * q]) * inv_l * unit, __uint_as_float(orr[8 * i + 2 * q + 1]) * inv_l * unit);
             p4[i] = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
       }
-      // The TMEM loads above have completed (tmem_ld_wait); the next item's first PV product waits for
+      if (!whole) {
+        part[PF_TILE * D + r] = m_ref;
+        part[PF_TILE * (D + 1) + r] = l;
+        part[PF_TILE * (D + 2) + r] = __int_as_float(e0);
+      }
+      // The TMEM loads above have completed (tmem_ld_wait); the next part's first PV product waits for
       // this warpgroup's next arrives on p_full, so O_t is not overwritten before it was read.
       tc_fence_before();
     }
@@ -562,80 +722,163 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
-int pf_tiles(int max_kv) { return (max_kv + PF_TILE - 1) / PF_TILE; }
-long long pf_align(long long n) { return (n + 255) / 256 * 256; }
+// Joins the parts of query tiles that lie in several stretches: 16 values of 128 rows of a (unit, pair, tile) per block, two
+// threads per row.
+template <int D>
+__global__ void __launch_bounds__(256)
+pf_merge_kernel(const __grid_constant__ PfArgs a) {
+  const int unit = blockIdx.x, pair = blockIdx.y, t = blockIdx.z & 1;
+  const PfItem it(a.line, pair);
+  asm volatile("griddepcontrol.wait;" ::: "memory");             // every CTA, so that this grid ends behind the one before
+  const int Jt = t ? it.J[1] : it.J[0];
+  if (!(t ? it.live[1] : it.live[0]) || Jt == 0) return;
+  const int per = a.plan.per(), rem = a.plan.rem(), u0 = a.plan.begin()[pair] + unit * it.steps;
+  const int c0 = pf_owner(per, rem, u0), c1 = pf_owner(per, rem, u0 + Jt - 1);
+  if (c0 == c1) return;                           // written by that CTA
+  const int r = threadIdx.x >> 1, v0 = (blockIdx.z >> 1) * 4 + (threadIdx.x & 1) * 2;      // row, first group of four values
+  const auto part = [&](int c) {
+    return a.parts + (long long)((c * 2 + (u0 > pf_start(per, rem, c) ? 1 : 0)) * 2 + t) * pf_part_floats<D>();
+  };
+  float M = -INFINITY, l = 0.f;
+  int e0 = 0;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 2
+  for (int c = c0; c <= c1; ++c) {
+    const float* p = part(c);
+    const float m = p[PF_TILE * D + r], lc = p[PF_TILE * (D + 1) + r];
+    const int e = __float_as_int(p[PF_TILE * (D + 2) + r]);
+    float4 v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) v[k] = *reinterpret_cast<const float4*>(p + ((v0 + k) * PF_TILE + r) * 4);
+    if (lc == 0.f) continue;                      // nothing seen (a NaN is not nothing)
+    if (l == 0.f) e0 = e;
+    const float Mn = fmaxf(M, m), w0 = l == 0.f ? 0.f : fast_exp2(M - Mn), w = fast_exp2(m - Mn);
+    M = Mn;
+    l = fmaf(w * pf_pow2(e0 - e), lc, l * w0);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      acc[k].x = fmaf(w, v[k].x, acc[k].x * w0);
+      acc[k].y = fmaf(w, v[k].y, acc[k].y * w0);
+      acc[k].z = fmaf(w, v[k].z, acc[k].z * w0);
+      acc[k].w = fmaf(w, v[k].w, acc[k].w * w0);
+    }
+  }
+  const int tok = (t ? it.tok[1] : it.tok[0]) + r / a.line.pack, head = unit * a.line.pack + r % a.line.pack, row = it.row0 + tok;
+  if (tok >= it.q_len || (unsigned)row >= (unsigned)a.total_q) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l, u = pf_pow2(e0);
+  uint32_t y[4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    y[2 * k] = l == 0.f ? 0u : pack_bf16x2(acc[k].x * inv * u, acc[k].y * inv * u);
+    y[2 * k + 1] = l == 0.f ? 0u : pack_bf16x2(acc[k].z * inv * u, acc[k].w * inv * u);
+  }
+  *reinterpret_cast<uint4*>(a.out + (long long)row * a.o_stride + (long long)head * D + v0 * 4) = make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+// Sizes of a call's workspace and launches.
+struct PfSizes {
+  int tiles, pack, units, n_qb, ctas;
+  bool whole;
+  long long kv_tiles, pairs, steps;     // steps: at most
+  long long kv, q, factor, exponents, plan, parts, total;    // bytes, each a multiple of 256
+};
+PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int D) {
+  const auto align = [](long long n) { return (n + 255) / 256 * 256; };
+  PfSizes z;
+  const int G = heads / kv_heads;
+  z.tiles = std::max(1, (max_kv + PF_TILE - 1) / PF_TILE);
+  z.pack = PF_TILE % G == 0 ? G : 1;
+  z.units = heads / z.pack;
+  z.n_qb = (int)(((long long)max_q * z.pack + 2 * PF_TILE - 1) / (2 * PF_TILE));
+  z.kv_tiles = (long long)batch * kv_heads * z.tiles;
+  z.pairs = (long long)batch * z.n_qb;
+  z.steps = z.pairs * z.units * z.tiles;
+  z.whole = z.pairs * z.units <= sm_count() && z.tiles <= PF_WHOLE_STEPS;
+  z.ctas = (int)(z.whole ? std::max(1LL, z.pairs * z.units) : std::max(1LL, std::min((long long)sm_count(), z.steps / PF_MIN_STEPS)));
+  z.kv = align(z.kv_tiles * PF_TILE * D * 2);
+  z.q = align((long long)total_q * heads * D * 2);
+  z.factor = align((long long)total_q * heads * 4);
+  z.exponents = align(z.kv_tiles * 4);
+  z.plan = align((4 + z.pairs + 4LL * z.ctas) * 4);
+  z.parts = z.whole ? 0 : align(4LL * z.ctas * PF_TILE * (D + 4) * 4);
+  z.total = 2 * z.kv + z.q + z.factor + z.exponents + z.plan + z.parts;
+  return z;
+}
 
 }  // namespace
 
-long long prompt_int4_workspace(int batch, int total_q, int max_kv, int heads, int kv_heads, int head_dim) {
-  const long long tiles = (long long)batch * kv_heads * pf_tiles(max_kv);
-  return 2 * tiles * PF_TILE * head_dim * 2 + pf_align((long long)total_q * heads * head_dim * 2) +
-         pf_align((long long)total_q * heads * 4) + pf_align(tiles * 4);
+long long prompt_int4_workspace(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int head_dim) {
+  return pf_sizes(batch, total_q, max_q, max_kv, heads, kv_heads, head_dim).total;
 }
 
 void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                  long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,
                  int* status, cudaStream_t stream) {
-  const int D = c.head_dim, G = heads / c.kv_heads, tiles = pf_tiles(max_kv);
-  const int pack = 128 % G == 0 ? G : 1;
-  const long long all = (long long)batch * c.kv_heads * tiles;
+  const int D = c.head_dim;
+  const PfSizes z = pf_sizes(batch, total_q, max_q, max_kv, heads, c.kv_heads, D);
   uint8_t* p = (uint8_t*)workspace;
+  const auto take = [&](long long bytes) {
+    uint8_t* at = p;
+    p += bytes;
+    return at;
+  };
   PfExpand x{(const uint8_t*)c.k, (const uint8_t*)c.v,
              {c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)}, kv_lens,
              (const __nv_bfloat16*)q, q_stride};
-  x.k = (__half*)p;
-  x.v = x.k + all * PF_TILE * D;
-  p += 2 * all * PF_TILE * D * 2;
-  x.qh = (__half*)p;
-  p += pf_align((long long)total_q * heads * D * 2);
-  x.q_factor = (float*)p;
-  p += pf_align((long long)total_q * heads * 4);
-  x.exponents = (int*)p;
+  x.k = (__half*)take(z.kv);
+  x.v = (__half*)take(z.kv);
+  x.qh = (__half*)take(z.q);
+  x.q_factor = (float*)take(z.factor);
+  x.exponents = (int*)take(z.exponents);
+  x.plan = {(int*)take(z.plan), (int)z.pairs};
   x.kv_heads = c.kv_heads;
   x.heads = heads;
-  x.tiles = tiles;
+  x.tiles = z.tiles;
   x.total_q = total_q;
+  x.line = {cu_q, kv_lens, batch, z.pack, z.units, z.n_qb, z.tiles};
+  x.ctas = z.ctas;
+  x.whole = z.whole;
   x.status = status;
   const int rows_per = PF_EXPAND / (D / 8);
   const long long q_blocks = ((long long)total_q * heads + rows_per - 1) / rows_per;
-  MB_REQUIRE(all + q_blocks < (1LL << 31) && all < (1LL << 31), "paged_attn_prefill_int4: batch too large");
-  x.kv_blocks = (int)all;
-  if (D == 128) kv4_expand_kernel<128><<<(unsigned)(all + q_blocks), PF_EXPAND, 0, stream>>>(x);
-  else kv4_expand_kernel<64><<<(unsigned)(all + q_blocks), PF_EXPAND, 0, stream>>>(x);
+  MB_REQUIRE(z.kv_tiles + q_blocks + 1 < (1LL << 31) && z.steps < (1LL << 31) && z.pairs <= 65535, "paged_attn_prefill_int4: batch too large");
+  x.kv_blocks = (int)z.kv_tiles;
+  x.q_blocks = (int)q_blocks;
+  const unsigned blocks = (unsigned)(z.kv_tiles + q_blocks + 1);
+  if (D == 128) kv4_expand_kernel<128><<<blocks, PF_EXPAND, 0, stream>>>(x);
+  else kv4_expand_kernel<64><<<blocks, PF_EXPAND, 0, stream>>>(x);
   count_launch();
   check_launch();
 
   // (copies only: TMA moves fp16 as it moves bf16)
   uint64_t qd[3] = {(uint64_t)D, (uint64_t)heads, (uint64_t)total_q}, qs[2] = {(uint64_t)D * 2, (uint64_t)heads * D * 2};
-  uint32_t qb[3] = {64, (uint32_t)pack, (uint32_t)(PF_TILE / pack)};
-  uint64_t kd[3] = {(uint64_t)D, (uint64_t)tiles * PF_TILE, (uint64_t)batch * c.kv_heads};
-  uint64_t ks[2] = {(uint64_t)D * 2, (uint64_t)tiles * PF_TILE * D * 2};
+  uint32_t qb[3] = {64, (uint32_t)z.pack, (uint32_t)(PF_TILE / z.pack)};
+  uint64_t kd[3] = {(uint64_t)D, (uint64_t)z.tiles * PF_TILE, (uint64_t)batch * c.kv_heads};
+  uint64_t ks[2] = {(uint64_t)D * 2, (uint64_t)z.tiles * PF_TILE * D * 2};
   uint32_t kb[3] = {64, PF_TILE, 1};
   const CUtensorMap tq = make_tensor_map(x.qh, TmaDType::BF16, 3, qd, qs, qb, true);
   const CUtensorMap tk = make_tensor_map(x.k, TmaDType::BF16, 3, kd, ks, kb, true);
   const CUtensorMap tv = make_tensor_map(x.v, TmaDType::BF16, 3, kd, ks, kb, true);
-  PfArgs a{cu_q, kv_lens, x.q_factor, x.exponents, (__nv_bfloat16*)out, o_stride};
-  a.batch = batch;
-  a.heads = heads;
-  a.group = G;
-  a.pack = pack;
-  a.units = heads / pack;
-  a.n_qb = (int)(((long long)max_q * pack + 2 * PF_TILE - 1) / (2 * PF_TILE));
-  MB_REQUIRE((long long)a.n_qb * a.units * batch < (1LL << 31), "paged_attn_prefill_int4: batch too large");
-  a.n_items = a.n_qb * a.units * batch;
-  a.tiles = tiles;
-  a.total_q = total_q;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.status = status;
-  const int grid = a.n_items < sm_count() ? a.n_items : sm_count();
-  const auto go = [&](auto kern, int smem) {
+  PfArgs a{x.line, x.plan, x.q_factor, x.exponents, (__nv_bfloat16*)out, (float*)take(z.parts), o_stride, heads, heads / c.kv_heads, total_q,
+           scale * 1.4426950408889634f, status};
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(z.units, (unsigned)z.pairs, 2 * (D / 16));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const auto go = [&](auto kern, auto merge, int smem) {
     MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kern<<<grid, PF_THREADS, smem, stream>>>(tq, tk, tv, a);
+    kern<<<z.ctas, PF_THREADS, smem, stream>>>(tq, tk, tv, a);
+    check_launch();
+    if (!z.whole) MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, merge, a));
   };
-  if (D == 128) go(fa_int4_kernel<128>, PfCfg<128>::SMEM_BYTES);
-  else go(fa_int4_kernel<64>, PfCfg<64>::SMEM_BYTES);
-  count_launch();
-  check_launch();
+  if (D == 128) go(fa_int4_kernel<128>, pf_merge_kernel<128>, PfCfg<128>::SMEM_BYTES);
+  else go(fa_int4_kernel<64>, pf_merge_kernel<64>, PfCfg<64>::SMEM_BYTES);
+  count_launch(z.whole ? 1 : 2);
 }
 
 }  // namespace mb
