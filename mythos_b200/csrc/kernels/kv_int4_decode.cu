@@ -552,7 +552,7 @@ __device__ __forceinline__ void p4_store(__nv_bfloat16* dst, const float4& v, fl
   if (dst) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
 }
 
-// ------------------------------------------------------------------------------------------------ few units
+// ------------------------------------------------------------------------------------------------ short contexts
 // One unit per cluster, whose CTAs split its chunks and join their sums through distributed shared memory: one launch, which
 // counts where the whole call takes a few microseconds.
 __device__ __forceinline__ uint32_t p4_rank() {
@@ -591,7 +591,7 @@ struct P4SmemCluster {
 };
 
 template <int D, int COLS>
-__global__ void __launch_bounds__(P4_THREADS, COLS == 8 ? 3 : 2)
+__global__ void __launch_bounds__(P4_THREADS, COLS == 8 ? 4 : 2)
 paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   using C = P4Cfg<D, COLS>;
   using S = P4SmemCluster<D, COLS>;
@@ -665,7 +665,7 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   p4_cluster_sync();                              // nobody leaves while a peer still reads its shared memory
 }
 
-// ------------------------------------------------------------------------------------------------ many units
+// ------------------------------------------------------------------------------------------------ long contexts
 // A unit has n = ceil(keys / 32) chunks. All chunks of all units stand in one line, units of a sequence side by side, and every
 // warp takes an equal stretch of it, so that ragged batches and any number of units load the GPU evenly (with equal splits
 // of each unit, 148 SMs x 16 warps were filled to three quarters: 8 x 32768 tokens and 5 kv heads took 73 us, 60 this way). A
@@ -963,9 +963,13 @@ P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, long long max_tokens) 
   p.chunks = std::max(1LL, (max_tokens + P4_CHUNK - 1) / P4_CHUNK);
   const long long resident = (p.cols == 8 ? 4LL : 2LL) * sm_count();
   p.ctas = (int)std::max(1LL, std::min(resident, (p.units * p.chunks + P4_WARPS - 1) / P4_WARPS));
-  // A cluster per unit while sixteen CTAs a unit fit beside each other and no warp gets more than eight chunks.
+  // A cluster per unit, of as many CTAs as the units leave room for, while no warp gets more than sixteen chunks. One launch,
+  // no scratch and no walk along the line: 64 x 512 tokens (8 kv heads, one query) take 12.9 us (18.0 as a line), 64 x 1280 27.0
+  // (32.6), 512 ragged x 512 76.3 (99.6), 4 x 1000 with five queries 10.9 (17.2). Longer contexts want the line's evenness:
+  // 32 ragged x 4096 take 35.6 there (37.0), 64 ragged x 2560 40.6 (41.8).
   const long long want = std::min(16LL, (p.chunks + P4_WARPS - 1) / P4_WARPS);
-  p.splits = p.units * want <= resident && p.chunks <= 8 * P4_WARPS * want ? (int)want : 0;
+  const long long room = std::max(1LL, std::min(want, resident / std::max(1LL, p.units)));
+  p.splits = p.chunks <= 16 * P4_WARPS * room ? (int)room : 0;
   return p;
 }
 
