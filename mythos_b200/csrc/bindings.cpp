@@ -970,7 +970,7 @@ Tensor paged_attn_decode_int4(const Tensor& q, const Tensor& k_cache, const Tens
               ": one context length and one table row per query token");
   const auto c = kv4_cache(k_cache, v_cache, block_table, k_cache.size(1), q.size(2), who);
   c10::cuda::CUDAGuard guard(q.device());
-  const int64_t bytes = mb::paged_attn_int4_workspace(c, (int)q.size(0), (int)q.size(0), 1, c.max_pages * c.page_size, (int)q.size(1));
+  const int64_t bytes = mb::paged_attn_decode_int4_workspace(c, (int)q.size(0), (int)q.size(1));
   Tensor work;
   if (bytes > 0) work = torch::empty({bytes}, q.options().dtype(U8));
   mb::paged_attn_decode_int4(c, q.data_ptr(), kv4_stride(q), context_lens.data_ptr<int>(), out.data_ptr(), (int)q.size(0), (int)q.size(1),
@@ -996,7 +996,7 @@ Tensor paged_attn_prefill_int4(const Tensor& q, const Tensor& k_cache, const Ten
   TORCH_CHECK(max_q_len >= 0 && max_q_len <= q.size(0) && max_kv_len >= 0 && max_kv_len <= (int64_t)c.max_pages * c.page_size, who,
               ": max_q_len must be within q and max_kv_len within the table's pages");
   c10::cuda::CUDAGuard guard(q.device());
-  const int64_t bytes = mb::paged_attn_int4_workspace(c, (int)B, (int)q.size(0), (int)max_q_len, (int)max_kv_len, (int)q.size(1));
+  const int64_t bytes = mb::paged_attn_prefill_int4_workspace(c, (int)B, (int)q.size(0), (int)max_q_len, (int)max_kv_len, (int)q.size(1));
   Tensor work;
   if (bytes > 0) work = torch::empty({bytes}, q.options().dtype(U8));
   mb::paged_attn_prefill_int4(c, q.data_ptr(), kv4_stride(q), cu_q.data_ptr<int>(), kv_lens.data_ptr<int>(), out.data_ptr(), kv4_stride(out),

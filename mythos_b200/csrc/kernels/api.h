@@ -397,18 +397,22 @@ void qkv_rope_append_int4(float* acc, const int* pos, const int* seq_ids, void* 
 void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* context_lens, void* out, int batch,
                             int heads, float scale, void* workspace, int* status, cudaStream_t stream);
 // New tokens of several sequences packed back to back, causal over the pages (as flash_attn_paged_prefill). max_q: most new
-// tokens of a sequence, max_kv: most keys. Up to P4_FEW_COLUMNS query columns (new tokens x heads of a group) per kv head, a
-// split-context kernel reads the codes directly; above, prompt_int4 expands the sequences into the workspace, each once
-// for all of its queries.
-constexpr int P4_FEW_COLUMNS = 64;
-// Bytes of the workspace of both attention calls (decode: total_q = batch, max_q = 1); 16-byte aligned, free again when the call's
-// kernels have run.
-long long paged_attn_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads);
+// tokens of a sequence, max_kv: most keys; a sequence that has more is reported through the status word.
+// Bytes of the two calls' workspaces; 16-byte aligned, free again when the call's kernels have run.
+long long paged_attn_decode_int4_workspace(const KvInt4Cache& c, int batch, int heads);
+long long paged_attn_prefill_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads);
 void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                              long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale,
                              void* workspace, int* status, cudaStream_t stream);
 // Their two forms, arguments checked by the caller: kv_int4_decode.cu (cu_q null: one query token per sequence) and
 // kv_int4_prefill.cu.
+// few_query_int4 reads the codes once per 16 query columns (new tokens x heads of a group); prompt_int4 expands every sequence
+// once and costs 14 to 18 us before its first product. So the first form takes calls of up to 64 columns per kv head (16
+// sequences, 1000 keys, 32 heads over 8: 16 tokens 38 us against 44, 32 tokens 75 against 44; 64 x 128 keys, 16 tokens: 64
+// against 44), and larger ones whose blocks of columns run side by side with at most eight chunks of 32 keys per warp (one
+// sequence, 512 keys, 64 tokens: 11 us against 23; 4 x 1000 keys, 32 tokens: 20 against 29; twice that work, 4 x 1000, 64
+// tokens: 38 against 33; twice the blocks, 8 x 100, 100 tokens, 16 heads over 4: 19.5 against 12.4).
+bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads);
 long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads);
 void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                     long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,

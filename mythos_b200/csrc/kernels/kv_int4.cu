@@ -196,13 +196,16 @@ void kv4_workspace(const void* workspace, long long bytes) {
   MB_REQUIRE(bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
              "attention over 4-bit pages: workspace missing or not 16-byte aligned");
 }
-bool p4_few(int max_q, int group) { return (long long)max_q * group <= P4_FEW_COLUMNS; }
 }  // namespace
 
-long long paged_attn_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads) {
+long long paged_attn_decode_int4_workspace(const KvInt4Cache& c, int batch, int heads) {
+  return batch == 0 || c.kv_heads <= 0 ? 0 : few_query_int4_workspace(c, batch, 1, heads);
+}
+
+long long paged_attn_prefill_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads) {
   if (batch == 0 || max_q == 0 || c.kv_heads <= 0) return 0;
-  const int G = heads / c.kv_heads;
-  if (!p4_few(max_q, G)) return prompt_int4_workspace(batch, total_q, max_q, max_kv, heads, c.kv_heads, c.head_dim);
+  if (!few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads))
+    return prompt_int4_workspace(batch, total_q, max_q, max_kv, heads, c.kv_heads, c.head_dim);
   return few_query_int4_workspace(c, batch, max_q, heads);
 }
 
@@ -214,7 +217,7 @@ void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_str
              "paged_attn_decode_int4: q must be 16-byte aligned with a token stride of a multiple of 8 elements");
   MB_REQUIRE(scale > 0.f, "paged_attn_decode_int4: scale must be positive");
   if (batch == 0) return;
-  kv4_workspace(workspace, paged_attn_int4_workspace(c, batch, batch, 1, 0, heads));
+  kv4_workspace(workspace, paged_attn_decode_int4_workspace(c, batch, heads));
   few_query_int4(c, q, q_stride, nullptr, context_lens, out, (long long)heads * c.head_dim, batch, batch, 1, heads, scale, workspace,
                  status, stream);
 }
@@ -228,8 +231,8 @@ void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_st
              "paged_attn_prefill_int4: q and out must be 16-byte aligned with token strides of multiples of 8 elements");
   MB_REQUIRE(scale > 0.f, "paged_attn_prefill_int4: scale must be positive");
   if (batch == 0 || total_q == 0 || max_q == 0) return;
-  kv4_workspace(workspace, paged_attn_int4_workspace(c, batch, total_q, max_q, max_kv, heads));
-  if (p4_few(max_q, heads / c.kv_heads)) {
+  kv4_workspace(workspace, paged_attn_prefill_int4_workspace(c, batch, total_q, max_q, max_kv, heads));
+  if (few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads)) {
     few_query_int4(c, q, q_stride, cu_q, kv_lens, out, o_stride, batch, total_q, max_q, heads, scale, workspace, status, stream);
     return;
   }

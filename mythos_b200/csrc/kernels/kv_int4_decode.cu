@@ -87,15 +87,21 @@ struct P4Args {
   __nv_bfloat16* out;
   long long q_stride, o_stride;
   int batch, G, kv_heads, total_q;
+  int max_q, most_chunks;   // a sequence's: the tables' tokens, and one chunk more, which reports what lies behind them
   Kv4Div by_group, by_heads;
   float scale_log2;
   int* status;
 };
 
+// Chunks of a sequence, whatever stands in its length: counts and sums of them stay within the launch's limits.
+__device__ __forceinline__ int p4_chunks(int kv_len, int most) {
+  return (int)min(((unsigned)max(kv_len, 0) + P4_CHUNK - 1u) / P4_CHUNK, (unsigned)most);
+}
 // A unit: one (sequence, kv head, block of columns).
 struct P4Unit {
   int b, hkv, col0, n_cols, row0, q_len, kv_len;
   int to_some, to_all;      // tokens that some column sees, and that all see
+  __device__ __forceinline__ int chunks(const P4Args& a) const { return p4_chunks(kv_len, a.most_chunks); }
   __device__ __forceinline__ P4Unit(const P4Args& a, int cols, int b_, int y) : b(b_) {
     const int block = a.by_heads(y);
     hkv = y - block * a.kv_heads;
@@ -103,7 +109,7 @@ struct P4Unit {
     row0 = a.cu_q ? a.cu_q[b] : b;
     q_len = a.cu_q ? a.cu_q[b + 1] - row0 : 1;
     kv_len = a.kv_lens[b];
-    n_cols = min(cols, q_len * a.G - col0);
+    n_cols = min(cols, min(q_len, a.max_q) * a.G - col0);
     to_some = min(kv_len, kv_len - q_len + a.by_group(col0 + max(n_cols, 1) - 1) + 1);
     to_all = min(kv_len, kv_len - q_len + a.by_group(col0) + 1);
   }
@@ -114,6 +120,11 @@ struct P4Unit {
     return a.out + row * a.o_stride + (hkv * a.G + col - qi * a.G) * D + d;
   }
 };
+
+// Rows behind max_q have no unit: reported, left as they were.
+__device__ __forceinline__ void p4_too_long(const P4Args& a) {
+  if (a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (90 << 16));
+}
 
 // A warp's running state. Thread (r, t) of the warp holds columns 2 t and 2 t + 1 of every block of eight.
 template <int D, int COLS>
@@ -598,6 +609,7 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, splits = gridDim.z;
   const P4Unit u(a, COLS, blockIdx.x, blockIdx.y);
+  if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && u.q_len > a.max_q) p4_too_long(a);
   if (u.n_cols <= 0) return;                      // the same for every CTA of the cluster
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * C::STAGES;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::OFF_FLAG);
@@ -610,7 +622,7 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
     fence_mbar_init();
   }
   __syncthreads();
-  const int n = (max(u.kv_len, 0) + P4_CHUNK - 1) / P4_CHUNK, per = (n + splits - 1) / splits;
+  const int n = u.chunks(a), per = (n + splits - 1) / splits;
   const int chunk0 = blockIdx.z * per + warp, end = min(n, (int)blockIdx.z * per + per);
   const int mine = max(0, (end - chunk0 + P4_WARPS - 1) / P4_WARPS);        // chunk0, + 4, ...
   const auto locate = [&](int i) {
@@ -672,12 +684,15 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
 // warp that meets a whole unit writes its outputs; parts of units go to shared memory and are joined by the CTA, and what
 // crosses a CTA's border goes to a scratch buffer of the call (two slots a CTA) and is joined by p4_merge_kernel.
 struct P4Line {
-  int batch, G, kv_heads, cols;
+  int batch, G, kv_heads, cols, max_q, most_chunks;
   const int* kv_lens;
   const int* cu_q;
-  __device__ __forceinline__ int chunks(int b) const { return (max(kv_lens[b], 0) + P4_CHUNK - 1) / P4_CHUNK; }
+  __device__ __forceinline__ P4Line(const P4Args& a, int cols_)
+      : batch(a.batch), G(a.G), kv_heads(a.kv_heads), cols(cols_), max_q(a.max_q), most_chunks(a.most_chunks), kv_lens(a.kv_lens), cu_q(a.cu_q) {}
+  __device__ __forceinline__ int chunks(int b) const { return p4_chunks(kv_lens[b], most_chunks); }
   __device__ __forceinline__ int units(int b) const {
-    return kv_heads * (cu_q ? (max(cu_q[b + 1] - cu_q[b], 0) * G + cols - 1) / cols : (G + cols - 1) / cols);
+    const int q = cu_q ? max(min(cu_q[b + 1] - cu_q[b], max_q), 0) : 1;
+    return kv_heads * ((q * G + cols - 1) / cols);
   }
   __device__ __forceinline__ int size(int b) const { return b < batch ? chunks(b) * units(b) : 0; }
 };
@@ -768,7 +783,7 @@ paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict_
   if (lane < 2) s_unit[warp * 2 + lane] = make_int4(-1, 0, 0, 0);
   __syncthreads();
 
-  const P4Line line{a.batch, a.G, a.kv_heads, COLS, a.kv_lens, a.cu_q};
+  const P4Line line(a, COLS);
   const P4Scan scan(line, lane);
   const P4Share share(scan.total, gridDim.x * P4_WARPS);
   const int worker = blockIdx.x * P4_WARPS + warp;
@@ -881,7 +896,7 @@ p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scra
   __shared__ float s_w[P4_MERGE][COLS], s_lw[P4_MERGE][COLS], s_m[COLS];
   __shared__ int s_at[P4_MERGE];
   const int b = blockIdx.x, y = blockIdx.y, lane = threadIdx.x & 31;
-  const P4Line line{a.batch, a.G, a.kv_heads, COLS, a.kv_lens, a.cu_q};
+  const P4Line line(a, COLS);
   const P4Scan scan(line, lane);
   const P4Share share(scan.total, ctas * P4_WARPS);
   const int u0 = scan.begin(line, b, lane) + y * line.chunks(b), n = line.chunks(b);
@@ -892,6 +907,7 @@ p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scra
     c1 = share.worker(u0 + n - 1) / P4_WARPS;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");             // every CTA, so that this grid ends behind the one before
+  if (y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && a.cu_q && a.cu_q[b + 1] - a.cu_q[b] > a.max_q) p4_too_long(a);
   if (!here || (n > 0 && c0 == c1)) return;       // no such unit, or written by that CTA
   const P4Unit u(a, COLS, b, y);
   const int c = threadIdx.x >> 3, d = blockIdx.z * 32 + (threadIdx.x & 7) * 4;
@@ -953,7 +969,7 @@ void p4_configure(K kern, int smem, bool cluster, unsigned long long& seen) {
 // How a call runs, by its sizes (the table's width stands for the contexts, which only the device knows).
 struct P4Plan {
   int cols, ctas, splits;         // splits > 0: clusters; else stretches of the line over that many CTAs
-  long long blocks, units, chunks;
+  long long blocks, units, chunks, resident;      // resident: CTAs side by side
 };
 P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, long long max_tokens) {
   P4Plan p;
@@ -961,14 +977,14 @@ P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, long long max_tokens) 
   p.blocks = ((long long)max_q * G + p.cols - 1) / p.cols;
   p.units = (long long)batch * kv_heads * p.blocks;
   p.chunks = std::max(1LL, (max_tokens + P4_CHUNK - 1) / P4_CHUNK);
-  const long long resident = (p.cols == 8 ? 4LL : 2LL) * sm_count();
-  p.ctas = (int)std::max(1LL, std::min(resident, (p.units * p.chunks + P4_WARPS - 1) / P4_WARPS));
+  p.resident = (p.cols == 8 ? 4LL : 2LL) * sm_count();
+  p.ctas = (int)std::max(1LL, std::min(p.resident, (p.units * p.chunks + P4_WARPS - 1) / P4_WARPS));
   // A cluster per unit, of as many CTAs as the units leave room for, while no warp gets more than sixteen chunks. One launch,
   // no scratch and no walk along the line: 64 x 512 tokens (8 kv heads, one query) take 12.9 us (18.0 as a line), 64 x 1280 27.0
   // (32.6), 512 ragged x 512 76.3 (99.6), 4 x 1000 with five queries 10.9 (17.2). Longer contexts want the line's evenness:
   // 32 ragged x 4096 take 35.6 there (37.0), 64 ragged x 2560 40.6 (41.8).
   const long long want = std::min(16LL, (p.chunks + P4_WARPS - 1) / P4_WARPS);
-  const long long room = std::max(1LL, std::min(want, resident / std::max(1LL, p.units)));
+  const long long room = std::max(1LL, std::min(want, p.resident / std::max(1LL, p.units)));
   p.splits = p.chunks <= 16 * P4_WARPS * room ? (int)room : 0;
   return p;
 }
@@ -976,7 +992,7 @@ P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, long long max_tokens) 
 template <int D, int COLS>
 void p4_launch(P4Args& a, const P4Plan& plan, float* scratch, cudaStream_t stream) {
   MB_REQUIRE(plan.blocks * a.kv_heads <= 65535, "paged attention over 4-bit pages: too many query columns for one launch");
-  MB_REQUIRE(plan.units * plan.chunks < (1LL << 31), "paged attention over 4-bit pages: too many chunks for one launch");
+  MB_REQUIRE(plan.units * (plan.chunks + 1) < (1LL << 31), "paged attention over 4-bit pages: too many chunks for one launch");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.stream = stream;
@@ -1011,6 +1027,11 @@ void p4_launch(P4Args& a, const P4Plan& plan, float* scratch, cudaStream_t strea
 
 }  // namespace
 
+bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads) {
+  const P4Plan p = p4_plan(batch, max_q, heads / kv_heads, kv_heads, max_kv);
+  return p.blocks * p.cols <= 64 || (p.units <= p.resident && p.units * p.chunks <= 8 * P4_WARPS * p.resident);
+}
+
 long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads) {
   const P4Plan p = p4_plan(batch, max_q, heads / c.kv_heads, c.kv_heads, (long long)c.max_pages * c.page_size);
   return p.splits > 0 ? 0 : 2LL * p.ctas * p.cols * (c.head_dim + 2) * 4;
@@ -1023,7 +1044,7 @@ void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, con
   const P4Plan plan = p4_plan(batch, max_q, G, c.kv_heads, (long long)c.max_pages * c.page_size);
   P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v,
            {c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)}, kv_lens, cu_q,
-           (__nv_bfloat16*)out, q_stride, o_stride, batch, G, c.kv_heads, total_q, kv4_div(G), kv4_div(c.kv_heads),
+           (__nv_bfloat16*)out, q_stride, o_stride, batch, G, c.kv_heads, total_q, max_q, (int)(plan.chunks + 1), kv4_div(G), kv4_div(c.kv_heads),
            scale * 1.4426950408889634f, status};
   float* scratch = (float*)workspace;
   if (c.head_dim == 128) {

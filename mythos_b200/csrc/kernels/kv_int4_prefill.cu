@@ -123,6 +123,7 @@ struct PfExpand {
   float* q_factor;      // [total_q, heads]: 2^eq
   int* exponents;       // [batch * kv_heads, tiles]: ek in the low, ev in the high half
   int kv_heads, heads, tiles, kv_blocks, q_blocks, total_q;
+  int most_q;           // new tokens that the items of a sequence cover
   PfLine line;
   PfPlan plan;
   int ctas;
@@ -140,6 +141,9 @@ __device__ void pf_make_plan(const PfExpand& a) {
   __shared__ int s_sum[PF_EXPAND / 32], s_total;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int each = (a.plan.pairs + PF_EXPAND - 1) / PF_EXPAND, p0 = min(a.plan.pairs, (int)threadIdx.x * each), p1 = min(a.plan.pairs, p0 + each);
+  for (int b = threadIdx.x; b < a.line.batch; b += PF_EXPAND)     // more tokens than the caller said: not all are dealt with
+    if (a.status && (a.line.kv_lens[b] > a.tiles * PF_TILE || a.line.cu_q[b + 1] - a.line.cu_q[b] > a.most_q))
+      atomicCAS(a.status, 0, ST_BAD_ARG | (90 << 16));
   int sum = 0;
   for (int p = p0; p < p1; ++p) sum += PfItem(a.line, p).steps * a.line.units;
   int up = sum;
@@ -835,6 +839,7 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.heads = heads;
   x.tiles = z.tiles;
   x.total_q = total_q;
+  x.most_q = z.n_qb * (2 * PF_TILE / z.pack);
   x.line = {cu_q, kv_lens, batch, z.pack, z.units, z.n_qb, z.tiles};
   x.ctas = z.ctas;
   x.whole = z.whole;
