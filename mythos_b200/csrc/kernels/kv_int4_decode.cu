@@ -1,7 +1,9 @@
 // Attention over the 4-bit paged KV cache for one or a few query tokens per sequence (format: kv_int4.cuh).
 //
 // Queries of one (sequence, kv head) are columns: column c is head c % G of token c / G. A warp takes chunks of 32 tokens
-// (two tiles) for a block of COLS columns through a ring of its own, filled with one bulk copy per tile for K and one for V.
+// (two tiles) for a block of COLS columns through a ring of its own. The ring is filled by 16-byte asynchronous copies, eight
+// lanes to a tile: a bulk copy takes its addresses from uniform registers, and four lanes with a copy each cost 61 instructions
+// a chunk, of 675, where these nine take twelve.
 //
 // What bounds it is the integer pipe (half rate) that takes the codes apart, so operands are formed by one AND each:
 // the low eleven bits of an fp16 are linear in its value (subnormals and the first normal binade share one step,
@@ -61,9 +63,8 @@ __device__ __forceinline__ void p4_mma0(float (&c)[4], uint32_t a0, uint32_t a1,
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ void p4_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void p4_copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ uint32_t p4_half2(float lo, float hi) {
   uint32_t r;
@@ -135,6 +136,8 @@ struct P4State {
   int limit[NB][2];
   float o[NB][GR][4][4];                  // units of 2^-24 (even i) and 2^-20
   float z[NB][GR][2], m[NB][2], l[NB][2];
+  uint32_t unseen;                        // bit 2 nb + c: the column has seen no score yet (its reference is 0)
+  bool fresh;                             // some column of the warp has seen none
 };
 
 // One chunk: tile u (0, 1) at `at` + u * TILE_BYTES for K, HALF behind for V; tok0: its first token.
@@ -200,11 +203,6 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
   float x[2][NB][2][2];                           // [tile][block][j][c]
   float top = -INFINITY;
   const int tok_r = tok0 + ((r >> 1) & 3) + ((r & 1) << 2);                // token of key row r of the first tile; row r + 8: 8 on
-  float mm[NB][2];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) mm[nb][c] = s.m[nb][c] == -INFINITY ? 0.f : s.m[nb][c];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -225,22 +223,18 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
           if constexpr (GR == 2) v = fmaf(kv4_low(kq[1]), s.qsum[nb][1][c], v);
 #pragma unroll
           for (int g = 0; g < GR; ++g) v = fmaf(kv4_scale(kq[g]), sc[u][nb][g][2 * j + c], v);
-          v = fmaf(v, s.factor[nb][c], -mm[nb][c]);
+          v = fmaf(v, s.factor[nb][c], -s.m[nb][c]);
           if (MASK && (tok_r + 16 * u + 8 * j >= s.limit[nb][c] || (absent >> u & 1u))) v = -INFINITY;
           x[u][nb][j][c] = v;
         }
     }
-  bool first = false;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) first = first || s.m[nb][c] == -INFINITY;
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < 2; ++j) top = fmax3(top, x[u][nb][j][0], x[u][nb][j][1]);
-  }
-  if (__any_sync(0xffffffffu, first || top + ev > 6.f)) {
+  if (s.fresh || __any_sync(0xffffffffu, top + ev > 6.f)) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -249,9 +243,11 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         mx += ev;                                 // relative to the reference used so far
-        if (s.m[nb][c] == -INFINITY ? mx > -INFINITY : mx > 0.f) {
-          const float alpha = s.m[nb][c] == -INFINITY ? 0.f : fast_exp2(-mx);
-          s.m[nb][c] = mm[nb][c] + mx;
+        const bool first = s.unseen >> (2 * nb + c) & 1u;
+        if (first ? mx > -INFINITY : mx > 0.f) {
+          const float alpha = first ? 0.f : fast_exp2(-mx);
+          s.unseen &= ~(1u << (2 * nb + c));
+          s.m[nb][c] += mx;
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -268,6 +264,7 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
           }
         }
       }
+    s.fresh = __any_sync(0xffffffffu, s.unseen != 0u);
   }
   // ---- weights p scale as the B operand (k = tokens, n = columns): transposed in blocks of eight by eight. Odd key rows
   // are the tokens that enter with the complement of their codes.
@@ -401,10 +398,12 @@ __device__ __forceinline__ void p4_queries(P4State<D, COLS>& s, const P4Args& a,
       const int from = 8 * t + 4 * c;
       s.limit[nb][c] = __shfl_sync(0xffffffffu, limit, from);
       s.factor[nb][c] = a.scale_log2 * 0x1p21f * p4_pow2(__shfl_sync(0xffffffffu, eq, from));
-      s.m[nb][c] = -INFINITY;
+      s.m[nb][c] = 0.f;
       s.l[nb][c] = 0.f;
     }
   }
+  s.unseen = (1u << (2 * NB)) - 1u;
+  s.fresh = true;
 }
 
 // The state's sums, complete over the warp: into `out` (whole) or as a part to w_acc [COLS][D] with references and row sums
@@ -424,7 +423,7 @@ __device__ __forceinline__ void p4_result(const P4State<D, COLS>& s, const P4Arg
       for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
       const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;      // nothing visible: zeros
       if (!whole && r == 0) {
-        ml[cc] = s.m[nb][c];
+        ml[cc] = l == 0.f ? -INFINITY : s.m[nb][c];
         ml[COLS + cc] = l;
       }
       __nv_bfloat16* dst = whole ? u.out(a, D, cc, 8 * r) : nullptr;
@@ -453,73 +452,71 @@ __device__ __forceinline__ void p4_result(const P4State<D, COLS>& s, const P4Arg
 }
 
 // A warp's chunks 0 .. mine - 1 through its ring. locate(i) gives the tile of the lane's half (lane & 1) of chunk i: -1 without
-// a page (reported, left out), -2 behind the keys.
+// a page (reported, left out), -2 behind the keys. Lanes 8 n .. 8 n + 7 copy tile n % 2 of K (n < 2) or V.
 template <int D, int COLS>
 struct P4Feed {
   using L = KvInt4<D>;
   using C = P4Cfg<D, COLS>;
-  const P4Args& a;
-  uint8_t* ring;
-  uint64_t* full;
+  static constexpr int PIECES = L::TILE_BYTES / 16;
+  const uint8_t* ring;
+  const uint8_t* from;            // the lane's first piece of tile 0
+  uint32_t to;                    // of stage 0
+  int* status;
   int lane, mine;
   int ids = -2, ids_next = -2;    // lane l: tile l % 2 of chunk 16 n + l / 2 for the block n being issued, and of the next one
-  uint32_t absent = 0u, parity = 0u;   // bits 2 s, 2 s + 1: tiles of stage s that were not loaded
-  int st = 0;                     // stage of the next chunk to use
+  uint32_t none = 0u;             // bit l: that tile does not exist
+  uint32_t gone = 0u, gone_next = 0u;  // bits 0, 1: tiles of the chunk in use, and of the next one, that were not loaded
+  int off = 0;                    // of the stage in use (0 or STAGE)
+  __device__ __forceinline__ P4Feed(const P4Args& a, uint8_t* ring_, int lane_, int mine_) : ring(ring_), status(a.status), lane(lane_), mine(mine_) {
+    from = ((lane & 16) ? a.v_cache : a.k_cache) + (lane & 7) * 16;
+    to = smem_u32(ring_) + ((lane & 16) ? C::HALF : 0) + ((lane & 8) ? L::TILE_BYTES : 0) + (lane & 7) * 16;
+  }
   template <class F>
   __device__ __forceinline__ void issue(int i, int stage, const F& locate) {
-    if ((i & 15) == 0) ids = i == 0 ? locate(lane >> 1) : ids_next;
-    if ((i & 15) == 4 && i + 12 < mine) ids_next = locate(i + 12 + (lane >> 1));
-    const int id = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + (lane & 1));
-    const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 3u;
-    absent = (absent & ~(3u << (2 * stage))) | gone << (2 * stage);
-    if (lane == 0) {
-      if (gone == 3u) mbar_arrive(&full[stage]);
-      else mbar_arrive_expect_tx(&full[stage], gone ? C::STAGE / 2 : C::STAGE);
+    if (i < mine) {
+      const int k = i & 15;
+      if (k == 0) {
+        ids = i == 0 ? locate(lane >> 1) : ids_next;
+        none = __ballot_sync(0xffffffffu, ids < 0);
+        if (ids == -1 && status) atomicCAS(status, 0, ST_BAD_ARG | (92 << 16));
+      }
+      if (k == 4 && i + 12 < mine) ids_next = locate(i + 12 + (lane >> 1));
+      const int id = __shfl_sync(0xffffffffu, ids, 2 * k + (lane >> 3 & 1));
+      gone_next = none >> (2 * k) & 3u;
+      if (id >= 0) {
+        const uint8_t* src = from + (long long)id * L::TILE_BYTES;
+#pragma unroll
+        for (int j = 0; j < PIECES / 8; ++j) p4_copy16(to + stage + 128 * j, src + 128 * j);
+        if (PIECES % 8 && (lane & 7) < PIECES % 8) p4_copy16(to + stage + PIECES / 8 * 128, src + PIECES / 8 * 128);
+      }
     }
-    if (lane < 4) {               // one copy each: tile lane % 2, K (lane < 2) or V
-      if (id >= 0)
-        p4_bulk_load(smem_u32(ring) + stage * C::STAGE + ((lane & 2) ? C::HALF : 0) + (lane & 1) * L::TILE_BYTES,
-                     ((lane & 2) ? a.v_cache : a.k_cache) + (long long)id * L::TILE_BYTES, L::TILE_BYTES, &full[stage]);
-      else if (id == -1 && a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (92 << 16));
-    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // Waits for chunk i, with the next one under way. False: the wait ran out.
+  // Waits for chunk i, with the next one under way.
   template <class F>
-  __device__ __forceinline__ bool wait(int i, volatile int* abort_flag, const F& locate) {
-    // the stage read in the step before is free now: every value read from it has gone through a product
-    if (i + 1 < mine) issue(i + 1, st ^ 1, locate);
-    if (__all_sync(0xffffffffu, mbar_try_wait(&full[st], parity))) return true;
-    const bool ok = mbar_wait(&full[st], parity, abort_flag, a.status, 93);
-    return __all_sync(0xffffffffu, ok);
+  __device__ __forceinline__ void wait(int i, const F& locate) {
+    gone = gone_next;
+    issue(i + 1, off ^ C::STAGE, locate);         // (every lane is done with that stage: next())
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
   }
-  __device__ __forceinline__ const uint8_t* at() const { return ring + st * C::STAGE; }
-  __device__ __forceinline__ uint32_t gone() const { return absent >> (2 * st) & 3u; }
+  __device__ __forceinline__ const uint8_t* at() const { return ring + off; }
   __device__ __forceinline__ void next() {
     __syncwarp();
-    parity ^= (uint32_t)st;
-    st ^= 1;
-  }
-  // After a wait that ran out at chunk i: copies in flight land before the ring's memory goes away.
-  __device__ __forceinline__ void drain(int i) {
-    for (int k = 0; k < C::STAGES && i + k < mine; ++k) {
-      mbar_drain(&full[st], parity);
-      parity ^= (uint32_t)st;
-      st ^= 1;
-    }
+    off ^= C::STAGE;
   }
 };
 static_assert(P4Cfg<128, 8>::STAGES == 2, "P4Feed alternates between two stages");
 
-// Chunks i .. end - 1 of the warp, which are the unit's chunks chunk, chunk + step, ...; false: a wait ran out. Those that every
-// column sees whole come first and have a loop of their own: with both forms in one loop the accumulators were copied
-// between them.
+// Chunks i .. end - 1 of the warp, which are the unit's chunks chunk, chunk + step, ... Those that every column sees whole come
+// first and have a loop of their own: with both forms in one loop the accumulators were copied between them.
 template <int D, int COLS, class F>
-__device__ __forceinline__ bool p4_run(P4State<D, COLS>& s, P4Feed<D, COLS>& feed, const P4Unit& u, int& i, int end, int chunk, int step,
-                                       volatile int* abort_flag, const F& locate) {
+__device__ __forceinline__ void p4_run(P4State<D, COLS>& s, P4Feed<D, COLS>& feed, const P4Unit& u, int& i, int end, int chunk, int step,
+                                       const F& locate) {
   bool waited = false;
   for (; i < end && (chunk + 1) * P4_CHUNK <= u.to_all; ++i, chunk += step) {
-    if (!feed.wait(i, abort_flag, locate)) return false;
-    if (feed.gone() != 0u) {
+    feed.wait(i, locate);
+    if (feed.gone != 0u) {
       waited = true;
       break;
     }
@@ -528,12 +525,11 @@ __device__ __forceinline__ bool p4_run(P4State<D, COLS>& s, P4Feed<D, COLS>& fee
   }
 #pragma unroll 1
   for (; i < end; ++i, chunk += step) {
-    if (!waited && !feed.wait(i, abort_flag, locate)) return false;
+    if (!waited) feed.wait(i, locate);
     waited = false;
-    p4_chunk<D, COLS, true>(s, feed.at(), chunk * P4_CHUNK, feed.lane, u.to_some, feed.gone());
+    p4_chunk<D, COLS, true>(s, feed.at(), chunk * P4_CHUNK, feed.lane, u.to_some, feed.gone);
     feed.next();
   }
-  return true;
 }
 
 // Joins the parts of a unit that shared memory holds (bits of `parts`), column c, values d .. d + 3: sums, and the column's
@@ -596,9 +592,7 @@ struct P4SmemCluster {
   static constexpr int OFF_CTA = P4_WARPS * C::WARP_BYTES;                  // the CTA's sums
   static constexpr int OFF_ML = OFF_CTA + C::PART;                          // [warps][m, l][COLS]
   static constexpr int OFF_CML = OFF_ML + P4_WARPS * 2 * COLS * 4;          // of the CTA: [m, l][COLS]
-  static constexpr int OFF_BAR = OFF_CML + 2 * COLS * 4;
-  static constexpr int OFF_FLAG = OFF_BAR + P4_WARPS * C::STAGES * 8;
-  static constexpr int BYTES = OFF_FLAG + 16;
+  static constexpr int BYTES = OFF_CML + 2 * COLS * 4;
 };
 
 template <int D, int COLS>
@@ -611,17 +605,9 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   const P4Unit u(a, COLS, blockIdx.x, blockIdx.y);
   if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && u.q_len > a.max_q) p4_too_long(a);
   if (u.n_cols <= 0) return;                      // the same for every CTA of the cluster
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * C::STAGES;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::OFF_FLAG);
   float* s_ml = reinterpret_cast<float*>(smem + S::OFF_ML);
   float* s_cml = reinterpret_cast<float*>(smem + S::OFF_CML);
   float* s_cta = reinterpret_cast<float*>(smem + S::OFF_CTA);
-  if (threadIdx.x == 0) *abort_flag = 0;
-  if (lane == 0) {
-    for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
-    fence_mbar_init();
-  }
-  __syncthreads();
   const int n = u.chunks(a), per = (n + splits - 1) / splits;
   const int chunk0 = blockIdx.z * per + warp, end = min(n, (int)blockIdx.z * per + per);
   const int mine = max(0, (end - chunk0 + P4_WARPS - 1) / P4_WARPS);        // chunk0, + 4, ...
@@ -629,16 +615,13 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
     const int token = (chunk0 + P4_WARPS * i) * P4_CHUNK + (lane & 1) * 16;
     return i < mine && token < u.kv_len ? a.pages.tile(u.b, token, u.hkv) : -2;
   };
-  P4Feed<D, COLS> feed{a, smem + warp * C::WARP_BYTES, full, lane, mine};
-  if (mine > 0) feed.issue(0, 0, locate);
+  P4Feed<D, COLS> feed(a, smem + warp * C::WARP_BYTES, lane, mine);
+  feed.issue(0, 0, locate);
   P4State<D, COLS> s;
   p4_queries(s, a, u, lane);
   int i = 0;
-  const bool ok = p4_run(s, feed, u, i, mine, chunk0, P4_WARPS, abort_flag, locate);
-  if (!ok) feed.drain(i);
-  p4_result(s, a, u, false, reinterpret_cast<float*>(feed.ring), s_ml + warp * 2 * COLS, lane);
-  __syncwarp();
-  if (!ok) s_ml[warp * 2 * COLS + COLS + lane % COLS] = 0.f;                // counts as nothing seen
+  p4_run(s, feed, u, i, mine, chunk0, P4_WARPS, locate);
+  p4_result(s, a, u, false, reinterpret_cast<float*>(smem + warp * C::WARP_BYTES), s_ml + warp * 2 * COLS, lane);
   __syncthreads();
   for (int k = threadIdx.x; k < COLS * D / 4; k += P4_THREADS) {
     const int c = 4 * k / D, d = 4 * k % D;
@@ -756,9 +739,7 @@ struct P4SmemLine {
   static constexpr int OFF_ML = OFF_HEAD + P4_WARPS * C::PART;              // [warps][head, tail][m, l][COLS]
   static constexpr int OFF_UNIT = OFF_ML + P4_WARPS * 4 * COLS * 4;         // [warps][head, tail] int4: sequence, unit, begins, ends
   static constexpr int OFF_LEAD = OFF_UNIT + P4_WARPS * 2 * 16;             // int2: sequence and unit of the CTA's first chunk
-  static constexpr int OFF_BAR = OFF_LEAD + 16;
-  static constexpr int OFF_FLAG = OFF_BAR + P4_WARPS * C::STAGES * 8;
-  static constexpr int BYTES = OFF_FLAG + 16;
+  static constexpr int BYTES = OFF_LEAD + 16;
 };
 
 template <int D, int COLS>
@@ -768,20 +749,13 @@ paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict_
   using S = P4SmemLine<D, COLS>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR) + warp * C::STAGES;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::OFF_FLAG);
   float* s_ml = reinterpret_cast<float*>(smem + S::OFF_ML);
   int4* s_unit = reinterpret_cast<int4*>(smem + S::OFF_UNIT);
   int2* s_lead = reinterpret_cast<int2*>(smem + S::OFF_LEAD);
   // the merge may start as soon as there is room; it waits for this grid's end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) *abort_flag = 0;
-  if (lane == 0) {
-    for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
-    fence_mbar_init();
-  }
   if (lane < 2) s_unit[warp * 2 + lane] = make_int4(-1, 0, 0, 0);
-  __syncthreads();
+  __syncwarp();                                   // (the warp's own, until the CTA meets)
 
   const P4Line line(a, COLS);
   const P4Scan scan(line, lane);
@@ -810,8 +784,8 @@ paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict_
     const int at = f - lbegin, ly = at / ln, token = (at - ly * ln) * P4_CHUNK + (lane & 1) * 16;
     return token < a.kv_lens[lb] ? a.pages.tile(lb, token, ly - a.by_heads(ly) * a.kv_heads) : -2;
   };
-  P4Feed<D, COLS> feed{a, smem + warp * C::WARP_BYTES, full, lane, mine};
-  if (mine > 0) feed.issue(0, 0, locate);
+  P4Feed<D, COLS> feed(a, smem + warp * C::WARP_BYTES, lane, mine);
+  feed.issue(0, 0, locate);
   P4State<D, COLS> s;
   int i = 0;
   while (i < mine) {
@@ -820,14 +794,11 @@ paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict_
     const bool begins = chunk == 0;
     p4_queries(s, a, u, lane);
     const int part = min(n - chunk, mine - i);
-    if (!p4_run(s, feed, u, i, i + part, chunk, 1, abort_flag, locate)) {
-      feed.drain(i);
-      break;
-    }
+    p4_run(s, feed, u, i, i + part, chunk, 1, locate);
     chunk += part;
     const bool ends = chunk == n;
     const int slot = ends ? 0 : 1;                // (a part that does not end its unit is the warp's last)
-    p4_result(s, a, u, begins && ends, reinterpret_cast<float*>(slot ? feed.ring : smem + S::OFF_HEAD + warp * C::PART),
+    p4_result(s, a, u, begins && ends, reinterpret_cast<float*>(smem + (slot ? warp * C::WARP_BYTES : S::OFF_HEAD + warp * C::PART)),
               s_ml + (warp * 2 + slot) * 2 * COLS, lane);
     if (!(begins && ends) && lane == 0) s_unit[warp * 2 + slot] = make_int4(b, y, begins ? 1 : 0, ends ? 1 : 0);
     if (ends) {
