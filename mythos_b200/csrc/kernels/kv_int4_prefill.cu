@@ -432,141 +432,145 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
-
-  if (warp == 2) {
-    // ------------------------------------------------------------------ Q loader
-    if (lane == 0) {
-      uint32_t n_q[2] = {0, 0};   // loads issued per tile (phase of q_free / q_full)
-      bool ok = true;
-      for (PfCursor c(a); c.more() && ok;) {
-        const PfItem it = c.next(a);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (min(c.j1, it.J[t]) <= c.j0 || !ok) continue;
-          if (!mbar_wait(&q_free[t], (n_q[t] & 1) ^ 1, abort_flag, status, 94)) { ok = false; break; }
-          mbar_arrive_expect_tx(&q_full[t], Cfg::TILE_BYTES);
-          for (int k = 0; k < CHUNKS; ++k)
-            tma_load_3d(smem + Cfg::OFF_Q + t * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_q, &q_full[t], k * 64,
-                        c.of_unit * a.line.pack, it.row0 + it.tok[t]);
-          ++n_q[t];
-        }
-      }
-    }
-  } else if (warp == 0) {
-    // ------------------------------------------------------------------ K / V loader
-    if (lane == 0) {
-      uint32_t kc = 0, vc = 0;
-      bool ok = true;
-      for (PfCursor c(a); c.more() && ok;) {
-        const PfItem it = c.next(a);
-        const int bh = it.b * kv_heads + c.of_unit * a.line.pack / a.group, end = min(c.j1, max(it.J[0], it.J[1]));
-        for (int j = c.j0; j < end; ++j) {
-          const int ks = kc % KS, vs = vc % VS;
-          if (!mbar_wait(&k_empty[ks], ((kc / KS) & 1) ^ 1, abort_flag, status, 95)) { ok = false; break; }
-          mbar_arrive_expect_tx(&k_full[ks], Cfg::TILE_BYTES);
-          for (int k = 0; k < CHUNKS; ++k)
-            tma_load_3d(smem + Cfg::OFF_K + ks * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_k, &k_full[ks], k * 64, j * PF_TILE, bh);
-          ++kc;
-          if (!mbar_wait(&v_empty[vs], ((vc / VS) & 1) ^ 1, abort_flag, status, 96)) { ok = false; break; }
-          mbar_arrive_expect_tx(&v_full[vs], Cfg::TILE_BYTES);
-          for (int k = 0; k < CHUNKS; ++k)
-            tma_load_3d(smem + Cfg::OFF_V + vs * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_v, &v_full[vs], k * 64, j * PF_TILE, bh);
-          ++vc;
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t IDESC_S = pf_idesc(PF_TILE, PF_TILE, false);
-      constexpr uint32_t IDESC_O = pf_idesc(PF_TILE, D, true);
-      const uint32_t q_addr = smem_u32(smem + Cfg::OFF_Q);
-      const uint32_t k_addr = smem_u32(smem + Cfg::OFF_K);
-      const uint32_t v_addr = smem_u32(smem + Cfg::OFF_V);
-      uint32_t kc = 0, vc = 0;              // K / V tiles consumed so far (ring position and phase)
-      uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
-      bool ok = true;
-      auto issue_s = [&](int t, uint32_t kpos) {
-        const uint32_t qa = q_addr + t * Cfg::TILE_BYTES;
-        const uint32_t ka = k_addr + (kpos % KS) * Cfg::TILE_BYTES;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const int c = k >> 2, kk = k & 3;
-          umma_f16(tmem_base + Cfg::COL_S + t * 128, umma_desc_sw128(qa + c * (PF_TILE * 128) + kk * 32, 0, 1024),
-                   umma_desc_sw128(ka + c * (PF_TILE * 128) + kk * 32, 0, 1024), IDESC_S, k > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[t]);
-      };
-      for (PfCursor c(a); c.more() && ok;) {
-        const PfItem it = c.next(a);
-        const int j0 = c.j0;
-        int end[2];                         // steps of each tile in this part: j0 .. end - 1
-#pragma unroll
-        for (int t = 0; t < 2; ++t) end[t] = min(c.j1, it.J[t]);
-        const int last = max(end[0], end[1]);
-        if (last <= j0) continue;
-        // scores of the first step for both tiles
-        if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 97)) { ok = false; break; }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (end[t] <= j0 || !ok) continue;
-          if (!mbar_wait(&q_full[t], n_q[t] & 1, abort_flag, status, 98)) { ok = false; break; }
-          tc_fence_after();
-          issue_s(t, kc);
-          if (end[t] == j0 + 1) umma_commit(&q_free[t]);
-        }
-        if (!ok) break;
-        umma_commit(&k_empty[kc % KS]);   // every score product of the first key tile has been issued
-        ++kc;
-        for (int j = j0; j < last && ok; ++j) {
-          bool v_ready = false, k_ready = false;
-          const bool have_next = j + 1 < last;
+  // 384 threads start with 168 registers each (64512); 128 x 96 + 256 x 200 = 63488
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 2) {
+      // ------------------------------------------------------------------ Q loader
+      if (lane == 0) {
+        uint32_t n_q[2] = {0, 0};   // loads issued per tile (phase of q_free / q_full)
+        bool ok = true;
+        for (PfCursor c(a); c.more() && ok;) {
+          const PfItem it = c.next(a);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (j >= end[t] || !ok) continue;
-            if (!mbar_wait(&p_full[2 * t], n_p[t] & 1, abort_flag, status, 99)) { ok = false; break; }
-            if (!v_ready) {
-              if (!mbar_wait(&v_full[vc % VS], (vc / VS) & 1, abort_flag, status, 100)) { ok = false; break; }
-              v_ready = true;
-            }
-            tc_fence_after();
-            const uint32_t va = v_addr + (vc % VS) * Cfg::TILE_BYTES;
-#pragma unroll
-            for (int k = 0; k < PF_TILE / 16; ++k) {   // O_t += P_t(tmem) V, the second half while its exponentials run
-              if (k == PF_TILE / 32) {
-                if (!mbar_wait(&p_full[2 * t + 1], n_p[t] & 1, abort_flag, status, 104)) { ok = false; break; }
-                tc_fence_after();
-              }
-              umma_f16_ts(tmem_base + Cfg::COL_O + t * D, tmem_base + Cfg::COL_S + t * 128 + k * 8,
-                          umma_desc_sw128(va + k * 2048, PF_TILE * 128, 1024), IDESC_O, (j > j0 || k > 0) ? 1u : 0u);
-            }
-            if (!ok) break;
-            ++n_p[t];
-            if (j == end[t] - 1) umma_commit(&o_full[t]);
-            if (j + 1 < end[t]) {
-              if (!k_ready) {
-                if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 101)) { ok = false; break; }
-                tc_fence_after();
-                k_ready = true;
-              }
-              issue_s(t, kc);               // overwrites S_t / P_t: ordered behind the PV product just issued
-              if (j + 2 == end[t]) umma_commit(&q_free[t]);   // that was the tile's last score product
-            }
-          }
-          if (!ok) break;
-          umma_commit(&v_empty[vc % VS]);
-          ++vc;
-          if (have_next) {
-            umma_commit(&k_empty[kc % KS]);
-            ++kc;
+            if (min(c.j1, it.J[t]) <= c.j0 || !ok) continue;
+            if (!mbar_wait(&q_free[t], (n_q[t] & 1) ^ 1, abort_flag, status, 94)) { ok = false; break; }
+            mbar_arrive_expect_tx(&q_full[t], Cfg::TILE_BYTES);
+            for (int k = 0; k < CHUNKS; ++k)
+              tma_load_3d(smem + Cfg::OFF_Q + t * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_q, &q_full[t], k * 64,
+                          c.of_unit * a.line.pack, it.row0 + it.tok[t]);
+            ++n_q[t];
           }
         }
+      }
+    } else if (warp == 0) {
+      // ------------------------------------------------------------------ K / V loader
+      if (lane == 0) {
+        uint32_t kc = 0, vc = 0;
+        bool ok = true;
+        for (PfCursor c(a); c.more() && ok;) {
+          const PfItem it = c.next(a);
+          const int bh = it.b * kv_heads + c.of_unit * a.line.pack / a.group, end = min(c.j1, max(it.J[0], it.J[1]));
+          for (int j = c.j0; j < end; ++j) {
+            const int ks = kc % KS, vs = vc % VS;
+            if (!mbar_wait(&k_empty[ks], ((kc / KS) & 1) ^ 1, abort_flag, status, 95)) { ok = false; break; }
+            mbar_arrive_expect_tx(&k_full[ks], Cfg::TILE_BYTES);
+            for (int k = 0; k < CHUNKS; ++k)
+              tma_load_3d(smem + Cfg::OFF_K + ks * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_k, &k_full[ks], k * 64, j * PF_TILE, bh);
+            ++kc;
+            if (!mbar_wait(&v_empty[vs], ((vc / VS) & 1) ^ 1, abort_flag, status, 96)) { ok = false; break; }
+            mbar_arrive_expect_tx(&v_full[vs], Cfg::TILE_BYTES);
+            for (int k = 0; k < CHUNKS; ++k)
+              tma_load_3d(smem + Cfg::OFF_V + vs * Cfg::TILE_BYTES + k * (PF_TILE * 128), &tm_v, &v_full[vs], k * 64, j * PF_TILE, bh);
+            ++vc;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t IDESC_S = pf_idesc(PF_TILE, PF_TILE, false);
+        constexpr uint32_t IDESC_O = pf_idesc(PF_TILE, D, true);
+        const uint32_t q_addr = smem_u32(smem + Cfg::OFF_Q);
+        const uint32_t k_addr = smem_u32(smem + Cfg::OFF_K);
+        const uint32_t v_addr = smem_u32(smem + Cfg::OFF_V);
+        uint32_t kc = 0, vc = 0;              // K / V tiles consumed so far (ring position and phase)
+        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
+        bool ok = true;
+        auto issue_s = [&](int t, uint32_t kpos) {
+          const uint32_t qa = q_addr + t * Cfg::TILE_BYTES;
+          const uint32_t ka = k_addr + (kpos % KS) * Cfg::TILE_BYTES;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (end[t] > j0) ++n_q[t];
+          for (int k = 0; k < D / 16; ++k) {
+            const int c = k >> 2, kk = k & 3;
+            umma_f16(tmem_base + Cfg::COL_S + t * 128, umma_desc_sw128(qa + c * (PF_TILE * 128) + kk * 32, 0, 1024),
+                     umma_desc_sw128(ka + c * (PF_TILE * 128) + kk * 32, 0, 1024), IDESC_S, k > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[t]);
+        };
+        for (PfCursor c(a); c.more() && ok;) {
+          const PfItem it = c.next(a);
+          const int j0 = c.j0;
+          int end[2];                         // steps of each tile in this part: j0 .. end - 1
+#pragma unroll
+          for (int t = 0; t < 2; ++t) end[t] = min(c.j1, it.J[t]);
+          const int last = max(end[0], end[1]);
+          if (last <= j0) continue;
+          // scores of the first step for both tiles
+          if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 97)) { ok = false; break; }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (end[t] <= j0 || !ok) continue;
+            if (!mbar_wait(&q_full[t], n_q[t] & 1, abort_flag, status, 98)) { ok = false; break; }
+            tc_fence_after();
+            issue_s(t, kc);
+            if (end[t] == j0 + 1) umma_commit(&q_free[t]);
+          }
+          if (!ok) break;
+          umma_commit(&k_empty[kc % KS]);   // every score product of the first key tile has been issued
+          ++kc;
+          for (int j = j0; j < last && ok; ++j) {
+            bool v_ready = false, k_ready = false;
+            const bool have_next = j + 1 < last;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (j >= end[t] || !ok) continue;
+              if (!mbar_wait(&p_full[2 * t], n_p[t] & 1, abort_flag, status, 99)) { ok = false; break; }
+              if (!v_ready) {
+                if (!mbar_wait(&v_full[vc % VS], (vc / VS) & 1, abort_flag, status, 100)) { ok = false; break; }
+                v_ready = true;
+              }
+              tc_fence_after();
+              const uint32_t va = v_addr + (vc % VS) * Cfg::TILE_BYTES;
+#pragma unroll
+              for (int k = 0; k < PF_TILE / 16; ++k) {   // O_t += P_t(tmem) V, the second half while its exponentials run
+                if (k == PF_TILE / 32) {
+                  if (!mbar_wait(&p_full[2 * t + 1], n_p[t] & 1, abort_flag, status, 104)) { ok = false; break; }
+                  tc_fence_after();
+                }
+                umma_f16_ts(tmem_base + Cfg::COL_O + t * D, tmem_base + Cfg::COL_S + t * 128 + k * 8,
+                            umma_desc_sw128(va + k * 2048, PF_TILE * 128, 1024), IDESC_O, (j > j0 || k > 0) ? 1u : 0u);
+              }
+              if (!ok) break;
+              ++n_p[t];
+              if (j == end[t] - 1) umma_commit(&o_full[t]);
+              if (j + 1 < end[t]) {
+                if (!k_ready) {
+                  if (!mbar_wait(&k_full[kc % KS], (kc / KS) & 1, abort_flag, status, 101)) { ok = false; break; }
+                  tc_fence_after();
+                  k_ready = true;
+                }
+                issue_s(t, kc);               // overwrites S_t / P_t: ordered behind the PV product just issued
+                if (j + 2 == end[t]) umma_commit(&q_free[t]);   // that was the tile's last score product
+              }
+            }
+            if (!ok) break;
+            umma_commit(&v_empty[vc % VS]);
+            ++vc;
+            if (have_next) {
+              umma_commit(&k_empty[kc % KS]);
+              ++kc;
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (end[t] > j0) ++n_q[t];
+        }
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------------ softmax + epilogue
     const int t = (warp - 4) >> 2;           // query tile
     const int quarter = warp & 3;            // TMEM lane quarter this warp may access
@@ -603,16 +607,43 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         ++n_s;
         tc_fence_after();
         uint32_t sr[4][32];
+        float* s = reinterpret_cast<float*>(&sr[0][0]);
+        const int kv0 = j * PF_TILE;
+        const auto hide = [&](int from, int to) {
+          if (kv0 + to - 1 > limit) {
+#pragma unroll
+            for (int i = from; i < to; ++i)
+              if (kv0 + i > limit) s[i] = -INFINITY;
+          }
+        };
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, sr[c]);
         tmem_ld_wait();
-        float* s = reinterpret_cast<float*>(&sr[0][0]);
-        const int kv0 = j * PF_TILE;
-        if (kv0 + PF_TILE - 1 > limit) {
+        hide(0, 128);
+        uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
+        uint32_t pk[2][32];
+        const auto exponentials = [&](int h) {   // of half h of the keys: fp16 pairs to pk[h], sums to rs2
+          const float shift = ev - m_ref;
+          const uint64_t sc2 = f32x2(sc, sc), nm2 = f32x2(shift, shift);
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (kv0 + i > limit) s[i] = -INFINITY;
-        }
+          for (int i = 64 * h; i < 64 * h + 64; i += 2) {
+            float e0f, e1f;
+            f32x2_unpack(fma_f32x2(f32x2(s[i], s[i + 1]), sc2, nm2), e0f, e1f);
+            const float p0 = fast_exp2(e0f), p1 = fast_exp2(e1f);
+            rs2[(i >> 1) & 3] = add_f32x2(rs2[(i >> 1) & 3], f32x2(p0, p1));
+            pk[h][(i >> 1) & 31] = pf_half2(p0, p1);
+          }
+        };
+        const auto publish = [&](int h) {        // P_t: fp16 pairs over the first 64 columns of S_t
+          tmem_st32(t_s + 32 * h, pk[h]);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&p_full[2 * t + h]);
+        };
+        // The reference rarely moves: the first half's exponentials are taken with the one there is, with the maximum of all
+        // 128 scores in their shadow, and again where it does (257 us -> 242 at 2048 over 6144; the registers that takes come from
+        // the service warps).
+        if (j > j0) exponentials(0);
         float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
         for (int i = 4; i < 124; i += 8) {
@@ -624,51 +655,38 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         mx4[0] = fmax3(mx4[0], s[124], s[125]);
         mx4[1] = fmax3(mx4[1], s[126], s[127]);
         const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sc, ev);
-        float alpha = 1.f;
-        bool need = false;
-        if (j == j0) {
-          m_ref = (m_new == -INFINITY) ? 0.f : m_new;
-        } else if (m_new - m_ref > 6.f) {     // lazy: p up to 2^6 until the reference moves
-          need = true;
-          alpha = fast_exp2(m_ref - m_new);
-          m_ref = m_new;
-        }
-        // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):
-        // O_t is quiescent until this warpgroup arrives on p_full, so a rescale can happen right here.
-        if (j > j0 && __any_sync(0xffffffffu, need)) {
+        const bool need = j == j0 || m_new - m_ref > 6.f;      // p up to 2^6 until the reference moves
+        if (__any_sync(0xffffffffu, need)) {
+          const float alpha = need ? fast_exp2(m_ref - m_new) : 1.f;
+          if (need) m_ref = m_new == -INFINITY ? 0.f : m_new;
+          if (j > j0) {
+            l *= alpha;
+            // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):
+            // O_t is quiescent until this warpgroup arrives on p_full, so a rescale can happen right here.
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t orr[32];
-            tmem_ld32(t_o + c * 32, orr);
+            for (int c = 0; c < D / 32; ++c) {
+              tmem_ld32(t_o + c * 32, pk[0]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) pk[0][i] = __float_as_uint(__uint_as_float(pk[0][i]) * alpha);
+              tmem_st32(t_o + c * 32, pk[0]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) rs2[q] = 0ull;
+            tmem_ld32(t_s, sr[0]);               // (the first half again: its registers need not outlive the exponentials)
+            tmem_ld32(t_s + 32, sr[1]);
             tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * alpha);
-            tmem_st32(t_o + c * 32, orr);
+            hide(0, 64);
           }
+          exponentials(0);
         }
-        const float shift = ev - m_ref;
-        const uint64_t sc2 = f32x2(sc, sc), nm2 = f32x2(shift, shift);
-        uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
-        uint32_t* pk = &sr[0][0];         // packed in place: pair i lands in word i / 2, behind the read position
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int i = 64 * h; i < 64 * h + 64; i += 2) {
-            float e0f, e1f;
-            f32x2_unpack(fma_f32x2(f32x2(s[i], s[i + 1]), sc2, nm2), e0f, e1f);
-            const float p0 = fast_exp2(e0f), p1 = fast_exp2(e1f);
-            rs2[(i >> 1) & 3] = add_f32x2(rs2[(i >> 1) & 3], f32x2(p0, p1));
-            pk[i >> 1] = pf_half2(p0, p1);
-          }
-          tmem_st32(t_s + 32 * h, sr[h]);   // P_t: fp16 pairs over the first 64 columns of S_t
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&p_full[2 * t + h]);
-        }
+        publish(0);
+        exponentials(1);
+        publish(1);
         float rs[8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
-        l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(e0 - e);
+        l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(e0 - e);
       }
       if (!ok) break;
       if (end > j0) {
