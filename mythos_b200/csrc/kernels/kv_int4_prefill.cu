@@ -51,6 +51,34 @@ __device__ __forceinline__ uint32_t pf_half2(float a, float b) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
+// tcgen05.mma on fp16 with the descriptors' low words (address / 16) in registers and their high words constant: formed anew for
+// every product, they took the issuing thread longer than the product takes.
+constexpr uint32_t PF_DESC_HI = 1024 / 16 | 1u << 14 | 2u << 29;      // atoms 1024 bytes apart, version, 128-byte swizzle
+template <uint32_t IDESC, uint32_t A_HI, uint32_t B_HI>
+__device__ __forceinline__ void pf_mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 a, b;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "mov.b64 a, {%1, %2};\n"
+      "mov.b64 b, {%3, %4};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n"
+      "}\n" ::"r"(d), "r"(a_lo), "n"(A_HI), "r"(b_lo), "n"(B_HI), "r"(IDESC), "r"(accumulate)
+      : "memory");
+}
+template <uint32_t IDESC, uint32_t B_HI>
+__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 b;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "mov.b64 b, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n"
+      "}\n" ::"r"(d), "r"(a), "r"(b_lo), "n"(B_HI), "r"(IDESC), "r"(accumulate)
+      : "memory");
+}
 // Eight values times inv (a power of two) as fp16. 0x4300 | code is the bf16 number 128 + code; the 128 scale leaves with the low
 // (both exact to 2^-17 of a step, far below fp16's rounding).
 __device__ __forceinline__ uint4 pf_expand8(uint32_t w, uint32_t pair, float inv) {
@@ -482,20 +510,21 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (lane == 0) {
         constexpr uint32_t IDESC_S = pf_idesc(PF_TILE, PF_TILE, false);
         constexpr uint32_t IDESC_O = pf_idesc(PF_TILE, D, true);
-        const uint32_t q_addr = smem_u32(smem + Cfg::OFF_Q);
-        const uint32_t k_addr = smem_u32(smem + Cfg::OFF_K);
-        const uint32_t v_addr = smem_u32(smem + Cfg::OFF_V);
+        const uint32_t q_addr = smem_u32(smem + Cfg::OFF_Q) / 16;
+        const uint32_t k_addr = smem_u32(smem + Cfg::OFF_K) / 16;
+        // (V: keys are rows; the halves of its columns lie PF_TILE * 128 bytes apart)
+        const uint32_t v_addr = smem_u32(smem + Cfg::OFF_V) / 16 + ((PF_TILE * 128 / 16) << 16);
         uint32_t kc = 0, vc = 0;              // K / V tiles consumed so far (ring position and phase)
         uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
         bool ok = true;
         auto issue_s = [&](int t, uint32_t kpos) {
-          const uint32_t qa = q_addr + t * Cfg::TILE_BYTES;
-          const uint32_t ka = k_addr + (kpos % KS) * Cfg::TILE_BYTES;
+          const uint32_t qa = q_addr + t * (Cfg::TILE_BYTES / 16);
+          const uint32_t ka = k_addr + (kpos % KS) * (Cfg::TILE_BYTES / 16);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const int c = k >> 2, kk = k & 3;
-            umma_f16(tmem_base + Cfg::COL_S + t * 128, umma_desc_sw128(qa + c * (PF_TILE * 128) + kk * 32, 0, 1024),
-                     umma_desc_sw128(ka + c * (PF_TILE * 128) + kk * 32, 0, 1024), IDESC_S, k > 0 ? 1u : 0u);
+            pf_mma<IDESC_S, PF_DESC_HI, PF_DESC_HI>(tmem_base + Cfg::COL_S + t * 128, qa + (c * (PF_TILE * 128) + kk * 32) / 16,
+                                        ka + (c * (PF_TILE * 128) + kk * 32) / 16, k > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[t]);
         };
@@ -532,15 +561,15 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 v_ready = true;
               }
               tc_fence_after();
-              const uint32_t va = v_addr + (vc % VS) * Cfg::TILE_BYTES;
+              const uint32_t va = v_addr + (vc % VS) * (Cfg::TILE_BYTES / 16);
 #pragma unroll
               for (int k = 0; k < PF_TILE / 16; ++k) {   // O_t += P_t(tmem) V, the second half while its exponentials run
                 if (k == PF_TILE / 32) {
                   if (!mbar_wait(&p_full[2 * t + 1], n_p[t] & 1, abort_flag, status, 104)) { ok = false; break; }
                   tc_fence_after();
                 }
-                umma_f16_ts(tmem_base + Cfg::COL_O + t * D, tmem_base + Cfg::COL_S + t * 128 + k * 8,
-                            umma_desc_sw128(va + k * 2048, PF_TILE * 128, 1024), IDESC_O, (j > j0 || k > 0) ? 1u : 0u);
+                pf_mma_ts<IDESC_O, PF_DESC_HI>(tmem_base + Cfg::COL_O + t * D, tmem_base + Cfg::COL_S + t * 128 + k * 8, va + k * 128,
+                                     (j > j0 || k > 0) ? 1u : 0u);
               }
               if (!ok) break;
               ++n_p[t];
