@@ -452,6 +452,41 @@ def bench_paged_decode(t: Timer, B: int, ctx: int, H: int, Hkv: int, D: int, spl
     return ms, 2.0 * B * ctx * Hkv * D * 2 / ms / 1e6, "GB/s"
 
 
+def bench_kv_int4(t: Timer, op: str, B: int, ctx: int, new: int, H: int, Hkv: int, D: int):
+    """4-bit pages of 16 tokens: decode attention (KV bytes per second: codes, scales and lows), append and read-back
+    (bytes moved), and attention of ``new`` tokens per sequence at the end of ``ctx`` (FLOP/s of the causal products)."""
+    from mythos_b200.ops import functional as F
+
+    pages = (ctx + 15) // 16
+    bytes_token = Hkv * F.kv4_token_bytes(D)
+    kc = torch.zeros(B * pages, Hkv, 16 * F.kv4_token_bytes(D), device="cuda", dtype=torch.uint8)
+    vc = torch.zeros_like(kc)
+    table = torch.randperm(B * pages, device="cuda").to(torch.int32).view(B, pages)
+    lens = torch.full((B,), ctx, device="cuda", dtype=torch.int32)
+    pos = torch.arange(ctx, device="cuda", dtype=torch.int32)
+    k, v = (torch.randn(ctx, Hkv, D, device="cuda").to(torch.bfloat16) for _ in range(2))
+    for b in range(B):
+        F.kv_append_int4(k, v, kc, vc, table, pos, torch.full_like(pos, b))
+    if op in ("append", "read"):
+        pos, sid = pos.repeat(B), torch.arange(B, device="cuda", dtype=torch.int32).repeat_interleave(ctx)
+        k, v = k.repeat(B, 1, 1), v.repeat(B, 1, 1)
+        call = (lambda: F.kv_append_int4(k, v, kc, vc, table, pos, sid)) if op == "append" else \
+            (lambda: F.kv_read_int4(kc, vc, table, pos, sid, D))
+        ms = graph_time(t, call)
+        return ms, 2.0 * B * ctx * (Hkv * D * 2 + bytes_token) / ms / 1e6, "GB/s"
+    if op == "decode":
+        q = torch.randn(B, H, D, device="cuda").to(torch.bfloat16)
+        ms = graph_time(t, lambda: F.paged_attn_decode_int4(q, kc, vc, table, lens))
+        return ms, 2.0 * B * ctx * bytes_token / ms / 1e6, "GB/s"
+    q = torch.randn(B * new, H, D, device="cuda").to(torch.bfloat16)
+    cu = torch.arange(B + 1, device="cuda", dtype=torch.int32) * new
+    ms = graph_time(t, lambda: F.paged_attn_prefill_int4(q, kc, vc, table, cu, lens, new, ctx))
+    return ms, 4.0 * B * H * D * (new * (ctx - new) + new * (new + 1) / 2) / ms / 1e9, "TFLOP/s"
+
+
+KV_INT4_OPS = ("append", "read", "decode", "prefill")
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--kernel", default="all")
@@ -472,6 +507,7 @@ def main():
     ap.add_argument("--no-flush", action="store_true")
     ap.add_argument("--fmt", default="oil8", choices=["oil8", "oil4", "i2s"])
     ap.add_argument("--ctx", type=int, default=1024)
+    ap.add_argument("--new", type=int, default=2048, help="new tokens per sequence of kv_int4_prefill")
     ap.add_argument("--splits", type=int, default=0, help="KV splits of paged_decode (0 = the engine's choice)")
     ap.add_argument("--coalesced-epilogue", type=int, default=1,
                     help="paired GEMM: 1 stores through a shared-memory transpose, 0 straight from registers")
@@ -552,6 +588,13 @@ def main():
         for B, ctx, H, Hkv in [(64, 1024, 32, 8), (64, 1024, 4, 1), (8, 32768, 20, 20)]:
             report(f"paged_decode_b{B}_ctx{ctx}_h{H}_kv{Hkv}_d128", bench_paged_decode(t, B, ctx, H, Hkv, 128))
         report("paged_decode_int8_b8_ctx32768_h32_kv8_d128", bench_paged_decode(t, 8, 32768, 32, 8, 128, int8=True))
+    if k in [f"kv_int4_{op}" for op in KV_INT4_OPS]:
+        report(f"{k}_b{args.batch}_ctx{args.ctx}_new{args.new}_h{args.heads}_kv{hkv}_d{args.head_dim}",
+               bench_kv_int4(t, k[8:], args.batch, args.ctx, args.new, args.heads, hkv, args.head_dim))
+    if k == "all":
+        for op, B, ctx, new, H, Hkv in [("append", 4, 2048, 1, 32, 8), ("read", 8, 4096, 1, 32, 8), ("decode", 64, 1024, 1, 32, 8),
+                                        ("decode", 8, 32768, 1, 32, 8), ("prefill", 1, 8192, 2048, 32, 8)]:
+            report(f"kv_int4_{op}_b{B}_ctx{ctx}_new{new}_h{H}_kv{Hkv}_d128", bench_kv_int4(t, op, B, ctx, new, H, Hkv, 128))
     for name, r, d in [("rmsnorm", args.rows, args.dim), ("swiglu", args.rows, 11008), ("ce", 4096, 32000),
                        ("adamw", 16384, 4096), ("fake_quant", 16384, 4096)]:
         if k in (name, "all"):
