@@ -79,6 +79,10 @@ __device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo,
       "}\n" ::"r"(d), "r"(a), "r"(b_lo), "n"(B_HI), "r"(IDESC), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ void pf_store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 // Eight values times inv (a power of two) as fp16. 0x4300 | code is the bf16 number 128 + code; the 128 scale leaves with the low
 // (both exact to 2^-17 of a step, far below fp16's rounding).
 __device__ __forceinline__ uint4 pf_expand8(uint32_t w, uint32_t pair, float inv) {
@@ -98,14 +102,15 @@ __device__ __forceinline__ uint4 pf_expand8(uint32_t w, uint32_t pair, float inv
 struct PfLine {
   const int* cu_q;
   const int* kv_lens;
-  int batch, pack, units, n_qb, tiles;
+  int batch, pack, log_pack, units, n_qb, tiles;
+  Kv4Div by_blocks, by_share;       // query blocks of a sequence; units of a kv head
 };
 struct PfItem {
   int b, row0, q_len, q_off, kv_len, tok[2], J[2], steps;   // tok: first token of each tile; J: its key tiles
   bool live[2];
   __device__ __forceinline__ PfItem(const PfLine& a, int pair) {
-    b = pair / a.n_qb;
-    const int blk = pair - b * a.n_qb, per = PF_TILE / a.pack;     // tokens of a tile
+    b = a.by_blocks(pair);
+    const int blk = pair - b * a.n_qb, per = PF_TILE >> a.log_pack;     // tokens of a tile
     row0 = a.cu_q[b];
     q_len = a.cu_q[b + 1] - row0;
     kv_len = a.kv_lens[b];
@@ -489,7 +494,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         bool ok = true;
         for (PfCursor c(a); c.more() && ok;) {
           const PfItem it = c.next(a);
-          const int bh = it.b * kv_heads + c.of_unit * a.line.pack / a.group, end = min(c.j1, max(it.J[0], it.J[1]));
+          const int bh = it.b * kv_heads + a.line.by_share(c.of_unit), end = min(c.j1, max(it.J[0], it.J[1]));
           for (int j = c.j0; j < end; ++j) {
             const int ks = kc % KS, vs = vc % VS;
             if (!mbar_wait(&k_empty[ks], ((kc / KS) & 1) ^ 1, abort_flag, status, 95)) { ok = false; break; }
@@ -607,6 +612,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem_base + Cfg::COL_S + t * 128 + lane_sel;
     const uint32_t t_o = tmem_base + Cfg::COL_O + t * D + lane_sel;
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.o_stride * 2)) & 31) == 0;
     uint32_t n_s = 0, n_o = 0;
     bool ok = true;
     for (PfCursor c(a); c.more() && ok;) {
@@ -615,11 +621,11 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int Jt = t ? it.J[1] : it.J[0], j0 = c.j0, end = min(c.j1, Jt);
       const bool whole = j0 == 0 && end == Jt && (t ? it.live[1] : it.live[0]);     // the tile's outputs are complete here
       if (end <= j0 && !whole) continue;
-      const int tok = (t ? it.tok[1] : it.tok[0]) + r / a.line.pack, head = c.of_unit * a.line.pack + r % a.line.pack;
+      const int tok = (t ? it.tok[1] : it.tok[0]) + (r >> a.line.log_pack), head = c.of_unit * a.line.pack + (r & (a.line.pack - 1));
       const int row = it.row0 + tok;
       const bool live = tok < it.q_len && (unsigned)row < (unsigned)a.total_q;
       const int limit = min(it.kv_len - 1, it.q_off + tok);
-      const int* ex = a.exponents + (long long)(it.b * kv_heads + c.of_unit * a.line.pack / a.group) * a.line.tiles;
+      const int* ex = a.exponents + (long long)(it.b * kv_heads + a.line.by_share(c.of_unit)) * a.line.tiles;
       const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 1.f;
       float m_ref = 0.f, l = 0.f;
       int e0 = 0;                             // exponent of the part's first values: the row sum is kept in units of 2^-e0
@@ -740,15 +746,18 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             *reinterpret_cast<uint4*>(part + ((k * 8 + i) * PF_TILE + r) * 4) =
                 make_uint4(orr[4 * i], orr[4 * i + 1], orr[4 * i + 2], orr[4 * i + 3]);
         } else if (live) {
-          uint4* p4 = reinterpret_cast<uint4*>(orow + k * 32);
+          uint32_t v[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t v[4];
+          for (int i = 0; i < 16; ++i)
+            v[i] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(orr[2 * i]) * inv_l * unit, __uint_as_float(orr[2 * i + 1]) * inv_l * unit);
+          // rows lie far apart: a lane writes whole 32-byte sectors where they are aligned
+          __nv_bfloat16* at = orow + k * 32;
+          if (wide) {
+            pf_store32(at, v);
+            pf_store32(at + 16, v + 8);
+          } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              v[q] = l == 0.f ? 0u
-                              : pack_bf16x2(__uint_as_float(orr[8 * i + 2 * q]) * inv_l * unit, __uint_as_float(orr[8 * i + 2 * q + 1]) * inv_l * unit);
-            p4[i] = make_uint4(v[0], v[1], v[2], v[3]);
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(at)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
         }
       }
@@ -814,7 +823,7 @@ pf_merge_kernel(const __grid_constant__ PfArgs a) {
       acc[k].w = fmaf(w, v[k].w, acc[k].w * w0);
     }
   }
-  const int tok = (t ? it.tok[1] : it.tok[0]) + r / a.line.pack, head = unit * a.line.pack + r % a.line.pack, row = it.row0 + tok;
+  const int tok = (t ? it.tok[1] : it.tok[0]) + (r >> a.line.log_pack), head = unit * a.line.pack + (r & (a.line.pack - 1)), row = it.row0 + tok;
   if (tok >= it.q_len || (unsigned)row >= (unsigned)a.total_q) return;
   const float inv = l == 0.f ? 0.f : 1.f / l, u = pf_pow2(e0);
   uint32_t y[4];
@@ -887,7 +896,9 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.tiles = z.tiles;
   x.total_q = total_q;
   x.most_q = z.n_qb * (2 * PF_TILE / z.pack);
-  x.line = {cu_q, kv_lens, batch, z.pack, z.units, z.n_qb, z.tiles};
+  int log_pack = 0;
+  while (1 << log_pack < z.pack) ++log_pack;
+  x.line = {cu_q, kv_lens, batch, z.pack, log_pack, z.units, z.n_qb, z.tiles, kv4_div(std::max(1, z.n_qb)), kv4_div(z.units / c.kv_heads)};
   x.ctas = z.ctas;
   x.whole = z.whole;
   x.status = status;
