@@ -98,7 +98,10 @@ __device__ __forceinline__ uint4 pf_expand8(uint32_t w, uint32_t pair, float inv
 
 // ------------------------------------------------------------------------------------------------ the line of steps
 // A pair is (sequence, block of 256 query rows); its items, one per unit (`pack` heads of a kv head), stand side by side, each
-// with as many steps as its last row sees key tiles (at least one, so that rows that see nothing get their zeros).
+// with as many steps as its last row sees key tiles (at least one, so that rows that see nothing get their zeros), behind
+// PF_SETUP places that stand for what an item costs beside its steps (8500 cycles of 3350 a step: equal numbers of steps alone
+// gave the stretches of short items 40 of them, and 4 prompts of 2048 tokens took 296 us instead of 195).
+constexpr int PF_SETUP = 2;
 struct PfLine {
   const int* cu_q;
   const int* kv_lens;
@@ -108,6 +111,7 @@ struct PfLine {
 struct PfItem {
   int b, row0, q_len, q_off, kv_len, tok[2], J[2], steps;   // tok: first token of each tile; J: its key tiles
   bool live[2];
+  __device__ __forceinline__ int places() const { return steps > 0 ? steps + PF_SETUP : 0; }
   __device__ __forceinline__ PfItem(const PfLine& a, int pair) {
     b = a.by_blocks(pair);
     const int blk = pair - b * a.n_qb, per = PF_TILE >> a.log_pack;     // tokens of a tile
@@ -126,16 +130,14 @@ struct PfItem {
     }
   }
 };
-// Written by the expansion, read by the attention and the merge: [0] steps of a stretch, [1] how many stretches have one more,
-// [2] stretches; then where every pair begins (pairs + 1), then (pair, unit, step, steps) of every stretch's start.
+// Written by the expansion, read by the attention and the merge: [0] places of a stretch, [1] how many stretches have one more,
+// [2] stretches; then (pair, unit, place in the item, places) of every stretch's start.
 struct PfPlan {
   int* p;
-  int pairs;
   __device__ __forceinline__ int per() const { return p[0]; }
   __device__ __forceinline__ int rem() const { return p[1]; }
   __device__ __forceinline__ int count() const { return p[2]; }
-  __device__ __forceinline__ int* begin() const { return p + 3; }
-  __device__ __forceinline__ int* start(int c) const { return p + 4 + pairs + 4 * c; }
+  __device__ __forceinline__ int* start(int c) const { return p + 4 + 4 * c; }
 };
 __device__ __forceinline__ int pf_start(int per, int rem, int c) { return c * per + min(c, rem); }
 __device__ __forceinline__ int pf_owner(int per, int rem, int place) {       // whose stretch holds it
@@ -156,6 +158,7 @@ struct PfExpand {
   float* q_factor;      // [total_q, heads]: 2^eq
   int* exponents;       // [batch * kv_heads, tiles]: ek in the low, ev in the high half
   int kv_heads, heads, tiles, kv_blocks, q_blocks, total_q;
+  int pairs;
   int most_q;           // new tokens that the items of a sequence cover
   PfLine line;
   PfPlan plan;
@@ -164,7 +167,8 @@ struct PfExpand {
   int* status;
 };
 
-constexpr int PF_MIN_STEPS = 4;   // of a stretch: a step is about 2 us, setting up and writing a part a few
+constexpr int PF_MIN_STEPS = 6;   // places of a stretch: a step is about 2 us, setting up and writing a part five
+static_assert(PF_MIN_STEPS > PF_SETUP, "a stretch holds a step");
 // Where there are no more items than CTAs and none has more steps than this, every CTA takes a whole one, and there is no merge:
 // 6 ragged prompts of up to 700 tokens take 21 us so and 26 with equal stretches.
 constexpr int PF_WHOLE_STEPS = 12;
@@ -173,12 +177,12 @@ constexpr int PF_WHOLE_STEPS = 12;
 __device__ void pf_make_plan(const PfExpand& a) {
   __shared__ int s_sum[PF_EXPAND / 32], s_total;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int each = (a.plan.pairs + PF_EXPAND - 1) / PF_EXPAND, p0 = min(a.plan.pairs, (int)threadIdx.x * each), p1 = min(a.plan.pairs, p0 + each);
+  const int each = (a.pairs + PF_EXPAND - 1) / PF_EXPAND, p0 = min(a.pairs, (int)threadIdx.x * each), p1 = min(a.pairs, p0 + each);
   for (int b = threadIdx.x; b < a.line.batch; b += PF_EXPAND)     // more tokens than the caller said: not all are dealt with
     if (a.status && (a.line.kv_lens[b] > a.tiles * PF_TILE || a.line.cu_q[b + 1] - a.line.cu_q[b] > a.most_q))
       atomicCAS(a.status, 0, ST_BAD_ARG | (90 << 16));
   int sum = 0;
-  for (int p = p0; p < p1; ++p) sum += PfItem(a.line, p).steps * a.line.units;
+  for (int p = p0; p < p1; ++p) sum += PfItem(a.line, p).places() * a.line.units;
   int up = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -200,29 +204,28 @@ __device__ void pf_make_plan(const PfExpand& a) {
   const int total = s_total;
   if (a.whole) {                                  // one item per stretch; items without steps in between are none
     for (int p = p0; p < p1; ++p) {
-      const int steps = PfItem(a.line, p).steps;
+      const int places = PfItem(a.line, p).places();
       for (int u = 0; u < a.line.units; ++u) {
         int* s = a.plan.start(p * a.line.units + u);
         s[0] = p;
         s[1] = u;
         s[2] = 0;
-        s[3] = steps;
+        s[3] = places;
       }
     }
-    if (threadIdx.x == 0) a.plan.p[2] = a.plan.pairs * a.line.units;
+    if (threadIdx.x == 0) a.plan.p[2] = a.pairs * a.line.units;
     return;
   }
   const int count = max(1, min(a.ctas, total / PF_MIN_STEPS)), per = total / count, rem = total - per * count;
   int place = s_sum[warp] + up - sum;
   for (int p = p0; p < p1; ++p) {
-    const int steps = PfItem(a.line, p).steps, end = place + steps * a.line.units;
-    a.plan.begin()[p] = place;
+    const int places = PfItem(a.line, p).places(), end = place + places * a.line.units;
     for (int c = place > 0 ? pf_owner(per, rem, place - 1) + 1 : 0; c < count && pf_start(per, rem, c) < end; ++c) {
       const int at = pf_start(per, rem, c) - place;
       int* s = a.plan.start(c);
       s[0] = p;
-      s[1] = at / steps;
-      s[2] = at - at / steps * steps;
+      s[1] = at / places;
+      s[2] = at - at / places * places;
       s[3] = per + (c < rem ? 1 : 0);
     }
     place = end;
@@ -231,7 +234,6 @@ __device__ void pf_make_plan(const PfExpand& a) {
     a.plan.p[0] = per;
     a.plan.p[1] = rem;
     a.plan.p[2] = total > 0 ? count : 0;
-    a.plan.begin()[a.plan.pairs] = total;
   }
 }
 
@@ -374,19 +376,19 @@ __host__ __device__ constexpr int pf_part_floats() { return PF_TILE * (D + 4); }
 
 // The parts of a CTA's stretch, in order: the steps j0 .. j1 of an item.
 struct PfCursor {
-  int pair, unit, step, left, slot = -1;
+  int pair, unit, at, left, slot = -1;
   int j0, j1;           // of the part
   int of_pair, of_unit;
   __device__ __forceinline__ explicit PfCursor(const PfArgs& a) {
     const int c = blockIdx.x;
     left = 0;
-    pair = unit = step = 0;
+    pair = unit = at = 0;
     if (c < a.plan.count()) {
       const int* s = a.plan.start(c);
       left = s[3];
       pair = s[0];
       unit = s[1];
-      step = s[2];
+      at = s[2];
     }
   }
   __device__ __forceinline__ bool more() const { return left > 0; }
@@ -397,10 +399,12 @@ struct PfCursor {
     slot = slot < 0 ? 0 : 1;
     of_pair = pair;
     of_unit = unit;
-    j0 = step;
-    j1 = min(it.steps, step + left);
-    left -= j1 - j0;
-    step = 0;
+    const int end = min(it.places(), at + left);
+    j0 = max(0, at - PF_SETUP);
+    j1 = end - PF_SETUP;          // (more than j0: a stretch is longer than PF_SETUP)
+    left -= end - at;
+    at = 0;
+    if (left <= PF_SETUP) left = 0;                        // no step of the next item
     if (j1 == it.steps) {
       if (++unit == a.line.units) {
         unit = 0;
@@ -782,20 +786,23 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
-// Joins the parts of query tiles that lie in several stretches: 16 values of 128 rows of a (unit, pair, tile) per block, two
-// threads per row.
+// Joins the parts of query tiles that lie in several stretches: blockIdx.x names the border (the start of a stretch) that cuts
+// the item first; 16 values of 128 rows of one of its tiles per block, two threads per row.
 template <int D>
 __global__ void __launch_bounds__(256)
 pf_merge_kernel(const __grid_constant__ PfArgs a) {
-  const int unit = blockIdx.x, pair = blockIdx.y, t = blockIdx.z & 1;
-  const PfItem it(a.line, pair);
+  const int border = blockIdx.x + 1, t = blockIdx.y & 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");             // every CTA, so that this grid ends behind the one before
+  if (border >= a.plan.count()) return;
+  const int* start = a.plan.start(border);
+  const int per = a.plan.per(), rem = a.plan.rem(), pair = start[0], unit = start[1], u0 = pf_start(per, rem, border) - start[2];
+  if (start[2] == 0 || pf_start(per, rem, border - 1) > u0) return;      // no cut, or not the item's first
+  const PfItem it(a.line, pair);
   const int Jt = t ? it.J[1] : it.J[0];
   if (!(t ? it.live[1] : it.live[0]) || Jt == 0) return;
-  const int per = a.plan.per(), rem = a.plan.rem(), u0 = a.plan.begin()[pair] + unit * it.steps;
-  const int c0 = pf_owner(per, rem, u0), c1 = pf_owner(per, rem, u0 + Jt - 1);
+  const int first = u0 + PF_SETUP, c0 = pf_owner(per, rem, first), c1 = pf_owner(per, rem, first + Jt - 1);
   if (c0 == c1) return;                           // written by that CTA
-  const int r = threadIdx.x >> 1, v0 = (blockIdx.z >> 1) * 4 + (threadIdx.x & 1) * 2;      // row, first group of four values
+  const int r = threadIdx.x >> 1, v0 = (blockIdx.y >> 1) * 4 + (threadIdx.x & 1) * 2;      // row, first group of four values
   const auto part = [&](int c) {
     return a.parts + (long long)((c * 2 + (u0 > pf_start(per, rem, c) ? 1 : 0)) * 2 + t) * pf_part_floats<D>();
   };
@@ -839,7 +846,7 @@ pf_merge_kernel(const __grid_constant__ PfArgs a) {
 struct PfSizes {
   int tiles, pack, units, n_qb, ctas;
   bool whole;
-  long long kv_tiles, pairs, steps;     // steps: at most
+  long long kv_tiles, pairs, steps;     // steps: places on the line, at most
   long long kv, q, factor, exponents, plan, parts, total;    // bytes, each a multiple of 256
 };
 PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int D) {
@@ -852,14 +859,14 @@ PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int k
   z.n_qb = (int)(((long long)max_q * z.pack + 2 * PF_TILE - 1) / (2 * PF_TILE));
   z.kv_tiles = (long long)batch * kv_heads * z.tiles;
   z.pairs = (long long)batch * z.n_qb;
-  z.steps = z.pairs * z.units * z.tiles;
+  z.steps = z.pairs * z.units * (z.tiles + PF_SETUP);
   z.whole = z.pairs * z.units <= sm_count() && z.tiles <= PF_WHOLE_STEPS;
   z.ctas = (int)(z.whole ? std::max(1LL, z.pairs * z.units) : std::max(1LL, std::min((long long)sm_count(), z.steps / PF_MIN_STEPS)));
   z.kv = align(z.kv_tiles * PF_TILE * D * 2);
   z.q = align((long long)total_q * heads * D * 2);
   z.factor = align((long long)total_q * heads * 4);
   z.exponents = align(z.kv_tiles * 4);
-  z.plan = align((4 + z.pairs + 4LL * z.ctas) * 4);
+  z.plan = align((4 + 4LL * z.ctas) * 4);
   z.parts = z.whole ? 0 : align(4LL * z.ctas * PF_TILE * (D + 4) * 4);
   z.total = 2 * z.kv + z.q + z.factor + z.exponents + z.plan + z.parts;
   return z;
@@ -890,7 +897,8 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.qh = (__half*)take(z.q);
   x.q_factor = (float*)take(z.factor);
   x.exponents = (int*)take(z.exponents);
-  x.plan = {(int*)take(z.plan), (int)z.pairs};
+  x.plan = {(int*)take(z.plan)};
+  x.pairs = (int)z.pairs;
   x.kv_heads = c.kv_heads;
   x.heads = heads;
   x.tiles = z.tiles;
@@ -904,7 +912,7 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.status = status;
   const int rows_per = PF_EXPAND / (D / 8);
   const long long q_blocks = ((long long)total_q * heads + rows_per - 1) / rows_per;
-  MB_REQUIRE(z.kv_tiles + q_blocks + 1 < (1LL << 31) && z.steps < (1LL << 31) && z.pairs <= 65535, "paged_attn_prefill_int4: batch too large");
+  MB_REQUIRE(z.kv_tiles + q_blocks + 1 < (1LL << 31) && z.steps < (1LL << 31) && z.pairs < (1LL << 31), "paged_attn_prefill_int4: batch too large");
   x.kv_blocks = (int)z.kv_tiles;
   x.q_blocks = (int)q_blocks;
   const unsigned blocks = (unsigned)(z.kv_tiles + q_blocks + 1);
@@ -926,7 +934,7 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
            scale * 1.4426950408889634f, status};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(z.units, (unsigned)z.pairs, 2 * (D / 16));
+  cfg.gridDim = dim3((unsigned)std::max(1, z.ctas - 1), 2 * (D / 16));
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
