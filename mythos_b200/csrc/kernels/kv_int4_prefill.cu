@@ -170,8 +170,9 @@ struct PfExpand {
 constexpr int PF_MIN_STEPS = 6;   // places of a stretch: a step is about 2 us, setting up and writing a part five
 static_assert(PF_MIN_STEPS > PF_SETUP, "a stretch holds a step");
 // Where there are no more items than CTAs and none has more steps than this, every CTA takes a whole one, and there is no merge:
-// 6 ragged prompts of up to 700 tokens take 21 us so and 26 with equal stretches.
-constexpr int PF_WHOLE_STEPS = 12;
+// 6 ragged prompts of up to 700 tokens (6 steps) take 23 us so and 27 with equal stretches, 3 of 500 over up to 500 (8) 31 and
+// 35; one of 700 over 700 (11) 33 and 31.
+constexpr int PF_WHOLE_STEPS = 8;
 
 // One block: the plan. Every thread takes a run of pairs.
 __device__ void pf_make_plan(const PfExpand& a) {
