@@ -703,6 +703,7 @@ mb::KvInt4Cache kv4_cache(const Tensor& k_cache, const Tensor& v_cache, const Te
                   v_cache.sizes() == k_cache.sizes(),
               who, ": caches must be [pages, ", kv_heads, ", page_size * ", token, "] with page_size a multiple of 16");
   TORCH_CHECK(block_table.dim() == 2, who, ": block_table must be [sequences, pages]");
+  TORCH_CHECK(block_table.size(1) * (k_cache.size(2) / token) < (int64_t)1 << 31, who, ": a row of block_table holds more than 2^31 tokens");
   TORCH_CHECK(v_cache.device() == k_cache.device() && block_table.device() == k_cache.device(), who, ": tensors on several devices");
   return {k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr<int>(), (int)k_cache.size(0), (int)kv_heads, (int)head_dim,
           (int)(k_cache.size(2) / token), (int)block_table.size(0), (int)block_table.size(1)};
@@ -730,11 +731,14 @@ void qkv_rope_append(Tensor& acc, const Tensor& pos, const Tensor& seq_ids, cons
   chk_c(block_table, I32, "block_table");
   chk_c(q_out, BF16, "q_out");
   if (k_cache.scalar_type() == U8) {   // 4-bit pages
+    TORCH_CHECK(q_out.dim() == 3 && k_cache.dim() == 3,
+                "qkv_rope_append: q_out must be [tokens, heads, head_dim], 4-bit caches [pages, kv_heads, page bytes]");
     const int64_t T4 = q_out.size(0), H4 = q_out.size(1), D4 = q_out.size(2), Hkv4 = k_cache.size(1);
     TORCH_CHECK(!k_scale.has_value() && !v_scale.has_value(), "qkv_rope_append: 4-bit pages hold their scales");
     TORCH_CHECK(acc.numel() == T4 * (H4 + 2 * Hkv4) * D4, "qkv_rope_append: accumulator shape mismatch");
     const auto c = kv4_cache(k_cache, v_cache, block_table, Hkv4, D4, "qkv_rope_append");
     kv4_tokens(pos, seq_ids, k_cache, T4, "qkv_rope_append");
+    TORCH_CHECK(acc.device() == k_cache.device() && q_out.device() == k_cache.device(), "qkv_rope_append: tensors on several devices");
     c10::cuda::CUDAGuard guard4(acc.device());
     mb::qkv_rope_append_int4(acc.data_ptr<float>(), pos.data_ptr<int>(), seq_ids.data_ptr<int>(), q_out.data_ptr(), c, (int)T4, (int)H4,
                              (float)theta, cur_stream());

@@ -162,8 +162,8 @@ void kv_append_int4(const KvInt4Cache& c, const void* k, const void* v, const in
   if (tokens == 0) return;
   const int units = kv4_units(c, tokens, 16, "kv_append_int4"), per_token = c.kv_heads * (c.head_dim / 16);
   const auto go = [&](auto kern) {
-    kern<<<(units + KV4_APPEND - 1) / KV4_APPEND, KV4_APPEND, 0, stream>>>((const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (uint8_t*)c.k, (uint8_t*)c.v,
-                                                  kv4_pages(c), positions, seq_ids, units, kv4_div(per_token), k_stride, v_stride);
+    kern<<<(units + KV4_APPEND - 1) / KV4_APPEND, KV4_APPEND, 0, stream>>>(
+        (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (uint8_t*)c.k, (uint8_t*)c.v, kv4_pages(c), positions, seq_ids, units, kv4_div(per_token), k_stride, v_stride);
   };
   if (c.head_dim == 128) go(kv_append_int4_kernel<128>);
   else go(kv_append_int4_kernel<64>);

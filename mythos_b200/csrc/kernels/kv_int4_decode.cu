@@ -23,6 +23,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "api.h"
 #include "common.cuh"
@@ -928,7 +929,7 @@ p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scra
 
 // A kernel's limits, raised once per device.
 template <typename K>
-void p4_configure(K kern, int smem, bool cluster, unsigned long long& seen) {
+void p4_configure(K kern, int smem, bool cluster, std::atomic<unsigned long long>& seen) {
   int dev = 0;
   MB_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 64 && (seen >> dev & 1ull)) return;
@@ -970,7 +971,7 @@ void p4_launch(P4Args& a, const P4Plan& plan, float* scratch, cudaStream_t strea
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (plan.splits > 0) {
-    static unsigned long long seen = 0;
+    static std::atomic<unsigned long long> seen{0};
     p4_configure(paged_attn_int4_cluster_kernel<D, COLS>, P4SmemCluster<D, COLS>::BYTES, true, seen);
     cfg.gridDim = dim3(a.batch, (unsigned)(plan.blocks * a.kv_heads), plan.splits);
     cfg.blockDim = dim3(P4_THREADS);
@@ -983,7 +984,7 @@ void p4_launch(P4Args& a, const P4Plan& plan, float* scratch, cudaStream_t strea
     count_launch();
     return;
   }
-  static unsigned long long seen = 0;
+  static std::atomic<unsigned long long> seen{0};
   p4_configure(paged_attn_int4_line_kernel<D, COLS>, P4SmemLine<D, COLS>::BYTES, false, seen);
   paged_attn_int4_line_kernel<D, COLS><<<plan.ctas, P4_THREADS, P4SmemLine<D, COLS>::BYTES, stream>>>(a, scratch);
   count_launch();

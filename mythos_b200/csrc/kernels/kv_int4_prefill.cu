@@ -844,8 +844,12 @@ pf_merge_kernel(const __grid_constant__ PfArgs a) {
 }
 
 // Sizes of a call's workspace and launches.
+// Bytes of the images of keys and values: every sequence has room for the longest, so a batch that holds a long one beside many
+// short ones would ask for far more than it reads. What does not fit is dealt with in slices of the batch, one after the other.
+constexpr long long PF_IMAGES = 1LL << 31;
 struct PfSizes {
   int tiles, pack, units, n_qb, ctas;
+  int slice;                            // sequences at a time; the rest is for one slice
   bool whole;
   long long kv_tiles, pairs, steps;     // steps: places on the line, at most
   long long kv, q, factor, exponents, plan, parts, total;    // bytes, each a multiple of 256
@@ -858,8 +862,9 @@ PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int k
   z.pack = PF_TILE % G == 0 ? G : 1;
   z.units = heads / z.pack;
   z.n_qb = (int)(((long long)max_q * z.pack + 2 * PF_TILE - 1) / (2 * PF_TILE));
-  z.kv_tiles = (long long)batch * kv_heads * z.tiles;
-  z.pairs = (long long)batch * z.n_qb;
+  z.slice = (int)std::max(1LL, std::min((long long)batch, PF_IMAGES / (4LL * kv_heads * z.tiles * PF_TILE * D)));
+  z.kv_tiles = (long long)z.slice * kv_heads * z.tiles;
+  z.pairs = (long long)z.slice * z.n_qb;
   z.steps = z.pairs * z.units * (z.tiles + PF_SETUP);
   z.whole = z.pairs * z.units <= sm_count() && z.tiles <= PF_WHOLE_STEPS;
   z.ctas = (int)(z.whole ? std::max(1LL, z.pairs * z.units) : std::max(1LL, std::min((long long)sm_count(), z.steps / PF_MIN_STEPS)));
@@ -899,58 +904,67 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.q_factor = (float*)take(z.factor);
   x.exponents = (int*)take(z.exponents);
   x.plan = {(int*)take(z.plan)};
-  x.pairs = (int)z.pairs;
+  float* parts = (float*)take(z.parts);
   x.kv_heads = c.kv_heads;
   x.heads = heads;
   x.tiles = z.tiles;
   x.total_q = total_q;
   x.most_q = z.n_qb * (2 * PF_TILE / z.pack);
+  x.status = status;
   int log_pack = 0;
   while (1 << log_pack < z.pack) ++log_pack;
-  x.line = {cu_q, kv_lens, batch, z.pack, log_pack, z.units, z.n_qb, z.tiles, kv4_div(std::max(1, z.n_qb)), kv4_div(z.units / c.kv_heads)};
-  x.ctas = z.ctas;
-  x.whole = z.whole;
-  x.status = status;
   const int rows_per = PF_EXPAND / (D / 8);
   const long long q_blocks = ((long long)total_q * heads + rows_per - 1) / rows_per;
   MB_REQUIRE(z.kv_tiles + q_blocks + 1 < (1LL << 31) && z.steps < (1LL << 31) && z.pairs < (1LL << 31), "paged_attn_prefill_int4: batch too large");
-  x.kv_blocks = (int)z.kv_tiles;
-  x.q_blocks = (int)q_blocks;
-  const unsigned blocks = (unsigned)(z.kv_tiles + q_blocks + 1);
-  if (D == 128) kv4_expand_kernel<128><<<blocks, PF_EXPAND, 0, stream>>>(x);
-  else kv4_expand_kernel<64><<<blocks, PF_EXPAND, 0, stream>>>(x);
-  count_launch();
-  check_launch();
-
   // (copies only: TMA moves fp16 as it moves bf16)
   uint64_t qd[3] = {(uint64_t)D, (uint64_t)heads, (uint64_t)total_q}, qs[2] = {(uint64_t)D * 2, (uint64_t)heads * D * 2};
   uint32_t qb[3] = {64, (uint32_t)z.pack, (uint32_t)(PF_TILE / z.pack)};
-  uint64_t kd[3] = {(uint64_t)D, (uint64_t)z.tiles * PF_TILE, (uint64_t)batch * c.kv_heads};
-  uint64_t ks[2] = {(uint64_t)D * 2, (uint64_t)z.tiles * PF_TILE * D * 2};
-  uint32_t kb[3] = {64, PF_TILE, 1};
   const CUtensorMap tq = make_tensor_map(x.qh, TmaDType::BF16, 3, qd, qs, qb, true);
-  const CUtensorMap tk = make_tensor_map(x.k, TmaDType::BF16, 3, kd, ks, kb, true);
-  const CUtensorMap tv = make_tensor_map(x.v, TmaDType::BF16, 3, kd, ks, kb, true);
-  PfArgs a{x.line, x.plan, x.q_factor, x.exponents, (__nv_bfloat16*)out, (float*)take(z.parts), o_stride, heads, heads / c.kv_heads, total_q,
-           scale * 1.4426950408889634f, status};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3((unsigned)std::max(1, z.ctas - 1), 2 * (D / 16));
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const auto go = [&](auto kern, auto merge, int smem) {
-    MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kern<<<z.ctas, PF_THREADS, smem, stream>>>(tq, tk, tv, a);
+
+  for (int b0 = 0; b0 < batch; b0 += z.slice) {
+    const int nb = std::min(z.slice, batch - b0);
+    const PfSizes s = pf_sizes(nb, total_q, max_q, max_kv, heads, c.kv_heads, D);
+    x.pages.block_table = c.block_table + (long long)b0 * c.max_pages;
+    x.pages.n_seqs = c.n_seqs - b0;
+    x.kv_lens = kv_lens + b0;
+    x.line = {cu_q + b0, kv_lens + b0, nb, s.pack, log_pack, s.units, s.n_qb, s.tiles, kv4_div(std::max(1, s.n_qb)), kv4_div(s.units / c.kv_heads)};
+    x.pairs = (int)s.pairs;
+    x.ctas = s.ctas;
+    x.whole = s.whole;
+    x.kv_blocks = (int)s.kv_tiles;
+    x.q_blocks = b0 == 0 ? (int)q_blocks : 0;
+    const unsigned blocks = (unsigned)x.kv_blocks + (unsigned)x.q_blocks + 1u;
+    if (D == 128) kv4_expand_kernel<128><<<blocks, PF_EXPAND, 0, stream>>>(x);
+    else kv4_expand_kernel<64><<<blocks, PF_EXPAND, 0, stream>>>(x);
+    count_launch();
     check_launch();
-    if (!z.whole) MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, merge, a));
-  };
-  if (D == 128) go(fa_int4_kernel<128>, pf_merge_kernel<128>, PfCfg<128>::SMEM_BYTES);
-  else go(fa_int4_kernel<64>, pf_merge_kernel<64>, PfCfg<64>::SMEM_BYTES);
-  count_launch(z.whole ? 1 : 2);
+
+    uint64_t kd[3] = {(uint64_t)D, (uint64_t)s.tiles * PF_TILE, (uint64_t)nb * c.kv_heads};
+    uint64_t ks[2] = {(uint64_t)D * 2, (uint64_t)s.tiles * PF_TILE * D * 2};
+    uint32_t kb[3] = {64, PF_TILE, 1};
+    const CUtensorMap tk = make_tensor_map(x.k, TmaDType::BF16, 3, kd, ks, kb, true);
+    const CUtensorMap tv = make_tensor_map(x.v, TmaDType::BF16, 3, kd, ks, kb, true);
+    PfArgs a{x.line, x.plan, x.q_factor, x.exponents, (__nv_bfloat16*)out, parts, o_stride, heads, heads / c.kv_heads, total_q,
+             scale * 1.4426950408889634f, status};
+    cfg.gridDim = dim3((unsigned)std::max(1, s.ctas - 1), 2 * (D / 16));
+    const auto go = [&](auto kern, auto merge, int smem) {
+      MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      kern<<<s.ctas, PF_THREADS, smem, stream>>>(tq, tk, tv, a);
+      check_launch();
+      if (!s.whole) MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, merge, a));
+    };
+    if (D == 128) go(fa_int4_kernel<128>, pf_merge_kernel<128>, PfCfg<128>::SMEM_BYTES);
+    else go(fa_int4_kernel<64>, pf_merge_kernel<64>, PfCfg<64>::SMEM_BYTES);
+    count_launch(s.whole ? 1 : 2);
+  }
 }
 
 }  // namespace mb

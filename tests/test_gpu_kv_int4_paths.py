@@ -244,3 +244,79 @@ def test_pages_behind_two_gibibytes():
         assert _same_bits(F.paged_attn_decode_int4(q[:2], kc, vc, t, ctx), F.paged_attn_decode_int4(q[:2], kf, vf, f, ctx))
     assert _same_bits(F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, 600, 700), F.paged_attn_prefill_int4(q, kf, vf, far, cu, ctx, 600, 700))
     native.check_status("cuda")
+
+
+def test_a_batch_whose_images_do_not_fit_at_once():
+    """Ten sequences announced at up to 65536 keys: images of 2.7 GB, dealt with eight sequences at a time."""
+    H, Hk, D, page, most = 8, 8, 128, 16, 65536
+    new, old = [130, 0, 70, 1, 200, 90, 33, 5, 260, 128], [700, 30, 0, 500, 90, 0, 5, 1000, 3, 400]
+    lens = [a + b for a, b in zip(new, old)]
+    kc, vc, table = filled(lens, Hk, D, page, "cuda", seed=8)
+    wide = _widen(table, most, page)
+    q = torch.randn(sum(new), H, D, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).cuda()
+    cu, kv = _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    res = oracle(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1.0 / math.sqrt(D))
+    out = F.paged_attn_prefill_int4(q, kc, vc, wide, cu, kv, max(new), most)
+    off = (out.cpu().double() - res["out"]).abs()
+    assert (off <= _prefill_bound(res)).all(), float((off / _prefill_bound(res)).max())
+    native.check_status("cuda")
+
+
+@pytest.mark.parametrize("form", ["few", "prompt"])
+def test_queries_that_see_nothing_get_zeros(form):
+    H, Hk, D, page = 4, 2, 128, 16
+    new, lens = ([6, 3], [2, 3]) if form == "few" else ([900, 800], [300, 800])      # more new tokens than keys
+    kc, vc, table = filled(lens, Hk, D, page, "cuda", seed=8)
+    q = torch.randn(sum(new), H, D, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).cuda()
+    cu, kv = _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    res = oracle(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1.0 / math.sqrt(D))
+    for t in (table, _widen(table, 40000, page)):
+        out = torch.full_like(q, 3.0)
+        F.paged_attn_prefill_int4(q, kc, vc, t, cu, kv, max(new), max(lens), out=out)
+        off = (out.cpu().double() - res["out"]).abs()
+        assert (off <= _prefill_bound(res)).all(), float((off / _prefill_bound(res)).max())
+        assert not out[: new[0] - lens[0]].any()
+    native.check_status("cuda")
+
+
+@pytest.mark.parametrize("form", ["cluster", "line", "prompt"])
+def test_a_query_that_is_not_finite_reaches_its_own_row_only_and_results_may_replace_the_queries(form):
+    H, Hk, D, page = 4, 2, 128, 16
+    new = [800, 700] if form == "prompt" else [1, 1]
+    lens = [900, 700]
+    kc, vc, table = filled(lens, Hk, D, page, "cuda", seed=5)
+    q = torch.randn(sum(new), H, D, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).cuda()
+    cu, ctx = _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def call(q, out=None):
+        if form == "prompt":
+            return F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens), out=out)
+        return F.paged_attn_decode_int4(q, kc, vc, table if form == "cluster" else _widen(table, 40000, page), ctx, out=out)
+
+    want = call(q)
+    bad = q.clone()
+    bad[0, 1, 5] = math.nan
+    bad[1, 3, 60] = math.inf
+    got = call(bad)
+    odd = torch.zeros(got.shape[:2], dtype=torch.bool, device="cuda")
+    odd[0, 1] = odd[1, 3] = True
+    assert torch.equal((~got.isfinite()).any(-1), odd) and _same_bits(got[~odd], want[~odd])
+    assert _same_bits(call(q, out=q), want)
+    native.check_status("cuda")
+
+
+def test_a_context_without_any_page_gives_zeros_and_is_reported():
+    H, Hk, D, page = 4, 2, 128, 16
+    kc, vc, table = filled([64, 40], Hk, D, page, "cuda", seed=4)
+    q = torch.randn(2, H, D, device="cuda").to(torch.bfloat16)
+    ctx = torch.tensor([64, 40], dtype=torch.int32, device="cuda")
+    table[0] = -1
+    for t in (table, _widen(table, 40000, page)):
+        out = F.paged_attn_decode_int4(q, kc, vc, t, ctx)
+        with pytest.raises(RuntimeError, match="status 2"):
+            native.check_status("cuda")
+        assert not out[0].any() and out[1].any()
+    nothing = F.paged_attn_decode_int4(q, kc[:0], vc[:0], table[:, :0], ctx)         # no pages, no columns
+    with pytest.raises(RuntimeError, match="status 2"):
+        native.check_status("cuda")
+    assert not nothing.any()
