@@ -106,6 +106,7 @@ struct PfLine {
   const int* cu_q;
   const int* kv_lens;
   int batch, pack, log_pack, units, n_qb, tiles;
+  int per_item;                     // query tiles of an item: two, one where that fills the GPU
   Kv4Div by_blocks, by_share;       // query blocks of a sequence; units of a kv head
 };
 struct PfItem {
@@ -122,8 +123,8 @@ struct PfItem {
     steps = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      tok[t] = (2 * blk + t) * per;
-      live[t] = tok[t] < q_len;
+      tok[t] = (a.per_item * blk + t) * per;
+      live[t] = t < a.per_item && tok[t] < q_len;
       const int hi = live[t] ? min(kv_len, q_off + min(q_len, tok[t] + per)) : 0;
       J[t] = min(a.tiles, (max(hi, 0) + PF_TILE - 1) / PF_TILE);
       if (live[t]) steps = max(steps, max(1, J[t]));
@@ -163,16 +164,17 @@ struct PfExpand {
   PfLine line;
   PfPlan plan;
   int ctas;
-  bool whole;           // a whole item per stretch
   int* status;
 };
 
 constexpr int PF_MIN_STEPS = 6;   // places of a stretch: a step is about 2 us, setting up and writing a part five
 static_assert(PF_MIN_STEPS > PF_SETUP, "a stretch holds a step");
 // Where there are no more items than CTAs and none has more steps than this, every CTA takes a whole one, and there is no merge:
-// 6 ragged prompts of up to 700 tokens (6 steps) take 23 us so and 27 with equal stretches, 3 of 500 over up to 500 (8) 31 and
-// 35; one of 700 over 700 (11) 33 and 31.
+// 3 prompts of 500 over up to 500 tokens (8 steps) take 31 us so and 35 with equal stretches, one of 700 over 700 (11) 33 and 31.
 constexpr int PF_WHOLE_STEPS = 8;
+// The same for items of a single query tile, whose steps are shorter (2400 cycles to 3350): 6 ragged prompts of up to 700 tokens
+// (6 steps) take 20.7 us so and 22.9 with two tiles, 700 over 700 (11) 29.3 and 31.0, 1500 (12) 30.4 and 29.4.
+constexpr int PF_SINGLE_STEPS = 11;
 
 // One block: the plan. Every thread takes a run of pairs.
 __device__ void pf_make_plan(const PfExpand& a) {
@@ -203,20 +205,6 @@ __device__ void pf_make_plan(const PfExpand& a) {
   }
   __syncthreads();
   const int total = s_total;
-  if (a.whole) {                                  // one item per stretch; items without steps in between are none
-    for (int p = p0; p < p1; ++p) {
-      const int places = PfItem(a.line, p).places();
-      for (int u = 0; u < a.line.units; ++u) {
-        int* s = a.plan.start(p * a.line.units + u);
-        s[0] = p;
-        s[1] = u;
-        s[2] = 0;
-        s[3] = places;
-      }
-    }
-    if (threadIdx.x == 0) a.plan.p[2] = a.pairs * a.line.units;
-    return;
-  }
   const int count = max(1, min(a.ctas, total / PF_MIN_STEPS)), per = total / count, rem = total - per * count;
   int place = s_sum[warp] + up - sum;
   for (int p = p0; p < p1; ++p) {
@@ -244,6 +232,7 @@ __global__ void __launch_bounds__(PF_EXPAND)
 kv4_expand_kernel(const __grid_constant__ PfExpand a) {
   using L = KvInt4<D>;
   constexpr int WORDS = D / 8;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the attention waits for this grid's end before it reads
   if ((int)blockIdx.x == a.kv_blocks + a.q_blocks) {
     pf_make_plan(a);
     return;
@@ -370,6 +359,8 @@ struct PfArgs {
   int heads, group, total_q;
   float scale_log2;
   int* status;
+  bool whole;           // a whole item per CTA
+  Kv4Div by_units;
 };
 // A part of a query tile: sums [D / 4][128 rows][4], reference, row sum and its exponent per row.
 template <int D>
@@ -384,7 +375,11 @@ struct PfCursor {
     const int c = blockIdx.x;
     left = 0;
     pair = unit = at = 0;
-    if (c < a.plan.count()) {
+    if (a.whole) {                        // one item per stretch, which needs no plan
+      pair = a.by_units(c);
+      unit = c - pair * a.line.units;
+      left = PfItem(a.line, pair).places();
+    } else if (c < a.plan.count()) {
       const int* s = a.plan.start(c);
       left = s[3];
       pair = s[0];
@@ -415,6 +410,10 @@ struct PfCursor {
     return it;
   }
 };
+
+// Where every CTA has an item of its own the kernel is launched ahead of the expansion's end, and finds its item meanwhile (6 ragged
+// prompts of up to 700 tokens: 20.7 us -> 19.7; with stretches, which wait for the plan first, it gains nothing).
+__device__ __forceinline__ void pf_wait_expansion() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __host__ __device__ constexpr uint32_t pf_idesc(int M, int N, bool b_mn_major) {   // fp16 operands, fp32 accumulator
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
@@ -478,7 +477,9 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (lane == 0) {
         uint32_t n_q[2] = {0, 0};   // loads issued per tile (phase of q_free / q_full)
         bool ok = true;
-        for (PfCursor c(a); c.more() && ok;) {
+        PfCursor c(a);
+        pf_wait_expansion();
+        while (c.more() && ok) {
           const PfItem it = c.next(a);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
@@ -497,7 +498,9 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (lane == 0) {
         uint32_t kc = 0, vc = 0;
         bool ok = true;
-        for (PfCursor c(a); c.more() && ok;) {
+        PfCursor c(a);
+        pf_wait_expansion();
+        while (c.more() && ok) {
           const PfItem it = c.next(a);
           const int bh = it.b * kv_heads + a.line.by_share(c.of_unit), end = min(c.j1, max(it.J[0], it.J[1]));
           for (int j = c.j0; j < end; ++j) {
@@ -538,7 +541,9 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           }
           umma_commit(&s_full[t]);
         };
-        for (PfCursor c(a); c.more() && ok;) {
+        PfCursor c(a);
+        pf_wait_expansion();
+        while (c.more() && ok) {
           const PfItem it = c.next(a);
           const int j0 = c.j0;
           int end[2];                         // steps of each tile in this part: j0 .. end - 1
@@ -620,7 +625,9 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.o_stride * 2)) & 31) == 0;
     uint32_t n_s = 0, n_o = 0;
     bool ok = true;
-    for (PfCursor c(a); c.more() && ok;) {
+    PfCursor c(a);
+    pf_wait_expansion();
+    while (c.more() && ok) {
       const PfItem it = c.next(a);
       // (selects, not indexing: the item stays in registers)
       const int Jt = t ? it.J[1] : it.J[0], j0 = c.j0, end = min(c.j1, Jt);
@@ -849,6 +856,7 @@ pf_merge_kernel(const __grid_constant__ PfArgs a) {
 constexpr long long PF_IMAGES = 1LL << 31;
 struct PfSizes {
   int tiles, pack, units, n_qb, ctas;
+  int per_item;
   int slice;                            // sequences at a time; the rest is for one slice
   bool whole;
   long long kv_tiles, pairs, steps;     // steps: places on the line, at most
@@ -861,12 +869,14 @@ PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int k
   z.tiles = std::max(1, (max_kv + PF_TILE - 1) / PF_TILE);
   z.pack = PF_TILE % G == 0 ? G : 1;
   z.units = heads / z.pack;
-  z.n_qb = (int)(((long long)max_q * z.pack + 2 * PF_TILE - 1) / (2 * PF_TILE));
   z.slice = (int)std::max(1LL, std::min((long long)batch, PF_IMAGES / (4LL * kv_heads * z.tiles * PF_TILE * D)));
   z.kv_tiles = (long long)z.slice * kv_heads * z.tiles;
+  const long long q_tiles = ((long long)max_q * z.pack + PF_TILE - 1) / PF_TILE;
+  z.per_item = z.slice * q_tiles * z.units <= sm_count() && z.tiles <= PF_SINGLE_STEPS ? 1 : 2;
+  z.n_qb = (int)((q_tiles + z.per_item - 1) / z.per_item);
   z.pairs = (long long)z.slice * z.n_qb;
   z.steps = z.pairs * z.units * (z.tiles + PF_SETUP);
-  z.whole = z.pairs * z.units <= sm_count() && z.tiles <= PF_WHOLE_STEPS;
+  z.whole = z.per_item == 1 || (z.pairs * z.units <= sm_count() && z.tiles <= PF_WHOLE_STEPS);
   z.ctas = (int)(z.whole ? std::max(1LL, z.pairs * z.units) : std::max(1LL, std::min((long long)sm_count(), z.steps / PF_MIN_STEPS)));
   z.kv = align(z.kv_tiles * PF_TILE * D * 2);
   z.q = align((long long)total_q * heads * D * 2);
@@ -909,7 +919,6 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.heads = heads;
   x.tiles = z.tiles;
   x.total_q = total_q;
-  x.most_q = z.n_qb * (2 * PF_TILE / z.pack);
   x.status = status;
   int log_pack = 0;
   while (1 << log_pack < z.pack) ++log_pack;
@@ -922,12 +931,10 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   const CUtensorMap tq = make_tensor_map(x.qh, TmaDType::BF16, 3, qd, qs, qb, true);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.blockDim = dim3(256);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
 
   for (int b0 = 0; b0 < batch; b0 += z.slice) {
     const int nb = std::min(z.slice, batch - b0);
@@ -935,10 +942,10 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
     x.pages.block_table = c.block_table + (long long)b0 * c.max_pages;
     x.pages.n_seqs = c.n_seqs - b0;
     x.kv_lens = kv_lens + b0;
-    x.line = {cu_q + b0, kv_lens + b0, nb, s.pack, log_pack, s.units, s.n_qb, s.tiles, kv4_div(std::max(1, s.n_qb)), kv4_div(s.units / c.kv_heads)};
+    x.line = {cu_q + b0, kv_lens + b0, nb, s.pack, log_pack, s.units, s.n_qb, s.tiles, s.per_item, kv4_div(std::max(1, s.n_qb)), kv4_div(s.units / c.kv_heads)};
     x.pairs = (int)s.pairs;
+    x.most_q = s.n_qb * s.per_item * (PF_TILE / s.pack);
     x.ctas = s.ctas;
-    x.whole = s.whole;
     x.kv_blocks = (int)s.kv_tiles;
     x.q_blocks = b0 == 0 ? (int)q_blocks : 0;
     const unsigned blocks = (unsigned)x.kv_blocks + (unsigned)x.q_blocks + 1u;
@@ -953,13 +960,20 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
     const CUtensorMap tk = make_tensor_map(x.k, TmaDType::BF16, 3, kd, ks, kb, true);
     const CUtensorMap tv = make_tensor_map(x.v, TmaDType::BF16, 3, kd, ks, kb, true);
     PfArgs a{x.line, x.plan, x.q_factor, x.exponents, (__nv_bfloat16*)out, parts, o_stride, heads, heads / c.kv_heads, total_q,
-             scale * 1.4426950408889634f, status};
-    cfg.gridDim = dim3((unsigned)std::max(1, s.ctas - 1), 2 * (D / 16));
+             scale * 1.4426950408889634f, status, s.whole, kv4_div(s.units)};
     const auto go = [&](auto kern, auto merge, int smem) {
       MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      kern<<<s.ctas, PF_THREADS, smem, stream>>>(tq, tk, tv, a);
-      check_launch();
-      if (!s.whole) MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, merge, a));
+      cfg.gridDim = dim3((unsigned)s.ctas);
+      cfg.blockDim = dim3(PF_THREADS);
+      cfg.dynamicSmemBytes = smem;
+      cfg.numAttrs = s.whole ? 1 : 0;
+      MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, a));
+      if (s.whole) return;
+      cfg.gridDim = dim3((unsigned)std::max(1, s.ctas - 1), 2 * (D / 16));
+      cfg.blockDim = dim3(256);
+      cfg.dynamicSmemBytes = 0;
+      cfg.numAttrs = 1;
+      MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, merge, a));
     };
     if (D == 128) go(fa_int4_kernel<128>, pf_merge_kernel<128>, PfCfg<128>::SMEM_BYTES);
     else go(fa_int4_kernel<64>, pf_merge_kernel<64>, PfCfg<64>::SMEM_BYTES);
