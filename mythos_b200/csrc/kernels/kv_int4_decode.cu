@@ -165,21 +165,23 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
         kw[j][0][0] = x.x; kw[j][0][1] = x.y;
       }
     }
+    // (groups innermost: products of one sum wait for one another; 8 x 32768 tokens: 53.1 -> 51.9 us)
 #pragma unroll
-    for (int g = 0; g < GR; ++g)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t w0 = kw[0][g][h], w1 = kw[1][g][h], v0 = __funnelshift_r(w0, w0, 8), v1 = __funnelshift_r(w1, w1, 8);
-        const uint32_t a0 = w0 & 0x00780078u, a1 = w1 & 0x00780078u, a2 = w0 & 0x07800780u, a3 = w1 & 0x07800780u;
-        const uint32_t b0 = v0 & 0x00780078u, b1 = v1 & 0x00780078u, b2 = v0 & 0x07800780u, b3 = v1 & 0x07800780u;
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float (&c)[4] = sc[u][nb][g];
-          if (h == 0) p4_mma0(c, a0, a1, a2, a3, s.qb[nb][g][0], s.qb[nb][g][1]);
-          else p4_mma(c, a0, a1, a2, a3, s.qb[nb][g][4], s.qb[nb][g][5]);
-          p4_mma(c, b0, b1, b2, b3, s.qb[nb][g][4 * h + 2], s.qb[nb][g][4 * h + 3]);
+        for (int g = 0; g < GR; ++g) {
+          const uint32_t k0 = kw[0][g][h], k1 = kw[1][g][h];
+          const uint32_t w0 = e ? __funnelshift_r(k0, k0, 8) : k0, w1 = e ? __funnelshift_r(k1, k1, 8) : k1;
+          const uint32_t a0 = w0 & 0x00780078u, a1 = w1 & 0x00780078u, a2 = w0 & 0x07800780u, a3 = w1 & 0x07800780u;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float (&c)[4] = sc[u][nb][g];
+            if (h == 0 && e == 0) p4_mma0(c, a0, a1, a2, a3, s.qb[nb][g][0], s.qb[nb][g][1]);
+            else p4_mma(c, a0, a1, a2, a3, s.qb[nb][g][4 * h + 2 * e], s.qb[nb][g][4 * h + 2 * e + 1]);
+          }
         }
-      }
   }
   // ---- exponent of the chunk's values: one group of one token per thread and tile
   float mag = 0.f;
