@@ -448,6 +448,8 @@ void qkv_rope_append_int4(float* acc, const int* pos, const int* seq_ids, void* 
                           float theta, cudaStream_t stream) {
   MB_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "qkv_rope_append: 4-bit pages need a head_dim of 64 or 128");
   MB_REQUIRE(c.page_size > 0 && c.page_size % 16 == 0, "qkv_rope_append: 4-bit pages hold a multiple of 16 tokens");
+  MB_REQUIRE(c.kv_heads > 0 && (long long)c.n_pages * c.kv_heads * (c.page_size / 16) < (1LL << 31), "qkv_rope_append: too many tiles in the 4-bit cache");
+  MB_REQUIRE(((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15) == 0, "qkv_rope_append: 4-bit caches must be 16-byte aligned");
   if (tokens == 0) return;
   const long long work = (long long)tokens * (heads + 2 * c.kv_heads) * (c.head_dim / 16);
   qkv_rope_append_kernel<true><<<(unsigned)ceil_div(work, 128), 128, 0, stream>>>(
