@@ -157,7 +157,7 @@ struct PfExpand {
   __half* v;
   __half* qh;           // [total_q, heads, D]
   float* q_factor;      // [total_q, heads]: 2^eq
-  int* exponents;       // [batch * kv_heads, tiles]: ek in the low, ev in the high half
+  int* exponents;       // [batch * kv_heads, tiles]: ek in the low byte, ev in the high half; between them, a bit per 16 tokens that have no page
   int kv_heads, heads, tiles, kv_blocks, q_blocks, total_q;
   int pairs;
   int most_q;           // new tokens that the items of a sequence cover
@@ -311,7 +311,12 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
     vm = fmaxf(vm, s_max[1][w]);
   }
   const int ek = pf_exponent(km), ev = pf_exponent(vm);
-  if (threadIdx.x == 0) a.exponents[blockIdx.x] = (ek & 0xFFFF) | ev << 16;
+  if (threadIdx.x == 0) {
+    int absent = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) absent |= (s_tile[u] < 0 && n0 + 16 * u < len ? 1 : 0) << u;
+    a.exponents[blockIdx.x] = (ek & 0xFF) | absent << 8 | ev << 16;
+  }
   const float ik = pf_pow2(-ek), iv = pf_pow2(-ev);
   const long long out = ((long long)bh * a.tiles + j) * PF_TILE * D;
 #pragma unroll 4
@@ -643,7 +648,8 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       int e0 = 0;                             // exponent of the part's first values: the row sum is kept in units of 2^-e0
       int e_next = end > j0 ? ex[j0] : 0;
       for (int j = j0; j < end && ok; ++j) {
-        const int ek = (short)e_next, e = e_next >> 16;
+        const int ek = (signed char)e_next, e = e_next >> 16;
+        const uint32_t absent = (uint32_t)e_next >> 8 & 0xFFu;     // sixteens of keys without a page: no query sees them
         if (j + 1 < end) e_next = ex[j + 1];
         if (j == j0) e0 = e;
         // (never zero: a masked score of minus infinity has to stay one)
@@ -661,6 +667,11 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
             for (int i = from; i < to; ++i)
               if (kv0 + i > limit) s[i] = -INFINITY;
+          }
+          if (absent) {
+#pragma unroll
+            for (int i = from; i < to; ++i)
+              if (absent >> (i >> 4) & 1u) s[i] = -INFINITY;
           }
         };
 #pragma unroll

@@ -314,10 +314,11 @@ def kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim: in
 
 def paged_attn_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, scale: float):
     """Causal attention of packed new tokens q [T, heads, D] (sequence b: rows cu_q[b] .. cu_q[b + 1], the last of its
-    kv_lens[b] keys) over 4-bit pages. A sequence without keys, and a query that sees none, give zeros."""
+    kv_lens[b] keys) over 4-bit pages. A sequence without keys, and a query that sees none, give zeros; a key without a page
+    is seen by none."""
     T, H, D = q.shape
     Hk = k_cache.shape[1]
-    kv4_check(k_cache, v_cache, block_table, Hk, D)
+    page_size = kv4_check(k_cache, v_cache, block_table, Hk, D)
     if Hk == 0 or H % Hk or cu_q.numel() != kv_lens.numel() + 1 or block_table.shape[0] < kv_lens.numel():
         raise ValueError("paged_attn_int4: heads in groups of the kv heads, cu_q with one entry more than kv_lens")
     out = torch.zeros_like(q)
@@ -331,6 +332,7 @@ def paged_attn_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, scale: floa
         k, v = (x.repeat_interleave(H // Hk, 1) for x in (k, v))
         s = torch.einsum("qhd,khd->hqk", q[a:e].float(), k) * scale
         hidden = pos[None] > n - (e - a) + torch.arange(e - a, device=q.device)[:, None]
+        hidden = hidden | ~kv4_places(block_table, page_size, k_cache.shape[0], pos, torch.full_like(pos, b))[3]
         p = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
         p = torch.where(hidden.all(-1)[:, None], torch.zeros_like(p), p)
         out[a:e] = torch.einsum("hqk,khd->qhd", p, v).to(q.dtype)

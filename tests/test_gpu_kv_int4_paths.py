@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from kv_int4_util import filled, make_cache, oracle, random_rows, token_lists
-from mythos_b200.ops import functional as F, native
+from mythos_b200.ops import functional as F, native, reference as ref
 from test_gpu_kv_int4 import HALF, _decode_bound, _prefill_bound, _same_bits
 
 pytestmark = pytest.mark.gpu
@@ -320,3 +320,58 @@ def test_a_context_without_any_page_gives_zeros_and_is_reported():
     with pytest.raises(RuntimeError, match="status 2"):
         native.check_status("cuda")
     assert not nothing.any()
+
+
+@pytest.mark.parametrize("D,form", [(128, "prompt"), (64, "prompt"), (128, "stretches"), (128, "few")])
+def test_keys_without_a_page_are_seen_by_no_query(D, form):
+    H, Hk, page = 4, 2, 16
+    new, lens = {"prompt": ([700, 300], [900, 700]), "stretches": ([1000], [3000]), "few": ([6, 3], [200, 90])}[form]
+    kc, vc, table = filled(lens, Hk, D, page, "cuda", seed=6)
+    q = torch.randn(sum(new), H, D, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16).cuda()
+    cu, kv = _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    # the first sixteen tokens, whole 128-token tiles, one in the middle of a tile, the last
+    gaps, last = table.clone(), (lens[0] - 1) // page
+    gone = sorted({0, 5, last} | ({*range(8, 16), 17, 19, 40} if form != "few" else set()))
+    gaps[0, gone] = -1
+    got = F.paged_attn_prefill_int4(q, kc, vc, gaps, cu, kv, max(new), max(lens))
+    with pytest.raises(RuntimeError, match="status 2"):
+        native.check_status("cuda")
+    whole = F.paged_attn_prefill_int4(q, kc, vc, table, cu, kv, max(new), max(lens))
+    native.check_status("cuda")
+    assert _same_bits(got[new[0]:], whole[new[0]:])         # the other sequence
+    # attention over the tokens that are left: they move up, the queries keep what they see
+    left = [t for t in range(lens[0]) if t // page not in gone]
+    at = torch.tensor(left)
+    k, v = (x.double() for x in ref.kv_read_int4(kc.cpu(), vc.cpu(), table.cpu(), at, torch.zeros_like(at), D, torch.float32))
+    hidden = at > lens[0] - new[0] + torch.arange(new[0])[:, None]
+    for h in range(H):
+        qh = q[: new[0], h].cpu().double()
+        kh, vh = k[:, h // 2], v[:, h // 2]
+        p = torch.softmax((qh @ kh.T / math.sqrt(D)).masked_fill(hidden, -math.inf), -1).nan_to_num(0.0)
+        o = p @ vh
+        # the same roundings as everywhere, with |v| + |o| in place of |v - o|
+        res = {"out": o, "plain": p @ vh.abs(), "centred": p @ vh.abs() + o.abs(), "spread": p @ vh.abs() + o.abs(),
+               "logit": (qh.abs() @ kh.abs().T).masked_fill(hidden, 0).amax(-1, keepdim=True) / math.sqrt(D)}
+        off = (got[: new[0], h].cpu().double() - o).abs()
+        assert (off <= _prefill_bound(res)).all(), float((off / _prefill_bound(res)).max())
+        assert float(off.norm() / o.norm()) < 5e-3
+
+
+def test_fused_epilogue_refuses_what_its_stores_cannot_reach():
+    C = native.require()
+    H, Hk, D, page = 4, 2, 128, 16
+    bytes_ = 3 * Hk * page * F.kv4_token_bytes(D)
+    flat = torch.zeros(2, bytes_ + 16, device="cuda", dtype=torch.uint8)
+    kc, vc = (x[:bytes_].view(3, Hk, -1) for x in flat)
+    table = torch.arange(2, device="cuda", dtype=torch.int32)[:, None]
+    acc = torch.randn(2, (H + 2 * Hk) * D, device="cuda")
+    pos, sid = torch.zeros(2, device="cuda", dtype=torch.int32), torch.arange(2, device="cuda", dtype=torch.int32)
+    q = torch.empty(2, H, D, device="cuda", dtype=torch.bfloat16)
+    for off in (1, 2, 4, 8):
+        odd = flat[0, off:bytes_ + off].view(3, Hk, -1)
+        for caches in ((odd, vc), (kc, odd)):
+            with pytest.raises(ValueError, match="aligned"):
+                C.qkv_rope_append(acc, pos, sid, table, q, *caches, 10000.0)
+    assert not flat.any()
+    C.qkv_rope_append(acc, pos, sid, table, q, kc, vc, 10000.0)
+    assert kc[:2].any() and not kc[2].any()

@@ -104,6 +104,23 @@ def test_tokens_without_a_page():
         assert not x.any()
 
 
+def test_a_key_without_a_page_is_seen_by_no_query():
+    H, Hk, D, page = 4, 2, 64, 16
+    kc, vc, table = filled([50], Hk, D, page, "cpu")
+    gaps = table.clone()
+    gaps[0, 1], gaps[0, 3] = -1, kc.shape[0]
+    q = torch.randn(20, H, D, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    lens = torch.tensor([50], dtype=torch.int32)
+    out = F.paged_attn_prefill_int4(q, kc, vc, gaps, torch.tensor([0, 20], dtype=torch.int32), lens, 20, 50)
+    here = torch.tensor([*range(16), *range(32, 48)])
+    k, v = (x.double() for x in ref.kv_read_int4(kc, vc, table, here, torch.zeros_like(here), D, torch.float32))
+    for h in range(H):
+        sc = q[:, h].double() @ k[:, h // 2].T / math.sqrt(D)
+        want = torch.softmax(sc.masked_fill(here > 30 + torch.arange(20)[:, None], -math.inf), -1) @ v[:, h // 2]
+        # (the output's rounding; sums of 64 terms in 32 bits)
+        assert ((out[:, h].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all()
+
+
 def test_refusals():
     kc, vc, table = make_cache([16], 2, 128, 16, "cpu")
     pos, sid = token_lists([0], [4], "cpu")
