@@ -412,7 +412,7 @@ void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_st
 // against 44), and larger ones whose blocks of columns run side by side with at most eight chunks of 32 keys per warp (one
 // sequence, 512 keys, 64 tokens: 11 us against 23; 4 x 1000 keys, 32 tokens: 20 against 29; twice that work, 4 x 1000, 64
 // tokens: 38 against 33; twice the blocks, 8 x 100, 100 tokens, 16 heads over 4: 19.5 against 12.4).
-bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads);
+bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
 long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads);
 void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                     long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,

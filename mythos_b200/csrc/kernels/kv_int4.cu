@@ -206,7 +206,7 @@ long long paged_attn_decode_int4_workspace(const KvInt4Cache& c, int batch, int 
 
 long long paged_attn_prefill_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads) {
   if (batch == 0 || max_q == 0 || c.kv_heads <= 0) return 0;
-  if (!few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads))
+  if (!few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads, c.head_dim))
     return prompt_int4_workspace(batch, total_q, max_q, max_kv, heads, c.kv_heads, c.head_dim);
   return few_query_int4_workspace(c, batch, max_q, heads);
 }
@@ -234,7 +234,7 @@ void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_st
   MB_REQUIRE(scale > 0.f, "paged_attn_prefill_int4: scale must be positive");
   if (batch == 0 || total_q == 0 || max_q == 0) return;
   kv4_workspace(workspace, paged_attn_prefill_int4_workspace(c, batch, total_q, max_q, max_kv, heads));
-  if (few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads)) {
+  if (few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads, c.head_dim)) {
     few_query_int4(c, q, q_stride, cu_q, kv_lens, out, o_stride, batch, total_q, max_q, heads, scale, workspace, status, stream);
     return;
   }

@@ -247,7 +247,8 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         mx += ev;                                 // relative to the reference used so far
         const bool first = s.unseen >> (2 * nb + c) & 1u;
-        if (first ? mx > -INFINITY : mx > 0.f) {
+        // (by the column's own scores alone: what the others hold, a NaN say, does not reach its bits)
+        if (first ? mx > -INFINITY : mx > 6.f) {
           const float alpha = first ? 0.f : fast_exp2(-mx);
           s.unseen &= ~(1u << (2 * nb + c));
           s.m[nb][c] += mx;
@@ -682,11 +683,16 @@ struct P4Line {
   }
   __device__ __forceinline__ int size(int b) const { return b < batch ? chunks(b) * units(b) : 0; }
 };
-// Equal stretches: the first `rem` of them one chunk longer.
+// Equal stretches: the first `rem` of them one chunk longer. No more stretches than leave each two chunks: every part costs the
+// merge more than a chunk costs a warp.
 struct P4Share {
-  int per, rem;
-  __device__ __forceinline__ P4Share(int total, int workers) : per(total / workers), rem(total - total / workers * workers) {}
-  __device__ __forceinline__ int start(int worker) const { return worker * per + min(worker, rem); }
+  int workers, per, rem;
+  __device__ __forceinline__ P4Share(int total, int most)
+      : workers(max(1, min(most, total / 2))), per(total / workers), rem(total - per * workers) {}
+  __device__ __forceinline__ int start(int worker) const {
+    const int w = min(worker, workers);            // (the warps that are left have none)
+    return w * per + min(w, rem);
+  }
   __device__ __forceinline__ int worker(int place) const {       // whose stretch holds it
     const int longer = rem * (per + 1);
     return place < longer ? place / (per + 1) : rem + (place - longer) / max(per, 1);
@@ -861,13 +867,16 @@ paged_attn_int4_line_kernel(const __grid_constant__ P4Args a, float* __restrict_
 }
 
 // One CTA per unit and 32 of its values: joins the parts of a unit that lies in several CTAs' stretches; zeros for a sequence
-// without keys. First the weights of all parts (one thread per part and column), then the sums with every load in flight.
+// without keys. First the weights of the parts (one thread per part and column), then the sums: slices of the CTA share
+// the parts, with their loads in flight (one slice takes 0.3 us a part: one sequence of 16384 tokens, one kv head, in a wide table: 44.6
+// us with a part for every chunk, 11.7 with four slices and two chunks a stretch; 8 x 32768 of 5 heads: 54.7 -> 49.9).
 constexpr int P4_MERGE = 64;      // parts whose weights are held at a time
-template <int D, int COLS>
-__global__ void __launch_bounds__(COLS * 8)
+template <int D, int COLS, int SLICES>
+__global__ void __launch_bounds__(COLS * 8 * SLICES)
 p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scratch, int ctas) {
-  constexpr int PART = COLS * (D + 2);
-  __shared__ float s_w[P4_MERGE][COLS], s_lw[P4_MERGE][COLS], s_m[COLS];
+  constexpr int PART = COLS * (D + 2), THREADS = COLS * 8 * SLICES;
+  __shared__ float s_w[P4_MERGE][COLS], s_lw[P4_MERGE][COLS], s_l[SLICES][COLS];
+  __shared__ float4 s_acc[SLICES][COLS * 8];
   __shared__ int s_at[P4_MERGE];
   const int b = blockIdx.x, y = blockIdx.y, lane = threadIdx.x & 31;
   const P4Line line(a, COLS);
@@ -884,37 +893,34 @@ p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scra
   if (y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && a.cu_q && a.cu_q[b + 1] - a.cu_q[b] > a.max_q) p4_too_long(a);
   if (!here || (n > 0 && c0 == c1)) return;       // no such unit, or written by that CTA
   const P4Unit u(a, COLS, b, y);
-  const int c = threadIdx.x >> 3, d = blockIdx.z * 32 + (threadIdx.x & 7) * 4;
+  const int slice = threadIdx.x / (COLS * 8), at_col = threadIdx.x % (COLS * 8), c = at_col >> 3, part_of = threadIdx.x & 7;
+  const int d = blockIdx.z * 32 + part_of * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f, M = -INFINITY;
   for (int k0 = c0; k0 <= c1; k0 += P4_MERGE) {   // (a unit of more than 64 CTAs: joined in turns)
     const int parts = min(P4_MERGE, c1 - k0 + 1);
     __syncthreads();
-    for (int i = threadIdx.x; i < parts * COLS; i += COLS * 8) {
+    for (int i = threadIdx.x; i < parts * COLS; i += THREADS) {
       const int p = i / COLS, cc = i % COLS, k = k0 + p;
-      // the first CTA has the unit in its first slot only where the unit holds the first chunk of its stretch; with fewer
-      // chunks than warps a CTA in between may have an empty stretch
-      const int first = share.start(k * P4_WARPS);
-      const bool empty = first == share.start((k + 1) * P4_WARPS);
-      const int at = (2 * k + (u0 > first ? 1 : 0)) * PART;
-      if (cc == 0) s_at[p] = empty ? -1 : at;
-      s_w[p][cc] = empty ? -INFINITY : scratch[at + COLS * D + cc];
-      s_lw[p][cc] = empty ? 0.f : scratch[at + COLS * D + COLS + cc];
+      // the first CTA has the unit in its first slot only where the unit holds the first chunk of its stretch; a CTA's stretch is
+      // never empty between others
+      const int at = (2 * k + (u0 > share.start(k * P4_WARPS) ? 1 : 0)) * PART;
+      if (cc == 0) s_at[p] = at;
+      s_w[p][cc] = scratch[at + COLS * D + cc];
+      s_lw[p][cc] = scratch[at + COLS * D + COLS + cc];
     }
     __syncthreads();
-    if (threadIdx.x < COLS) {
-      float m = -INFINITY;
-      for (int p = 0; p < parts; ++p)
-        if (s_lw[p][threadIdx.x] != 0.f) m = fmaxf(m, s_w[p][threadIdx.x]);    // nothing seen is left out, a NaN is not
-      s_m[threadIdx.x] = m;
-    }
-    __syncthreads();
+    float Mn = M;                                 // the eight threads of a column look through every eighth part
+    for (int p = part_of; p < parts; p += 8)
+      if (s_lw[p][c] != 0.f) Mn = fmaxf(Mn, s_w[p][c]);          // nothing seen is left out, a NaN is not
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, o));
+    const float e = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
+    acc.x *= e; acc.y *= e; acc.z *= e; acc.w *= e; l *= e;
+    M = Mn;
     if (c < u.n_cols) {
-      const float Mn = fmaxf(M, s_m[c]), e = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
-      acc.x *= e; acc.y *= e; acc.z *= e; acc.w *= e; l *= e;
-      M = Mn;
 #pragma unroll 8
-      for (int p = 0; p < parts; ++p) {
+      for (int p = slice; p < parts; p += SLICES) {
         const float lw = s_lw[p][c];
         const float4 v = lw != 0.f ? *reinterpret_cast<const float4*>(scratch + s_at[p] + c * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
         const float w = lw != 0.f ? fast_exp2(s_w[p][c] - M) : 0.f;
@@ -924,6 +930,18 @@ p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scra
         acc.z = fmaf(w, v.z, acc.z);
         acc.w = fmaf(w, v.w, acc.w);
       }
+    }
+  }
+  if constexpr (SLICES > 1) {
+    s_acc[slice][at_col] = acc;
+    if (part_of == 0) s_l[slice][c] = l;
+    __syncthreads();
+    if (slice > 0) return;
+#pragma unroll
+    for (int k = 1; k < SLICES; ++k) {
+      const float4 v = s_acc[k][at_col];
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+      l += s_l[k][c];
     }
   }
   p4_store(u.out(a, D, c, d), acc, l);
@@ -940,12 +958,41 @@ void p4_configure(K kern, int smem, bool cluster, std::atomic<unsigned long long
   if (dev < 64) seen |= 1ull << dev;
 }
 
+// Clusters of `splits` CTAs that run side by side. A cluster lies within one of the GPU's partitions, which are not of one size: 40
+// clusters of 14 CTAs are fewer CTAs than fit, but take two turns (8 x 2048 tokens, 5 kv heads: 18.5 us, 10.7 in smaller ones).
+template <int D, int COLS>
+int p4_capacity(int splits) {
+  static std::atomic<int> known[17];
+  static std::atomic<unsigned long long> seen{0};
+  int n = known[splits];
+  if (n > 0) return n;
+  p4_configure(paged_attn_int4_cluster_kernel<D, COLS>, P4SmemCluster<D, COLS>::BYTES, true, seen);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(1, 1, splits);
+  cfg.blockDim = dim3(P4_THREADS);
+  cfg.dynamicSmemBytes = P4SmemCluster<D, COLS>::BYTES;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = splits;
+  MB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, paged_attn_int4_cluster_kernel<D, COLS>, &cfg));
+  known[splits] = std::max(1, n);
+  return std::max(1, n);
+}
+int p4_capacity(int D, int cols, int splits) {
+  if (D == 128) return cols == 16 ? p4_capacity<128, 16>(splits) : p4_capacity<128, 8>(splits);
+  return cols == 16 ? p4_capacity<64, 16>(splits) : p4_capacity<64, 8>(splits);
+}
+
 // How a call runs, by its sizes (the table's width stands for the contexts, which only the device knows).
 struct P4Plan {
   int cols, ctas, splits;         // splits > 0: clusters; else stretches of the line over that many CTAs
   long long blocks, units, chunks, resident;      // resident: CTAs side by side
 };
-P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, long long max_tokens) {
+P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, int D, long long max_tokens) {
   P4Plan p;
   p.cols = (long long)max_q * G > 8 ? 16 : 8;
   p.blocks = ((long long)max_q * G + p.cols - 1) / p.cols;
@@ -953,13 +1000,15 @@ P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, long long max_tokens) 
   p.chunks = std::max(1LL, (max_tokens + P4_CHUNK - 1) / P4_CHUNK);
   p.resident = (p.cols == 8 ? 4LL : 2LL) * sm_count();
   p.ctas = (int)std::max(1LL, std::min(p.resident, (p.units * p.chunks + P4_WARPS - 1) / P4_WARPS));
-  // A cluster per unit, of as many CTAs as the units leave room for, while no warp gets more than sixteen chunks. One launch,
-  // no scratch and no walk along the line: 64 x 512 tokens (8 kv heads, one query) take 12.9 us (18.0 as a line), 64 x 1280 27.0
-  // (32.6), 512 ragged x 512 76.3 (99.6), 4 x 1000 with five queries 10.9 (17.2). Longer contexts want the line's evenness:
-  // 32 ragged x 4096 take 35.6 there (37.0), 64 ragged x 2560 40.6 (41.8).
+  // A cluster per unit, of as many CTAs as the units leave room for, while no warp gets more than sixteen chunks (eight, where a
+  // larger cluster would have been of use). One launch, no scratch and no walk along the line: 64 x 1024 tokens (8 kv heads, one
+  // query) take 22.0 us (27.5 as a line), 64 x 2048 36.9 (41.6), 64 ragged x 1280 23.7 (27.2), 1 x 1024 6.3 (9.3), 8 x 8192 23.2
+  // (26.5). Longer contexts want the line's evenness: 1 x 32768 take 22.6 there (24.2), 2 x 32768 27.1 (31.3), and what lies between
+  // is even: 1 x 16384 15.5 (15.5).
   const long long want = std::min(16LL, (p.chunks + P4_WARPS - 1) / P4_WARPS);
-  const long long room = std::max(1LL, std::min(want, p.resident / std::max(1LL, p.units)));
-  p.splits = p.chunks <= 16 * P4_WARPS * room ? (int)room : 0;
+  long long room = std::max(1LL, std::min(want, p.resident / std::max(1LL, p.units)));
+  while (room > 1 && p4_capacity(D, p.cols, (int)room) < p.units) --room;
+  p.splits = p.chunks <= (room == 16 ? 8 : 16) * P4_WARPS * room ? (int)room : 0;
   return p;
 }
 
@@ -992,22 +1041,27 @@ void p4_launch(P4Args& a, const P4Plan& plan, float* scratch, cudaStream_t strea
   count_launch();
   check_launch();
   cfg.gridDim = dim3(a.batch, (unsigned)(plan.blocks * a.kv_heads), D / 32);
-  cfg.blockDim = dim3(COLS * 8);
+  const auto merge = [&](auto kern, int slices) {
+    cfg.blockDim = dim3(COLS * 8 * slices);
+    MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, (const float*)scratch, plan.ctas));
+  };
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, p4_merge_kernel<D, COLS>, a, (const float*)scratch, plan.ctas));
+  // (units of a few parts each want no slices: 64 x 1024 tokens, 8 kv heads, in a wide table: 27.6 us with one, 34.6 with four)
+  if (plan.ctas >= 8 * plan.units) merge(p4_merge_kernel<D, COLS, 4>, 4);
+  else merge(p4_merge_kernel<D, COLS, 1>, 1);
   count_launch();
 }
 
 }  // namespace
 
-bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads) {
-  const P4Plan p = p4_plan(batch, max_q, heads / kv_heads, kv_heads, max_kv);
+bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads, int head_dim) {
+  const P4Plan p = p4_plan(batch, max_q, heads / kv_heads, kv_heads, head_dim, max_kv);
   return p.blocks * p.cols <= 64 || (p.units <= p.resident && p.units * p.chunks <= 8 * P4_WARPS * p.resident);
 }
 
 long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads) {
-  const P4Plan p = p4_plan(batch, max_q, heads / c.kv_heads, c.kv_heads, (long long)c.max_pages * c.page_size);
+  const P4Plan p = p4_plan(batch, max_q, heads / c.kv_heads, c.kv_heads, c.head_dim, (long long)c.max_pages * c.page_size);
   return p.splits > 0 ? 0 : 2LL * p.ctas * p.cols * (c.head_dim + 2) * 4;
 }
 
@@ -1015,7 +1069,7 @@ void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, con
                     long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,
                     cudaStream_t stream) {
   const int G = heads / c.kv_heads;
-  const P4Plan plan = p4_plan(batch, max_q, G, c.kv_heads, (long long)c.max_pages * c.page_size);
+  const P4Plan plan = p4_plan(batch, max_q, G, c.kv_heads, c.head_dim, (long long)c.max_pages * c.page_size);
   P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v,
            {c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)}, kv_lens, cu_q,
            (__nv_bfloat16*)out, q_stride, o_stride, batch, G, c.kv_heads, total_q, max_q, (int)(plan.chunks + 1), kv4_div(G), kv4_div(c.kv_heads),
