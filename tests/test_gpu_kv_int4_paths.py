@@ -375,3 +375,45 @@ def test_fused_epilogue_refuses_what_its_stores_cannot_reach():
     assert not flat.any()
     C.qkv_rope_append(acc, pos, sid, table, q, kc, vc, 10000.0)
     assert kc[:2].any() and not kc[2].any()
+
+
+@pytest.mark.parametrize("H,Hk,D,lens,width", [
+    (4, 1, 128, [40000], 300000),                                  # parts in more CTAs than the merge holds weights of
+    (2, 1, 64, [34000, 20000, 1, 0, 700], 300000),
+    (20, 5, 128, [2048, 2000, 1500, 2048, 33, 64, 1900, 2047], 0),  # 40 clusters: of fewer CTAs than would fit by number
+    (8, 1, 128, [1100] * 32, 0), (16, 2, 128, [900, 31000], 0)])
+def test_decode_over_many_parts_and_cluster_sizes(H, Hk, D, lens, width):
+    kc, vc, table = filled(lens, Hk, D, 16, "cuda", seed=9)
+    B = len(lens)
+    q = torch.randn(B, H, D, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).cuda()
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    if width:
+        table = _widen(table, width, 16)
+    out = F.paged_attn_decode_int4(q, kc, vc, table, ctx)
+    res = oracle(q, kc, vc, table, range(B), [1] * B, lens, 1.0 / math.sqrt(D))
+    off = (out.cpu().double() - res["out"]).abs()
+    assert (off <= _decode_bound(res)).all(), float((off / _decode_bound(res)).max())
+    assert not out[ctx == 0].any() and _same_bits(F.paged_attn_decode_int4(q, kc, vc, table, ctx), out)
+    native.check_status("cuda")
+
+
+@pytest.mark.parametrize("form", ["cluster", "line", "several"])
+def test_a_heads_bits_do_not_depend_on_its_neighbours(form):
+    H, Hk, D, page = 8, 2, 128, 16
+    lens = [3000, 777]
+    kc, vc, table = filled(lens, Hk, D, page, "cuda", seed=2)
+    new = [3, 2] if form == "several" else [1, 1]
+    q = torch.randn(sum(new), H, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    cu, ctx = _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def call(q):
+        if form == "several":
+            return F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens))
+        return F.paged_attn_decode_int4(q, kc, vc, table if form == "cluster" else _widen(table, 400000, page), ctx)
+
+    want = call(q)
+    other = q.clone()
+    other[:, ::2] *= 40                                     # every second head's maximum moves all the time
+    got = call(other)
+    assert _same_bits(got[:, 1::2], want[:, 1::2]) and not _same_bits(got[:, ::2], want[:, ::2])
+    native.check_status("cuda")
