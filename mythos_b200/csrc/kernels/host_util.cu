@@ -57,7 +57,12 @@ CUtensorMap make_tensor_map(const void* base, TmaDType dt, int rank, const uint6
   // that has made no runtime call yet (an autograd worker) has none until the runtime binds one.
   static thread_local bool ctx_bound = false;
   if (!ctx_bound) {
-    MB_CUDA_CHECK(cudaFree(nullptr));
+    // (a thread's first call may be one that is captured into a graph, which allows this only in the relaxed mode)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    MB_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t bound = cudaFree(nullptr);
+    MB_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    MB_CUDA_CHECK(bound);
     ctx_bound = true;
   }
   CUtensorMap m;

@@ -417,3 +417,39 @@ def test_a_heads_bits_do_not_depend_on_its_neighbours(form):
     got = call(other)
     assert _same_bits(got[:, 1::2], want[:, 1::2]) and not _same_bits(got[:, ::2], want[:, ::2])
     native.check_status("cuda")
+
+
+@pytest.mark.parametrize("form", ["line", "prompt"])
+def test_a_threads_first_call_may_be_captured(form):
+    import threading
+
+    H, Hk, D, page = 8, 2, 128, 16
+    new, lens = ([800, 700], [900, 700]) if form == "prompt" else ([1, 1], [900, 700])
+    kc, vc, table = filled(lens, Hk, D, page, "cuda", seed=1)
+    q = torch.randn(sum(new), H, D, device="cuda").to(torch.bfloat16)
+    cu, ctx = _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    wide = _widen(table, 40000, page)
+    native.status_word(q.device)
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens)) if form == "prompt" else \
+                    F.paged_attn_decode_int4(q, kc, vc, wide, ctx)
+            g.replay()
+            torch.cuda.synchronize()
+            got.append(out.clone())
+        except Exception as e:
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert isinstance(got[0], torch.Tensor), got[0]
+    want = F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens)) if form == "prompt" else \
+        F.paged_attn_decode_int4(q, kc, vc, wide, ctx)
+    assert _same_bits(got[0], want)
+    native.check_status("cuda")
