@@ -655,7 +655,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int limit = min(it.kv_len - 1, it.q_off + tok);
       const int* ex = a.exponents + (long long)(it.b * kv_heads + a.line.by_share(c.of_unit)) * a.line.tiles;
       const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 1.f;
-      float m_ref = 0.f, l = 0.f;
+      float m_ref = -INFINITY, l = 0.f;       // (no key seen yet)
       int e0 = 0;                             // exponent of the part's first values: the row sum is kept in units of 2^-e0
       int e_next = end > j0 ? ex[j0] : 0;
       for (int j = j0; j < end && ok; ++j) {
@@ -692,7 +692,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
         uint32_t pk[2][32];
         const auto exponentials = [&](int h) {   // of half h of the keys: fp16 pairs to pk[h], sums to rs2
-          const float shift = ev - m_ref;
+          const float shift = m_ref == -INFINITY ? 0.f : ev - m_ref;      // (without a key every score is minus infinity)
           const uint64_t sc2 = f32x2(sc, sc), nm2 = f32x2(shift, shift);
 #pragma unroll
           for (int i = 64 * h; i < 64 * h + 64; i += 2) {
@@ -724,10 +724,12 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         mx4[0] = fmax3(mx4[0], s[124], s[125]);
         mx4[1] = fmax3(mx4[1], s[126], s[127]);
         const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sc, ev);
-        const bool need = j == j0 || m_new - m_ref > 6.f;      // p up to 2^6 until the reference moves
-        if (__any_sync(0xffffffffu, need)) {
+        // p up to 2^6 until the reference moves. The first score that is seen always sets it, in whatever tile it stands: a
+        // reference of zero kept from a tile without a visible key left p as 2^(score + ev), which fp16 may not hold.
+        const bool need = m_new - m_ref > 6.f;
+        if (j == j0 || __any_sync(0xffffffffu, need)) {
           const float alpha = need ? fast_exp2(m_ref - m_new) : 1.f;
-          if (need) m_ref = m_new == -INFINITY ? 0.f : m_new;
+          if (need) m_ref = m_new;
           if (j > j0) {
             l *= alpha;
             // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):

@@ -1,0 +1,55 @@
+"""Corners of attention over 4-bit pages: first tiles that hold nothing, value sizes that change along a context, tokens of any size that
+a query does not see, lengths that were not announced."""
+import math
+
+import pytest
+import torch
+
+from kv_int4_bounds import attention, check
+from kv_int4_util import filled, make_cache, random_rows, token_lists
+from mythos_b200.ops import functional as F, native
+
+pytestmark = pytest.mark.gpu
+
+
+def _cu(new):
+    return torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+
+
+def _wide(table, tokens, page):
+    wide = torch.full((table.shape[0], (tokens + page - 1) // page), -1, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    return wide
+
+
+def _written(k, v, lens, Hk, D, seed=0):
+    kc, vc, table = make_cache(lens, Hk, D, 16, "cuda", seed=seed)
+    pos, sid = token_lists([0] * len(lens), lens, "cuda")
+    F.kv_append_int4(k.to(torch.bfloat16).contiguous(), v.to(torch.bfloat16).contiguous(), kc, vc, table, pos, sid)
+    return kc, vc, table
+
+
+def _queries(T, H, D, seed=8):
+    return torch.randn(T, H, D, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).cuda()
+
+
+# new tokens, keys, tiles of 128 keys without pages: whole items per CTA, and stretches that begin at any tile
+HIDDEN = [([700, 300], [900, 700], [0]), ([700, 300], [900, 700], [0, 1]), ([2500], [2500], [0, 1]), ([1000], [3000], [0, 1, 3, 4, 5, 8, 10, 11, 12, 20])]
+
+
+@pytest.mark.parametrize("size,offset", [(1.0, 0.0), (0.01, -8.0), (1e-4, -4.0), (1e-3, 12.0)])
+@pytest.mark.parametrize("new,lens,tiles", HIDDEN)
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_without_pages_leave_the_rest_as_exact(D, new, lens, tiles, size, offset):
+    H, Hk = 4, 2
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    q = _queries(sum(new), H, D)
+    k[..., 0], q[..., 0] = 4.0, offset * math.sqrt(D) / 4       # moves every score by the offset
+    kc, vc, table = _written(k, v.float() * size, lens, Hk, D)
+    for t in tiles:
+        table[0, 8 * t:8 * t + 8] = -1
+    cu, ctx = _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens))
+    with pytest.raises(RuntimeError, match="status 2"):
+        native.check_status("cuda")
+    check(got, *attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D)))
