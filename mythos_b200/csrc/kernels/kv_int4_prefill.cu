@@ -12,7 +12,10 @@
 //     multiplies it back with the softmax scale;
 //   * a tile of keys (128 tokens of one head) is divided by 2^ek, which joins the same factor per step;
 //   * a tile of values is divided by 2^ev, and the probabilities of the step are multiplied by it: the running reference
-//     M is the maximum of score + ev, so that p 2^(ev - M) stays within fp16, and the row sum is taken back by 2^-ev.
+//     M is the maximum of score + ev, so that p 2^(ev - M) stays within fp16, and the row sum is taken back by 2^-ev. What it
+//     is taken back to is sum 2^(score - M), between 2^-113 and 2^116 a key for ev of -110 to 113: it is kept in units of 2^10 (units of the
+//     first tile's ev overflowed where later values were 2^130 times as large). Values below 2^-124 lose bits, and the weights of tiles
+//     whose values are less than 2^-120 of another tile's leave the sum.
 // The matrix product multiplies masked probabilities of zero by whatever the value rows hold, so nothing that is not
 // finite goes there: tokens behind a sequence's end are zeros, and a token with a scale that is not finite gets values of
 // zero and NaN keys, which reach the queries that see it through their scores, and no others.
@@ -46,6 +49,8 @@ __device__ __forceinline__ int pf_exponent(float m) {
   const int e = (int)(__float_as_uint(m) >> 23) - 127 - 14;      // subnormals: -141 -> bounded
   return max(-126, min(113, e));
 }
+constexpr int PF_EV_MIN = -110;   // of a tile of values
+constexpr float PF_SUM_UNIT = 0x1p10f;      // of a row sum
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
 __device__ __forceinline__ uint32_t pf_half2(float a, float b) {
   uint32_t r;
@@ -321,7 +326,7 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
     km = fmaxf(km, s_max[0][w]);
     vm = fmaxf(vm, s_max[1][w]);
   }
-  const int ek = pf_exponent(km), ev = pf_exponent(vm);
+  const int ek = pf_exponent(km), ev = max(PF_EV_MIN, pf_exponent(vm));
   if (threadIdx.x == 0) {
     int absent = 0;
 #pragma unroll
@@ -378,9 +383,9 @@ struct PfArgs {
   bool whole;           // a whole item per CTA
   Kv4Div by_units;
 };
-// A part of a query tile: sums [D / 4][128 rows][4], reference, row sum and its exponent per row.
+// A part of a query tile: sums [D / 4][128 rows][4], reference and row sum per row.
 template <int D>
-__host__ __device__ constexpr int pf_part_floats() { return PF_TILE * (D + 4); }
+__host__ __device__ constexpr int pf_part_floats() { return PF_TILE * (D + 2); }
 
 // The parts of a CTA's stretch, in order: the steps j0 .. j1 of an item.
 struct PfCursor {
@@ -656,13 +661,11 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int* ex = a.exponents + (long long)(it.b * kv_heads + a.line.by_share(c.of_unit)) * a.line.tiles;
       const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 1.f;
       float m_ref = -INFINITY, l = 0.f;       // (no key seen yet)
-      int e0 = 0;                             // exponent of the part's first values: the row sum is kept in units of 2^-e0
       int e_next = end > j0 ? ex[j0] : 0;
       for (int j = j0; j < end && ok; ++j) {
         const int ek = (signed char)e_next, e = e_next >> 16;
         const uint32_t absent = (uint32_t)e_next >> 8 & 0xFFu;     // sixteens of keys without a page: no query sees them
         if (j + 1 < end) e_next = ex[j + 1];
-        if (j == j0) e0 = e;
         // (never zero: a masked score of minus infinity has to stay one)
         const float sc = fmaxf(row_f * pf_pow2(ek), 1e-37f), ev = (float)e;
         ok = mbar_wait(&s_full[t], n_s & 1, abort_flag, status, 102);
@@ -757,7 +760,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         float rs[8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
-        l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(e0 - e);
+        l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(-e) * (1.f / PF_SUM_UNIT);
       }
       if (!ok) break;
       if (end > j0) {
@@ -767,8 +770,8 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         ++n_o;
         tc_fence_after();
       }
-      // p 2^ev and the values' 2^-ev cancel in O; l is in units of 2^-e0
-      const float inv_l = l == 0.f ? 0.f : 1.f / l, unit = pf_pow2(e0);
+      // p 2^ev and the values' 2^-ev cancel in O
+      const float inv_l = l == 0.f ? 0.f : 1.f / PF_SUM_UNIT / l;
       __nv_bfloat16* orow = a.out + (long long)row * a.o_stride + (long long)head * D;
       float* part = a.parts + (long long)((blockIdx.x * 2 + c.slot) * 2 + t) * pf_part_floats<D>();
 #pragma unroll 1
@@ -785,7 +788,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           uint32_t v[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            v[i] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(orr[2 * i]) * inv_l * unit, __uint_as_float(orr[2 * i + 1]) * inv_l * unit);
+            v[i] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(orr[2 * i]) * inv_l, __uint_as_float(orr[2 * i + 1]) * inv_l);
           // rows lie far apart: a lane writes whole 32-byte sectors where they are aligned
           __nv_bfloat16* at = orow + k * 32;
           if (wide) {
@@ -800,7 +803,6 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (!whole) {
         part[PF_TILE * D + r] = m_ref;
         part[PF_TILE * (D + 1) + r] = l;
-        part[PF_TILE * (D + 2) + r] = __int_as_float(e0);
       }
       // The TMEM loads above have completed (tmem_ld_wait); the next part's first PV product waits for
       // this warpgroup's next arrives on p_full, so O_t is not overwritten before it was read.
@@ -839,21 +841,18 @@ pf_merge_kernel(const __grid_constant__ PfArgs a) {
     return a.parts + (long long)((c * 2 + (u0 > pf_start(per, rem, c) ? 1 : 0)) * 2 + t) * pf_part_floats<D>();
   };
   float M = -INFINITY, l = 0.f;
-  int e0 = 0;
   float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 2
   for (int c = c0; c <= c1; ++c) {
     const float* p = part(c);
     const float m = p[PF_TILE * D + r], lc = p[PF_TILE * (D + 1) + r];
-    const int e = __float_as_int(p[PF_TILE * (D + 2) + r]);
     float4 v[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) v[k] = *reinterpret_cast<const float4*>(p + ((v0 + k) * PF_TILE + r) * 4);
     if (lc == 0.f) continue;                      // nothing seen (a NaN is not nothing)
-    if (l == 0.f) e0 = e;
     const float Mn = fmaxf(M, m), w0 = l == 0.f ? 0.f : fast_exp2(M - Mn), w = fast_exp2(m - Mn);
     M = Mn;
-    l = fmaf(w * pf_pow2(e0 - e), lc, l * w0);
+    l = fmaf(w, lc, l * w0);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       acc[k].x = fmaf(w, v[k].x, acc[k].x * w0);
@@ -864,12 +863,12 @@ pf_merge_kernel(const __grid_constant__ PfArgs a) {
   }
   const int tok = (t ? it.tok[1] : it.tok[0]) + (r >> a.line.log_pack), head = unit * a.line.pack + (r & (a.line.pack - 1)), row = it.row0 + tok;
   if (tok >= it.q_len || (unsigned)row >= (unsigned)a.total_q) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l, u = pf_pow2(e0);
+  const float inv = l == 0.f ? 0.f : 1.f / PF_SUM_UNIT / l;
   uint32_t y[4];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    y[2 * k] = l == 0.f ? 0u : pack_bf16x2(acc[k].x * inv * u, acc[k].y * inv * u);
-    y[2 * k + 1] = l == 0.f ? 0u : pack_bf16x2(acc[k].z * inv * u, acc[k].w * inv * u);
+    y[2 * k] = l == 0.f ? 0u : pack_bf16x2(acc[k].x * inv, acc[k].y * inv);
+    y[2 * k + 1] = l == 0.f ? 0u : pack_bf16x2(acc[k].z * inv, acc[k].w * inv);
   }
   *reinterpret_cast<uint4*>(a.out + (long long)row * a.o_stride + (long long)head * D + v0 * 4) = make_uint4(y[0], y[1], y[2], y[3]);
 }
@@ -907,7 +906,7 @@ PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int k
   z.factor = align((long long)total_q * heads * 4);
   z.exponents = align(z.kv_tiles * 4);
   z.plan = align((4 + 4LL * z.ctas) * 4);
-  z.parts = z.whole ? 0 : align(4LL * z.ctas * PF_TILE * (D + 4) * 4);
+  z.parts = z.whole ? 0 : align(4LL * z.ctas * PF_TILE * (D + 2) * 4);
   z.total = 2 * z.kv + z.q + z.factor + z.exponents + z.plan + z.parts;
   return z;
 }

@@ -53,3 +53,22 @@ def test_tiles_without_pages_leave_the_rest_as_exact(D, new, lens, tiles, size, 
     with pytest.raises(RuntimeError, match="status 2"):
         native.check_status("cuda")
     check(got, *attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D)))
+
+
+# sizes of the values, 128 tokens after 128
+SIZES = [[1e-35, 4.0], [1e-35, 1e-3, 4.0, 1e-20, 1.0], [2.0 ** (20 * (-1) ** i) for i in range(30)], [1.0] + [1e-36] * 3 + [1e-12] * 9]
+
+
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("new,lens", [([700, 300], [900, 700]), ([2500], [2500]), ([1000], [3000]), ([1, 1], [3000, 700])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_sizes_that_change_along_a_context(D, new, lens, sizes):
+    H, Hk = 4, 2
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    size = torch.cat([torch.tensor(sizes)[(torch.arange(n) // 128).clamp_max(len(sizes) - 1)] for n in lens]).cuda()
+    kc, vc, table = _written(k, v.float() * size[:, None, None], lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    for t in (table, _wide(table, 40000, 16)):
+        check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
+    native.check_status("cuda")
