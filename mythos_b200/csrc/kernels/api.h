@@ -397,7 +397,8 @@ void qkv_rope_append_int4(float* acc, const int* pos, const int* seq_ids, void* 
 void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* context_lens, void* out, int batch,
                             int heads, float scale, void* workspace, int* status, cudaStream_t stream);
 // New tokens of several sequences packed back to back, causal over the pages (as flash_attn_paged_prefill). max_q: most new
-// tokens of a sequence, max_kv: most keys; a sequence that has more is reported through the status word.
+// tokens of a sequence, max_kv: most keys; a sequence that has more is reported through the status word, and what lies behind
+// them may be left out.
 // Bytes of the two calls' workspaces; 16-byte aligned, free again when the call's kernels have run.
 long long paged_attn_decode_int4_workspace(const KvInt4Cache& c, int batch, int heads);
 long long paged_attn_prefill_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads);
@@ -415,8 +416,8 @@ void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_st
 bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
 long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads);
 void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
-                    long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,
-                    cudaStream_t stream);
+                    long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,
+                    int* status, cudaStream_t stream);
 long long prompt_int4_workspace(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int head_dim);
 void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
                  long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,

@@ -4,6 +4,8 @@
 //   kv_read_int4              tokens of the cache -> bf16 rows
 //   paged_attn_decode_int4    one query token per sequence
 //   paged_attn_prefill_int4   several new query tokens per sequence, causal, over everything in the pages
+#include <climits>
+
 #include "api.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -205,7 +207,7 @@ long long paged_attn_decode_int4_workspace(const KvInt4Cache& c, int batch, int 
 }
 
 long long paged_attn_prefill_int4_workspace(const KvInt4Cache& c, int batch, int total_q, int max_q, int max_kv, int heads) {
-  if (batch == 0 || max_q == 0 || c.kv_heads <= 0) return 0;
+  if (batch == 0 || c.kv_heads <= 0) return 0;
   if (!few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads, c.head_dim))
     return prompt_int4_workspace(batch, total_q, max_q, max_kv, heads, c.kv_heads, c.head_dim);
   return few_query_int4_workspace(c, batch, max_q, heads);
@@ -220,8 +222,8 @@ void paged_attn_decode_int4(const KvInt4Cache& c, const void* q, long long q_str
   MB_REQUIRE(scale > 0.f, "paged_attn_decode_int4: scale must be positive");
   if (batch == 0) return;
   kv4_workspace(workspace, paged_attn_decode_int4_workspace(c, batch, heads));
-  few_query_int4(c, q, q_stride, nullptr, context_lens, out, (long long)heads * c.head_dim, batch, batch, 1, heads, scale, workspace,
-                 status, stream);
+  few_query_int4(c, q, q_stride, nullptr, context_lens, out, (long long)heads * c.head_dim, batch, batch, 1, INT_MAX, heads, scale,
+                 workspace, status, stream);
 }
 
 void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
@@ -232,10 +234,10 @@ void paged_attn_prefill_int4(const KvInt4Cache& c, const void* q, long long q_st
   MB_REQUIRE(q_stride % 8 == 0 && o_stride % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
              "paged_attn_prefill_int4: q and out must be 16-byte aligned with token strides of multiples of 8 elements");
   MB_REQUIRE(scale > 0.f, "paged_attn_prefill_int4: scale must be positive");
-  if (batch == 0 || total_q == 0 || max_q == 0) return;
+  if (batch == 0) return;         // (without queries: the lengths are still looked at)
   kv4_workspace(workspace, paged_attn_prefill_int4_workspace(c, batch, total_q, max_q, max_kv, heads));
   if (few_query_int4_takes(batch, max_q, max_kv, heads, c.kv_heads, c.head_dim)) {
-    few_query_int4(c, q, q_stride, cu_q, kv_lens, out, o_stride, batch, total_q, max_q, heads, scale, workspace, status, stream);
+    few_query_int4(c, q, q_stride, cu_q, kv_lens, out, o_stride, batch, total_q, max_q, max_kv, heads, scale, workspace, status, stream);
     return;
   }
   prompt_int4(c, q, q_stride, cu_q, kv_lens, out, o_stride, batch, total_q, max_q, max_kv, heads, scale, workspace, status, stream);

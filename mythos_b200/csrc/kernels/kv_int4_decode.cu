@@ -89,7 +89,8 @@ struct P4Args {
   __nv_bfloat16* out;
   long long q_stride, o_stride;
   int batch, G, kv_heads, total_q;
-  int max_q, most_chunks;   // a sequence's: the tables' tokens, and one chunk more, which reports what lies behind them
+  int max_q, max_kv;        // what the call announced of a sequence
+  int most_chunks;          // a sequence's: the tables' tokens, and one chunk more, which reports what lies behind them
   Kv4Div by_group, by_heads;
   float scale_log2;
   int* status;
@@ -123,9 +124,10 @@ struct P4Unit {
   }
 };
 
-// Rows behind max_q have no unit: reported, left as they were.
-__device__ __forceinline__ void p4_too_long(const P4Args& a) {
-  if (a.status) atomicCAS(a.status, 0, ST_BAD_ARG | (90 << 16));
+// A sequence with more new tokens or keys than the call announced is reported. Rows behind max_q have no unit and are left as they
+// were; keys are all dealt with.
+__device__ __forceinline__ void p4_announced(const P4Args& a, int q_len, int kv_len) {
+  if (a.status && (q_len > a.max_q || kv_len > a.max_kv)) atomicCAS(a.status, 0, ST_BAD_ARG | (90 << 16));
 }
 
 // A warp's running state. Thread (r, t) of the warp holds columns 2 t and 2 t + 1 of every block of eight.
@@ -607,7 +609,7 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, splits = gridDim.z;
   const P4Unit u(a, COLS, blockIdx.x, blockIdx.y);
-  if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && u.q_len > a.max_q) p4_too_long(a);
+  if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) p4_announced(a, u.q_len, u.kv_len);
   if (u.n_cols <= 0) return;                      // the same for every CTA of the cluster
   float* s_ml = reinterpret_cast<float*>(smem + S::OFF_ML);
   float* s_cml = reinterpret_cast<float*>(smem + S::OFF_CML);
@@ -890,7 +892,7 @@ p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scra
     c1 = share.worker(u0 + n - 1) / P4_WARPS;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");             // every CTA, so that this grid ends behind the one before
-  if (y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && a.cu_q && a.cu_q[b + 1] - a.cu_q[b] > a.max_q) p4_too_long(a);
+  if (y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && a.cu_q) p4_announced(a, a.cu_q[b + 1] - a.cu_q[b], a.kv_lens[b]);
   if (!here || (n > 0 && c0 == c1)) return;       // no such unit, or written by that CTA
   const P4Unit u(a, COLS, b, y);
   const int slice = threadIdx.x / (COLS * 8), at_col = threadIdx.x % (COLS * 8), c = at_col >> 3, part_of = threadIdx.x & 7;
@@ -994,6 +996,7 @@ struct P4Plan {
 };
 P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, int D, long long max_tokens) {
   P4Plan p;
+  max_q = std::max(1, max_q);       // (a call that announces no new tokens still looks at the lengths)
   p.cols = (long long)max_q * G > 8 ? 16 : 8;
   p.blocks = ((long long)max_q * G + p.cols - 1) / p.cols;
   p.units = (long long)batch * kv_heads * p.blocks;
@@ -1057,7 +1060,7 @@ void p4_launch(P4Args& a, const P4Plan& plan, float* scratch, cudaStream_t strea
 
 bool few_query_int4_takes(int batch, int max_q, int max_kv, int heads, int kv_heads, int head_dim) {
   const P4Plan p = p4_plan(batch, max_q, heads / kv_heads, kv_heads, head_dim, max_kv);
-  return p.blocks * p.cols <= 64 || (p.units <= p.resident && p.units * p.chunks <= 8 * P4_WARPS * p.resident);
+  return max_q == 0 || p.blocks * p.cols <= 64 || (p.units <= p.resident && p.units * p.chunks <= 8 * P4_WARPS * p.resident);
 }
 
 long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, int heads) {
@@ -1066,13 +1069,13 @@ long long few_query_int4_workspace(const KvInt4Cache& c, int batch, int max_q, i
 }
 
 void few_query_int4(const KvInt4Cache& c, const void* q, long long q_stride, const int* cu_q, const int* kv_lens, void* out,
-                    long long o_stride, int batch, int total_q, int max_q, int heads, float scale, void* workspace, int* status,
-                    cudaStream_t stream) {
+                    long long o_stride, int batch, int total_q, int max_q, int max_kv, int heads, float scale, void* workspace,
+                    int* status, cudaStream_t stream) {
   const int G = heads / c.kv_heads;
   const P4Plan plan = p4_plan(batch, max_q, G, c.kv_heads, c.head_dim, (long long)c.max_pages * c.page_size);
   P4Args a{(const __nv_bfloat16*)q, (const uint8_t*)c.k, (const uint8_t*)c.v,
            {c.block_table, c.n_seqs, c.max_pages, c.n_pages, c.kv_heads, c.page_size, kv4_div(c.page_size)}, kv_lens, cu_q,
-           (__nv_bfloat16*)out, q_stride, o_stride, batch, G, c.kv_heads, total_q, max_q, (int)(plan.chunks + 1), kv4_div(G), kv4_div(c.kv_heads),
+           (__nv_bfloat16*)out, q_stride, o_stride, batch, G, c.kv_heads, total_q, max_q, max_kv, (int)(plan.chunks + 1), kv4_div(G), kv4_div(c.kv_heads),
            scale * 1.4426950408889634f, status};
   float* scratch = (float*)workspace;
   if (c.head_dim == 128) {

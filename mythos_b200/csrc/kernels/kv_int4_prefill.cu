@@ -167,7 +167,7 @@ struct PfExpand {
   int kv_heads, heads, tiles, kv_blocks, q_blocks, q_rows;     // q_rows: total_q * heads
   Kv4Div by_heads;
   int pairs;
-  int most_q;           // new tokens that the items of a sequence cover
+  int max_q, max_kv;    // what the call announced of a sequence
   PfLine line;
   PfPlan plan;
   int ctas;
@@ -188,8 +188,8 @@ __device__ void pf_make_plan(const PfExpand& a) {
   __shared__ int s_sum[PF_EXPAND / 32], s_total;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int each = (a.pairs + PF_EXPAND - 1) / PF_EXPAND, p0 = min(a.pairs, (int)threadIdx.x * each), p1 = min(a.pairs, p0 + each);
-  for (int b = threadIdx.x; b < a.line.batch; b += PF_EXPAND)     // more tokens than the caller said: not all are dealt with
-    if (a.status && (a.line.kv_lens[b] > a.tiles * PF_TILE || a.line.cu_q[b + 1] - a.line.cu_q[b] > a.most_q))
+  for (int b = threadIdx.x; b < a.line.batch; b += PF_EXPAND)     // more tokens than the caller said: not all may be dealt with
+    if (a.status && (a.line.kv_lens[b] > a.max_kv || a.line.cu_q[b + 1] - a.line.cu_q[b] > a.max_q))
       atomicCAS(a.status, 0, ST_BAD_ARG | (90 << 16));
   int sum = 0;
   for (int p = p0; p < p1; ++p) sum += PfItem(a.line, p).places() * a.line.units;
@@ -943,6 +943,8 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.tiles = z.tiles;
   x.q_rows = (int)((long long)total_q * heads);
   x.by_heads = kv4_div(heads);
+  x.max_q = max_q;
+  x.max_kv = max_kv;
   x.status = status;
   int log_pack = 0;
   while (1 << log_pack < z.pack) ++log_pack;
@@ -969,7 +971,6 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
     x.kv_lens = kv_lens + b0;
     x.line = {cu_q + b0, kv_lens + b0, nb, s.pack, log_pack, s.units, s.n_qb, s.tiles, s.per_item, kv4_div(std::max(1, s.n_qb)), kv4_div(s.units / c.kv_heads)};
     x.pairs = (int)s.pairs;
-    x.most_q = s.n_qb * s.per_item * (PF_TILE / s.pack);
     x.ctas = s.ctas;
     x.kv_blocks = (int)s.kv_tiles;
     x.q_blocks = b0 == 0 ? (int)q_blocks : 0;

@@ -746,8 +746,9 @@ def paged_attn_prefill_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, max
                             scale: float | None = None, out=None):
     """Causal attention of the new tokens of several sequences (q bf16 [tokens, heads, head_dim], sequence b = rows
     ``cu_q[b] .. cu_q[b + 1]``, already in the pages) over 4-bit pages; ``kv_lens[b]`` counts the keys its last token
-    sees. ``max_q_len`` / ``max_kv_len``: host integers that no sequence's new tokens / keys exceed. Rows of ``out`` behind the
-    last sequence are left as they are."""
+    sees. ``max_q_len`` / ``max_kv_len``: host integers that no sequence's new tokens / keys exceed; on the GPU a sequence that has
+    more is reported (``native.check_status``) and what lies behind them may be left out. Rows of ``out`` that belong to no sequence
+    are left as they are (without ``out`` they hold nothing)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if not q.is_cuda:
         o = ref.paged_attn_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, scale)

@@ -72,3 +72,34 @@ def test_value_sizes_that_change_along_a_context(D, new, lens, sizes):
     for t in (table, _wide(table, 40000, 16)):
         check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
     native.check_status("cuda")
+
+
+@pytest.mark.parametrize("width", [0, 40000])
+def test_new_tokens_of_a_call_that_announces_none_are_reported(width):
+    H, Hk, D = 4, 2, 128
+    kc, vc, table = filled([64, 40], Hk, D, 16, "cuda", seed=4)
+    t = _wide(table, width, 16) if width else table
+    q, ctx = _queries(9, H, D), torch.tensor([64, 40], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 3.0)
+    F.paged_attn_prefill_int4(q, kc, vc, t, _cu([5, 4]), ctx, 0, 64, out=out)
+    with pytest.raises(RuntimeError, match="status 2"):
+        native.check_status("cuda")
+    F.paged_attn_prefill_int4(q, kc, vc, t, _cu([0, 0]), ctx, 0, 64, out=out)       # none: nothing to report
+    native.check_status("cuda")
+    assert bool((out == 3.0).all())
+
+
+@pytest.mark.parametrize("new,lens,most_new,most", [
+    ([5, 4], [64, 40], 5, 63), ([5, 4], [64, 40], 4, 64), ([700], [700], 700, 699), ([700], [700], 699, 700), ([1000], [3000], 1000, 2999),
+    ([1000], [3000], 999, 3000)])
+@pytest.mark.parametrize("width", [0, 40000])
+def test_one_token_more_than_announced_is_reported(new, lens, most_new, most, width):
+    H, Hk, D = 4, 2, 128
+    kc, vc, table = filled(lens, Hk, D, 16, "cuda", seed=4)
+    t = _wide(table, width, 16) if width else table
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens))
+    native.check_status("cuda")
+    F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, most_new, most)
+    with pytest.raises(RuntimeError, match="status 2"):
+        native.check_status("cuda")
