@@ -335,5 +335,9 @@ def paged_attn_int4(q, k_cache, v_cache, block_table, cu_q, kv_lens, scale: floa
         hidden = hidden | ~kv4_places(block_table, page_size, k_cache.shape[0], pos, torch.full_like(pos, b))[3]
         p = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
         p = torch.where(hidden.all(-1)[:, None], torch.zeros_like(p), p)
-        out[a:e] = torch.einsum("hqk,khd->qhd", p, v).to(q.dtype)
+        bad = ~v.isfinite()                    # left out where they are not seen: a weight of zero would not do
+        o = torch.einsum("hqk,khd->qhd", p, v.masked_fill(bad, 0.0))
+        if bad.any():
+            o = o.masked_fill(torch.einsum("qk,khd->qhd", (~hidden).float(), bad.float()) > 0, math.nan)
+        out[a:e] = o.to(q.dtype)
     return out
