@@ -16,8 +16,8 @@
 // second sum a scalar per column and group in fp32. The tensor cores truncate what they add, and the codes are all
 // positive: over a long context that would drift. So every second token (the upper halves of the operand) enters as
 // -(p scale) (15 - c) + p (low + 15 scale): complementing costs one NOT per word, and the running sum stays near zero.
-// p_t scale_t is rounded to fp16 (2^-12 of each term); the running reference M is the maximum of the scores plus the
-// exponent of the chunk's values, so it fits whatever the values' size. Everything else is fp32. mma.sync rather than tcgen05:
+// p_t scale_t is rounded to fp16 (2^-11 of each term); the running reference M is the maximum of score plus exponent of the values
+// over the tokens, so it fits whatever the values' size. Everything else is fp32. mma.sync rather than tcgen05:
 // with 8 columns a 128-row tile would be filled to a sixteenth, and the codes would have to go through shared memory
 // once more.
 #include <cuda_fp16.h>
@@ -140,8 +140,14 @@ struct P4State {
   float o[NB][GR][4][4];                  // units of 2^-24 (even i) and 2^-20
   float z[NB][GR][2], m[NB][2], l[NB][2];
   uint32_t unseen;                        // bit 2 nb + c: the column has seen no score yet (its reference is 0)
-  bool fresh;                             // some column of the warp has seen none
 };
+
+// Exponent that values of magnitude `mag` enter the reference with. p is kept up to 2^8 (and 2^6 more until the reference moves) times
+// the inverse of the token's largest magnitude, which is at least 7 scales: p times a scale then stays below 2^13, and is exact to 2^-11
+// over 19 octaves below the reference. Bounded so that p, its sum and its product with any value stay within fp32.
+__device__ __forceinline__ float p4_exponent(float mag) {
+  return fminf(fmaxf(__uint_as_float(0x4B000000u | (__float_as_uint(mag) >> 23)) - (8388608.f + 127.f), -80.f), 112.f) - 8.f;
+}
 
 // One chunk: tile u (0, 1) at `at` + u * TILE_BYTES for K, HALF behind for V; tok0: its first token.
 // MASK: some token is not seen by some column (visible: those seen by any), or not held at all.
@@ -185,7 +191,7 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
           }
         }
   }
-  // ---- exponent of the chunk's values: one group of one token per thread and tile
+  // ---- largest exponent of the chunk's values, which decides whether the reference may have to move: one group of one token per thread and tile
   float mag = 0.f;
 #pragma unroll
   for (int u = 0; u < GR; ++u) {                  // (one group a token: the warp's halves take the two tiles)
@@ -199,11 +205,7 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
     }
     mag = fmax3(mag, use ? fabsf(top) : 0.f, use ? fabsf(kv4_low(p)) : 0.f);
   }
-  // p is kept up to 2^8 (and 2^6 more until the reference moves) times the inverse of the largest magnitude, which is at
-  // least 7 scales: p times a scale then stays below 2^13, and is exact to 2^-12 over 24 octaves below. Bounded so that p, its
-  // sum and its product with any value stay within fp32.
-  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(mag));
-  const float ev = fminf(fmaxf(__uint_as_float(0x4B000000u | (bits >> 23)) - (8388608.f + 127.f), -80.f), 112.f) - 8.f;
+  const float ev = p4_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mag))));
   // ---- online softmax: scores relative to the reference; it moves only when one of them passes it by 2^6
   float x[2][NB][2][2];                           // [tile][block][j][c]
   float top = -INFINITY;
@@ -239,15 +241,37 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < 2; ++j) top = fmax3(top, x[u][nb][j][0], x[u][nb][j][1]);
-  if (s.fresh || __any_sync(0xffffffffu, top + ev > 6.f)) {
+  if (__any_sync(0xffffffffu, s.unseen != 0u || top + ev > 6.f)) {
+    // where it moves to goes by every token's own score and exponent: with the chunk's exponent, one large token that a column
+    // hardly weighs or does not see took the others' products below what fp16 holds (8 x 32768 tokens: 49.6 -> 50.7 us for it)
+    float most[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) most[nb][0] = most[nb][1] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t w[2];
+        const uint32_t vp = smem_u32(at) + C::HALF + u * L::TILE_BYTES + L::OFF_PAIR + (8 * j + r) * L::PAIR;
+        if constexpr (GR == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(vp));
+        else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(vp));
+        float m = 0.f;
+#pragma unroll
+        for (int g = 0; g < GR; ++g) m = fmax3(m, fabsf(fmaf(15.f, kv4_scale(w[g]), kv4_low(w[g]))), fabsf(kv4_low(w[g])));
+        const float own = p4_exponent(m);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          most[nb][0] = fmaxf(most[nb][0], x[u][nb][j][0] + own);
+          most[nb][1] = fmaxf(most[nb][1], x[u][nb][j][1] + own);
+        }
+      }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float mx = fmaxf(fmax3(x[0][nb][0][c], x[0][nb][1][c], x[1][nb][0][c]), x[1][nb][1][c]);
+        float mx = most[nb][c];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        mx += ev;                                 // relative to the reference used so far
         const bool first = s.unseen >> (2 * nb + c) & 1u;
         // (by the column's own scores alone: what the others hold, a NaN say, does not reach its bits)
         if (first ? mx > -INFINITY : mx > 6.f) {
@@ -270,7 +294,6 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
           }
         }
       }
-    s.fresh = __any_sync(0xffffffffu, s.unseen != 0u);
   }
   // ---- weights p scale as the B operand (k = tokens, n = columns): transposed in blocks of eight by eight. Odd key rows
   // are the tokens that enter with the complement of their codes.
@@ -409,7 +432,6 @@ __device__ __forceinline__ void p4_queries(P4State<D, COLS>& s, const P4Args& a,
     }
   }
   s.unseen = (1u << (2 * NB)) - 1u;
-  s.fresh = true;
 }
 
 // The state's sums, complete over the warp: into `out` (whole) or as a part to w_acc [COLS][D] with references and row sums

@@ -103,3 +103,49 @@ def test_one_token_more_than_announced_is_reported(new, lens, most_new, most, wi
     F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, most_new, most)
     with pytest.raises(RuntimeError, match="status 2"):
         native.check_status("cuda")
+
+
+def _one_large(D, Hk, lens, at, size, score):
+    """Rows whose token ``at`` of every sequence has values ``size`` times larger and a score lower by ``score``."""
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    k[..., 0] = 0.0
+    first = 0
+    for n in lens:
+        if at < n:
+            v[first + at] = (v[first + at].float() * size).to(torch.bfloat16)
+            k[first + at, :, 0] = -score * math.sqrt(D) / 8
+        first += n
+    return k, v
+
+
+@pytest.mark.parametrize("size", [1e4, 1e9, 1e30])
+@pytest.mark.parametrize("D,lens,at", [(128, [300, 70], 20), (64, [300, 70], 65), (128, [3000, 33], 32)])
+def test_decode_beside_a_large_token_that_hardly_counts(D, lens, at, size):
+    H, Hk = 4, 2
+    k, v = _one_large(D, Hk, lens, at, size, 100.0)            # a weight of e^-100
+    kc, vc, table = _written(k, v, lens, Hk, D)
+    q = _queries(2, H, D)
+    q[..., 0] = 8.0
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = attention(q, kc, vc, table, [0, 1], [1, 1], lens, 1 / math.sqrt(D))
+    for t in (table, _wide(table, 40000, 16)):
+        check(F.paged_attn_decode_int4(q, kc, vc, t, ctx), *want)
+    native.check_status("cuda")
+
+
+@pytest.mark.parametrize("ks,vs", [(1.0, 1e9), (1.0, 1e30), (1e30, 1.0), (1e30, 1e30)])
+def test_a_few_queries_are_not_reached_by_a_large_token_behind_them(ks, vs):
+    H, Hk, D, lens, new = 4, 2, 128, [300, 70], [6, 5]
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    last = [299, 369]
+    small = _written(k, v, lens, Hk, D)
+    k[last], v[last] = (k[last].float() * ks).to(torch.bfloat16), (v[last].float() * vs).to(torch.bfloat16)
+    large = _written(k, v, lens, Hk, D)
+    rows = [r for r in range(sum(new)) if r not in (5, 10)]     # the others see neither
+    want = attention(q, *small, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    for width in (0, 40000):
+        t = _wide(large[2], width, 16) if width else large[2]
+        got = F.paged_attn_prefill_int4(q, large[0], large[1], t, cu, ctx, 6, 300)
+        check(got[rows], *(w[rows] for w in want))
+    native.check_status("cuda")
