@@ -326,7 +326,8 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
     km = fmaxf(km, s_max[0][w]);
     vm = fmaxf(vm, s_max[1][w]);
   }
-  const int ek = pf_exponent(km), ev = max(PF_EV_MIN, pf_exponent(vm));
+  // (values of zero must not raise the reference: with an exponent of 0 they took thirteen bits and more from the other tiles' p)
+  const int ek = pf_exponent(km), ev = vm > 0.f ? max(PF_EV_MIN, pf_exponent(vm)) : PF_EV_MIN;
   if (threadIdx.x == 0) {
     int absent = 0;
 #pragma unroll

@@ -149,3 +149,19 @@ def test_a_few_queries_are_not_reached_by_a_large_token_behind_them(ks, vs):
         got = F.paged_attn_prefill_int4(q, large[0], large[1], t, cu, ctx, 6, 300)
         check(got[rows], *(w[rows] for w in want))
     native.check_status("cuda")
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-6])
+@pytest.mark.parametrize("new,lens", [([700, 300], [900, 700]), ([2500], [2500]), ([1000], [3000]), ([1, 1], [3000, 700])])
+def test_128_tokens_whose_values_are_zero(new, lens, size):
+    H, Hk, D = 4, 2, 128
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    v = v.float() * size
+    for first in [0, lens[0]] if len(lens) > 1 else [0]:
+        v[first + 256:first + 384] = 0.0
+    kc, vc, table = _written(k, v, lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    for t in (table, _wide(table, 40000, 16)):
+        check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
+    native.check_status("cuda")
