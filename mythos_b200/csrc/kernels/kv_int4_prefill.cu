@@ -16,6 +16,9 @@
 //     is taken back to is sum 2^(score - M), between 2^-113 and 2^116 a key for ev of -110 to 113: it is kept in units of 2^10 (units of the
 //     first tile's ev overflowed where later values were 2^130 times as large). Values below 2^-124 lose bits, and the weights of tiles
 //     whose values are less than 2^-120 of another tile's leave the sum.
+// Tokens of a tile whose magnitudes lie more than 2^8 apart get exponents of their own (PF_SPREAD), so that a large token takes no
+// bits from the others for the queries that give it no weight or do not see it: the softmax then adds every key's own to its score
+// first. (That the kernel can do so costs 2048 tokens over 6144 256 -> 260 us, 6 ragged prompts of up to 700 21.0 -> 22.3.)
 // The matrix product multiplies masked probabilities of zero by whatever the value rows hold, so nothing that is not
 // finite goes there: tokens behind a sequence's end are zeros, and a token with a scale that is not finite gets values of
 // zero and NaN keys, which reach the queries that see it through their scores, and no others.
@@ -50,8 +53,11 @@ __device__ __forceinline__ int pf_exponent(float m) {
   return max(-126, min(113, e));
 }
 constexpr int PF_EV_MIN = -110;   // of a tile of values
-constexpr float PF_SUM_UNIT = 0x1p10f;      // of a row sum
+constexpr int PF_SPREAD = 8;      // octaves between the tokens of a tile that share an exponent: p keeps 2^-17 of the largest term
+constexpr float PF_SUM_UNIT = 0x1p10f, PF_SUM_LOG = 10.f;      // of a row sum
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
+// Of values: zeros must not raise the reference (with an exponent of 0 they took thirteen bits and more from the other tiles' p).
+__device__ __forceinline__ int pf_value_exponent(float m) { return m > 0.f ? max(PF_EV_MIN, pf_exponent(m)) : PF_EV_MIN; }
 __device__ __forceinline__ uint32_t pf_half2(float a, float b) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
@@ -163,7 +169,8 @@ struct PfExpand {
   __half* v;
   __half* qh;           // [total_q, heads, D]
   float* q_factor;      // [total_q, heads]: 2^eq
-  int* exponents;       // [batch * kv_heads, tiles]: ek in the low byte, ev in the high half; between them, a bit per 16 tokens that have no page
+  int* exponents;       // [batch * kv_heads, tiles]: from the low byte on ek, a bit per 16 tokens that have no page, ev, 1 where tokens have their own
+  int16_t* own;         // [batch * kv_heads, tiles, 128]: there, ek and ev of every token
   int kv_heads, heads, tiles, kv_blocks, q_blocks, q_rows;     // q_rows: total_q * heads
   Kv4Div by_heads;
   int pairs;
@@ -275,7 +282,8 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
   }
   __shared__ uint32_t s_pair[2][PF_TILE][L::GROUPS];
   __shared__ int s_tile[8];
-  __shared__ float s_max[2][PF_EXPAND / 32];
+  __shared__ uint32_t s_ext[4][PF_EXPAND / 32];       // largest magnitude of K and V, smallest that is not zero
+  __shared__ int8_t s_own[2][PF_TILE];
   const int j = blockIdx.x % a.tiles, bh = blockIdx.x / a.tiles, b = bh / a.kv_heads, head = bh % a.kv_heads;
   const int len = a.kv_lens[b], n0 = j * PF_TILE;
   if (n0 >= len) return;
@@ -289,8 +297,9 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
   }
   __syncthreads();
   // pairs of both tensors; the largest magnitude a group can stand for lies at one of its ends
-  float km = 0.f, vm = 0.f;
-  for (int i = threadIdx.x; i < PF_TILE * L::GROUPS; i += PF_EXPAND) {
+  static_assert(PF_TILE * L::GROUPS <= PF_EXPAND && PF_TILE * L::GROUPS % 32 == 0, "a thread holds one group at most, and warps go together");
+  float km = 0.f, vm = 0.f;            // of the thread's token
+  if (const int i = threadIdx.x; i < PF_TILE * L::GROUPS) {
     const int n = i / L::GROUPS, g = i % L::GROUPS, tile = s_tile[n >> 4];
     uint32_t kp = 0u, vp = 0u;
     if (tile >= 0 && n0 + n < len) {
@@ -310,31 +319,47 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
     }
     s_pair[0][n][g] = kp;
     s_pair[1][n][g] = vp;
-    if (kv4_finite(kp)) km = fmaxf(km, fmaxf(fabsf(kv4_low(kp)), fabsf(fmaf(15.f, kv4_scale(kp), kv4_low(kp)))));
-    vm = fmaxf(vm, fmaxf(fabsf(kv4_low(vp)), fabsf(fmaf(15.f, kv4_scale(vp), kv4_low(vp)))));
+    if (kv4_finite(kp)) km = fmaxf(fabsf(kv4_low(kp)), fabsf(fmaf(15.f, kv4_scale(kp), kv4_low(kp))));
+    vm = fmaxf(fabsf(kv4_low(vp)), fabsf(fmaf(15.f, kv4_scale(vp), kv4_low(vp))));
+    if constexpr (L::GROUPS == 2) {
+      km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, 1));
+      vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
+    }
+    if (g == 0) {
+      s_own[0][n] = (int8_t)pf_exponent(km);
+      s_own[1][n] = (int8_t)pf_value_exponent(vm);
+    }
   }
-  km = warp_max(km);
-  vm = warp_max(vm);
-  if ((threadIdx.x & 31) == 0) {
-    s_max[0][threadIdx.x >> 5] = km;
-    s_max[1][threadIdx.x >> 5] = vm;
+  {                                    // (as integers: they are not negative)
+    const uint32_t kb = __float_as_uint(km), vb = __float_as_uint(vm);
+    const uint32_t k1 = __reduce_max_sync(0xffffffffu, kb), v1 = __reduce_max_sync(0xffffffffu, vb);
+    const uint32_t k0 = __reduce_min_sync(0xffffffffu, kb ? kb : ~0u), v0 = __reduce_min_sync(0xffffffffu, vb ? vb : ~0u);
+    if ((threadIdx.x & 31) == 0) {
+      s_ext[0][threadIdx.x >> 5] = k1;
+      s_ext[1][threadIdx.x >> 5] = v1;
+      s_ext[2][threadIdx.x >> 5] = k0;
+      s_ext[3][threadIdx.x >> 5] = v0;
+    }
   }
   __syncthreads();
-  km = vm = 0.f;
+  uint32_t k1 = 0u, v1 = 0u, k0 = ~0u, v0 = ~0u;
 #pragma unroll
   for (int w = 0; w < PF_EXPAND / 32; ++w) {
-    km = fmaxf(km, s_max[0][w]);
-    vm = fmaxf(vm, s_max[1][w]);
+    k1 = max(k1, s_ext[0][w]);
+    v1 = max(v1, s_ext[1][w]);
+    k0 = min(k0, s_ext[2][w]);
+    v0 = min(v0, s_ext[3][w]);
   }
-  // (values of zero must not raise the reference: with an exponent of 0 they took thirteen bits and more from the other tiles' p)
-  const int ek = pf_exponent(km), ev = vm > 0.f ? max(PF_EV_MIN, pf_exponent(vm)) : PF_EV_MIN;
+  const int ek = pf_exponent(__uint_as_float(k1)), ev = pf_value_exponent(__uint_as_float(v1));
+  const bool apart = (int)(k1 >> 23) - (int)(min(k0, k1) >> 23) > PF_SPREAD || (int)(v1 >> 23) - (int)(min(v0, v1) >> 23) > PF_SPREAD;
   if (threadIdx.x == 0) {
     int absent = 0;
 #pragma unroll
     for (int u = 0; u < 8; ++u) absent |= (s_tile[u] < 0 && n0 + 16 * u < len ? 1 : 0) << u;
-    a.exponents[blockIdx.x] = (ek & 0xFF) | absent << 8 | ev << 16;
+    a.exponents[blockIdx.x] = (ek & 0xFF) | absent << 8 | (ev & 0xFF) << 16 | (apart ? 1 : 0) << 24;
   }
-  const float ik = pf_pow2(-ek), iv = pf_pow2(-ev);
+  if (apart && threadIdx.x < PF_TILE)
+    a.own[(long long)blockIdx.x * PF_TILE + threadIdx.x] = (int16_t)((s_own[0][threadIdx.x] & 0xFF) | s_own[1][threadIdx.x] * 256);
   const long long out = ((long long)bh * a.tiles + j) * PF_TILE * D;
 #pragma unroll 4
   for (int i = threadIdx.x; i < PF_TILE * WORDS; i += PF_EXPAND) {
@@ -346,8 +371,8 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
       kw = kv4_unrotate(*reinterpret_cast<const uint32_t*>(a.k_cache + at + kv4_key_word<D>(n & 15, g, u)));
       vw = *reinterpret_cast<const uint32_t*>(a.v_cache + at + kv4_value_word<D>(n & 15, g, u));
     }
-    *reinterpret_cast<uint4*>(a.k + out + (long long)i * 8) = pf_expand8(kw, kp, ik);
-    *reinterpret_cast<uint4*>(a.v + out + (long long)i * 8) = pf_expand8(vw, vp, iv);
+    *reinterpret_cast<uint4*>(a.k + out + (long long)i * 8) = pf_expand8(kw, kp, pf_pow2(apart ? -s_own[0][n] : -ek));
+    *reinterpret_cast<uint4*>(a.v + out + (long long)i * 8) = pf_expand8(vw, vp, pf_pow2(apart ? -s_own[1][n] : -ev));
   }
 }
 
@@ -364,7 +389,8 @@ struct PfCfg {
   static constexpr int OFF_V = OFF_K + KS * TILE_BYTES;
   static constexpr int OFF_BAR = OFF_V + VS * TILE_BYTES;
   static constexpr int NUM_BARS = 4 + 2 * KS + 2 * VS + 8;
-  static constexpr int SMEM_BYTES = OFF_BAR + NUM_BARS * 8 + 16 + 1024;
+  static constexpr int OFF_SUM = OFF_BAR + NUM_BARS * 8 + 16;          // a float per softmax thread
+  static constexpr int SMEM_BYTES = OFF_SUM + 2 * PF_TILE * 4 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
   static constexpr int COL_S = 0;     // S_t at t * 128 (P_t over its first 64 columns)
   static constexpr int COL_O = 256;   // O_t at 256 + t * D
@@ -375,6 +401,7 @@ struct PfArgs {
   PfPlan plan;
   const float* q_factor;
   const int* exponents;
+  const int16_t* own;
   __nv_bfloat16* out;
   float* parts;         // [stretches][2 slots][2 tiles]: see pf_part_floats
   long long o_stride;
@@ -439,6 +466,40 @@ __device__ __forceinline__ void pf_wait_expansion() { asm volatile("griddepcontr
 
 __host__ __device__ constexpr uint32_t pf_idesc(int M, int N, bool b_mn_major) {   // fp16 operands, fp32 accumulator
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// A row's scores over a tile whose tokens have exponents of their own: in tensor memory they are replaced by score + ev of the token - ev of
+// the tile (e), as they enter the softmax. The row sum goes without the tokens' exponents: its logarithm is returned, minus infinity where
+// nothing is seen; it is formed from the scores as they were rounded there, and rounded as scores of its size are. Four at a time and ahead of
+// everything else, since the loop around it has to carry the code (32 at a time, with the sum between the halves of p: 6 ragged prompts of up to
+// 700 tokens without such tiles took 22.5 us, 22.3 this way).
+__device__ __forceinline__ float pf_own_scores(uint32_t t_s, const int16_t* own, float row_f, int limit, uint32_t absent, int e) {
+  float sum = 0.f, top = -1e30f;
+#pragma unroll 1
+  for (int c = 0; c < PF_TILE; c += 4) {
+    uint32_t x[4];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(t_s + c) : "memory");
+    const uint2 w = *reinterpret_cast<const uint2*>(own + c);
+    tmem_ld_wait();
+    float y[4];
+    const float before = top;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int both = (int16_t)((i < 2 ? w.x : w.y) >> (16 * (i & 1)));          // ek, ev
+      const bool seen = c + i <= limit && !(absent >> (c >> 4) & 1u);
+      const float more = (float)((both >> 8) - e);
+      const float z = seen ? fmaf(__uint_as_float(x[i]), fmaxf(row_f * pf_pow2((signed char)both), 1e-37f), more) : -INFINITY;
+      x[i] = __float_as_uint(z);
+      y[i] = z - more;
+      top = fmaxf(top, y[i]);
+    }
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t_s + c), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+    sum *= fast_exp2(before - top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += fast_exp2(y[i] - top);
+  }
+  tmem_st_wait();
+  return top + __log2f(sum);
 }
 
 template <int D>
@@ -644,6 +705,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem_base + Cfg::COL_S + t * 128 + lane_sel;
     const uint32_t t_o = tmem_base + Cfg::COL_O + t * D + lane_sel;
+    float* own_sum = reinterpret_cast<float*>(smem + Cfg::OFF_SUM) - PF_TILE;     // (indexed by threads 128 ..; a register for it would spill)
     const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.o_stride * 2)) & 31) == 0;
     uint32_t n_s = 0, n_o = 0;
     bool ok = true;
@@ -664,11 +726,12 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       float m_ref = -INFINITY, l = 0.f;       // (no key seen yet)
       int e_next = end > j0 ? ex[j0] : 0;
       for (int j = j0; j < end && ok; ++j) {
-        const int ek = (signed char)e_next, e = e_next >> 16;
+        const int ek = (signed char)e_next, e = (signed char)(e_next >> 16);
+        const bool apart = e_next >> 24;      // (for the whole CTA)
         const uint32_t absent = (uint32_t)e_next >> 8 & 0xFFu;     // sixteens of keys without a page: no query sees them
         if (j + 1 < end) e_next = ex[j + 1];
         // (never zero: a masked score of minus infinity has to stay one)
-        const float sc = fmaxf(row_f * pf_pow2(ek), 1e-37f), ev = (float)e;
+        const float sc = apart ? 1.f : fmaxf(row_f * pf_pow2(ek), 1e-37f), ev = (float)e;
         ok = mbar_wait(&s_full[t], n_s & 1, abort_flag, status, 102);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -689,6 +752,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
               if (absent >> (i >> 4) & 1u) s[i] = -INFINITY;
           }
         };
+        if (apart) own_sum[threadIdx.x] = pf_own_scores(t_s, a.own + (ex + j - a.exponents) * PF_TILE, row_f, limit - kv0, absent, e);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, sr[c]);
         tmem_ld_wait();
@@ -761,7 +825,10 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         float rs[8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
-        l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(-e) * (1.f / PF_SUM_UNIT);
+        if (apart) {
+          const float own = own_sum[threadIdx.x];
+          l += own == -INFINITY ? 0.f : fast_exp2(own - m_ref - PF_SUM_LOG);       // (nothing seen: the reference may be infinite)
+        } else l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(-e) * (1.f / PF_SUM_UNIT);
       }
       if (!ok) break;
       if (end > j0) {
@@ -884,7 +951,7 @@ struct PfSizes {
   int slice;                            // sequences at a time; the rest is for one slice
   bool whole;
   long long kv_tiles, pairs, steps;     // steps: places on the line, at most
-  long long kv, q, factor, exponents, plan, parts, total;    // bytes, each a multiple of 256
+  long long kv, q, factor, exponents, own, plan, parts, total;    // bytes, each a multiple of 256
 };
 PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int kv_heads, int D) {
   const auto align = [](long long n) { return (n + 255) / 256 * 256; };
@@ -906,9 +973,10 @@ PfSizes pf_sizes(int batch, int total_q, int max_q, int max_kv, int heads, int k
   z.q = align((long long)total_q * heads * D * 2);
   z.factor = align((long long)total_q * heads * 4);
   z.exponents = align(z.kv_tiles * 4);
+  z.own = align(z.kv_tiles * PF_TILE * 2);
   z.plan = align((4 + 4LL * z.ctas) * 4);
   z.parts = z.whole ? 0 : align(4LL * z.ctas * PF_TILE * (D + 2) * 4);
-  z.total = 2 * z.kv + z.q + z.factor + z.exponents + z.plan + z.parts;
+  z.total = 2 * z.kv + z.q + z.factor + z.exponents + z.own + z.plan + z.parts;
   return z;
 }
 
@@ -937,6 +1005,7 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
   x.qh = (__half*)take(z.q);
   x.q_factor = (float*)take(z.factor);
   x.exponents = (int*)take(z.exponents);
+  x.own = (int16_t*)take(z.own);
   x.plan = {(int*)take(z.plan)};
   float* parts = (float*)take(z.parts);
   x.kv_heads = c.kv_heads;
@@ -986,7 +1055,7 @@ void prompt_int4(const KvInt4Cache& c, const void* q, long long q_stride, const 
     uint32_t kb[3] = {64, PF_TILE, 1};
     const CUtensorMap tk = make_tensor_map(x.k, TmaDType::BF16, 3, kd, ks, kb, true);
     const CUtensorMap tv = make_tensor_map(x.v, TmaDType::BF16, 3, kd, ks, kb, true);
-    PfArgs a{x.line, x.plan, x.q_factor, x.exponents, (__nv_bfloat16*)out, parts, o_stride, heads, heads / c.kv_heads, total_q,
+    PfArgs a{x.line, x.plan, x.q_factor, x.exponents, x.own, (__nv_bfloat16*)out, parts, o_stride, heads, heads / c.kv_heads, total_q,
              scale * 1.4426950408889634f, status, s.whole, kv4_div(s.units)};
     const auto go = [&](auto kern, auto merge, int smem) {
       MB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));

@@ -165,3 +165,65 @@ def test_128_tokens_whose_values_are_zero(new, lens, size):
     for t in (table, _wide(table, 40000, 16)):
         check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
     native.check_status("cuda")
+
+
+@pytest.mark.parametrize("ks,vs", [(1.0, 1e4), (1.0, 1e9), (1.0, 1e30), (1e4, 1.0), (1e30, 1.0), (1e30, 1e30)])
+@pytest.mark.parametrize("D,new,lens", [(128, [700, 300], [900, 700]), (64, [2500], [2500]), (128, [1000], [3000])])
+def test_a_prompt_is_not_reached_by_a_large_token_behind_it(D, new, lens, ks, vs):
+    H, Hk = 4, 2
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    at = lens[0] - 200                                          # of the first sequence; its last 200 queries see the token
+    k[at], v[at] = (k[at].float() * ks).to(torch.bfloat16), (v[at].float() * vs).to(torch.bfloat16)
+    kc, vc, table = _written(k, v, lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    got = F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens))
+    # (a key of 1e30 gives scores whose difference from others no 32-bit number holds: what sees it is only finite)
+    rows = [r for r in range(sum(new)) if not new[0] - 200 <= r < new[0]] if ks > 1e4 else list(range(sum(new)))
+    assert bool(got.isfinite().all())
+    check(got[rows], *(w[rows] for w in want))
+    native.check_status("cuda")
+
+
+@pytest.mark.parametrize("size", [1e4, 1e9, 1e30])
+@pytest.mark.parametrize("D,new,lens", [(128, [700, 300], [900, 700]), (64, [2500], [2500]), (128, [1000], [3000])])
+def test_a_prompt_beside_a_large_token_that_hardly_counts(D, new, lens, size):
+    H, Hk = 4, 2
+    k, v = _one_large(D, Hk, lens, 20, size, 100.0)
+    kc, vc, table = _written(k, v, lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q[..., 0] = 8.0
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    check(F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens)), *want)
+    native.check_status("cuda")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_tokens_of_every_size_side_by_side(D):
+    H, Hk, new, lens = 4, 2, [900, 800], [1500, 800]
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    size = torch.exp2(torch.randint(-40, 41, (sum(lens), 1, 1), generator=torch.Generator().manual_seed(2)).float()).cuda()
+    kc, vc, table = _written(k * size.clamp(1e-6, 1.0), v.float() * size.flip(0), lens, Hk, D)
+    for t in range(0, 12, 3):
+        table[0, 8 * t + 3] = -1                                # and gaps among them
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens))
+    with pytest.raises(RuntimeError, match="status 2"):
+        native.check_status("cuda")
+    check(got, *attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D)))
+
+
+def test_large_scores_beside_a_token_of_another_size():
+    """Scores around 1e5 are off by 2^-7 in 32 bits; weights and their sum have to be off together."""
+    H, Hk, D, lens = 4, 2, 128, [900]
+    k, v = random_rows(900, Hk, D, 6, "cuda")
+    k[..., 0] = 0.0
+    k[::7, :, 0] = 10.0                                         # every seventh key far above the others
+    v = v.float()
+    v[5::128] *= 1e6
+    kc, vc, table = _written(k, v, lens, Hk, D)
+    q = torch.zeros(700, H, D, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1e5
+    want = attention(q, kc, vc, table, [0], [700], lens, 1 / math.sqrt(D))
+    check(F.paged_attn_prefill_int4(q, kc, vc, table, _cu([700]), torch.tensor(lens, dtype=torch.int32, device="cuda"), 700, 900), *want)
+    native.check_status("cuda")
