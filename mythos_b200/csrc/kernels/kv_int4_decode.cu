@@ -275,14 +275,14 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
         const bool first = s.unseen >> (2 * nb + c) & 1u;
         // (by the column's own scores alone: what the others hold, a NaN say, does not reach its bits)
         if (first ? mx > -INFINITY : mx > 6.f) {
-          const float alpha = first ? 0.f : fast_exp2(-mx);
+          const float half = first ? 0.f : fast_exp2(-0.5f * mx), alpha = half * half;
           s.unseen &= ~(1u << (2 * nb + c));
           s.m[nb][c] += mx;
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int j = 0; j < 2; ++j) x[u][nb][j][c] -= mx;
-          s.l[nb][c] *= alpha;
+          s.l[nb][c] = s.l[nb][c] * half * half;  // (the sum may outlast what the products are: exponents of values are in them only)
 #pragma unroll
           for (int g = 0; g < GR; ++g) {
             s.z[nb][g][c] *= alpha;
@@ -561,7 +561,7 @@ __device__ __forceinline__ void p4_run(P4State<D, COLS>& s, P4Feed<D, COLS>& fee
 }
 
 // Joins the parts of a unit that shared memory holds (bits of `parts`), column c, values d .. d + 3: sums, and the column's
-// reference and row sum.
+// reference and row sum. References may lie further apart than 2^126 where values do: row sums are scaled in two steps, here and below.
 template <int D, int COLS, class At>
 __device__ __forceinline__ float4 p4_join(uint32_t parts, const float* ml, const At& at, int c, int d, float& M, float& l) {
   M = -INFINITY;
@@ -572,9 +572,9 @@ __device__ __forceinline__ float4 p4_join(uint32_t parts, const float* ml, const
     const int k = __ffs(w) - 1;
     const float lk = ml[(2 * k + 1) * COLS + c];
     if (lk == 0.f) continue;                      // nothing seen (a NaN is not nothing)
-    const float e = fast_exp2(ml[2 * k * COLS + c] - M);
+    const float half = fast_exp2(0.5f * (ml[2 * k * COLS + c] - M)), e = half * half;
     const float4 v = *reinterpret_cast<const float4*>(at(k) + c * D + d);
-    l = fmaf(e, lk, l);
+    l = fmaf(half, half * lk, l);
     acc.x = fmaf(e, v.x, acc.x);
     acc.y = fmaf(e, v.y, acc.y);
     acc.z = fmaf(e, v.z, acc.z);
@@ -675,12 +675,13 @@ paged_attn_int4_cluster_kernel(const __grid_constant__ P4Args a) {
       const float m = p4_ld_cluster(p4_mapa(m_at, p)), lp = p4_ld_cluster(p4_mapa(l_at, p));
       const float4 v = p4_ld_cluster4(p4_mapa(v_at, p));
       if (lp == 0.f) continue;
-      const float Mn = fmaxf(M, m), e0 = M == -INFINITY ? 0.f : fast_exp2(M - Mn), e1 = fast_exp2(m - Mn);
+      const float Mn = fmaxf(M, m), h0 = M == -INFINITY ? 0.f : fast_exp2(0.5f * (M - Mn)), h1 = fast_exp2(0.5f * (m - Mn));
+      const float e0 = h0 * h0, e1 = h1 * h1;
       acc.x = fmaf(e1, v.x, acc.x * e0);
       acc.y = fmaf(e1, v.y, acc.y * e0);
       acc.z = fmaf(e1, v.z, acc.z * e0);
       acc.w = fmaf(e1, v.w, acc.w * e0);
-      l = fmaf(e1, lp, l * e0);
+      l = fmaf(h1, h1 * lp, h0 * (h0 * l));
       M = Mn;
     }
     p4_store(u.out(a, D, c, d), acc, l);
@@ -939,16 +940,17 @@ p4_merge_kernel(const __grid_constant__ P4Args a, const float* __restrict__ scra
       if (s_lw[p][c] != 0.f) Mn = fmaxf(Mn, s_w[p][c]);          // nothing seen is left out, a NaN is not
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, o));
-    const float e = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
-    acc.x *= e; acc.y *= e; acc.z *= e; acc.w *= e; l *= e;
+    const float half = M == -INFINITY ? 0.f : fast_exp2(0.5f * (M - Mn)), e = half * half;
+    acc.x *= e; acc.y *= e; acc.z *= e; acc.w *= e;
+    l = l * half * half;
     M = Mn;
     if (c < u.n_cols) {
 #pragma unroll 8
       for (int p = slice; p < parts; p += SLICES) {
         const float lw = s_lw[p][c];
         const float4 v = lw != 0.f ? *reinterpret_cast<const float4*>(scratch + s_at[p] + c * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float w = lw != 0.f ? fast_exp2(s_w[p][c] - M) : 0.f;
-        l = fmaf(w, lw, l);
+        const float half = lw != 0.f ? fast_exp2(0.5f * (s_w[p][c] - M)) : 0.f, w = half * half;
+        l = fmaf(half, half * lw, l);
         acc.x = fmaf(w, v.x, acc.x);
         acc.y = fmaf(w, v.y, acc.y);
         acc.z = fmaf(w, v.z, acc.z);

@@ -14,8 +14,7 @@
 //   * a tile of values is divided by 2^ev, and the probabilities of the step are multiplied by it: the running reference
 //     M is the maximum of score + ev, so that p 2^(ev - M) stays within fp16, and the row sum is taken back by 2^-ev. What it
 //     is taken back to is sum 2^(score - M), between 2^-113 and 2^116 a key for ev of -110 to 113: it is kept in units of 2^10 (units of the
-//     first tile's ev overflowed where later values were 2^130 times as large). Values below 2^-124 lose bits, and the weights of tiles
-//     whose values are less than 2^-120 of another tile's leave the sum.
+//     first tile's ev overflowed where later values were 2^130 times as large). Values below 2^-124 lose bits.
 // Tokens of a tile whose magnitudes lie more than 2^8 apart get exponents of their own (PF_SPREAD), so that a large token takes no
 // bits from the others for the queries that give it no weight or do not see it: the softmax then adds every key's own to its score
 // first. (That the kernel can do so costs 2048 tokens over 6144 256 -> 260 us, 6 ragged prompts of up to 700 21.0 -> 22.3.)
@@ -54,6 +53,9 @@ __device__ __forceinline__ int pf_exponent(float m) {
 }
 constexpr int PF_EV_MIN = -110;   // of a tile of values
 constexpr int PF_SPREAD = 8;      // octaves between the tokens of a tile that share an exponent: p keeps 2^-17 of the largest term
+// Octaves below the reference up to which the row sum is taken from p. What lies further below counts for nothing in the products, but does in
+// the sum where it is the values that are small.
+constexpr float PF_FAR = 100.f;
 constexpr float PF_SUM_UNIT = 0x1p10f, PF_SUM_LOG = 10.f;      // of a row sum
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
 // Of values: zeros must not raise the reference (with an exponent of 0 they took thirteen bits and more from the other tiles' p).
@@ -473,13 +475,16 @@ __host__ __device__ constexpr uint32_t pf_idesc(int M, int N, bool b_mn_major) {
 // nothing is seen; it is formed from the scores as they were rounded there, and rounded as scores of its size are. Four at a time and ahead of
 // everything else, since the loop around it has to carry the code (32 at a time, with the sum between the halves of p: 6 ragged prompts of up to
 // 700 tokens without such tiles took 22.5 us, 22.3 this way).
+// Otherwise (OWN false) nothing is replaced, and row_f is the factor of the scores as they stand there.
+template <bool OWN>
 __device__ __forceinline__ float pf_own_scores(uint32_t t_s, const int16_t* own, float row_f, int limit, uint32_t absent, int e) {
   float sum = 0.f, top = -1e30f;
 #pragma unroll 1
   for (int c = 0; c < PF_TILE; c += 4) {
     uint32_t x[4];
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(t_s + c) : "memory");
-    const uint2 w = *reinterpret_cast<const uint2*>(own + c);
+    uint2 w = make_uint2(0u, 0u);
+    if constexpr (OWN) w = *reinterpret_cast<const uint2*>(own + c);
     tmem_ld_wait();
     float y[4];
     const float before = top;
@@ -487,18 +492,23 @@ __device__ __forceinline__ float pf_own_scores(uint32_t t_s, const int16_t* own,
     for (int i = 0; i < 4; ++i) {
       const int both = (int16_t)((i < 2 ? w.x : w.y) >> (16 * (i & 1)));          // ek, ev
       const bool seen = c + i <= limit && !(absent >> (c >> 4) & 1u);
-      const float more = (float)((both >> 8) - e);
-      const float z = seen ? fmaf(__uint_as_float(x[i]), fmaxf(row_f * pf_pow2((signed char)both), 1e-37f), more) : -INFINITY;
-      x[i] = __float_as_uint(z);
-      y[i] = z - more;
+      if constexpr (OWN) {
+        const float more = (float)((both >> 8) - e);
+        const float z = seen ? fmaf(__uint_as_float(x[i]), fmaxf(row_f * pf_pow2((signed char)both), 1e-37f), more) : -INFINITY;
+        x[i] = __float_as_uint(z);
+        y[i] = z - more;
+      } else {
+        y[i] = seen ? __uint_as_float(x[i]) * row_f : -INFINITY;
+      }
       top = fmaxf(top, y[i]);
     }
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t_s + c), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+    if constexpr (OWN)
+      asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t_s + c), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
     sum *= fast_exp2(before - top);
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum += fast_exp2(y[i] - top);
   }
-  tmem_st_wait();
+  if constexpr (OWN) tmem_st_wait();
   return top + __log2f(sum);
 }
 
@@ -722,12 +732,13 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const bool live = tok < it.q_len && (unsigned)row < (unsigned)a.total_q;
       const int limit = min(it.kv_len - 1, it.q_off + tok);
       const int* ex = a.exponents + (long long)(it.b * kv_heads + a.line.by_share(c.of_unit)) * a.line.tiles;
-      const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 1.f;
+      const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 0.f;      // (other rows: no spread)
       float m_ref = -INFINITY, l = 0.f;       // (no key seen yet)
       int e_next = end > j0 ? ex[j0] : 0;
       for (int j = j0; j < end && ok; ++j) {
         const int ek = (signed char)e_next, e = (signed char)(e_next >> 16);
         const bool apart = e_next >> 24;      // (for the whole CTA)
+        bool by_itself = apart;               // the row's sum over the tile lies in shared memory
         const uint32_t absent = (uint32_t)e_next >> 8 & 0xFFu;     // sixteens of keys without a page: no query sees them
         if (j + 1 < end) e_next = ex[j + 1];
         // (never zero: a masked score of minus infinity has to stay one)
@@ -752,7 +763,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
               if (absent >> (i >> 4) & 1u) s[i] = -INFINITY;
           }
         };
-        if (apart) own_sum[threadIdx.x] = pf_own_scores(t_s, a.own + (ex + j - a.exponents) * PF_TILE, row_f, limit - kv0, absent, e);
+        if (apart) own_sum[threadIdx.x] = pf_own_scores<true>(t_s, a.own + (ex + j - a.exponents) * PF_TILE, row_f, limit - kv0, absent, e);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, sr[c]);
         tmem_ld_wait();
@@ -794,12 +805,13 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sc, ev);
         // p up to 2^6 until the reference moves. The first score that is seen always sets it, in whatever tile it stands: a
         // reference of zero kept from a tile without a visible key left p as 2^(score + ev), which fp16 may not hold.
-        const bool need = m_new - m_ref > 6.f;
-        if (j == j0 || __any_sync(0xffffffffu, need)) {
-          const float alpha = need ? fast_exp2(m_ref - m_new) : 1.f;
+        const float up = m_new - m_ref;
+        const bool need = up > 6.f, far = up < -PF_FAR && up > -INFINITY;
+        if (j == j0 || __any_sync(0xffffffffu, need || far)) {
+          const float half = need ? fast_exp2(0.5f * (m_ref - m_new)) : 1.f, alpha = half * half;
           if (need) m_ref = m_new;
           if (j > j0) {
-            l *= alpha;
+            l = l * half * half;             // (the sum may outlast what the products are: exponents of values are in them only)
             // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):
             // O_t is quiescent until this warpgroup arrives on p_full, so a rescale can happen right here.
 #pragma unroll 1
@@ -817,6 +829,11 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             tmem_ld_wait();
             hide(0, 64);
           }
+          if (!apart && __any_sync(0xffffffffu, far)) {
+            const float own = pf_own_scores<false>(t_s, nullptr, sc, limit - kv0, absent, 0);
+            by_itself = far;
+            if (far) own_sum[threadIdx.x] = own;
+          }
           exponentials(0);
         }
         publish(0);
@@ -825,7 +842,7 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         float rs[8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
-        if (apart) {
+        if (by_itself) {
           const float own = own_sum[threadIdx.x];
           l += own == -INFINITY ? 0.f : fast_exp2(own - m_ref - PF_SUM_LOG);       // (nothing seen: the reference may be infinite)
         } else l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(-e) * (1.f / PF_SUM_UNIT);
@@ -918,9 +935,9 @@ pf_merge_kernel(const __grid_constant__ PfArgs a) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) v[k] = *reinterpret_cast<const float4*>(p + ((v0 + k) * PF_TILE + r) * 4);
     if (lc == 0.f) continue;                      // nothing seen (a NaN is not nothing)
-    const float Mn = fmaxf(M, m), w0 = l == 0.f ? 0.f : fast_exp2(M - Mn), w = fast_exp2(m - Mn);
+    const float Mn = fmaxf(M, m), h0 = l == 0.f ? 0.f : fast_exp2(0.5f * (M - Mn)), h = fast_exp2(0.5f * (m - Mn)), w0 = h0 * h0, w = h * h;
     M = Mn;
-    l = fmaf(w, lc, l * w0);
+    l = fmaf(h, h * lc, h0 * (h0 * l));
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       acc[k].x = fmaf(w, v[k].x, acc[k].x * w0);

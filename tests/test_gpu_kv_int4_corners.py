@@ -227,3 +227,22 @@ def test_large_scores_beside_a_token_of_another_size():
     want = attention(q, kc, vc, table, [0], [700], lens, 1 / math.sqrt(D))
     check(F.paged_attn_prefill_int4(q, kc, vc, table, _cu([700]), torch.tensor(lens, dtype=torch.int32, device="cuda"), 700, 900), *want)
     native.check_status("cuda")
+
+
+# further apart than 32-bit numbers go below one
+FAR = [[1e-35, 1e10], [1e30, 1e-35], [1e-35, 1e30, 1e-30, 1e20, 1.0], [1e-30, 0.0, 1e25, 1e-30]]
+
+
+@pytest.mark.parametrize("sizes", FAR)
+@pytest.mark.parametrize("new,lens", [([700, 300], [900, 700]), ([2500], [2500]), ([1000], [3000]), ([1, 1], [3000, 700]), ([6, 2], [600, 300])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_sizes_further_apart_than_32_bits_go(D, new, lens, sizes):
+    H, Hk = 4, 2
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    size = torch.cat([torch.tensor(sizes)[(torch.arange(n) // 128).clamp_max(len(sizes) - 1)] for n in lens]).cuda()
+    kc, vc, table = _written(k, v.float() * size[:, None, None], lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    for t in (table, _wide(table, 40000, 16)):
+        check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
+    native.check_status("cuda")
