@@ -988,10 +988,11 @@ void p4_configure(K kern, int smem, bool cluster, std::atomic<unsigned long long
 // clusters of 14 CTAs are fewer CTAs than fit, but take two turns (8 x 2048 tokens, 5 kv heads: 18.5 us, 10.7 in smaller ones).
 template <int D, int COLS>
 int p4_capacity(int splits) {
-  static std::atomic<int> known[17];
+  static std::atomic<int> known[64][17];          // per device
   static std::atomic<unsigned long long> seen{0};
-  int n = known[splits];
-  if (n > 0) return n;
+  int n = 0, dev = 0;
+  MB_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64 && (n = known[dev][splits]) > 0) return n;
   p4_configure(paged_attn_int4_cluster_kernel<D, COLS>, P4SmemCluster<D, COLS>::BYTES, true, seen);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -1005,8 +1006,9 @@ int p4_capacity(int splits) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = splits;
   MB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, paged_attn_int4_cluster_kernel<D, COLS>, &cfg));
-  known[splits] = std::max(1, n);
-  return std::max(1, n);
+  n = std::max(1, n);
+  if (dev < 64) known[dev][splits] = n;
+  return n;
 }
 int p4_capacity(int D, int cols, int splits) {
   if (D == 128) return cols == 16 ? p4_capacity<128, 16>(splits) : p4_capacity<128, 8>(splits);
