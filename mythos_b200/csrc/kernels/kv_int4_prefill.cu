@@ -17,7 +17,8 @@
 //     first tile's ev overflowed where later values were 2^130 times as large). Values below 2^-124 lose bits.
 // Tokens of a tile whose magnitudes lie more than 2^8 apart get exponents of their own (PF_SPREAD), so that a large token takes no
 // bits from the others for the queries that give it no weight or do not see it: the softmax then adds every key's own to its score
-// first. (That the kernel can do so costs 2048 tokens over 6144 256 -> 260 us, 6 ragged prompts of up to 700 21.0 -> 22.3.)
+// first. Such tiles, and tiles whose values lie 2^100 below the largest, take a step of their own (four times as long: 2048 tokens over 6144 with
+// one such token in every tile 850 us, not 226).
 // The matrix product multiplies masked probabilities of zero by whatever the value rows hold, so nothing that is not
 // finite goes there: tokens behind a sequence's end are zeros, and a token with a scale that is not finite gets values of
 // zero and NaN keys, which reach the queries that see it through their scores, and no others.
@@ -53,9 +54,9 @@ __device__ __forceinline__ int pf_exponent(float m) {
 }
 constexpr int PF_EV_MIN = -110;   // of a tile of values
 constexpr int PF_SPREAD = 8;      // octaves between the tokens of a tile that share an exponent: p keeps 2^-17 of the largest term
-// Octaves below the reference up to which the row sum is taken from p. What lies further below counts for nothing in the products, but does in
-// the sum where it is the values that are small.
-constexpr float PF_FAR = 100.f;
+// Octaves between the values' exponents of a part's tiles up to which row sums are taken from p, which goes with them: 26 are left for the scores
+// before fp32 ends. What lies below counts for nothing in the products, but would in the sum where it is the values that are small.
+constexpr int PF_ALIKE = 100;
 constexpr float PF_SUM_UNIT = 0x1p10f, PF_SUM_LOG = 10.f;      // of a row sum
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
 // Of values: zeros must not raise the reference (with an exponent of 0 they took thirteen bits and more from the other tiles' p).
@@ -391,8 +392,7 @@ struct PfCfg {
   static constexpr int OFF_V = OFF_K + KS * TILE_BYTES;
   static constexpr int OFF_BAR = OFF_V + VS * TILE_BYTES;
   static constexpr int NUM_BARS = 4 + 2 * KS + 2 * VS + 8;
-  static constexpr int OFF_SUM = OFF_BAR + NUM_BARS * 8 + 16;          // a float per softmax thread
-  static constexpr int SMEM_BYTES = OFF_SUM + 2 * PF_TILE * 4 + 1024;
+  static constexpr int SMEM_BYTES = OFF_BAR + NUM_BARS * 8 + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
   static constexpr int COL_S = 0;     // S_t at t * 128 (P_t over its first 64 columns)
   static constexpr int COL_O = 256;   // O_t at 256 + t * D
@@ -470,21 +470,21 @@ __host__ __device__ constexpr uint32_t pf_idesc(int M, int N, bool b_mn_major) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// A row's scores over a tile whose tokens have exponents of their own: in tensor memory they are replaced by score + ev of the token - ev of
-// the tile (e), as they enter the softmax. The row sum goes without the tokens' exponents: its logarithm is returned, minus infinity where
-// nothing is seen; it is formed from the scores as they were rounded there, and rounded as scores of its size are. Four at a time and ahead of
-// everything else, since the loop around it has to carry the code (32 at a time, with the sum between the halves of p: 6 ragged prompts of up to
-// 700 tokens without such tiles took 22.5 us, 22.3 this way).
-// Otherwise (OWN false) nothing is replaced, and row_f is the factor of the scores as they stand there.
-template <bool OWN>
-__device__ __forceinline__ float pf_own_scores(uint32_t t_s, const int16_t* own, float row_f, int limit, uint32_t absent, int e) {
-  float sum = 0.f, top = -1e30f;
+// One step of the softmax for parts whose exponents lie far apart, whatever they are: a row's scores over the tile at t_s are replaced by score +
+// ev of the token - ev of the tile (e), as they enter the softmax, and their sum goes without the tokens' exponents, from the scores as they were
+// rounded. `own`: the tokens' ek and ev, or null where all have the tile's. Four scores at a time, then 32: little code and few registers, since
+// the loops of ordinary parts must not pay for it (one loop with both cost 4 prompts of 2048 tokens 188 -> 195 us, 16 of 1024 with narrow heads
+// 196 -> 212). O_t is at t_o; `first`: the part's first step, which finds none.
+template <int D>
+__device__ __forceinline__ void pf_special_step(uint32_t t_s, uint32_t t_o, uint64_t* p_full, const int16_t* own, float row_f, int limit,
+                                                uint32_t absent, int ek, int e, bool first, float& m_ref, float& l) {
+  float sum = 0.f, top = -1e30f, m_new = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < PF_TILE; c += 4) {
     uint32_t x[4];
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(t_s + c) : "memory");
-    uint2 w = make_uint2(0u, 0u);
-    if constexpr (OWN) w = *reinterpret_cast<const uint2*>(own + c);
+    const uint32_t all = ((uint32_t)(ek & 0xFF) | (uint32_t)(e & 0xFF) << 8) * 0x10001u;
+    const uint2 w = own ? *reinterpret_cast<const uint2*>(own + c) : make_uint2(all, all);
     tmem_ld_wait();
     float y[4];
     const float before = top;
@@ -492,24 +492,56 @@ __device__ __forceinline__ float pf_own_scores(uint32_t t_s, const int16_t* own,
     for (int i = 0; i < 4; ++i) {
       const int both = (int16_t)((i < 2 ? w.x : w.y) >> (16 * (i & 1)));          // ek, ev
       const bool seen = c + i <= limit && !(absent >> (c >> 4) & 1u);
-      if constexpr (OWN) {
-        const float more = (float)((both >> 8) - e);
-        const float z = seen ? fmaf(__uint_as_float(x[i]), fmaxf(row_f * pf_pow2((signed char)both), 1e-37f), more) : -INFINITY;
-        x[i] = __float_as_uint(z);
-        y[i] = z - more;
-      } else {
-        y[i] = seen ? __uint_as_float(x[i]) * row_f : -INFINITY;
-      }
+      const float more = (float)((both >> 8) - e);
+      // (the factor is never zero: a masked score of minus infinity has to stay one)
+      const float z = seen ? fmaf(__uint_as_float(x[i]), fmaxf(row_f * pf_pow2((signed char)both), 1e-37f), more) : -INFINITY;
+      x[i] = __float_as_uint(z);
+      y[i] = z - more;
+      m_new = fmaxf(m_new, z);
       top = fmaxf(top, y[i]);
     }
-    if constexpr (OWN)
-      asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t_s + c), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t_s + c), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
     sum *= fast_exp2(before - top);
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum += fast_exp2(y[i] - top);
   }
-  if constexpr (OWN) tmem_st_wait();
-  return top + __log2f(sum);
+  tmem_st_wait();
+  const float ev = (float)e;
+  m_new += ev;
+  const bool need = m_new - m_ref > 6.f;         // as below
+  if (__any_sync(0xffffffffu, need)) {
+    // (the sum may outlast what the products are: exponents of values are in them only)
+    const float half = need ? fast_exp2(0.5f * (m_ref - m_new)) : 1.f, alpha = half * half;
+    if (need) m_ref = m_new;
+    l = l * half * half;
+    if (!first) {
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(t_o + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+        tmem_st16(t_o + c, o);
+      }
+    }
+  }
+  if (sum != 0.f) l += sum * fast_exp2(top - m_ref - PF_SUM_LOG);          // (nothing seen: the reference may be infinite)
+  const float shift = m_ref == -INFINITY ? 0.f : ev - m_ref;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {                  // P_t over columns of S_t that have been read
+    uint32_t x[32], pk[16];
+    tmem_ld32(t_s + c * 32, x);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) pk[i] = pf_half2(fast_exp2(__uint_as_float(x[2 * i]) + shift), fast_exp2(__uint_as_float(x[2 * i + 1]) + shift));
+    tmem_st16(t_s + c * 16, pk);
+    if (c & 1) {
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[c >> 1]);
+    }
+  }
 }
 
 template <int D>
@@ -715,7 +747,6 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem_base + Cfg::COL_S + t * 128 + lane_sel;
     const uint32_t t_o = tmem_base + Cfg::COL_O + t * D + lane_sel;
-    float* own_sum = reinterpret_cast<float*>(smem + Cfg::OFF_SUM) - PF_TILE;     // (indexed by threads 128 ..; a register for it would spill)
     const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.o_stride * 2)) & 31) == 0;
     uint32_t n_s = 0, n_o = 0;
     bool ok = true;
@@ -734,118 +765,140 @@ fa_int4_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int* ex = a.exponents + (long long)(it.b * kv_heads + a.line.by_share(c.of_unit)) * a.line.tiles;
       const float row_f = live ? a.q_factor[(long long)row * a.heads + head] * a.scale_log2 : 0.f;      // (other rows: no spread)
       float m_ref = -INFINITY, l = 0.f;       // (no key seen yet)
-      int e_next = end > j0 ? ex[j0] : 0;
-      for (int j = j0; j < end && ok; ++j) {
-        const int ek = (signed char)e_next, e = (signed char)(e_next >> 16);
-        const bool apart = e_next >> 24;      // (for the whole CTA)
-        bool by_itself = apart;               // the row's sum over the tile lies in shared memory
-        const uint32_t absent = (uint32_t)e_next >> 8 & 0xFFu;     // sixteens of keys without a page: no query sees them
-        if (j + 1 < end) e_next = ex[j + 1];
-        // (never zero: a masked score of minus infinity has to stay one)
-        const float sc = apart ? 1.f : fmaxf(row_f * pf_pow2(ek), 1e-37f), ev = (float)e;
-        ok = mbar_wait(&s_full[t], n_s & 1, abort_flag, status, 102);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        ++n_s;
-        tc_fence_after();
-        uint32_t sr[4][32];
-        float* s = reinterpret_cast<float*>(&sr[0][0]);
-        const int kv0 = j * PF_TILE;
-        const auto hide = [&](int from, int to) {
-          if (kv0 + to - 1 > limit) {
-#pragma unroll
-            for (int i = from; i < to; ++i)
-              if (kv0 + i > limit) s[i] = -INFINITY;
-          }
-          if (absent) {
-#pragma unroll
-            for (int i = from; i < to; ++i)
-              if (absent >> (i >> 4) & 1u) s[i] = -INFINITY;
-          }
-        };
-        if (apart) own_sum[threadIdx.x] = pf_own_scores<true>(t_s, a.own + (ex + j - a.exponents) * PF_TILE, row_f, limit - kv0, absent, e);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, sr[c]);
-        tmem_ld_wait();
-        hide(0, 128);
-        uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
-        uint32_t pk[2][32];
-        const auto exponentials = [&](int h) {   // of half h of the keys: fp16 pairs to pk[h], sums to rs2
-          const float shift = m_ref == -INFINITY ? 0.f : ev - m_ref;      // (without a key every score is minus infinity)
-          const uint64_t sc2 = f32x2(sc, sc), nm2 = f32x2(shift, shift);
-#pragma unroll
-          for (int i = 64 * h; i < 64 * h + 64; i += 2) {
-            float e0f, e1f;
-            f32x2_unpack(fma_f32x2(f32x2(s[i], s[i + 1]), sc2, nm2), e0f, e1f);
-            const float p0 = fast_exp2(e0f), p1 = fast_exp2(e1f);
-            rs2[(i >> 1) & 3] = add_f32x2(rs2[(i >> 1) & 3], f32x2(p0, p1));
-            pk[h][(i >> 1) & 31] = pf_half2(p0, p1);
-          }
-        };
-        const auto publish = [&](int h) {        // P_t: fp16 pairs over the first 64 columns of S_t
-          tmem_st32(t_s + 32 * h, pk[h]);
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&p_full[2 * t + h]);
-        };
-        // The reference rarely moves: the first half's exponentials are taken with the one there is, with the maximum of all
-        // 128 scores in their shadow, and again where it does (257 us -> 242 at 2048 over 6144; the registers that takes come from
-        // the service warps).
-        if (j > j0) exponentials(0);
-        float mx4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < 124; i += 8) {
-          mx4[0] = fmax3(mx4[0], s[i], s[i + 1]);
-          mx4[1] = fmax3(mx4[1], s[i + 2], s[i + 3]);
-          mx4[2] = fmax3(mx4[2], s[i + 4], s[i + 5]);
-          mx4[3] = fmax3(mx4[3], s[i + 6], s[i + 7]);
-        }
-        mx4[0] = fmax3(mx4[0], s[124], s[125]);
-        mx4[1] = fmax3(mx4[1], s[126], s[127]);
-        const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sc, ev);
-        // p up to 2^6 until the reference moves. The first score that is seen always sets it, in whatever tile it stands: a
-        // reference of zero kept from a tile without a visible key left p as 2^(score + ev), which fp16 may not hold.
-        const float up = m_new - m_ref;
-        const bool need = up > 6.f, far = up < -PF_FAR && up > -INFINITY;
-        if (j == j0 || __any_sync(0xffffffffu, need || far)) {
-          const float half = need ? fast_exp2(0.5f * (m_ref - m_new)) : 1.f, alpha = half * half;
-          if (need) m_ref = m_new;
-          if (j > j0) {
-            l = l * half * half;             // (the sum may outlast what the products are: exponents of values are in them only)
-            // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):
-            // O_t is quiescent until this warpgroup arrives on p_full, so a rescale can happen right here.
+      // The exponents of the part's tiles. Where some take a special step (tokens with their own, or far below the largest), the others are run
+      // stretch by stretch; otherwise nothing more is looked at.
+      int e_min = 127, e_max = -128, own = 0;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              tmem_ld32(t_o + c * 32, pk[0]);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) pk[0][i] = __float_as_uint(__uint_as_float(pk[0][i]) * alpha);
-              tmem_st32(t_o + c * 32, pk[0]);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) rs2[q] = 0ull;
-            tmem_ld32(t_s, sr[0]);               // (the first half again: its registers need not outlive the exponentials)
-            tmem_ld32(t_s + 32, sr[1]);
-            tmem_ld_wait();
-            hide(0, 64);
+      for (int j = j0 + lane; j < end; j += 32) {
+        const int w = ex[j], e = (signed char)(w >> 16);
+        e_min = min(e_min, e);
+        e_max = max(e_max, e);
+        own |= w >> 24;
+      }
+      e_max = __reduce_max_sync(0xffffffffu, e_max);
+      const bool plain = !__any_sync(0xffffffffu, own || e_max - e_min > PF_ALIKE);
+      for (int j = j0; j < end && ok;) {
+        int stop = end;                       // the next tile that takes a special step
+        if (!plain) {
+          for (int b = j; b < stop; b += 32) {
+            const int w = ex[min(b + lane, end - 1)], e = (signed char)(w >> 16);
+            const uint32_t found = __ballot_sync(0xffffffffu, b + lane < end && (w >> 24 || e < e_max - PF_ALIKE));
+            if (found) stop = b + __ffs(found) - 1;
           }
-          if (!apart && __any_sync(0xffffffffu, far)) {
-            const float own = pf_own_scores<false>(t_s, nullptr, sc, limit - kv0, absent, 0);
-            by_itself = far;
-            if (far) own_sum[threadIdx.x] = own;
+          if (stop == j) {
+            ok = mbar_wait(&s_full[t], n_s & 1, abort_flag, status, 102);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ++n_s;
+            tc_fence_after();
+            const int w = ex[j];
+            pf_special_step<D>(t_s, t_o, &p_full[2 * t], w >> 24 ? a.own + (ex + j - a.exponents) * PF_TILE : nullptr, row_f, limit - j * PF_TILE,
+                               (uint32_t)w >> 8 & 0xFFu, (signed char)w, (signed char)(w >> 16), j == j0, m_ref, l);
+            ++j;
+            continue;
           }
-          exponentials(0);
         }
-        publish(0);
-        exponentials(1);
-        publish(1);
-        float rs[8];
+        int e_next = ex[j];
+        for (; j < stop && ok; ++j) {
+          const int ek = (signed char)e_next, e = (signed char)(e_next >> 16);
+          const uint32_t absent = (uint32_t)e_next >> 8 & 0xFFu;     // sixteens of keys without a page: no query sees them
+          if (j + 1 < end) e_next = ex[j + 1];
+          // (never zero: a masked score of minus infinity has to stay one)
+          const float sc = fmaxf(row_f * pf_pow2(ek), 1e-37f), ev = (float)e;
+          ok = mbar_wait(&s_full[t], n_s & 1, abort_flag, status, 102);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          ++n_s;
+          tc_fence_after();
+          uint32_t sr[4][32];
+          float* s = reinterpret_cast<float*>(&sr[0][0]);
+          const int kv0 = j * PF_TILE;
+          const auto hide = [&](int from, int to) {
+            if (kv0 + to - 1 > limit) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
-        if (by_itself) {
-          const float own = own_sum[threadIdx.x];
-          l += own == -INFINITY ? 0.f : fast_exp2(own - m_ref - PF_SUM_LOG);       // (nothing seen: the reference may be infinite)
-        } else l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(-e) * (1.f / PF_SUM_UNIT);
+              for (int i = from; i < to; ++i)
+                if (kv0 + i > limit) s[i] = -INFINITY;
+            }
+            if (absent) {
+#pragma unroll
+              for (int i = from; i < to; ++i)
+                if (absent >> (i >> 4) & 1u) s[i] = -INFINITY;
+            }
+          };
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, sr[c]);
+          tmem_ld_wait();
+          hide(0, 128);
+          uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
+          uint32_t pk[2][32];
+          const auto exponentials = [&](int h) {   // of half h of the keys: fp16 pairs to pk[h], sums to rs2
+            const float shift = m_ref == -INFINITY ? 0.f : ev - m_ref;      // (without a key every score is minus infinity)
+            const uint64_t sc2 = f32x2(sc, sc), nm2 = f32x2(shift, shift);
+#pragma unroll
+            for (int i = 64 * h; i < 64 * h + 64; i += 2) {
+              float e0f, e1f;
+              f32x2_unpack(fma_f32x2(f32x2(s[i], s[i + 1]), sc2, nm2), e0f, e1f);
+              const float p0 = fast_exp2(e0f), p1 = fast_exp2(e1f);
+              rs2[(i >> 1) & 3] = add_f32x2(rs2[(i >> 1) & 3], f32x2(p0, p1));
+              pk[h][(i >> 1) & 31] = pf_half2(p0, p1);
+            }
+          };
+          const auto publish = [&](int h) {        // P_t: fp16 pairs over the first 64 columns of S_t
+            tmem_st32(t_s + 32 * h, pk[h]);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_full[2 * t + h]);
+          };
+          // The reference rarely moves: the first half's exponentials are taken with the one there is, with the maximum of all
+          // 128 scores in their shadow, and again where it does (257 us -> 242 at 2048 over 6144; the registers that takes come from
+          // the service warps).
+          if (j > j0) exponentials(0);
+          float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int i = 4; i < 124; i += 8) {
+            mx4[0] = fmax3(mx4[0], s[i], s[i + 1]);
+            mx4[1] = fmax3(mx4[1], s[i + 2], s[i + 3]);
+            mx4[2] = fmax3(mx4[2], s[i + 4], s[i + 5]);
+            mx4[3] = fmax3(mx4[3], s[i + 6], s[i + 7]);
+          }
+          mx4[0] = fmax3(mx4[0], s[124], s[125]);
+          mx4[1] = fmax3(mx4[1], s[126], s[127]);
+          const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sc, ev);
+          // p up to 2^6 until the reference moves. The first score that is seen always sets it, in whatever tile it stands: a
+          // reference of zero kept from a tile without a visible key left p as 2^(score + ev), which fp16 may not hold.
+          const bool need = m_new - m_ref > 6.f;
+          if (j == j0 || __any_sync(0xffffffffu, need)) {
+            const float half = need ? fast_exp2(0.5f * (m_ref - m_new)) : 1.f, alpha = half * half;
+            if (need) m_ref = m_new;
+            if (j > j0) {
+              l = l * half * half;             // (in two steps, as in special ones)
+              // S_t(j) complete implies PV_t(j-1) complete (same issuing thread, commit covers earlier MMAs):
+              // O_t is quiescent until this warpgroup arrives on p_full, so a rescale can happen right here.
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                tmem_ld32(t_o + c * 32, pk[0]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) pk[0][i] = __float_as_uint(__uint_as_float(pk[0][i]) * alpha);
+                tmem_st32(t_o + c * 32, pk[0]);
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) rs2[q] = 0ull;
+              tmem_ld32(t_s, sr[0]);               // (the first half again: its registers need not outlive the exponentials)
+              tmem_ld32(t_s + 32, sr[1]);
+              tmem_ld_wait();
+              hide(0, 64);
+            }
+            exponentials(0);
+          }
+          publish(0);
+          exponentials(1);
+          publish(1);
+          float rs[8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) f32x2_unpack(rs2[q], rs[2 * q], rs[2 * q + 1]);
+          l += (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]))) * pf_pow2(-e) * (1.f / PF_SUM_UNIT);
+        }
       }
       if (!ok) break;
       if (end > j0) {
