@@ -137,16 +137,19 @@ struct P4State {
   uint32_t qb[NB][GR][8];                 // B operand: column r
   float qsum[NB][GR][2], factor[NB][2];   // of columns 2 t, 2 t + 1, as everything below
   int limit[NB][2];
-  float o[NB][GR][4][4];                  // units of 2^-24 (even i) and 2^-20
+  float o[NB][GR][4][4];                  // units of 2^-(24 + P4_DOWN) (even i) and 2^-(20 + P4_DOWN)
   float z[NB][GR][2], m[NB][2], l[NB][2];
   uint32_t unseen;                        // bit 2 nb + c: the column has seen no score yet (its reference is 0)
 };
 
-// Exponent that values of magnitude `mag` enter the reference with. p is kept up to 2^8 (and 2^6 more until the reference moves) times
-// the inverse of the token's largest magnitude, which is at least 7 scales: p times a scale then stays below 2^13, and is exact to 2^-11
-// over 19 octaves below the reference. Bounded so that p, its sum and its product with any value stay within fp32.
+// Exponent that values of magnitude `mag` enter the reference with. p is kept up to 2^19 (and 2^6 more until the reference moves) times
+// the inverse of the token's largest magnitude, which is at least 7 scales: p times a scale times 2^-P4_DOWN then stays below 2^12, and is
+// exact to 2^-11 over 19 octaves below the reference. Every bf16 magnitude from 2^-81 on has its own: p is 2^-108 at least at the reference, so
+// that 18 octaves of weights below it count, and 2^106 at most, so that a million of them stay within fp32, and so does a product with any
+// value. (With 2^8 and without P4_DOWN magnitudes ended at 2^112, and p times a scale overflowed above 2^117.)
+constexpr int P4_DOWN = 11;
 __device__ __forceinline__ float p4_exponent(float mag) {
-  return fminf(fmaxf(__uint_as_float(0x4B000000u | (__float_as_uint(mag) >> 23)) - (8388608.f + 127.f), -80.f), 112.f) - 8.f;
+  return fminf(fmaxf(__uint_as_float(0x4B000000u | (__float_as_uint(mag) >> 23)) - (8388608.f + 127.f), -81.f), 127.f) - 19.f;
 }
 
 // One chunk: tile u (0, 1) at `at` + u * TILE_BYTES for K, HALF behind for V; tok0: its first token.
@@ -298,7 +301,7 @@ __device__ __forceinline__ void p4_chunk(P4State<D, COLS>& s, const uint8_t* at,
   // ---- weights p scale as the B operand (k = tokens, n = columns): transposed in blocks of eight by eight. Odd key rows
   // are the tokens that enter with the complement of their codes.
   uint32_t pb[2][NB][GR][2];
-  const float sign = (r & 1) ? -1.f : 1.f, whole = (r & 1) ? 15.f : 0.f;
+  const float sign = ((r & 1) ? -1.f : 1.f) / (1 << P4_DOWN), whole = (r & 1) ? 15.f : 0.f;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -463,7 +466,7 @@ __device__ __forceinline__ void p4_result(const P4State<D, COLS>& s, const P4Arg
         float v[8];                               // out of their units, with the offset sum
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float unit = (q & 1) ? 0x1p20f : 0x1p24f;
+          const float unit = ((q & 1) ? 0x1p20f : 0x1p24f) * (1 << P4_DOWN);
           v[2 * q] = fmaf(s.o[nb][g][q][c], unit, z) * inv;
           v[2 * q + 1] = fmaf(s.o[nb][g][q][2 + c], unit, z) * inv;
         }

@@ -246,3 +246,19 @@ def test_value_sizes_further_apart_than_32_bits_go(D, new, lens, sizes):
     for t in (table, _wide(table, 40000, 16)):
         check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
     native.check_status("cuda")
+
+
+@pytest.mark.parametrize("size", [1e33, 1e35, 1e37, 5e37])
+@pytest.mark.parametrize("new,lens", [([1, 1], [3000, 700]), ([6, 2], [600, 300]), ([700, 300], [900, 700])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_near_the_largest_there_are(D, new, lens, size):
+    H, Hk = 4, 2
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    k[..., 0] = torch.arange(sum(lens), device="cuda")[:, None].remainder(97) / 8        # scores that rise again and again
+    kc, vc, table = _written(k, v.float().clamp(-3, 3) * size, lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q[..., 0] = 4.0
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    for t in (table, _wide(table, 40000, 16)):
+        check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
+    native.check_status("cuda")
