@@ -285,7 +285,7 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
   }
   __shared__ uint32_t s_pair[2][PF_TILE][L::GROUPS];
   __shared__ int s_tile[8];
-  __shared__ uint32_t s_ext[4][PF_EXPAND / 32];       // largest magnitude of K and V, smallest that is not zero
+  __shared__ uint32_t s_ext[4][PF_EXPAND / 32];       // largest magnitudes of K and V, smallest
   __shared__ int8_t s_own[2][PF_TILE];
   const int j = blockIdx.x % a.tiles, bh = blockIdx.x / a.tiles, b = bh / a.kv_heads, head = bh % a.kv_heads;
   const int len = a.kv_lens[b], n0 = j * PF_TILE;
@@ -302,6 +302,7 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
   // pairs of both tensors; the largest magnitude a group can stand for lies at one of its ends
   static_assert(PF_TILE * L::GROUPS <= PF_EXPAND && PF_TILE * L::GROUPS % 32 == 0, "a thread holds one group at most, and warps go together");
   float km = 0.f, vm = 0.f;            // of the thread's token
+  bool held = false;                   // with values that are numbers
   if (const int i = threadIdx.x; i < PF_TILE * L::GROUPS) {
     const int n = i / L::GROUPS, g = i % L::GROUPS, tile = s_tile[n >> 4];
     uint32_t kp = 0u, vp = 0u;
@@ -315,6 +316,7 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
         finite = finite && kv4_finite(p);
         if (gg == g) vp = p;
       }
+      held = finite;
       if (!finite) {
         kp = 0x7FFF7FFFu;
         vp = 0u;
@@ -333,10 +335,12 @@ kv4_expand_kernel(const __grid_constant__ PfExpand a) {
       s_own[1][n] = (int8_t)pf_value_exponent(vm);
     }
   }
-  {                                    // (as integers: they are not negative)
+  // (As integers: they are not negative. Values of zero count as the smallest there are: a token of them that takes nearly all the weight
+  // must not push the others' p out of fp16. Keys of zero do no harm.)
+  {
     const uint32_t kb = __float_as_uint(km), vb = __float_as_uint(vm);
     const uint32_t k1 = __reduce_max_sync(0xffffffffu, kb), v1 = __reduce_max_sync(0xffffffffu, vb);
-    const uint32_t k0 = __reduce_min_sync(0xffffffffu, kb ? kb : ~0u), v0 = __reduce_min_sync(0xffffffffu, vb ? vb : ~0u);
+    const uint32_t k0 = __reduce_min_sync(0xffffffffu, kb ? kb : ~0u), v0 = __reduce_min_sync(0xffffffffu, held ? vb : ~0u);
     if ((threadIdx.x & 31) == 0) {
       s_ext[0][threadIdx.x >> 5] = k1;
       s_ext[1][threadIdx.x >> 5] = v1;

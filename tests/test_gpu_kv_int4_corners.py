@@ -262,3 +262,24 @@ def test_values_near_the_largest_there_are(D, new, lens, size):
     for t in (table, _wide(table, 40000, 16)):
         check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
     native.check_status("cuda")
+
+
+@pytest.mark.parametrize("score", [10.0, 30.0, 60.0])
+@pytest.mark.parametrize("new,lens", [([1, 1], [3000, 700]), ([700, 300], [900, 700]), ([2500], [2500])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_token_of_zeros_that_takes_nearly_all_the_weight(D, new, lens, score):
+    H, Hk = 4, 2
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    k[..., 0] = 0.0
+    first = 0
+    for n in lens:
+        for at in (3, 400):
+            v[first + at] = 0.0
+            k[first + at, :, 0] = score * math.sqrt(D) / 8
+        first += n
+    kc, vc, table = _written(k, v, lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q[..., 0] = 8.0
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    check(F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens)), *want)
+    native.check_status("cuda")
