@@ -57,7 +57,7 @@ constexpr int PF_SPREAD = 8;      // octaves between the tokens of a tile that s
 // Octaves between the values' exponents of a part's tiles up to which row sums are taken from p, which goes with them: 26 are left for the scores
 // before fp32 ends. What lies below counts for nothing in the products, but would in the sum where it is the values that are small.
 constexpr int PF_ALIKE = 100;
-constexpr float PF_SUM_UNIT = 0x1p10f, PF_SUM_LOG = 10.f;      // of a row sum
+constexpr float PF_SUM_UNIT = 0x1p10f;      // of a row sum
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
 // Of values: zeros must not raise the reference (with an exponent of 0 they took thirteen bits and more from the other tiles' p).
 __device__ __forceinline__ int pf_value_exponent(float m) { return m > 0.f ? max(PF_EV_MIN, pf_exponent(m)) : PF_EV_MIN; }
@@ -530,7 +530,11 @@ __device__ __forceinline__ void pf_special_step(uint32_t t_s, uint32_t t_o, uint
       }
     }
   }
-  if (sum != 0.f) l += sum * fast_exp2(top - m_ref - PF_SUM_LOG);          // (nothing seen: the reference may be infinite)
+  if (sum != 0.f) {                              // (nothing seen: the reference may be infinite)
+    // in two factors: beside the largest values the sum lies near fp32's smallest numbers, where ex2 gives zero
+    const float half = fast_exp2(0.5f * (top - m_ref));
+    l += sum * half * (1.f / PF_SUM_UNIT) * half;
+  }
   const float shift = m_ref == -INFINITY ? 0.f : ev - m_ref;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {                  // P_t over columns of S_t that have been read

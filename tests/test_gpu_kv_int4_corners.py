@@ -283,3 +283,26 @@ def test_a_token_of_zeros_that_takes_nearly_all_the_weight(D, new, lens, score):
     want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
     check(F.paged_attn_prefill_int4(q, kc, vc, table, cu, ctx, max(new), max(lens)), *want)
     native.check_status("cuda")
+
+
+@pytest.mark.parametrize("below", [2.0, 6.0, 10.0])
+@pytest.mark.parametrize("new,lens", [([1, 1], [3000, 700]), ([6, 2], [600, 300]), ([700, 300], [900, 700]), ([1000], [3000])])
+def test_small_weights_beside_the_largest_values_count_in_the_sum(new, lens, below):
+    H, Hk, D = 4, 2, 128
+    k, v = random_rows(sum(lens), Hk, D, 6, "cuda")
+    v = v.float() * 1e-10
+    k[..., 0] = 0.0
+    first = 0
+    for n in lens:                                              # a token of 1e37, scores of the others lower by `below`
+        v[first + 20] *= 1e23
+        v[first + 20] *= 1e24
+        k[first + 20, :, 0] = below * math.sqrt(D) / 8
+        first += n
+    k[..., 1:] *= 0.1
+    kc, vc, table = _written(k, v, lens, Hk, D)
+    q, cu, ctx = _queries(sum(new), H, D), _cu(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q[..., 0] = 8.0
+    want = attention(q, kc, vc, table, cu[:-1].tolist(), new, lens, 1 / math.sqrt(D))
+    for t in (table, _wide(table, 40000, 16)):
+        check(F.paged_attn_prefill_int4(q, kc, vc, t, cu, ctx, max(new), max(lens)), *want)
+    native.check_status("cuda")
