@@ -5,14 +5,14 @@
 // clamp(round_to_even((x - low) / scale), 0, 15); it stands for scale * code + low. The range is kept
 // asymmetric because keys carry per-channel offsets: a symmetric scale would spend codes on values that do
 // not occur. The scale is rounded to bf16 (half the bytes of fp32): codes are formed against the rounded
-// scale, so its rounding moves the grid by at most 2^-9 of a step per code and adds no error of its own.
+// scale, so its rounding moves the grid by at most 2^-8 of a step per code and adds no error of its own.
 // 64 values per group cost 4.5 bits a value; groups of 32 would cost 5 (one ninth more bytes to read per
 // decoded token). A group with a NaN, an infinity or a range beyond fp32 has a NaN or infinite scale and
 // reads back as NaN: nothing finite is made up.
 //
 // A cache is [pages, kv_heads, page_size / 16 tiles, TILE_BYTES] bytes. A tile is 16 tokens: 16 rows of codes
 // (D / 2 bytes each), then 16 rows of (scale, low) pairs (D / 16 bytes each); contiguous, a multiple of 16
-// bytes, so one bulk copy fetches it. The order inside a tile is that of the tensor-core fragments the attention
+// bytes, fetched in 16-byte pieces. The order inside a tile is that of the tensor-core fragments the attention
 // kernel builds, so that a thread reads its operands with 16-byte (keys) and 8-byte (values) shared loads,
 // without bank conflicts and without ldmatrix:
 //   * eight consecutive values share a 32-bit word; value 2 i + j sits in nibble i + 4 j: word >> 4 i masked by

@@ -5,7 +5,7 @@
 // lanes to a tile: a bulk copy takes its addresses from uniform registers, and four lanes with a copy each cost 61 instructions
 // a chunk, of 675, where these nine take twelve.
 //
-// What bounds it is the integer pipe (half rate) that takes the codes apart, so operands are formed by one AND each:
+// Most of its instructions take codes apart, on the integer pipe (half rate), so operands are formed by one AND each:
 // the low eleven bits of an fp16 are linear in its value (subnormals and the first normal binade share one step,
 // 2^-24), so a nibble anywhere in them is its code times a power of two. Keys: bits 3-6 (code 2^-21) and 7-10 (code 2^-17)
 // of a rotated word, then the word rotated by eight; queries of the second kind are multiplied by 2^-4. Values: bits 0-3
@@ -146,7 +146,8 @@ struct P4State {
 // the inverse of the token's largest magnitude, which is at least 7 scales: p times a scale times 2^-P4_DOWN then stays below 2^12, and is
 // exact to 2^-11 over 19 octaves below the reference. Every bf16 magnitude from 2^-81 on has its own: p is 2^-108 at least at the reference, so
 // that 18 octaves of weights below it count, and 2^106 at most, so that a million of them stay within fp32, and so does a product with any
-// value. (With 2^8 and without P4_DOWN magnitudes ended at 2^112, and p times a scale overflowed above 2^117.)
+// value. Smaller magnitudes lose bits, below 2^-110 all. (With 2^8 and without P4_DOWN magnitudes ended at 2^112, and p times a scale
+// overflowed above 2^117.)
 constexpr int P4_DOWN = 11;
 __device__ __forceinline__ float p4_exponent(float mag) {
   return fminf(fmaxf(__uint_as_float(0x4B000000u | (__float_as_uint(mag) >> 23)) - (8388608.f + 127.f), -81.f), 127.f) - 19.f;
@@ -1034,9 +1035,9 @@ P4Plan p4_plan(int batch, int max_q, int G, int kv_heads, int D, long long max_t
   p.ctas = (int)std::max(1LL, std::min(p.resident, (p.units * p.chunks + P4_WARPS - 1) / P4_WARPS));
   // A cluster per unit, of as many CTAs as the units leave room for, while no warp gets more than sixteen chunks (eight, where a
   // larger cluster would have been of use). One launch, no scratch and no walk along the line: 64 x 1024 tokens (8 kv heads, one
-  // query) take 22.0 us (27.5 as a line), 64 x 2048 36.9 (41.6), 64 ragged x 1280 23.7 (27.2), 1 x 1024 6.3 (9.3), 8 x 8192 23.2
-  // (26.5). Longer contexts want the line's evenness: 1 x 32768 take 22.6 there (24.2), 2 x 32768 27.1 (31.3), and what lies between
-  // is even: 1 x 16384 15.5 (15.5).
+  // query) take 22.1 us (27.4 as a line), 64 x 2048 37.2 (41.1), 64 ragged x 1280 24.2 (27.3), 1 x 1024 6.8 (9.3), 8 x 8192 23.9
+  // (26.8). Longer contexts want the line's evenness: 1 x 32768 take 23.1 there (24.2 before as clusters), 2 x 32768 27.5 (31.3), and what
+  // lies between is even: 1 x 16384 16.1 (15.5).
   const long long want = std::min(16LL, (p.chunks + P4_WARPS - 1) / P4_WARPS);
   long long room = std::max(1LL, std::min(want, p.resident / std::max(1LL, p.units)));
   while (room > 1 && p4_capacity(D, p.cols, (int)room) < p.units) --room;

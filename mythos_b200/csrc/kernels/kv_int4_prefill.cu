@@ -4,8 +4,8 @@
 // fp16 in a workspace, once for all the queries that read them, and the queries into fp16 rows; fa_int4_kernel is the
 // persistent two-tile flash attention kernel of attention_fwd2.cu over those images (128 x 128 score tiles, P in tensor memory).
 //
-// Why fp16 and not bf16: a value scale * code + low has up to 20 significant bits. Rounded to bf16 (half a step, 2^-9)
-// every key moves its score by 2^-9 of sum |q k|, which is several times the error of all other roundings together
+// Why fp16 and not bf16: a value scale * code + low has up to 20 significant bits. Rounded to bf16 (half a step, 2^-8)
+// every key moves its score by up to 2^-8 of sum |q k|, which is several times the error of all other roundings together
 // (measured 4.5e-3 of the output in bf16 against 1.7e-3 here, of which 1.65e-3 is the output's own rounding). fp16
 // has three bits more but a range of 2^-14 .. 2^15, so exponents are factored out, all powers of two (exact):
 //   * a query row is divided by 2^eq (its largest value then lies in 2^14 .. 2^15); the thread that owns the row's softmax

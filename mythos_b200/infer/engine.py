@@ -194,7 +194,9 @@ class InferenceEngine:
         """``kv_dtype``: "bf16", "int8" for pages of int8 rows with one scale per (token, kv head)
         (half the KV bytes per decode step; the reference's block-quantised cache mode,
         src/kv_cache.cpp:13-42, 78-137), or "int4" for pages of 4-bit codes with a scale and a minimum per 64
-        values (9/32 of the bytes; head widths 64 and 128)."""
+        values (9/32 of the bytes; head widths 64 and 128). With either a prompt that starts a sequence attends
+        over its own rows as they are; what follows, and portions of long prompts over 4-bit pages, over the
+        quantised ones."""
         if kv_dtype not in KV_DTYPES:
             raise ValueError(f"kv_dtype must be one of {sorted(KV_DTYPES)}, got {kv_dtype!r}")
         if kv_dtype == "int4" and (cfg.head_dim not in (64, 128) or page_size % 16):
