@@ -234,6 +234,20 @@ def kv4_quantise(x):
     return code.to(torch.uint8).flatten(-2), scale.squeeze(-1).to(torch.bfloat16), lo.squeeze(-1).to(torch.bfloat16)
 
 
+def kv4_values(code, scale, low, dtype=torch.bfloat16):
+    """scale * code + low (fp32 tensors that broadcast) rounded once to ``dtype``, as the kernels' fused multiply-add does: a sum in 32
+    bits would lose a low far below the product, and with it which way a bf16 tie goes."""
+    p, low = code.double() * scale.double(), low.double()
+    s = p + low
+    y = s.float()
+    if dtype == torch.bfloat16:
+        b = s - p
+        rest = (s - y.double()) + ((p - (s - b)) + (low - b))          # what y lacks (two-sum)
+        tie = (y.view(torch.int32) & 0xFFFF) == 0x8000
+        y = torch.where(tie & (rest != 0), torch.nextafter(y, torch.where(rest > 0, torch.inf, -torch.inf).to(y)), y)
+    return y.to(dtype)
+
+
 def _kv4_row(n):
     return (n & 8) + ((n & 3) << 1) + ((n >> 2) & 1)
 
@@ -307,8 +321,8 @@ def kv_read_int4(k_cache, v_cache, block_table, positions, seq_ids, head_dim: in
         w = w.gather(2, _kv4_word_order(D, n, is_key)[:, None].expand_as(w))
         code = (w[..., None] >> at & 15).flatten(2).float().unflatten(-1, (-1, KV4_GROUP))
         pair = pairs[page, :, tile, _kv4_row(n)].contiguous().view(torch.bfloat16).float().unflatten(-1, (-1, 2))
-        x = (code * pair[..., :1] + pair[..., 1:]).flatten(2)
-        out.append(torch.where(ok[:, None, None], x, torch.zeros_like(x)).to(dtype))
+        x = kv4_values(code, pair[..., :1], pair[..., 1:], dtype).flatten(2)
+        out.append(torch.where(ok[:, None, None], x, torch.zeros_like(x)))
     return out[0], out[1]
 
 
